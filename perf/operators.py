@@ -1,0 +1,455 @@
+"""The operators of a training step around its products, as cases that can be timed and compared.
+
+    layer_norm   a row's normalisation with the statistics it is differentiated from, and the gradient of
+                 input, gain and bias
+    dropout      a mask that a counter-based generator makes of a key and an element's position, with or
+                 without a residual that it is added to; its gradient is the same operator
+    log_probs    log probability of one token per row of logits, the distribution's entropy, the most
+                 likely tokens; and the gradient of the first two
+
+With ``own`` false the operators are elementary torch operations, with ``own`` true the calls that a
+program makes of ``raven_amd.nx_backend.Backend``, whose results go to tensors that the program keeps.
+"""
+
+from __future__ import annotations
+
+import functools
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+DTYPES = {"bfloat16": torch.bfloat16, "float16": torch.float16, "float32": torch.float32, "float64": torch.float64}
+SIZES = {"bfloat16": 2, "float16": 2, "float32": 4, "float64": 8}
+EPS = 1e-5
+
+
+# ── the cases ───────────────────────────────────────────────────────────────────────────────────
+
+def listed():
+    return [
+        # A step of eight sequences, one token each, through a norm of GPT-2 small: latency counts.
+        {"name": "norm_step", "op": "norm", "grad": False, "dtype": "bfloat16", "rows": 8, "n": 768, "affine": True},
+        # A norm of GPT-2 small over a training batch of 8 x 1024 tokens, forward and backward.
+        {"name": "norm_batch", "op": "norm", "grad": False, "dtype": "bfloat16", "rows": 8192, "n": 768, "affine": True},
+        {"name": "norm_batch_grad", "op": "norm", "grad": True, "dtype": "bfloat16", "rows": 8192, "n": 768, "affine": True},
+        # Queries or keys normalised per head: very many short rows.
+        {"name": "norm_heads_grad", "op": "norm", "grad": True, "dtype": "float16", "rows": 98304, "n": 64, "affine": True},
+        # Rows that are no whole number of vectors, in float32.
+        {"name": "norm_ragged_grad", "op": "norm", "grad": True, "dtype": "float32", "rows": 4097, "n": 1001, "affine": True},
+        # The hidden layer of a small classifier.
+        {"name": "drop_small", "op": "dropout", "dtype": "float32", "rows": 32, "n": 128, "rate": 0.5, "residual": False},
+        # The end of a sublayer of GPT-2 small: dropout, then the residual.
+        {"name": "drop_residual", "op": "dropout", "dtype": "bfloat16", "rows": 8192, "n": 768, "rate": 0.1, "residual": True},
+        # Attention probabilities of eight sequences of 1024 tokens and twelve heads.
+        {"name": "drop_scores", "op": "dropout", "dtype": "bfloat16", "rows": 98304, "n": 1024, "rate": 0.1, "residual": False},
+        # A decoding step of eight sequences: what was sampled, and the alternatives shown beside it. The logits
+        # are a matrix product's result, whose rows start on memory lines.
+        {"name": "lp_step", "op": "log_probs", "do": "score", "dtype": "bfloat16", "rows": 8, "vocab": 50257, "top": 20,
+         "entropy_grad": False, "pitched": True, "banned": 0.0},
+        # Two prompts of 1024 tokens scored in float32, five alternatives each.
+        {"name": "lp_score", "op": "log_probs", "do": "score", "dtype": "float32", "rows": 2048, "vocab": 50257, "top": 5,
+         "entropy_grad": False, "pitched": False, "banned": 0.01},
+        # The loss of a training batch of 8 x 1024 tokens over GPT-2's vocabulary and its gradient.
+        {"name": "lp_train", "op": "log_probs", "do": "train", "dtype": "bfloat16", "rows": 8192, "vocab": 50257, "top": 0,
+         "entropy_grad": False, "pitched": True, "banned": 0.0},
+        # The gradient alone, with an entropy bonus, over rows of an odd length.
+        {"name": "lp_grad_ragged", "op": "log_probs", "do": "grad", "dtype": "float16", "rows": 777, "vocab": 10007, "top": 0,
+         "entropy_grad": True, "pitched": False, "banned": 0.0},
+    ]
+
+
+def _log(rng, low, high):
+    """A whole number between low and high, spread over its logarithm."""
+    return max(low, min(high, round(math.exp(rng.uniform(math.log(low), math.log(high))))))
+
+
+def draw(rng):
+    op = rng.choice(["norm", "dropout", "log_probs"])
+    dtype = rng.choice(["bfloat16", "bfloat16", "float16", "float32", "float32", "float64"])
+    if op == "norm":
+        n = _log(rng, 8, 20000)
+        return {"op": op, "grad": rng.random() < 0.6, "dtype": dtype, "rows": _log(rng, 1, min(65536, (1 << 25) // n)),
+                "n": n, "affine": rng.random() < 0.8}
+    if op == "dropout":
+        n = _log(rng, 1, 8192)
+        return {"op": op, "dtype": dtype, "rows": _log(rng, 1, min(65536, (1 << 25) // n)), "n": n,
+                "rate": rng.choice([0.0, 0.1, 0.2, 0.5, 0.75]), "residual": rng.random() < 0.5}
+    vocab = _log(rng, 2, 200000)
+    do = rng.choice(["score", "score", "train", "grad"])
+    return {"op": op, "do": do, "dtype": dtype, "rows": _log(rng, 1, min(8192, (1 << 26) // vocab)), "vocab": vocab,
+            "top": min(vocab, rng.choice([0, 1, 5, 20, 64])) if do == "score" else 0,
+            "entropy_grad": do != "score" and rng.random() < 0.5, "pitched": rng.random() < 0.5,
+            "banned": rng.choice([0.0, 0.0, 0.01, 0.5])}
+
+
+def work(case):
+    e, s = SIZES[case["dtype"]], 8 if case["dtype"] == "float64" else 4
+    if case["op"] == "norm":
+        r, n, w = case["rows"], case["n"], 1 if case["affine"] else 0
+        if case["grad"]:
+            return {"bytes": 3 * r * n * e + (2 + w) * n * e + 2 * r * s, "flops": 14 * r * n}
+        return {"bytes": 2 * r * n * e + 2 * w * n * e + 2 * r * s, "flops": 8 * r * n}
+    if case["op"] == "dropout":
+        size = case["rows"] * case["n"]
+        return {"bytes": (3 if case["residual"] else 2) * size * e + 8, "flops": size * 22}
+    r, size = case["rows"], case["rows"] * case["vocab"]
+    score = size * e + r * (4 + 4 * s) + r * case["top"] * (4 + s)
+    grad = 2 * size * e + r * (4 + 3 * s) + (2 * r * s if case["entropy_grad"] else 0)
+    return {"bytes": {"score": score, "grad": grad, "train": score + grad}[case["do"]],
+            "flops": {"score": 6, "grad": 6, "train": 12}[case["do"]] * size}
+
+
+# ── inputs ──────────────────────────────────────────────────────────────────────────────────────
+
+class State:
+    """What a program has in hand: inputs, the tensors that results go to, and the backend's handles of both."""
+
+    def __init__(self, case, inputs, results):
+        self.case, self.inputs, self.results = case, inputs, results
+        self.handles = None
+
+
+def _wide(dtype):
+    """What sums and statistics are held in."""
+    return torch.float64 if dtype == torch.float64 else torch.float32
+
+
+def _norm_inputs(c, g):
+    dtype, wide = DTYPES[c["dtype"]], _wide(DTYPES[c["dtype"]])
+    r, n = c["rows"], c["n"]
+    # activations of a residual stream: rows of different scales, off zero
+    scale = torch.exp(torch.randn(r, 1, generator=g, device="cuda") * 0.5)
+    x = (torch.randn(r, n, generator=g, device="cuda") * scale + torch.randn(r, 1, generator=g, device="cuda") * 0.5).to(dtype)
+    inputs = {"x": x}
+    if c["affine"]:
+        inputs["gamma"] = (1 + 0.1 * torch.randn(n, generator=g, device="cuda")).to(dtype)
+        inputs["beta"] = (0.1 * torch.randn(n, generator=g, device="cuda")).to(dtype)
+    if not c["grad"]:
+        return inputs
+    inputs.pop("beta", None)
+    inputs["g"] = torch.randn(r, n, generator=g, device="cuda").to(dtype)
+    mean = torch.empty(r, dtype=wide, device="cuda")
+    rstd = torch.empty(r, dtype=wide, device="cuda")
+    step = max(1, (1 << 24) // n)
+    for at in range(0, r, step):
+        var, mu = torch.var_mean(x[at:at + step].double(), 1, unbiased=False)
+        mean[at:at + step], rstd[at:at + step] = mu, 1 / torch.sqrt(var + EPS)
+    inputs["mean"], inputs["rstd"] = mean, rstd
+    return inputs
+
+
+def _dropout_inputs(c, g):
+    shape = (c["rows"], c["n"])
+    inputs = {"x": torch.randn(shape, generator=g, device="cuda").to(DTYPES[c["dtype"]])}
+    if c["residual"]:
+        inputs["residual"] = torch.randn(shape, generator=g, device="cuda").to(DTYPES[c["dtype"]])
+    inputs["key"] = torch.randint(-2**31, 2**31, (2,), generator=g, device="cuda").int()
+    return inputs
+
+
+def _logits(c, g, like=None):
+    """Logits of a model that has learned something: a few tokens stand out. Rows of a matrix product start on lines of 128 bytes."""
+    dtype, (r, v) = DTYPES[c["dtype"]], (c["rows"], c["vocab"])
+    pitch = -(-v * SIZES[c["dtype"]] // 128) * 128 // SIZES[c["dtype"]] if c["pitched"] else v
+    x = torch.empty(r, pitch, dtype=dtype, device="cuda")[:, :v]
+    step = max(1, (1 << 26) // v)
+    for at in range(0, r, step):
+        x[at:at + step] = torch.randn(x[at:at + step].shape, generator=g, device="cuda") * 2.5
+    if c["banned"]:
+        ban = torch.rand(v, generator=g, device="cuda") < c["banned"]
+        ban[0] = False
+        x[:, ban] = -math.inf
+    return x
+
+
+def _log_probs_inputs(c, g):
+    wide = _wide(DTYPES[c["dtype"]])
+    r, v = c["rows"], c["vocab"]
+    x = _logits(c, g)
+    tokens = torch.randint(0, v, (r,), generator=g, device="cuda").int()
+    tokens = torch.where(torch.isinf(x.gather(1, tokens.long()[:, None])[:, 0]), 0, tokens).int()
+    if c["do"] != "score":  # the batch's last sequences are shorter: their ends are padding
+        tokens = torch.where(torch.rand(r, generator=g, device="cuda") < 0.05, -1, tokens).int()
+    inputs = {"logits": x, "tokens": tokens}
+    if c["do"] == "score":
+        return inputs
+    # one scalar for all rows, as the mean of a loss gives it; gradients in float16 are scaled up
+    one = (1024 if c["dtype"] == "float16" else 1) / r
+    inputs["g"] = torch.full((1,), -one, dtype=wide, device="cuda").expand(r)
+    if c["entropy_grad"]:
+        inputs["g_entropy"] = torch.randn(r, generator=g, device="cuda").to(wide) * (0.1 * one)
+    if c["do"] == "train":
+        return inputs
+    peak, total, entropy = (torch.empty(r, dtype=wide, device="cuda") for _ in range(3))
+    step = max(1, (1 << 24) // v)
+    for at in range(0, r, step):
+        z = x[at:at + step].double()
+        top = z.max(1).values
+        z -= top[:, None]
+        e = z.exp()
+        s = e.sum(1)
+        peak[at:at + step], total[at:at + step] = top, s
+        entropy[at:at + step] = s.log() - torch.where(e > 0, e * z, 0.0).sum(1) / s
+    inputs.update(peak=peak, total=total, entropy=entropy)
+    return inputs
+
+
+def _inputs(case, seed):
+    g = torch.Generator("cuda").manual_seed(seed)
+    return {"norm": _norm_inputs, "dropout": _dropout_inputs, "log_probs": _log_probs_inputs}[case["op"]](case, g)
+
+
+def prepare(case, seed):
+    inputs = _inputs(case, seed)
+    wide = _wide(DTYPES[case["dtype"]])
+
+    def rows():
+        return torch.empty(case["rows"], dtype=wide, device="cuda")
+
+    def like(x):
+        return torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device="cuda")
+
+    results = {}
+    if case["op"] == "norm" and case["grad"]:
+        results = {"dx": like(inputs["x"]), "dgamma": inputs["x"].new_empty(case["n"]), "dbeta": inputs["x"].new_empty(case["n"])}
+    elif case["op"] == "norm":
+        results = {"y": like(inputs["x"]), "mean": rows(), "rstd": rows()}
+    elif case["op"] == "dropout":
+        results = {"y": like(inputs["x"])}
+    else:
+        if case["do"] != "grad":
+            results = {"log_p": rows(), "entropy": rows(), "peak": rows(), "total": rows()}
+        if case["top"]:
+            results["top_log_p"] = torch.empty(case["rows"], case["top"], dtype=wide, device="cuda")
+            results["top_tokens"] = torch.empty(case["rows"], case["top"], dtype=torch.int32, device="cuda")
+        if case["do"] != "score":
+            results["d_logits"] = like(inputs["logits"])
+    torch.cuda.synchronize()
+    return State(case, inputs, results)
+
+
+# ── the operators in elementary operations ──────────────────────────────────────────────────────
+
+def _plain_norm(i):
+    x = i["x"].to(_wide(i["x"].dtype))
+    mean = x.mean(1, keepdim=True)
+    centred = x - mean
+    rstd = 1 / torch.sqrt((centred * centred).mean(1, keepdim=True) + EPS)
+    y = centred * rstd
+    if "gamma" in i:
+        y = y * i["gamma"] + i["beta"]
+    return {"y": y.to(i["x"].dtype), "mean": mean[:, 0], "rstd": rstd[:, 0]}
+
+
+def _plain_norm_grad(i):
+    dtype, wide = i["x"].dtype, _wide(i["x"].dtype)
+    g, rstd = i["g"].to(wide), i["rstd"][:, None]
+    h = (i["x"].to(wide) - i["mean"][:, None]) * rstd
+    w = g * i["gamma"] if "gamma" in i else g
+    dx = rstd * (w - w.mean(1, keepdim=True) - h * (w * h).mean(1, keepdim=True))
+    return {"dx": dx.to(dtype), "dgamma": (g * h).sum(0).to(dtype), "dbeta": g.sum(0).to(dtype)}
+
+
+_LOW = 0xFFFFFFFF
+_TURNS = (13, 15, 26, 6, 17, 29, 16, 24)
+
+
+def _round(words, r):
+    """One of Threefry-2x32's twenty rounds on 32-bit words held in 64; the key goes in after every fourth."""
+    x0, x1, ks = words
+    x0 = (x0 + x1) & _LOW
+    x1 = (((x1 << _TURNS[r % 8]) & _LOW) | (x1 >> (32 - _TURNS[r % 8]))) ^ x0
+    if r % 4 == 3:
+        s = r // 4 + 1
+        x0, x1 = (x0 + ks[s % 3]) & _LOW, (x1 + ks[(s + 1) % 3] + s) & _LOW
+    return x0, x1, ks
+
+
+def _random_bits(key, n):
+    """Sixteen bits for each of n elements: a block of the generator serves four."""
+    k0, k1 = key[0].long() & _LOW, key[1].long() & _LOW
+    block = torch.arange(-(-n // 4), device="cuda")
+    words = ((block & _LOW) + k0) & _LOW, ((block >> 32) + k1) & _LOW, (k0, k1, 0x1BD11BDA ^ k0 ^ k1)
+    x0, x1, _ = functools.reduce(_round, range(20), words)
+    return torch.stack((x0 & 0xFFFF, x0 >> 16, x1 & 0xFFFF, x1 >> 16), 1).reshape(-1)[:n]
+
+
+def _plain_dropout(i, rate):
+    x = i["x"]
+    cut = int(rate * 65536 + 0.5)
+    keep = (_random_bits(i["key"], x.numel()) >= cut).reshape(x.shape)
+    y = torch.where(keep, x.to(_wide(x.dtype)) * (65536 / (65536 - cut)), 0)
+    if "residual" in i:
+        y = y + i["residual"]
+    return {"y": y.to(x.dtype)}
+
+
+def _plain_log_probs(i, top):
+    x, tokens = i["logits"].to(_wide(i["logits"].dtype)), i["tokens"].long()
+    peak = x.max(1, keepdim=True).values
+    z = x - peak
+    e = torch.exp(z)
+    total = e.sum(1, keepdim=True)
+    log_total = torch.log(total)
+    at_token = z.gather(1, tokens.clamp(min=0)[:, None]) - log_total
+    out = {"log_p": torch.where(tokens >= 0, at_token[:, 0], 0),
+           "entropy": log_total[:, 0] - torch.where(e > 0, e * z, 0).sum(1) / total[:, 0],
+           "peak": peak[:, 0], "total": total[:, 0]}
+    if top:
+        order = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :top]
+        out["top_log_p"] = z.gather(1, order) - log_total
+        out["top_tokens"] = order.int()
+    return out
+
+
+def _plain_log_probs_grad(i):
+    dtype, tokens = i["logits"].dtype, i["tokens"].long()
+    z = i["logits"].to(_wide(dtype)) - i["peak"][:, None]
+    p = torch.exp(z) / i["total"][:, None]
+    g = torch.where(tokens >= 0, i["g"], 0)[:, None]
+    d = (-g * p).scatter_add(1, tokens.clamp(min=0)[:, None], g)
+    if "g_entropy" in i:
+        log_p = z - torch.log(i["total"])[:, None]
+        d = d - i["g_entropy"][:, None] * torch.where(p > 0, p * (log_p + i["entropy"][:, None]), 0)
+    return d.to(dtype)
+
+
+def _plain(state):
+    c, i = state.case, state.inputs
+    if c["op"] == "norm":
+        return _plain_norm_grad(i) if c["grad"] else _plain_norm(i)
+    if c["op"] == "dropout":
+        return _plain_dropout(i, c["rate"])
+    out = {} if c["do"] == "grad" else _plain_log_probs(i, c["top"])
+    if c["do"] != "score":
+        out["d_logits"] = _plain_log_probs_grad({**i, **out})
+    return out
+
+
+# ── the framework's calls ───────────────────────────────────────────────────────────────────────
+
+class _Storage:
+    """Device memory of a torch tensor, as the backend's handles hold it."""
+
+    def __init__(self, x):
+        self.tensor, self.ptr = x, x.data_ptr()
+        self.nbytes = x.untyped_storage().nbytes()
+
+
+@functools.lru_cache(maxsize=1)
+def _backend():
+    """A program has one context."""
+    from raven_amd.nx_backend import Backend
+
+    return Backend()
+
+
+def _handles(state):
+    """The handles of a state's tensors: its program makes them once, no data is touched."""
+    from raven_amd import dtype as dt
+    from raven_amd.nx_backend import Tensor
+    from raven_amd.view import View
+
+    return {name: Tensor(_Storage(x), View.create(x.shape, x.stride()), dt.BY_NAME[str(x.dtype).removeprefix("torch.")], _backend())
+            for name, x in (state.inputs | state.results).items()}
+
+
+def _run_own(state):
+    if state.handles is None:
+        state.handles = _handles(state)
+    c, h, B = state.case, state.handles, _backend()
+    if c["op"] == "norm":
+        if c["grad"]:
+            B.layer_norm_grad(h["g"], h["x"], h["mean"], h["rstd"], h.get("gamma"), out=(h["dx"], h["dgamma"], h["dbeta"]))
+        else:
+            B.layer_norm(h["x"], h.get("gamma"), h.get("beta"), EPS, out=(h["y"], h["mean"], h["rstd"]))
+    elif c["op"] == "dropout":
+        B.dropout(h["x"], h["key"], c["rate"], h.get("residual"), out=h["y"])
+    else:
+        if c["do"] != "grad":
+            B.log_probs(h["logits"], h["tokens"], c["top"],
+                        out=(h["log_p"], h["entropy"], h["peak"], h["total"], h.get("top_log_p"), h.get("top_tokens")))
+        if c["do"] != "score":
+            B.log_probs_grad(h["logits"], h["tokens"], h["peak"], h["total"], h["g"], h.get("g_entropy"),
+                             h["entropy"] if c["entropy_grad"] else None, out=h["d_logits"])
+    return state.results
+
+
+def run(state):
+    return _run_own(state) if own else _plain(state)
+
+
+# ── the operators in 64 bits ────────────────────────────────────────────────────────────────────
+
+def _exact_norm(c, i):
+    x = i["x"].double().requires_grad_(c["grad"])
+    one = torch.ones(c["n"], dtype=torch.float64, device="cuda")
+    gamma = (i["gamma"].double() if "gamma" in i else one).requires_grad_(c["grad"])
+    beta = (i["beta"].double() if "beta" in i else 0 * one).requires_grad_(c["grad"])
+    var, mean = torch.var_mean(x, 1, unbiased=False)
+    deviation = torch.sqrt(var + EPS)
+    y = gamma * ((x - mean[:, None]) / deviation[:, None]) + beta
+    if not c["grad"]:
+        return {"y": y, "mean": mean, "rstd": 1 / deviation}
+    return dict(zip(("dx", "dgamma", "dbeta"), torch.autograd.grad(y, (x, gamma, beta), i["g"].double())))
+
+
+def _exact_dropout(c, i):
+    """The generator on numpy's 32-bit words, as its authors describe it."""
+    x = i["x"].double()
+    n = x.numel()
+    k0, k1 = (np.uint32(int(k) & 0xFFFFFFFF) for k in i["key"].tolist())
+    keys = [k0, k1, np.uint32(0x1BD11BDA) ^ k0 ^ k1]
+    u = np.empty((-(-n // 4), 4), np.uint16)
+    with np.errstate(over="ignore"):
+        for at in range(0, len(u), 1 << 20):  # (so few blocks that the counter's high word is zero)
+            a = np.arange(at, min(len(u), at + (1 << 20)), dtype=np.uint32)
+            b = np.full_like(a, keys[1])
+            a += keys[0]
+            for group in range(5):
+                for turn in ((13, 15, 26, 6), (17, 29, 16, 24))[group % 2]:
+                    a += b
+                    b = (b << np.uint32(turn)) | (b >> np.uint32(32 - turn))
+                    b ^= a
+                a += keys[(group + 1) % 3]
+                b += keys[(group + 2) % 3] + np.uint32(group + 1)
+            u[at:at + len(a)] = np.stack([a, b], 1).astype("<u4").view("<u2")
+    dropped = math.floor(c["rate"] * 65536 + 0.5)
+    keep = torch.from_numpy((u.reshape(-1)[:n] >= dropped)).cuda().reshape(x.shape)
+    y = torch.zeros_like(x)
+    y[keep] = x[keep] / (1 - dropped / 65536)
+    return {"y": y + i["residual"].double() if "residual" in i else y}
+
+
+def _exact_log_probs(c, i):
+    x = i["logits"].double().requires_grad_(c["do"] != "score")
+    tokens = i["tokens"].long()
+    real = tokens >= 0
+    lse = torch.logsumexp(x, 1)
+    log_p = torch.where(real, x[torch.arange(len(x), device="cuda"), tokens.clamp(min=0)] - lse, 0.0)
+    finite = torch.where(torch.isinf(x.detach()), 0.0, x)
+    weights = torch.exp(x - lse[:, None]) if c["do"] == "score" or c["entropy_grad"] or c["do"] == "train" else None
+    entropy = lse - (weights * finite).sum(1) if weights is not None else None
+    out = {}
+    if c["do"] != "grad":
+        peak = x.detach().amax(1)
+        out = {"log_p": log_p.detach(), "entropy": entropy.detach(), "peak": peak, "total": torch.exp(lse.detach() - peak)}
+    if c["top"]:
+        order = torch.argsort(-x, dim=1, stable=True)[:, :c["top"]]
+        out["top_log_p"] = x.gather(1, order) - lse[:, None]
+        out["top_tokens"] = order.int()
+    if c["do"] != "score":
+        loss = (log_p * i["g"].double()).sum()
+        if c["entropy_grad"]:
+            loss = loss + (entropy * i["g_entropy"].double()).sum()
+        del weights, finite, entropy
+        out["d_logits"] = torch.autograd.grad(loss, x)[0]
+    return out
+
+
+def exact(case, seed):
+    i = _inputs(case, seed)
+    return {"norm": _exact_norm, "dropout": _exact_dropout, "log_probs": _exact_log_probs}[case["op"]](case, i)
