@@ -5,7 +5,8 @@
     dropout      a mask that a counter-based generator makes of a key and an element's position, with or
                  without a residual that it is added to; its gradient is the same operator
     log_probs    log probability of one token per row of logits, the distribution's entropy, the most
-                 likely tokens; and the gradient of the first two
+                 likely tokens; the gradient of the first two; and both at once, as a training step has it
+                 whose loss is a weighted sum of them
 
 With ``own`` false the operators are elementary torch operations, with ``own`` true the calls that a
 program makes of ``raven_amd.nx_backend.Backend``, whose results go to tensors that the program keeps.
@@ -98,7 +99,7 @@ def work(case):
     r, size = case["rows"], case["rows"] * case["vocab"]
     score = size * e + r * (4 + 4 * s) + r * case["top"] * (4 + s)
     grad = 2 * size * e + r * (4 + 3 * s) + (2 * r * s if case["entropy_grad"] else 0)
-    return {"bytes": {"score": score, "grad": grad, "train": score + grad}[case["do"]],
+    return {"bytes": score if case["do"] == "score" else grad,
             "flops": {"score": 6, "grad": 6, "train": 12}[case["do"]] * size}
 
 
@@ -221,7 +222,9 @@ def prepare(case, seed):
         results = {"y": like(inputs["x"])}
     else:
         if case["do"] != "grad":
-            results = {"log_p": rows(), "entropy": rows(), "peak": rows(), "total": rows()}
+            results = {"log_p": rows(), "entropy": rows()}
+        if case["do"] == "score":
+            results["peak"], results["total"] = rows(), rows()
         if case["top"]:
             results["top_log_p"] = torch.empty(case["rows"], case["top"], dtype=wide, device="cuda")
             results["top_tokens"] = torch.empty(case["rows"], case["top"], dtype=torch.int32, device="cuda")
@@ -323,9 +326,11 @@ def _plain(state):
         return _plain_norm_grad(i) if c["grad"] else _plain_norm(i)
     if c["op"] == "dropout":
         return _plain_dropout(i, c["rate"])
-    out = {} if c["do"] == "grad" else _plain_log_probs(i, c["top"])
-    if c["do"] != "score":
-        out["d_logits"] = _plain_log_probs_grad({**i, **out})
+    if c["do"] == "grad":
+        return {"d_logits": _plain_log_probs_grad(i)}
+    out = _plain_log_probs(i, c["top"])
+    if c["do"] == "train":
+        out = {"log_p": out["log_p"], "entropy": out["entropy"], "d_logits": _plain_log_probs_grad({**i, **out})}
     return out
 
 
@@ -368,13 +373,15 @@ def _run_own(state):
             B.layer_norm(h["x"], h.get("gamma"), h.get("beta"), EPS, out=(h["y"], h["mean"], h["rstd"]))
     elif c["op"] == "dropout":
         B.dropout(h["x"], h["key"], c["rate"], h.get("residual"), out=h["y"])
+    elif c["do"] == "score":
+        B.log_probs(h["logits"], h["tokens"], c["top"],
+                    out=(h["log_p"], h["entropy"], h["peak"], h["total"], h.get("top_log_p"), h.get("top_tokens")))
+    elif c["do"] == "grad":
+        B.log_probs_grad(h["g"], h["logits"], h["tokens"], h["peak"], h["total"], h.get("g_entropy"),
+                         h["entropy"] if c["entropy_grad"] else None, out=h["d_logits"])
     else:
-        if c["do"] != "grad":
-            B.log_probs(h["logits"], h["tokens"], c["top"],
-                        out=(h["log_p"], h["entropy"], h["peak"], h["total"], h.get("top_log_p"), h.get("top_tokens")))
-        if c["do"] != "score":
-            B.log_probs_grad(h["logits"], h["tokens"], h["peak"], h["total"], h["g"], h.get("g_entropy"),
-                             h["entropy"] if c["entropy_grad"] else None, out=h["d_logits"])
+        B.log_probs_with_grad(h["g"], h["logits"], h["tokens"], h.get("g_entropy"),
+                              out=(h["log_p"], h["entropy"], h["d_logits"]))
     return state.results
 
 
@@ -431,12 +438,14 @@ def _exact_log_probs(c, i):
     lse = torch.logsumexp(x, 1)
     log_p = torch.where(real, x[torch.arange(len(x), device="cuda"), tokens.clamp(min=0)] - lse, 0.0)
     finite = torch.where(torch.isinf(x.detach()), 0.0, x)
-    weights = torch.exp(x - lse[:, None]) if c["do"] == "score" or c["entropy_grad"] or c["do"] == "train" else None
+    weights = torch.exp(x - lse[:, None]) if c["do"] != "grad" or c["entropy_grad"] else None
     entropy = lse - (weights * finite).sum(1) if weights is not None else None
     out = {}
     if c["do"] != "grad":
-        peak = x.detach().amax(1)
-        out = {"log_p": log_p.detach(), "entropy": entropy.detach(), "peak": peak, "total": torch.exp(lse.detach() - peak)}
+        out = {"log_p": log_p.detach(), "entropy": entropy.detach()}
+    if c["do"] == "score":
+        out["peak"] = x.amax(1)
+        out["total"] = torch.exp(lse - out["peak"])
     if c["top"]:
         order = torch.argsort(-x, dim=1, stable=True)[:, :c["top"]]
         out["top_log_p"] = x.gather(1, order) - lse[:, None]
