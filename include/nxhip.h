@@ -345,6 +345,30 @@ int nxh_linear(nxh_context *ctx, const nxh_tensor *out, const nxh_tensor *x,
 int nxh_linear_gelu_tanh(nxh_context *ctx, const nxh_tensor *out, const nxh_tensor *x,
                          const nxh_tensor *w, const nxh_tensor *bias, const void *constants);
 
+/* ── training: norms, dropout, losses ────────────────────────────────────── */
+
+/* No counterpart in the reference's backend: Rune differentiates the primitives that
+   the frontend and Kaun issue (kaun/lib/layer_norm.ml:43-68 and the like) one by one. Each
+   call below is an operator of its own, computed in float32 (float64 for float64) with one
+   rounding on the way out. Floating dtypes f16/bf16/f32/f64; the rows (the last axis) of
+   inputs and results contiguous and at most 2^24 long, their other strides any (zero, a
+   broadcast, for inputs), anything else is Failure. Values that belong to a row have the
+   input's shape without the last axis, any strides, and float32 (float64 for float64
+   inputs). A result may be an input of its own shape (the same view); other overlaps
+   are undefined. Equal calls give equal bits. */
+
+/* out = (x - mean) * rstd [* gamma] [+ beta] over the last axis, mean = sum x / n,
+   rstd = 1 / sqrt (sum (x - mean)^2 / n + eps). mean and rstd are what the gradient
+   takes, each may be NULL; gamma and beta (rank 1, the row's length, x's dtype) too. */
+int nxh_layer_norm(nxh_context *ctx, const nxh_tensor *out, const nxh_tensor *mean, const nxh_tensor *rstd,
+                   const nxh_tensor *x, const nxh_tensor *gamma, const nxh_tensor *beta, double eps);
+/* The gradients of nxh_layer_norm for g, what flows back into its out; x, gamma as there,
+   mean and rstd as it gave them. dx, dgamma, dbeta (rank 1, any stride): each may be NULL,
+   not all. No rows: dgamma and dbeta are zeros. */
+int nxh_layer_norm_grad(nxh_context *ctx, const nxh_tensor *dx, const nxh_tensor *dgamma, const nxh_tensor *dbeta,
+                        const nxh_tensor *g, const nxh_tensor *x, const nxh_tensor *mean, const nxh_tensor *rstd,
+                        const nxh_tensor *gamma);
+
 /* ── Fourier transforms ──────────────────────────────────────────────────── */
 
 /* fft / ifft (backend_intf.ml:594-598; nx_backend.ml:507-528; nx_c_fft.c:940-956,

@@ -1,0 +1,370 @@
+// layer_norm_grad.hip — nxh_layer_norm_grad: the transposed step of nxh_layer_norm. With
+// h = (x - mean) rstd, w = g gamma and N the row's length:
+//
+//   dx = rstd (w - sum w / N - h sum (w h) / N),   dgamma = sum_rows g h,   dbeta = sum_rows g
+//
+// One pass over g and x makes all three. A group of lanes keeps a row in registers between its two
+// sums and dx, and the sums over rows of the columns that its lanes hold from row to row; a block
+// adds up its groups and writes one row of partial sums, a second launch adds those in a fixed order.
+// Nothing is added by atomics, so equal calls give equal bits. All sums are float32 (float64 for float64).
+//
+// Memory bounds it: g and x in, dx out; the partial sums are held to some percent of that by the
+// number of blocks.
+
+#include "layer_norm_train.hpp"
+
+namespace {
+
+enum { LG_DX, LG_G, LG_X, LG_MEAN, LG_RSTD, LG_OPERANDS };
+struct LayerNormGradArgs {
+  RowGeom g;
+  RowOperand o[LG_OPERANDS];  // dx: base may be null
+  const char *gamma;          // null: ones
+  void *partials;             // [blocks][2][n] sums of g h and of g; null: not wanted
+};
+
+// Adds up one value per lane over the groups of a wave: lanes with equal places in their groups.
+template <int G, class C>
+__device__ __forceinline__ C across_groups(C v) {
+  const Sum<C> sum;
+  if constexpr (G < 64) v = combine_step<32>(v, sum);
+  if constexpr (G < 32) v = combine_step<16>(v, sum);
+  if constexpr (G < 16) v = combine_step<8>(v, sum);
+  if constexpr (G < 8) v = v + __shfl_xor(v, 4, 64);
+  if constexpr (G < 4) v = combine_step<2>(v, sum);
+  if constexpr (G < 2) v = combine_step<1>(v, sum);
+  return v;
+}
+
+template <int DT, int G, int NV, bool RAGGED>
+__global__ __launch_bounds__(ln_threads(G)) void layer_norm_grad_kernel(LayerNormGradArgs a) {
+  using TX = Tr<DT>;
+  using C = typename TX::C;
+  using S = typename TX::S;
+  constexpr int V = VECTOR<S>, T = ln_threads(G), GROUPS = T / G, W = T / 64;
+  __shared__ C lds[G > 64 ? 2 * (G / 64) : 2 * W * G * V];
+  const int lane = threadIdx.x % G, n = a.g.n, nvec = (n + V - 1) / V;
+  const S *gamma = reinterpret_cast<const S *>(a.gamma);
+  Vec<S, V> gv[NV], xr[NV], gr[NV];
+  C dgamma[NV][V], dbeta[NV][V];
+#pragma unroll
+  for (int v = 0; v < NV; v++) {
+    if (v * G + lane < nvec && gamma) gv[v] = load_part<V, RAGGED>(gamma, v * G + lane, n, S{});
+#pragma unroll
+    for (int j = 0; j < V; j++) dgamma[v][j] = dbeta[v][j] = 0;
+  }
+  const C count = (C)n;
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G, at[LG_OPERANDS];
+  C mean = 0, rstd = 0;
+  auto request = [&](int64_t r) {  // row r's loads
+    row_starts(a.g, (uint32_t)r, a.o, at);
+    const S *x = reinterpret_cast<const S *>(a.o[LG_X].base) + at[LG_X];
+    const S *g = reinterpret_cast<const S *>(a.o[LG_G].base) + at[LG_G];
+    mean = reinterpret_cast<const C *>(a.o[LG_MEAN].base)[at[LG_MEAN]];
+    rstd = reinterpret_cast<const C *>(a.o[LG_RSTD].base)[at[LG_RSTD]];
+#pragma unroll
+    for (int v = 0; v < NV; v++)
+      if (v * G + lane < nvec) {
+        xr[v] = load_part<V, RAGGED>(x, v * G + lane, n, S{});
+        gr[v] = load_part<V, RAGGED>(g, v * G + lane, n, S{});
+      }
+  };
+  if (row < a.g.rows) request(row);
+  for (; row < a.g.rows; row += step) {
+    S *dx = reinterpret_cast<S *>(const_cast<char *>(a.o[LG_DX].base)) + at[LG_DX];
+    const C mu = mean, rs = rstd;
+    C h[NV][V], w[NV][V], s[2] = {0, 0};
+#pragma unroll
+    for (int v = 0; v < NV; v++)
+      if (v * G + lane < nvec)
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          // (past the row's end g was read as zero, which keeps the element out of every sum: h is finite wherever the row is)
+          const C gj = TX::ld(gr[v].v[j]);
+          h[v][j] = (TX::ld(xr[v].v[j]) - mu) * rs;
+          if (RAGGED && (v * G + lane) * V + j >= n) h[v][j] = 0;
+          w[v][j] = gamma ? gj * TX::ld(gv[v].v[j]) : gj;
+          s[0] = s[0] + w[v][j];
+          s[1] = fused(w[v][j], h[v][j], s[1]);
+          dgamma[v][j] = fused(gj, h[v][j], dgamma[v][j]);
+          dbeta[v][j] = dbeta[v][j] + gj;
+        }
+    if (row + step < a.g.rows) request(row + step);  // in flight while this row is finished
+    group_combine<G>(s, Sum<C>{}, lds);
+    if (a.o[LG_DX].base) {
+      const C c1 = s[0] / count, c2 = s[1] / count;
+#pragma unroll
+      for (int v = 0; v < NV; v++)
+        if (v * G + lane < nvec) {
+          Vec<S, V> o;
+#pragma unroll
+          for (int j = 0; j < V; j++) o.v[j] = TX::st(rs * fused(-h[v][j], c2, w[v][j] - c1));
+          store_part<V, RAGGED>(dx, v * G + lane, n, o);
+        }
+    }
+  }
+  if (!a.partials) return;
+  C *mine = reinterpret_cast<C *>(a.partials) + (int64_t)blockIdx.x * 2 * n;
+  if constexpr (G > 64) {  // the block's only group
+#pragma unroll
+    for (int v = 0; v < NV; v++)
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const int c = (v * G + lane) * V + j;
+        if (c < n) {
+          mine[c] = dgamma[v][j];
+          mine[n + c] = dbeta[v][j];
+        }
+      }
+  } else {
+    const int wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const C p = across_groups<G>(dgamma[v][j]), q = across_groups<G>(dbeta[v][j]);
+        if ((threadIdx.x & 63) < G) {
+          lds[(wave * 2 + 0) * G * V + lane * V + j] = p;
+          lds[(wave * 2 + 1) * G * V + lane * V + j] = q;
+        }
+      }
+      __syncthreads();
+      for (int e = threadIdx.x; e < 2 * G * V; e += T) {
+        C s = lds[e];
+#pragma unroll
+        for (int k = 1; k < W; k++) s = s + lds[k * 2 * G * V + e];
+        const int c = v * G * V + e % (G * V);
+        if (c < n) mine[(e / (G * V)) * n + c] = s;
+      }
+    }
+  }
+}
+
+// ── rows that registers do not hold ─────────────────────────────────────────
+// The rows' sums and dx by a block per row, which walks it twice; the columns' sums by blocks of 256 lanes that
+// own a vector of columns each and walk a share of the rows: g and x are read again, which such rows have caches for.
+constexpr int LONG_THREADS = 1024;
+template <int DT>
+__global__ __launch_bounds__(LONG_THREADS) void layer_norm_grad_long_kernel(LayerNormGradArgs a) {
+  using TX = Tr<DT>;
+  using C = typename TX::C;
+  using S = typename TX::S;
+  constexpr int V = VECTOR<S>;
+  __shared__ C lds[2 * (LONG_THREADS / 64)];
+  const int n = a.g.n, nvec = (n + V - 1) / V;
+  const S *gamma = reinterpret_cast<const S *>(a.gamma);
+  const C count = (C)n;
+  for (int64_t row = blockIdx.x; row < a.g.rows; row += gridDim.x) {
+    int64_t at[LG_OPERANDS];
+    row_starts(a.g, (uint32_t)row, a.o, at);
+    const S *x = reinterpret_cast<const S *>(a.o[LG_X].base) + at[LG_X];
+    const S *g = reinterpret_cast<const S *>(a.o[LG_G].base) + at[LG_G];
+    S *dx = reinterpret_cast<S *>(const_cast<char *>(a.o[LG_DX].base)) + at[LG_DX];
+    const C mu = reinterpret_cast<const C *>(a.o[LG_MEAN].base)[at[LG_MEAN]];
+    const C rs = reinterpret_cast<const C *>(a.o[LG_RSTD].base)[at[LG_RSTD]];
+    C s[2] = {0, 0};
+    auto walk = [&](auto &&body) {
+      for (int c = threadIdx.x; c < nvec; c += LONG_THREADS) {
+        const Vec<S, V> xv = load_part<V, true>(x, c, n, S{}), gv = load_part<V, true>(g, c, n, S{});
+        Vec<S, V> wv;
+        if (gamma) wv = load_part<V, true>(gamma, c, n, S{});
+        C h[V], w[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          h[j] = c * V + j < n ? (TX::ld(xv.v[j]) - mu) * rs : 0;
+          w[j] = gamma ? TX::ld(gv.v[j]) * TX::ld(wv.v[j]) : TX::ld(gv.v[j]);
+        }
+        body(c, h, w);
+      }
+    };
+    walk([&](int, const C *h, const C *w) {
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        s[0] = s[0] + w[j];
+        s[1] = fused(w[j], h[j], s[1]);
+      }
+    });
+    group_combine<LONG_THREADS>(s, Sum<C>{}, lds);
+    const C c1 = s[0] / count, c2 = s[1] / count;
+    walk([&](int c, const C *h, const C *w) {
+      Vec<S, V> o;
+#pragma unroll
+      for (int j = 0; j < V; j++) o.v[j] = TX::st(rs * fused(-h[j], c2, w[j] - c1));
+      store_part<V, true>(dx, c, n, o);
+    });
+  }
+}
+template <int DT>
+__global__ __launch_bounds__(256) void layer_norm_columns_kernel(LayerNormGradArgs a, int64_t share) {
+  using TX = Tr<DT>;
+  using C = typename TX::C;
+  using S = typename TX::S;
+  constexpr int V = VECTOR<S>;
+  const int n = a.g.n, c = blockIdx.x * 256 + threadIdx.x;
+  if ((int64_t)c * V >= n) return;
+  C dgamma[V], dbeta[V];
+#pragma unroll
+  for (int j = 0; j < V; j++) dgamma[j] = dbeta[j] = 0;
+  const int64_t first = (int64_t)blockIdx.y * share, end = first + share < a.g.rows ? first + share : a.g.rows;
+#pragma unroll 4
+  for (int64_t row = first; row < end; row++) {
+    int64_t at[LG_OPERANDS];
+    row_starts(a.g, (uint32_t)row, a.o, at);
+    const Vec<S, V> xv = load_part<V, true>(reinterpret_cast<const S *>(a.o[LG_X].base) + at[LG_X], c, n, S{});
+    const Vec<S, V> gv = load_part<V, true>(reinterpret_cast<const S *>(a.o[LG_G].base) + at[LG_G], c, n, S{});
+    const C mu = reinterpret_cast<const C *>(a.o[LG_MEAN].base)[at[LG_MEAN]];
+    const C rs = reinterpret_cast<const C *>(a.o[LG_RSTD].base)[at[LG_RSTD]];
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      const C gj = TX::ld(gv.v[j]);
+      dgamma[j] = fused(gj, (TX::ld(xv.v[j]) - mu) * rs, dgamma[j]);
+      dbeta[j] = dbeta[j] + gj;
+    }
+  }
+  C *mine = reinterpret_cast<C *>(a.partials) + (int64_t)blockIdx.y * 2 * n;
+#pragma unroll
+  for (int j = 0; j < V; j++)
+    if (c * V + j < n) {
+      mine[c * V + j] = dgamma[j];
+      mine[n + c * V + j] = dbeta[j];
+    }
+}
+
+// ── the partial sums ────────────────────────────────────────────────────────
+// 32 columns of a block, 32 lanes to each: a lane adds every 32nd partial sum, then the lanes' sums are added in order.
+struct JoinArgs {
+  const void *partials;
+  int64_t blocks;
+  int n;
+  char *out[2];  // dgamma, dbeta; null: not wanted
+  int64_t stride[2];
+};
+template <int DT>
+__global__ __launch_bounds__(1024) void layer_norm_join_kernel(JoinArgs a) {
+  using TX = Tr<DT>;
+  using C = typename TX::C;
+  using S = typename TX::S;
+  __shared__ C lds[32][33];
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+  const int64_t column = (int64_t)blockIdx.x * 32 + lane;
+  const C *p = reinterpret_cast<const C *>(a.partials);
+  C s = 0;
+  if (column < 2 * (int64_t)a.n)
+#pragma unroll 8
+    for (int64_t b = part; b < a.blocks; b += 32) s = s + p[b * 2 * a.n + column];
+  lds[part][lane] = s;
+  __syncthreads();
+  if (part != 0 || column >= 2 * (int64_t)a.n) return;
+#pragma unroll
+  for (int k = 1; k < 32; k++) s = s + lds[k][lane];
+  const int which = column >= a.n;
+  char *out = which ? a.out[1] : a.out[0];
+  const int64_t stride = which ? a.stride[1] : a.stride[0];
+  if (out) reinterpret_cast<S *>(out)[(column - (which ? a.n : 0)) * stride] = TX::st(s);
+}
+
+// ── host side ───────────────────────────────────────────────────────────────
+struct Plan {
+  void (*launch)(nxh_context *, const LayerNormGradArgs &, int64_t blocks);
+  int64_t blocks;  // rows of partial sums
+};
+template <int DT, int G, int NV>
+void launch(nxh_context *ctx, const LayerNormGradArgs &a, int64_t blocks) {
+  constexpr int V = VECTOR<typename Tr<DT>::S>;
+  const dim3 grid((unsigned)blocks);
+  if (a.g.n % V == 0) hipLaunchKernelGGL((layer_norm_grad_kernel<DT, G, NV, false>), grid, dim3(ln_threads(G)), 0, ctx->stream, a);
+  else hipLaunchKernelGGL((layer_norm_grad_kernel<DT, G, NV, true>), grid, dim3(ln_threads(G)), 0, ctx->stream, a);
+}
+template <int DT>
+void launch_long(nxh_context *ctx, const LayerNormGradArgs &a, int64_t blocks) {
+  constexpr int V = VECTOR<typename Tr<DT>::S>;
+  const int64_t units = ctx->compute_units > 0 ? ctx->compute_units : 256;
+  if (a.partials) {  // before dx, which may go where g or x is
+    const dim3 grid((unsigned)(((a.g.n + V - 1) / V + 255) / 256), (unsigned)blocks);
+    hipLaunchKernelGGL((layer_norm_columns_kernel<DT>), grid, dim3(256), 0, ctx->stream, a, (a.g.rows + blocks - 1) / blocks);
+  }
+  if (a.o[LG_DX].base)
+    hipLaunchKernelGGL((layer_norm_grad_long_kernel<DT>), dim3((unsigned)std::min(a.g.rows, units)), dim3(LONG_THREADS), 0, ctx->stream, a);
+}
+template <int DT>
+Plan plan(nxh_context *ctx, int n, int64_t rows) {
+  constexpr int V = VECTOR<typename Tr<DT>::S>;
+  const int64_t units = ctx->compute_units > 0 ? ctx->compute_units : 256;
+  const int nvec = (n + V - 1) / V;
+#define X(G, NV)                                                                                                \
+  if (nvec <= G * NV)                                                                                           \
+    return {launch<DT, G, NV>, std::min((rows + ln_threads(G) / G - 1) / (ln_threads(G) / G), 2 * units)};
+  LN_GROUPS(X)
+#undef X
+  const int64_t tiles = (nvec + 255) / 256;
+  return {launch_long<DT>, std::max<int64_t>(1, std::min(rows / 8, 2 * units / tiles))};
+}
+
+}  // namespace
+
+NXH_EXPORT int nxh_layer_norm_grad(nxh_context *ctx, const nxh_tensor *dx, const nxh_tensor *dgamma, const nxh_tensor *dbeta,
+                                   const nxh_tensor *g, const nxh_tensor *x, const nxh_tensor *mean, const nxh_tensor *rstd,
+                                   const nxh_tensor *gamma) {
+  NXH_DEFER_TOUCH(ctx, 3, dx, dgamma, dbeta, g, x, mean, rstd, gamma);
+  const char *op = "layer_norm_grad";
+  if (!ctx || !g || !x || !mean || !rstd || (!dx && !dgamma && !dbeta)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "null argument");
+  int rc = NXH_OK;
+  for (const nxh_tensor *t : {dx, dgamma, dbeta, g, x, mean, rstd, gamma})
+    if (t && (rc = nxh_check_tensor(op, t))) return rc;
+  const int dt = x->dtype;
+  LayerNormGradArgs a;
+  if ((rc = same_shape(op, g, x)) || (dx && (rc = same_shape(op, dx, x))) || (rc = rows_geometry(op, x, a.g))) return rc;
+  for (const nxh_tensor *t : {dx, dgamma, dbeta})
+    if (t && (rc = out_rows_ok(op, t))) return rc;
+  if (!float_dtype_ok(dt)) return nxh_fail(NXH_FAILURE, op, NXH_ERR_UNSUPPORTED);
+  for (const nxh_tensor *t : {dx, dgamma, dbeta, g, gamma})
+    if (t && t->dtype != dt) return nxh_fail(NXH_FAILURE, op, NXH_ERR_UNSUPPORTED);
+  for (const nxh_tensor *t : {mean, rstd})
+    if ((rc = row_values_ok(op, t, x, statistics_dtype(dt)))) return rc;
+  if (gamma && (rc = row_vector_ok(op, gamma, a.g.n))) return rc;
+  for (const nxh_tensor *t : {dgamma, dbeta})
+    if (t && (t->ndim != 1 || t->shape[0] != a.g.n)) return nxh_fail(NXH_INVALID_ARGUMENT, op, NXH_ERR_SHAPE);
+  if (a.g.rows > 0 && a.g.n == 0) return nxh_fail(NXH_INVALID_ARGUMENT, op, NXH_ERR_EMPTY_REDUCE);
+  if (a.g.n == 0) return NXH_OK;
+  if (a.g.rows > 0 && (!unit_stride(x) || !unit_stride(g) || (dx && !unit_stride(dx))))
+    return nxh_fail(NXH_FAILURE, op, "rows must be contiguous");
+  row_operand(dx, a.o[LG_DX]);
+  row_operand(g, a.o[LG_G]);
+  row_operand(x, a.o[LG_X]);
+  row_value_operand(mean, a.o[LG_MEAN]);
+  row_value_operand(rstd, a.o[LG_RSTD]);
+  merge_outer_dims(a.g, {&a.o[LG_DX], &a.o[LG_G], &a.o[LG_X], &a.o[LG_MEAN], &a.o[LG_RSTD]});
+  const int64_t es = nxh_elem_size(dt);
+  a.gamma = gamma ? (const char *)gamma->data + gamma->offset * es : nullptr;
+  a.partials = nullptr;
+  std::lock_guard<std::mutex> guard(ctx->mu);
+  NXH_HIP(op, hipSetDevice(ctx->device));
+  const bool weights = dgamma || dbeta;
+  nxh_set_path(a.g.n > LN_VECTORS * (16 / es) ? "layer_norm_grad_long" : "layer_norm_grad");
+  Plan p{nullptr, 0};  // no rows: sums of nothing
+  if (a.g.rows > 0)
+    p = dt == NXH_F32 ? plan<NXH_F32>(ctx, a.g.n, a.g.rows) : dt == NXH_BF16 ? plan<NXH_BF16>(ctx, a.g.n, a.g.rows)
+        : dt == NXH_F16 ? plan<NXH_F16>(ctx, a.g.n, a.g.rows) : plan<NXH_F64>(ctx, a.g.n, a.g.rows);
+  if (weights && p.launch)
+    if ((rc = nxh_alloc_locked(ctx, (size_t)p.blocks * 2 * (size_t)a.g.n * (dt == NXH_F64 ? 8 : 4), &a.partials))) return rc;
+  if (p.launch) p.launch(ctx, a, p.blocks);
+  if (weights) {
+    JoinArgs j{a.partials, p.blocks, a.g.n, {nullptr, nullptr}, {1, 1}};
+    const nxh_tensor *outs[2] = {dgamma, dbeta};
+    for (int k = 0; k < 2; k++)
+      if (outs[k]) {
+        j.out[k] = (char *)outs[k]->data + outs[k]->offset * es;
+        j.stride[k] = outs[k]->strides[0];
+      }
+    const dim3 grid((unsigned)((2 * (int64_t)a.g.n + 31) / 32));
+    if (dt == NXH_F32) hipLaunchKernelGGL((layer_norm_join_kernel<NXH_F32>), grid, dim3(1024), 0, ctx->stream, j);
+    else if (dt == NXH_BF16) hipLaunchKernelGGL((layer_norm_join_kernel<NXH_BF16>), grid, dim3(1024), 0, ctx->stream, j);
+    else if (dt == NXH_F16) hipLaunchKernelGGL((layer_norm_join_kernel<NXH_F16>), grid, dim3(1024), 0, ctx->stream, j);
+    else hipLaunchKernelGGL((layer_norm_join_kernel<NXH_F64>), grid, dim3(1024), 0, ctx->stream, j);
+    if (a.partials) nxh_free_locked(ctx, a.partials);  // (the stream orders its next use behind these launches)
+  }
+  NXH_HIP(op, hipGetLastError());
+  return NXH_OK;
+}

@@ -30,24 +30,13 @@
 #include "softmax_math.hpp"
 #include "stream_access.hpp"
 #include "map_ops.hpp"
+#include "rows.hpp"
 
 namespace {
 
-constexpr int ROW_MAXD = 8;
 constexpr int EPL = 32;  // elements per lane at most (rows held in registers)
 constexpr int ROW_REGS = 64 * 4 * EPL;  // the longest row a block holds in registers
 constexpr int LONG_THREADS = 1024, LONG_WAVES = LONG_THREADS / 64;  // a block of the long-row kernels
-constexpr int64_t ROW_MAX = (int64_t)1 << 24;  // the longest row at all (float32 counts it exactly)
-
-struct RowGeom {
-  int64_t rows;
-  int n, nouter;
-  uint32_t oshape[ROW_MAXD];
-};
-struct RowOperand {
-  const char *base;
-  int64_t stride[ROW_MAXD];  // per outer dim, elements
-};
 
 template <int DT>
 __device__ __forceinline__ typename Tr<DT>::C rnd(typename Tr<DT>::C v) {
@@ -576,8 +565,6 @@ __global__ __launch_bounds__(LUT_THREADS) void gelu_lut_kernel(const uint16_t *t
 }
 
 // ── host side ───────────────────────────────────────────────────────────────
-bool float_dtype_ok(int dt) { return dt == NXH_F32 || dt == NXH_F64 || dt == NXH_BF16 || dt == NXH_F16; }
-
 double decode_scalar(int dt, const void *p) {
   switch (dt) {
     case NXH_F32: return (double)*(const float *)p;
@@ -591,75 +578,6 @@ double decode_scalar(int dt, const void *p) {
       return (h & 0x8000) ? -v : v;
     }
   }
-}
-
-// Fills the row geometry from `x` (rows = product of the outer extents).
-int row_geometry(const char *op, const nxh_tensor *x, RowGeom &g) {
-  if (x->ndim < 1) return nxh_fail(NXH_INVALID_ARGUMENT, op, "input must not be a scalar");
-  if (x->ndim - 1 > ROW_MAXD) return nxh_fail(NXH_FAILURE, op, "more than 8 outer dimensions");
-  if (x->shape[x->ndim - 1] > ROW_MAX) return nxh_fail(NXH_FAILURE, op, "rows longer than 2^24 elements");
-  g.n = (int)x->shape[x->ndim - 1];
-  g.nouter = x->ndim - 1;
-  g.rows = 1;
-  for (int d = 0; d < g.nouter; d++) {
-    if (x->shape[d] > 0xffffffffLL) return nxh_fail(NXH_FAILURE, op, "extent exceeds 32 bits");
-    g.oshape[d] = (uint32_t)x->shape[d];
-    g.rows *= x->shape[d];
-  }
-  return NXH_OK;
-}
-void row_operand(const nxh_tensor *t, RowOperand &o) {
-  o.base = t ? (const char *)t->data + t->offset * (int64_t)nxh_elem_size(t->dtype) : nullptr;
-  for (int d = 0; d < ROW_MAXD; d++) o.stride[d] = (t && d < t->ndim - 1) ? t->strides[d] : 0;
-}
-// Outer dims that compose on every operand (stride[d - 1] == stride[d] * extent[d], a broadcast
-// with both strides 0 included) become one: contiguous rows end up with a single outer dim.
-void merge_outer_dims(RowGeom &g, std::initializer_list<RowOperand *> ops) {
-  int n = g.nouter;
-  for (int d = n - 1; d > 0; d--) {
-    bool composes = true;
-    for (RowOperand *o : ops) composes = composes && o->stride[d - 1] == o->stride[d] * (int64_t)g.oshape[d];
-    if (!composes || (uint64_t)g.oshape[d - 1] * g.oshape[d] > 0xffffffffULL) continue;
-    g.oshape[d - 1] *= g.oshape[d];
-    for (RowOperand *o : ops) o->stride[d - 1] = o->stride[d];
-    for (int e = d; e + 1 < n; e++) {
-      g.oshape[e] = g.oshape[e + 1];
-      for (RowOperand *o : ops) o->stride[e] = o->stride[e + 1];
-    }
-    n--;
-  }
-  g.nouter = n;
-}
-// A row operand can be moved V elements at a time when its rows are contiguous
-// and every row starts on a V-element boundary.
-bool rows_vector_ok(const nxh_tensor *t, int v) {
-  const int es = (int)nxh_elem_size(t->dtype);
-  if ((((uintptr_t)t->data + t->offset * es) % (uintptr_t)(es * v)) != 0) return false;
-  for (int d = 0; d < t->ndim - 1; d++)
-    if (t->shape[d] > 1 && t->strides[d] % v != 0) return false;
-  return true;
-}
-// Rows of a and b are off their V-element boundaries by the same amount, row by row: the
-// long-row kernels then peel the same head and tail from both.
-bool rows_congruent(const nxh_tensor *a, const nxh_tensor *b, int v) {
-  const uintptr_t ea = (uintptr_t)a->data / nxh_elem_size(a->dtype) + (uintptr_t)a->offset;
-  const uintptr_t eb = (uintptr_t)b->data / nxh_elem_size(b->dtype) + (uintptr_t)b->offset;
-  if ((uintptr_t)a->data % nxh_elem_size(a->dtype) || (uintptr_t)b->data % nxh_elem_size(b->dtype)) return false;
-  if (ea % v != eb % v) return false;
-  for (int d = 0; d < a->ndim - 1; d++)
-    if (a->shape[d] > 1 && ((a->strides[d] - b->strides[d]) % v) != 0) return false;
-  return true;
-}
-int same_shape(const char *op, const nxh_tensor *a, const nxh_tensor *b) {
-  if (a->ndim != b->ndim) return nxh_fail(NXH_INVALID_ARGUMENT, op, NXH_ERR_SHAPE);
-  for (int d = 0; d < a->ndim; d++)
-    if (a->shape[d] != b->shape[d]) return nxh_fail(NXH_INVALID_ARGUMENT, op, NXH_ERR_SHAPE);
-  return NXH_OK;
-}
-int out_rows_ok(const char *op, const nxh_tensor *out) {
-  for (int d = 0; d < out->ndim; d++)
-    if (out->shape[d] > 1 && out->strides[d] == 0) return nxh_fail(NXH_INVALID_ARGUMENT, op, NXH_ERR_OUT_ALIASED);
-  return NXH_OK;
 }
 
 // Elements per lane of the vector forms: the smallest of 8 / 16 / 32 that holds the row.

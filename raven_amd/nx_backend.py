@@ -550,6 +550,38 @@ class Backend(Calls):
                                             C.byref(m) if m is not None else None, pm, int(causal)))
         return out
 
+    # ── training: norms, dropout, losses (no counterpart in Backend_intf.S) ─
+    # ``out`` gives tensors the results go to (a training loop's own, or views); without it they are fresh ones.
+    @staticmethod
+    def _statistics_dtype(dtype: dt.DType) -> dt.DType:
+        """What statistics of ``dtype`` are held in: float64 for float64, else float32."""
+        return dt.float64 if dtype is dt.float64 else dt.float32
+
+    def layer_norm(self, x: Tensor, gamma: Tensor | None = None, beta: Tensor | None = None, eps: float = 1e-5, out=None):
+        """``(y, mean, rstd)``: ``x`` normalised over its last axis, times ``gamma``, plus ``beta``, rounded once, and
+        the statistics that ``layer_norm_grad`` takes (``layer_norm_rows`` rounds as the primitives do and keeps none)."""
+        if out is None:
+            stats = self._statistics_dtype(x.dtype)
+            out = self.buffer(x.dtype, x.shape), self.buffer(stats, x.shape[:-1]), self.buffer(stats, x.shape[:-1])
+        y, mean, rstd = out
+        rc = self._lib.nxh_layer_norm(self._h, y._desc(), mean and mean._desc(), rstd and rstd._desc(), x._desc(),
+                                      gamma and gamma._desc(), beta and beta._desc(), float(eps))
+        if rc:
+            self._check(rc)
+        return out
+
+    def layer_norm_grad(self, g: Tensor, x: Tensor, mean: Tensor, rstd: Tensor, gamma: Tensor | None = None, out=None):
+        """``(dx, dgamma, dbeta)``: the gradients of ``layer_norm`` for ``g``, what flows back into its ``y``. A None
+        in ``out`` leaves that gradient out."""
+        if out is None:
+            out = self.buffer(x.dtype, x.shape), self.buffer(x.dtype, x.shape[-1:]), self.buffer(x.dtype, x.shape[-1:])
+        dx, dgamma, dbeta = out
+        rc = self._lib.nxh_layer_norm_grad(self._h, dx and dx._desc(), dgamma and dgamma._desc(), dbeta and dbeta._desc(),
+                                           g._desc(), x._desc(), mean._desc(), rstd._desc(), gamma and gamma._desc())
+        if rc:
+            self._check(rc)
+        return out
+
     # ── fold family (nx_backend.ml:266-307) ─────────────────────────────────
     def _reduce_general(self, op: str, axes: Sequence[int], x: Tensor) -> Tensor:
         """``reduce`` of any axes: out of order, empty extents, errors."""

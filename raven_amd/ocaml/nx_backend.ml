@@ -549,6 +549,33 @@ module Fused = struct
     caml_linear out x w bias residual; out
 end
 
+(* Operators of a training step, each with what its gradient takes. [stats] is the dtype of
+   statistics: float64 for float64 tensors, float32 for all others. *)
+module Train = struct
+  external caml_layer_norm :
+    ('a, 'b) t -> ('c, 'd) t -> ('c, 'd) t -> ('a, 'b) t -> ('a, 'b) t option -> ('a, 'b) t option -> float -> unit
+    = "caml_nx_hip_layer_norm_bc" "caml_nx_hip_layer_norm"
+  external caml_layer_norm_grad :
+    ('a, 'b) t option -> ('a, 'b) t option -> ('a, 'b) t option -> ('a, 'b) t -> ('a, 'b) t -> ('c, 'd) t -> ('c, 'd) t ->
+    ('a, 'b) t option -> unit = "caml_nx_hip_layer_norm_grad_bc" "caml_nx_hip_layer_norm_grad"
+
+  let row_values x = Array.sub x.shape 0 (max 0 (Array.length x.shape - 1))
+  let columns x = [| x.shape.(Array.length x.shape - 1) |]
+
+  let layer_norm ?gamma ?beta ~eps ~stats x =
+    let out = create_tensor x.context x.dtype x.shape in
+    let mean = create_tensor x.context stats (row_values x) in
+    let rstd = create_tensor x.context stats (row_values x) in
+    caml_layer_norm out mean rstd x gamma beta eps; (out, mean, rstd)
+
+  (* dx, dgamma, dbeta for [g], what flows back into the norm's result *)
+  let layer_norm_grad ?gamma ~mean ~rstd x g =
+    let dx = create_tensor x.context x.dtype x.shape in
+    let dgamma = create_tensor x.context x.dtype (columns x) in
+    let dbeta = create_tensor x.context x.dtype (columns x) in
+    caml_layer_norm_grad (Some dx) (Some dgamma) (Some dbeta) g x mean rstd gamma; (dx, dgamma, dbeta)
+end
+
 (* Recorded sequences: every operation between [capture_begin] and [capture_end]
    is recorded instead of run; [Graph.launch] replays the whole sequence with
    one call, reading the inputs' current contents and writing the same outputs.

@@ -38,6 +38,7 @@
   X(triangular_solve) X(qr) X(eigh) X(svd) X(eig) X(device_info)              \
   X(memory_stats) X(trim) X(reduce_noalloc) X(softmax_rows) X(layer_norm_rows) \
   X(gelu_tanh) X(attention) X(linear) X(linear_gelu_tanh) X(set_deferred) X(deferred_stats)        \
+  X(layer_norm) X(layer_norm_grad)                                             \
   X(set_cache_policy) X(cache_policy_stats)                                    \
   X(capture_begin) X(capture_end) X(graph_launch) X(graph_destroy)             \
   X(timer_start) X(timer_stop) X(last_path)
@@ -735,6 +736,40 @@ CAMLprim value caml_nx_hip_linear_gelu_tanh(value vout, value vx, value vw, valu
   extract(vw, &w);
   check(c, L.linear_gelu_tanh(c, &o, &x, &w, optional(vbias, &b), Caml_ba_data_val(vconstants)));
   CAMLreturn(Val_unit);
+}
+
+/* training: results that are not wanted, and operands that are not there, are None */
+CAMLprim value caml_nx_hip_layer_norm(value vout, value vmean, value vrstd, value vx, value vgamma, value vbeta, value veps) {
+  CAMLparam5(vout, vmean, vrstd, vx, vgamma);
+  CAMLxparam2(vbeta, veps);
+  nxh_tensor o, m, r, x, g, b;
+  nxh_context *c = extract(vout, &o);
+  extract(vmean, &m);
+  extract(vrstd, &r);
+  extract(vx, &x);
+  check(c, L.layer_norm(c, &o, &m, &r, &x, optional(vgamma, &g), optional(vbeta, &b), Double_val(veps)));
+  CAMLreturn(Val_unit);
+}
+CAMLprim value caml_nx_hip_layer_norm_bc(value *argv, int argn) {
+  (void)argn;
+  return caml_nx_hip_layer_norm(argv[0], argv[1], argv[2], argv[3], argv[4], argv[5], argv[6]);
+}
+CAMLprim value caml_nx_hip_layer_norm_grad(value vdx, value vdgamma, value vdbeta, value vg, value vx, value vmean,
+                                           value vrstd, value vgamma) {
+  CAMLparam5(vdx, vdgamma, vdbeta, vg, vx);
+  CAMLxparam3(vmean, vrstd, vgamma);
+  nxh_tensor dx, dgamma, dbeta, g, x, m, r, w;
+  nxh_context *c = extract(vg, &g);
+  extract(vx, &x);
+  extract(vmean, &m);
+  extract(vrstd, &r);
+  check(c, L.layer_norm_grad(c, optional(vdx, &dx), optional(vdgamma, &dgamma), optional(vdbeta, &dbeta), &g, &x, &m, &r,
+                             optional(vgamma, &w)));
+  CAMLreturn(Val_unit);
+}
+CAMLprim value caml_nx_hip_layer_norm_grad_bc(value *argv, int argn) {
+  (void)argn;
+  return caml_nx_hip_layer_norm_grad(argv[0], argv[1], argv[2], argv[3], argv[4], argv[5], argv[6], argv[7]);
 }
 
 CAMLprim value caml_nx_hip_set_deferred(value vctx, value von) {
