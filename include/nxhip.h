@@ -369,6 +369,17 @@ int nxh_layer_norm_grad(nxh_context *ctx, const nxh_tensor *dx, const nxh_tensor
                         const nxh_tensor *g, const nxh_tensor *x, const nxh_tensor *mean, const nxh_tensor *rstd,
                         const nxh_tensor *gamma);
 
+/* out = [residual +] (kept ? x * scale : 0), x and residual of one shape and dtype, all of any
+   strides. What is kept is a function of the key (int32, shape [2], device memory: a recorded
+   graph uses what it holds at each replay) and of an element's row-major position i in x's
+   shape: block i / 4 of nxh_threefry (counter words: low 32 bits, high 32 bits) gives two words,
+   whose four halves (low, high, low, high) are the numbers u of the block's four elements; kept
+   is u >= cut, cut = floor (65536 rate + 1/2), scale = 65536 / (65536 - cut). rate 1 keeps
+   nothing. The gradient of x for g is nxh_dropout of g with the same key and rate, the
+   residual's is g itself. */
+int nxh_dropout(nxh_context *ctx, const nxh_tensor *out, const nxh_tensor *x, const nxh_tensor *residual,
+                const nxh_tensor *key, double rate);
+
 /* ── Fourier transforms ──────────────────────────────────────────────────── */
 
 /* fft / ifft (backend_intf.ml:594-598; nx_backend.ml:507-528; nx_c_fft.c:940-956,

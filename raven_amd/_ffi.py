@@ -128,6 +128,7 @@ SIGNATURES = {
     "nxh_attention": (C.c_int, [_CTX, _T, _T, _T, _T, C.c_void_p, _T, C.c_void_p, C.c_int]),
     "nxh_layer_norm": (C.c_int, [_CTX] + [_T] * 6 + [C.c_double]),
     "nxh_layer_norm_grad": (C.c_int, [_CTX] + [_T] * 8),
+    "nxh_dropout": (C.c_int, [_CTX] + [_T] * 4 + [C.c_double]),
     "nxh_set_deferred": (C.c_int, [_CTX, C.c_int]),
     "nxh_deferred_stats": (C.c_int, [_CTX, _P(C.c_uint64), C.c_int]),
     "nxh_set_cache_policy": (C.c_int, [_CTX, C.c_int]),

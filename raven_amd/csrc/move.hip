@@ -31,6 +31,7 @@
 // (key, counter) vector; normative bit for bit.
 
 #include "nxh_common.hpp"
+#include "threefry.hpp"
 #include "stream_access.hpp"
 
 struct alignas(16) G16 {
@@ -1105,7 +1106,6 @@ struct ThreefryArgs {
   int64_t kstride[NXH_MAX_NDIM], cstride[NXH_MAX_NDIM], ostride[NXH_MAX_NDIM];
   int64_t key_last, ctr_last, out_last;  // stride of the 2-word axis
 };
-__device__ __forceinline__ uint32_t rotl32(uint32_t x, int r) { return (x << r) | (x >> (32 - r)); }
 __global__ __launch_bounds__(256) void threefry_kernel(ThreefryArgs a) {
   const int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (it >= a.vectors) return;
@@ -1140,23 +1140,6 @@ __global__ __launch_bounds__(256) void threefry_kernel(ThreefryArgs a) {
 // for all vectors or dense too. A lane takes two neighbouring vectors with one 16-byte load and
 // one 16-byte store (two independent chains of rounds) and no division; a lane per vector with
 // 4-byte accesses and a 64-bit division left the call at half the memory rate.
-__device__ __forceinline__ void threefry_block(uint32_t k0, uint32_t k1, uint32_t &x0, uint32_t &x1) {
-  const uint32_t ks[3] = {k0, k1, 0x1BD11BDAu ^ k0 ^ k1};
-  x0 += k0;
-  x1 += k1;
-  constexpr int rots[8] = {13, 15, 26, 6, 17, 29, 16, 24};
-#pragma unroll
-  for (int r = 0; r < 20; r++) {
-    x0 += x1;
-    x1 = rotl32(x1, rots[r % 8]);
-    x1 ^= x0;
-    if ((r + 1) % 4 == 0) {
-      const int s = (r + 1) / 4;
-      x0 += ks[s % 3];
-      x1 += ks[(s + 1) % 3] + (uint32_t)s;
-    }
-  }
-}
 __global__ __launch_bounds__(256) void threefry_dense_kernel(const int32_t *key, int64_t key_step, int64_t key_last,
                                                              const int32_t *ctr, int32_t *out, int64_t vectors) {
   typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;

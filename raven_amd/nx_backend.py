@@ -582,6 +582,17 @@ class Backend(Calls):
             self._check(rc)
         return out
 
+    def dropout(self, x: Tensor, key: Tensor, rate: float, residual: Tensor | None = None, out: Tensor | None = None) -> Tensor:
+        """``residual +`` what of ``x`` a mask keeps, scaled by what it drops. The mask is a function of ``key`` (two
+        int32) and an element's position and is never stored: the gradient of ``x`` for ``g`` is
+        ``dropout(g, key, rate)``. Calls that are to drop independently take keys of their own."""
+        if out is None:
+            out = self.buffer(x.dtype, x.shape)
+        rc = self._lib.nxh_dropout(self._h, out._desc(), x._desc(), residual and residual._desc(), key._desc(), float(rate))
+        if rc:
+            self._check(rc)
+        return out
+
     # ── fold family (nx_backend.ml:266-307) ─────────────────────────────────
     def _reduce_general(self, op: str, axes: Sequence[int], x: Tensor) -> Tensor:
         """``reduce`` of any axes: out of order, empty extents, errors."""

@@ -574,6 +574,14 @@ module Train = struct
     let dgamma = create_tensor x.context x.dtype (columns x) in
     let dbeta = create_tensor x.context x.dtype (columns x) in
     caml_layer_norm_grad (Some dx) (Some dgamma) (Some dbeta) g x mean rstd gamma; (dx, dgamma, dbeta)
+
+  external caml_dropout :
+    ('a, 'b) t -> ('a, 'b) t -> ('a, 'b) t option -> (int32, Dtype.int32_elt) t -> float -> unit = "caml_nx_hip_dropout"
+
+  (* the gradient of [x] for [g] is [dropout ~rate ~key g] *)
+  let dropout ?residual ~rate ~key x =
+    let out = create_tensor x.context x.dtype x.shape in
+    caml_dropout out x residual key rate; out
 end
 
 (* Recorded sequences: every operation between [capture_begin] and [capture_end]

@@ -38,7 +38,7 @@
   X(triangular_solve) X(qr) X(eigh) X(svd) X(eig) X(device_info)              \
   X(memory_stats) X(trim) X(reduce_noalloc) X(softmax_rows) X(layer_norm_rows) \
   X(gelu_tanh) X(attention) X(linear) X(linear_gelu_tanh) X(set_deferred) X(deferred_stats)        \
-  X(layer_norm) X(layer_norm_grad)                                             \
+  X(layer_norm) X(layer_norm_grad) X(dropout)                                  \
   X(set_cache_policy) X(cache_policy_stats)                                    \
   X(capture_begin) X(capture_end) X(graph_launch) X(graph_destroy)             \
   X(timer_start) X(timer_stop) X(last_path)
@@ -770,6 +770,16 @@ CAMLprim value caml_nx_hip_layer_norm_grad(value vdx, value vdgamma, value vdbet
 CAMLprim value caml_nx_hip_layer_norm_grad_bc(value *argv, int argn) {
   (void)argn;
   return caml_nx_hip_layer_norm_grad(argv[0], argv[1], argv[2], argv[3], argv[4], argv[5], argv[6], argv[7]);
+}
+
+CAMLprim value caml_nx_hip_dropout(value vout, value vx, value vresidual, value vkey, value vrate) {
+  CAMLparam5(vout, vx, vresidual, vkey, vrate);
+  nxh_tensor o, x, r, k;
+  nxh_context *c = extract(vout, &o);
+  extract(vx, &x);
+  extract(vkey, &k);
+  check(c, L.dropout(c, &o, &x, optional(vresidual, &r), &k, Double_val(vrate)));
+  CAMLreturn(Val_unit);
 }
 
 CAMLprim value caml_nx_hip_set_deferred(value vctx, value von) {
