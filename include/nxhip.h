@@ -380,6 +380,31 @@ int nxh_layer_norm_grad(nxh_context *ctx, const nxh_tensor *dx, const nxh_tensor
 int nxh_dropout(nxh_context *ctx, const nxh_tensor *out, const nxh_tensor *x, const nxh_tensor *residual,
                 const nxh_tensor *key, double rate);
 
+/* Of each row of logits, p = softmax of the row, its token (int32, a value of the row): log_p =
+   log p[token], 0 for a token below zero (padding), NaN for one past the row (nothing waits for the
+   device to report it); entropy = - sum p log p; peak = the row's largest logit and total = sum
+   e^(logit - peak), which the gradient takes; and the most likely tokens with their log
+   probabilities, in descending order, equal logits by index, NaNs last: top_log_p, top_tokens
+   (int32), logits' shape with 0 to 64 as last extent, rows contiguous. Each result may be NULL, the
+   last two together. A logit of -inf has probability 0; a row with a NaN or +inf, or of -inf
+   alone, has NaN for all values but peak (the largest that is a number). */
+int nxh_log_probs(nxh_context *ctx, const nxh_tensor *log_p, const nxh_tensor *entropy, const nxh_tensor *peak,
+                  const nxh_tensor *total, const nxh_tensor *top_log_p, const nxh_tensor *top_tokens,
+                  const nxh_tensor *logits, const nxh_tensor *tokens);
+/* The gradient of the logits, out, for g, what flows back into log_p, and, not NULL, g_entropy,
+   what flows back into entropy (values of rows, broadcasts among them):
+     g (1[token] - p) - g_entropy p (log p + entropy)
+   peak, total and entropy as nxh_log_probs gave them; entropy is NULL where g_entropy is. The
+   first term is left out for padding; a token past the row makes its row NaN. */
+int nxh_log_probs_grad(nxh_context *ctx, const nxh_tensor *out, const nxh_tensor *g, const nxh_tensor *logits,
+                       const nxh_tensor *tokens, const nxh_tensor *peak, const nxh_tensor *total,
+                       const nxh_tensor *g_entropy, const nxh_tensor *entropy);
+/* Both at once, for losses whose g and g_entropy do not depend on log_p and entropy (a mean of
+   them, with weights): reads the logits from memory once. log_p, entropy, g_entropy may be NULL. */
+int nxh_log_probs_with_grad(nxh_context *ctx, const nxh_tensor *log_p, const nxh_tensor *entropy, const nxh_tensor *out,
+                            const nxh_tensor *g, const nxh_tensor *logits, const nxh_tensor *tokens,
+                            const nxh_tensor *g_entropy);
+
 /* ── Fourier transforms ──────────────────────────────────────────────────── */
 
 /* fft / ifft (backend_intf.ml:594-598; nx_backend.ml:507-528; nx_c_fft.c:940-956,

@@ -129,6 +129,9 @@ SIGNATURES = {
     "nxh_layer_norm": (C.c_int, [_CTX] + [_T] * 6 + [C.c_double]),
     "nxh_layer_norm_grad": (C.c_int, [_CTX] + [_T] * 8),
     "nxh_dropout": (C.c_int, [_CTX] + [_T] * 4 + [C.c_double]),
+    "nxh_log_probs": (C.c_int, [_CTX] + [_T] * 8),
+    "nxh_log_probs_grad": (C.c_int, [_CTX] + [_T] * 8),
+    "nxh_log_probs_with_grad": (C.c_int, [_CTX] + [_T] * 7),
     "nxh_set_deferred": (C.c_int, [_CTX, C.c_int]),
     "nxh_deferred_stats": (C.c_int, [_CTX, _P(C.c_uint64), C.c_int]),
     "nxh_set_cache_policy": (C.c_int, [_CTX, C.c_int]),

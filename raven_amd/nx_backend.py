@@ -593,6 +593,50 @@ class Backend(Calls):
             self._check(rc)
         return out
 
+    def log_probs(self, logits: Tensor, tokens: Tensor, top: int = 0, out=None):
+        """``(log_p, entropy, peak, total, top_log_p, top_tokens)`` of each row of ``logits``: the log probability of its
+        token (a negative one is padding: 0), the entropy of its softmax, the statistics ``log_probs_grad`` takes, and
+        the ``top`` most likely tokens, equal ones by index (None for ``top`` 0). A None in ``out`` leaves that result out."""
+        if out is None:
+            stats = self._statistics_dtype(logits.dtype)
+            rows = logits.shape[:-1]
+            out = tuple(self.buffer(stats, rows) for _ in range(4))
+            out += (self.buffer(stats, (*rows, top)), self.buffer(dt.int32, (*rows, top))) if top else (None, None)
+        log_p, entropy, peak, total, top_log_p, top_tokens = out
+        if (top_tokens.shape[-1] if top_tokens else 0) != top:
+            raise ValueError("log_probs: the results have room for another number of alternatives")
+        rc = self._lib.nxh_log_probs(self._h, log_p and log_p._desc(), entropy and entropy._desc(), peak and peak._desc(),
+                                     total and total._desc(), top_log_p and top_log_p._desc(), top_tokens and top_tokens._desc(),
+                                     logits._desc(), tokens._desc())
+        if rc:
+            self._check(rc)
+        return out
+
+    def log_probs_grad(self, g: Tensor, logits: Tensor, tokens: Tensor, peak: Tensor, total: Tensor,
+                       g_entropy: Tensor | None = None, entropy: Tensor | None = None, out: Tensor | None = None) -> Tensor:
+        """The gradient of ``logits`` for ``g``, what flows back into ``log_p``, and ``g_entropy``, what flows back
+        into ``entropy`` (which it then needs)."""
+        if out is None:
+            out = self.buffer(logits.dtype, logits.shape)
+        rc = self._lib.nxh_log_probs_grad(self._h, out._desc(), g._desc(), logits._desc(), tokens._desc(), peak._desc(),
+                                          total._desc(), g_entropy and g_entropy._desc(), entropy and entropy._desc())
+        if rc:
+            self._check(rc)
+        return out
+
+    def log_probs_with_grad(self, g: Tensor, logits: Tensor, tokens: Tensor, g_entropy: Tensor | None = None, out=None):
+        """``(log_p, entropy, d_logits)`` in one call, for losses whose ``g`` and ``g_entropy`` are known before it (means,
+        weighted sums): the logits are read from memory once."""
+        if out is None:
+            stats = self._statistics_dtype(logits.dtype)
+            out = self.buffer(stats, logits.shape[:-1]), self.buffer(stats, logits.shape[:-1]), self.buffer(logits.dtype, logits.shape)
+        log_p, entropy, d_logits = out
+        rc = self._lib.nxh_log_probs_with_grad(self._h, log_p and log_p._desc(), entropy and entropy._desc(), d_logits._desc(),
+                                               g._desc(), logits._desc(), tokens._desc(), g_entropy and g_entropy._desc())
+        if rc:
+            self._check(rc)
+        return out
+
     # ── fold family (nx_backend.ml:266-307) ─────────────────────────────────
     def _reduce_general(self, op: str, axes: Sequence[int], x: Tensor) -> Tensor:
         """``reduce`` of any axes: out of order, empty extents, errors."""

@@ -582,6 +582,42 @@ module Train = struct
   let dropout ?residual ~rate ~key x =
     let out = create_tensor x.context x.dtype x.shape in
     caml_dropout out x residual key rate; out
+
+  external caml_log_probs :
+    ('c, 'd) t option -> ('c, 'd) t option -> ('c, 'd) t option -> ('c, 'd) t option -> ('c, 'd) t option ->
+    (int32, Dtype.int32_elt) t option -> ('a, 'b) t -> (int32, Dtype.int32_elt) t -> unit
+    = "caml_nx_hip_log_probs_bc" "caml_nx_hip_log_probs"
+  external caml_log_probs_grad :
+    ('a, 'b) t -> ('c, 'd) t -> ('a, 'b) t -> (int32, Dtype.int32_elt) t -> ('c, 'd) t -> ('c, 'd) t ->
+    ('c, 'd) t option -> ('c, 'd) t option -> unit = "caml_nx_hip_log_probs_grad_bc" "caml_nx_hip_log_probs_grad"
+  external caml_log_probs_with_grad :
+    ('c, 'd) t option -> ('c, 'd) t option -> ('a, 'b) t -> ('c, 'd) t -> ('a, 'b) t -> (int32, Dtype.int32_elt) t ->
+    ('c, 'd) t option -> unit = "caml_nx_hip_log_probs_with_grad_bc" "caml_nx_hip_log_probs_with_grad"
+
+  (* log_p, entropy, peak, total of each row of [logits], and its [top] most likely tokens *)
+  let log_probs ?(top = 0) ~stats logits tokens =
+    let values () = create_tensor logits.context stats (row_values logits) in
+    let log_p, entropy, peak, total = (values (), values (), values (), values ()) in
+    let alternatives =
+      if top = 0 then None
+      else
+        let shape = Array.append (row_values logits) [| top |] in
+        Some (create_tensor logits.context stats shape, create_tensor logits.context Dtype.Int32 shape) in
+    caml_log_probs (Some log_p) (Some entropy) (Some peak) (Some total) (Option.map fst alternatives)
+      (Option.map snd alternatives) logits tokens;
+    (log_p, entropy, peak, total, alternatives)
+
+  (* the gradient of [logits] for [g] of log_p and, with the entropy, [g_entropy] *)
+  let log_probs_grad ?entropy ~peak ~total logits tokens g =
+    let out = create_tensor logits.context logits.dtype logits.shape in
+    let entropy, g_entropy = match entropy with Some (e, ge) -> (Some e, Some ge) | None -> (None, None) in
+    caml_log_probs_grad out g logits tokens peak total g_entropy entropy; out
+
+  let log_probs_with_grad ?g_entropy ~stats logits tokens g =
+    let values () = create_tensor logits.context stats (row_values logits) in
+    let log_p, entropy = (values (), values ()) in
+    let out = create_tensor logits.context logits.dtype logits.shape in
+    caml_log_probs_with_grad (Some log_p) (Some entropy) out g logits tokens g_entropy; (log_p, entropy, out)
 end
 
 (* Recorded sequences: every operation between [capture_begin] and [capture_end]

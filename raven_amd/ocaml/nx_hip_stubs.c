@@ -39,6 +39,7 @@
   X(memory_stats) X(trim) X(reduce_noalloc) X(softmax_rows) X(layer_norm_rows) \
   X(gelu_tanh) X(attention) X(linear) X(linear_gelu_tanh) X(set_deferred) X(deferred_stats)        \
   X(layer_norm) X(layer_norm_grad) X(dropout)                                  \
+  X(log_probs) X(log_probs_grad) X(log_probs_with_grad)                        \
   X(set_cache_policy) X(cache_policy_stats)                                    \
   X(capture_begin) X(capture_end) X(graph_launch) X(graph_destroy)             \
   X(timer_start) X(timer_stop) X(last_path)
@@ -780,6 +781,56 @@ CAMLprim value caml_nx_hip_dropout(value vout, value vx, value vresidual, value 
   extract(vkey, &k);
   check(c, L.dropout(c, &o, &x, optional(vresidual, &r), &k, Double_val(vrate)));
   CAMLreturn(Val_unit);
+}
+
+CAMLprim value caml_nx_hip_log_probs(value vlog_p, value ventropy, value vpeak, value vtotal, value vtop_log_p,
+                                     value vtop_tokens, value vlogits, value vtokens) {
+  CAMLparam5(vlog_p, ventropy, vpeak, vtotal, vtop_log_p);
+  CAMLxparam3(vtop_tokens, vlogits, vtokens);
+  nxh_tensor p, e, m, s, tp, tt, x, t;
+  nxh_context *c = extract(vlogits, &x);
+  extract(vtokens, &t);
+  check(c, L.log_probs(c, optional(vlog_p, &p), optional(ventropy, &e), optional(vpeak, &m), optional(vtotal, &s),
+                       optional(vtop_log_p, &tp), optional(vtop_tokens, &tt), &x, &t));
+  CAMLreturn(Val_unit);
+}
+CAMLprim value caml_nx_hip_log_probs_bc(value *argv, int argn) {
+  (void)argn;
+  return caml_nx_hip_log_probs(argv[0], argv[1], argv[2], argv[3], argv[4], argv[5], argv[6], argv[7]);
+}
+CAMLprim value caml_nx_hip_log_probs_grad(value vout, value vg, value vlogits, value vtokens, value vpeak, value vtotal,
+                                          value vg_entropy, value ventropy) {
+  CAMLparam5(vout, vg, vlogits, vtokens, vpeak);
+  CAMLxparam3(vtotal, vg_entropy, ventropy);
+  nxh_tensor o, g, x, t, m, s, ge, e;
+  nxh_context *c = extract(vout, &o);
+  extract(vg, &g);
+  extract(vlogits, &x);
+  extract(vtokens, &t);
+  extract(vpeak, &m);
+  extract(vtotal, &s);
+  check(c, L.log_probs_grad(c, &o, &g, &x, &t, &m, &s, optional(vg_entropy, &ge), optional(ventropy, &e)));
+  CAMLreturn(Val_unit);
+}
+CAMLprim value caml_nx_hip_log_probs_grad_bc(value *argv, int argn) {
+  (void)argn;
+  return caml_nx_hip_log_probs_grad(argv[0], argv[1], argv[2], argv[3], argv[4], argv[5], argv[6], argv[7]);
+}
+CAMLprim value caml_nx_hip_log_probs_with_grad(value vlog_p, value ventropy, value vout, value vg, value vlogits,
+                                               value vtokens, value vg_entropy) {
+  CAMLparam5(vlog_p, ventropy, vout, vg, vlogits);
+  CAMLxparam2(vtokens, vg_entropy);
+  nxh_tensor p, e, o, g, x, t, ge;
+  nxh_context *c = extract(vout, &o);
+  extract(vg, &g);
+  extract(vlogits, &x);
+  extract(vtokens, &t);
+  check(c, L.log_probs_with_grad(c, optional(vlog_p, &p), optional(ventropy, &e), &o, &g, &x, &t, optional(vg_entropy, &ge)));
+  CAMLreturn(Val_unit);
+}
+CAMLprim value caml_nx_hip_log_probs_with_grad_bc(value *argv, int argn) {
+  (void)argn;
+  return caml_nx_hip_log_probs_with_grad(argv[0], argv[1], argv[2], argv[3], argv[4], argv[5], argv[6]);
 }
 
 CAMLprim value caml_nx_hip_set_deferred(value vctx, value von) {
