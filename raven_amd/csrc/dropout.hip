@@ -30,13 +30,9 @@ struct DropoutArgs {
   int64_t shape[DROP_MAXD], stride[3][DROP_MAXD];
 };
 
-template <int DT>
-__device__ __forceinline__ typename Tr<DT>::S drop_one(typename Tr<DT>::S x, bool keep, typename Tr<DT>::C scale, bool add,
-                                                       typename Tr<DT>::S residual) {
-  using TX = Tr<DT>;
-  typename TX::C y = keep ? TX::ld(x) * scale : 0;  // (chosen, not multiplied: a NaN that is dropped is gone)
-  if (add) y = y + TX::ld(residual);
-  return TX::st(y);
+template <class C>
+__device__ __forceinline__ C drop_one(C x, bool keep, C scale) {
+  return keep ? x * scale : 0;  // (chosen, not multiplied: a NaN that is dropped is gone)
 }
 // Which of the four elements of block `b` are kept.
 struct Keep {
@@ -51,37 +47,50 @@ __device__ __forceinline__ Keep keep_four(uint32_t k0, uint32_t k1, uint64_t b, 
 // All operands dense: a lane takes the elements of one or two blocks, 16 bytes of a 16- or 32-bit dtype.
 template <int DT, bool RESIDUAL>
 __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
-  using C = typename Tr<DT>::C;
-  using S = typename Tr<DT>::S;
-  constexpr int V = VECTOR<S> < 4 ? 4 : VECTOR<S>;
+  using IO = Io<DT>;
+  using C = typename IO::C;
+  using S = typename IO::S;
+  constexpr int N = IO::V < 4 ? 4 : IO::V, L = N / IO::V;  // elements and vectors of a lane
   const uint32_t k0 = (uint32_t)a.key[0], k1 = (uint32_t)a.key[a.key_step];
   const C scale = (C)a.scale;
-  for (int64_t first = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; first < a.n; first += (int64_t)gridDim.x * 256 * V) {
-    const S *x = reinterpret_cast<const S *>(a.x) + first, *r = reinterpret_cast<const S *>(a.residual) + first;
-    S *out = reinterpret_cast<S *>(a.out) + first;
-    const int left = a.n - first < V ? (int)(a.n - first) : V;
-    Vec<S, V> xv, rv, o;
-    if (left == V) {
-      xv = load_vec<V>(x);
-      if (RESIDUAL) rv = load_vec<V>(r);
-    } else {
+  const S *x = reinterpret_cast<const S *>(a.x), *r = reinterpret_cast<const S *>(a.residual);
+  S *out = reinterpret_cast<S *>(a.out);
+  for (int64_t first = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N; first < a.n; first += (int64_t)gridDim.x * 256 * N) {
+    if (first + N <= a.n) {
+      Words xw[L], rw[L];
 #pragma unroll
-      for (int j = 0; j < V; j++) {
-        xv.v[j] = j < left ? x[j] : S{};
-        rv.v[j] = RESIDUAL && j < left ? r[j] : S{};
+      for (int l = 0; l < L; l++) {
+        xw[l] = load_words(x + first + l * IO::V);
+        if (RESIDUAL) rw[l] = load_words(r + first + l * IO::V);
+      }
+      bool keep[N];
+#pragma unroll
+      for (int q = 0; q < N / 4; q++) {
+        const Keep four = keep_four(k0, k1, (uint64_t)first / 4 + q, a.cut);
+#pragma unroll
+        for (int j = 0; j < 4; j++) keep[q * 4 + j] = four.k[j];
+      }
+#pragma unroll
+      for (int l = 0; l < L; l++) {
+        C y[IO::V], add[IO::V];
+        IO::widen(xw[l], y);
+        if (RESIDUAL) IO::widen(rw[l], add);
+#pragma unroll
+        for (int j = 0; j < IO::V; j++) {
+          y[j] = drop_one(y[j], keep[l * IO::V + j], scale);
+          if (RESIDUAL) y[j] = y[j] + add[j];
+        }
+        store_words(out + first + l * IO::V, IO::narrow(y));
+      }
+    } else {
+      for (int64_t i = first; i < a.n; i++) {
+        const Keep four = keep_four(k0, k1, (uint64_t)i / 4, a.cut);
+        const int j = (int)(i & 3);
+        C y = drop_one(IO::ld(x[i]), j < 2 ? (j ? four.k[1] : four.k[0]) : (j == 3 ? four.k[3] : four.k[2]), scale);
+        if (RESIDUAL) y = y + IO::ld(r[i]);
+        out[i] = IO::st(y);
       }
     }
-#pragma unroll
-    for (int q = 0; q < V / 4; q++) {
-      const Keep keep = keep_four(k0, k1, (uint64_t)first / 4 + q, a.cut);
-#pragma unroll
-      for (int j = 0; j < 4; j++) o.v[q * 4 + j] = drop_one<DT>(xv.v[q * 4 + j], keep.k[j], scale, RESIDUAL, rv.v[q * 4 + j]);
-    }
-    if (left == V) store_vec<V>(out, o);
-    else
-#pragma unroll
-      for (int j = 0; j < V; j++)
-        if (j < left) out[j] = o.v[j];
   }
 }
 
@@ -89,8 +98,9 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
 // cross its end; only then each has its own way through the extents.
 template <int DT>
 __global__ __launch_bounds__(256) void dropout_strided_kernel(DropoutArgs a) {
-  using C = typename Tr<DT>::C;
-  using S = typename Tr<DT>::S;
+  using IO = Io<DT>;
+  using C = typename IO::C;
+  using S = typename IO::S;
   const S *x = reinterpret_cast<const S *>(a.x), *r = reinterpret_cast<const S *>(a.residual);
   S *out = reinterpret_cast<S *>(a.out);
   const bool small = a.n <= 0xffffffffLL;
@@ -122,13 +132,19 @@ __global__ __launch_bounds__(256) void dropout_strided_kernel(DropoutArgs a) {
         rv[j] = r ? r[at[1] + j * a.stride[1][last]] : S{};
       }
 #pragma unroll
-      for (int j = 0; j < 4; j++) out[at[2] + j * a.stride[2][last]] = drop_one<DT>(xv[j], keep.k[j], scale, r != nullptr, rv[j]);
+      for (int j = 0; j < 4; j++) {
+        C y = drop_one(IO::ld(xv[j]), keep.k[j], scale);
+        if (r) y = y + IO::ld(rv[j]);
+        out[at[2] + j * a.stride[2][last]] = IO::st(y);
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < 4; j++)
         if (block * 4 + j < a.n) {
           find(block * 4 + j, at);
-          out[at[2]] = drop_one<DT>(x[at[0]], keep.k[j], scale, r != nullptr, r ? r[at[1]] : S{});
+          C y = drop_one(IO::ld(x[at[0]]), keep.k[j], scale);
+          if (r) y = y + IO::ld(r[at[1]]);
+          out[at[2]] = IO::st(y);
         }
     }
   }
@@ -155,8 +171,8 @@ void merge_dims(DropoutArgs &a) {
 
 template <int DT>
 void launch(nxh_context *ctx, const DropoutArgs &a, bool dense) {
-  constexpr int V = VECTOR<typename Tr<DT>::S> < 4 ? 4 : VECTOR<typename Tr<DT>::S>;
-  const int64_t lanes = dense ? (a.n + V - 1) / V : (a.n + 3) / 4;
+  constexpr int N = Io<DT>::V < 4 ? 4 : Io<DT>::V;
+  const int64_t lanes = dense ? (a.n + N - 1) / N : (a.n + 3) / 4;
   const dim3 grid((unsigned)std::min<int64_t>((lanes + 255) / 256, DROP_BLOCKS));
   if (!dense) hipLaunchKernelGGL((dropout_strided_kernel<DT>), grid, dim3(256), 0, ctx->stream, a);
   else if (a.residual) hipLaunchKernelGGL((dropout_kernel<DT, true>), grid, dim3(256), 0, ctx->stream, a);

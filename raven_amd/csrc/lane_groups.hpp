@@ -11,43 +11,130 @@ namespace {
 template <class S>
 constexpr int VECTOR = 16 / (int)sizeof(S);
 
-template <class S, int V>
-struct Vec {
-  S v[V];
-};
+// Sixteen bytes of a row, as words: elements are taken out where they are used (kept as an array of 16-bit elements between a load
+// and its use, the compiler takes them apart at the load, which waits for it).
+typedef uint32_t Words __attribute__((ext_vector_type(4)));
 // A 16-byte access needs no more than an element's alignment, so rows of odd lengths and views that
 // start anywhere are read and written as wide as aligned ones.
-template <int V, class S>
-__device__ __forceinline__ Vec<S, V> load_vec(const S *p) {
-  Vec<S, V> x;
-  __builtin_memcpy(&x, p, sizeof(S) * V);
-  return x;
+template <class S>
+__device__ __forceinline__ Words load_words(const S *p) {
+  Words w;
+  __builtin_memcpy(&w, p, sizeof w);
+  return w;
 }
-template <int V, class S>
-__device__ __forceinline__ void store_vec(S *p, const Vec<S, V> &x) {
-  __builtin_memcpy(p, &x, sizeof(S) * V);
+template <class S>
+__device__ __forceinline__ void store_words(S *p, Words w) {
+  __builtin_memcpy(p, &w, sizeof w);
 }
-// Vector c of a row of n elements. RAGGED: the last one may reach past the row; what is not there reads as `fill`.
-template <int V, bool RAGGED, class S>
-__device__ __forceinline__ Vec<S, V> load_part(const S *row, int c, int n, S fill) {
-  if (!RAGGED || (c + 1) * V <= n) return load_vec<V>(row + (int64_t)c * V);
-  Vec<S, V> x;
-#pragma unroll
-  for (int j = 0; j < V; j++) {
-    x.v[j] = fill;
-    if (c * V + j < n) x.v[j] = row[(int64_t)c * V + j];
+
+// What elements are computed as, and back, one or a vector at a time. float16 and bfloat16 take the hardware's conversions, which
+// round to nearest, ties to even, and keep a NaN a NaN; the primitives' keep its payload too, at some ten instructions an
+// element of float16.
+template <int DT>
+struct Io {
+  using S = typename Tr<DT>::S;
+  using C = typename Tr<DT>::C;
+  static constexpr int V = VECTOR<S>;
+  __device__ __forceinline__ static C ld(S s) {
+    if constexpr (DT == NXH_F16) return (float)__builtin_bit_cast(_Float16, s);
+    else return Tr<DT>::ld(s);
   }
-  return x;
+  __device__ __forceinline__ static S st(C c) {
+    if constexpr (DT == NXH_F16) {
+      asm("" : "+v"(c));  // (a product folded into the conversion would lose the sign of zero)
+      return __builtin_bit_cast(uint16_t, (_Float16)c);
+    } else {
+      return Tr<DT>::st(c);
+    }
+  }
+  __device__ __forceinline__ static void widen(Words w, C (&x)[V]) {
+    if constexpr (sizeof(S) == 2) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        if constexpr (DT == NXH_BF16) {
+          x[2 * k] = u2f(w[k] << 16);
+          x[2 * k + 1] = u2f(w[k] & 0xffff0000u);
+        } else {
+          x[2 * k] = ld((S)(w[k] & 0xffffu));
+          x[2 * k + 1] = ld((S)(w[k] >> 16));
+        }
+      }
+    } else {
+      struct Elements { C x[V]; } e = __builtin_bit_cast(Elements, w);
+#pragma unroll
+      for (int j = 0; j < V; j++) x[j] = e.x[j];
+    }
+  }
+  __device__ __forceinline__ static Words narrow(const C (&x)[V]) {
+    Words w;
+    if constexpr (sizeof(S) == 2) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        if constexpr (DT == NXH_BF16) w[k] = f32x2_to_bf16x2(x[2 * k], x[2 * k + 1]);
+        else w[k] = (uint32_t)st(x[2 * k]) | (uint32_t)st(x[2 * k + 1]) << 16;
+      }
+    } else {
+      struct Elements { C x[V]; } e;
+#pragma unroll
+      for (int j = 0; j < V; j++) e.x[j] = x[j];
+      w = __builtin_bit_cast(Words, e);
+    }
+    return w;
+  }
+  __device__ __forceinline__ static Words all(C c) {
+    C x[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) x[j] = c;
+    return narrow(x);
+  }
+};
+
+// Vector c of a row of n elements. WHOLE: n is a number of vectors. RAGGED: it is none and more than one; the last vector is the
+// row's last V elements, of which it has the first in common with the one before it: they are loaded, computed and stored
+// twice, with equal results, and belong to sums once. SHORT: less than a vector, which is taken element by element.
+enum Rows { WHOLE, RAGGED, SHORT };
+template <int V, Rows R>
+__device__ __forceinline__ int vec_start(int c, int n) {
+  return R != RAGGED || (c + 1) * V <= n ? c * V : n - V;
 }
-template <int V, bool RAGGED, class S>
-__device__ __forceinline__ void store_part(S *row, int c, int n, const Vec<S, V> &x) {
-  if (!RAGGED || (c + 1) * V <= n) {
-    store_vec<V>(row + (int64_t)c * V, x);
+// Whether element j of vector c belongs to it.
+template <int V, Rows R>
+__device__ __forceinline__ bool vec_owns(int c, int j, int n) {
+  return R == WHOLE ? true : R == SHORT ? j < n : j >= c * V - vec_start<V, R>(c, n);
+}
+template <Rows R, class S>
+__device__ __forceinline__ Words load_part(const S *row, int c, int n) {
+  constexpr int V = VECTOR<S>;
+  if constexpr (R != SHORT) return load_words(row + vec_start<V, R>(c, n));
+  struct Elements { S x[V]; } e;
+#pragma unroll
+  for (int j = 0; j < V; j++) e.x[j] = row[j < n ? j : 0];
+  return __builtin_bit_cast(Words, e);
+}
+template <Rows R, class S>
+__device__ __forceinline__ void store_part(S *row, int c, int n, Words w) {
+  constexpr int V = VECTOR<S>;
+  if constexpr (R != SHORT) {
+    store_words(row + vec_start<V, R>(c, n), w);
+  } else {
+    struct Elements { S x[V]; } e = __builtin_bit_cast(Elements, w);
+#pragma unroll
+    for (int j = 0; j < V; j++)
+      if (j < n) row[j] = e.x[j];
+  }
+}
+// Only what the vector owns: for results that replace what other lanes may not have read yet.
+template <class S>
+__device__ __forceinline__ void store_own(S *row, int c, int n, Words w) {
+  constexpr int V = VECTOR<S>;
+  if ((c + 1) * V <= n) {
+    store_words(row + c * V, w);
     return;
   }
+  struct Elements { S x[V]; } e = __builtin_bit_cast(Elements, w);
 #pragma unroll
   for (int j = 0; j < V; j++)
-    if (c * V + j < n) row[(int64_t)c * V + j] = x.v[j];
+    if (vec_owns<V, RAGGED>(c, j, n)) row[vec_start<V, RAGGED>(c, n) + j] = e.x[j];
 }
 
 // ── exchanges between lanes ─────────────────────────────────────────────────

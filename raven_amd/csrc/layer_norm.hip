@@ -26,53 +26,59 @@ struct LayerNormArgs {
 __device__ __forceinline__ float reciprocal_root(float v) { return 1.0f / sqrtf(v); }
 __device__ __forceinline__ double reciprocal_root(double v) { return 1.0 / sqrt(v); }
 
-template <int DT, int G, int NV, bool RAGGED>
+template <int DT, int G, int NV, Rows R>
 __global__ __launch_bounds__(ln_threads(G)) void layer_norm_kernel(LayerNormArgs a) {
-  using TX = Tr<DT>;
-  using C = typename TX::C;
-  using S = typename TX::S;
-  constexpr int V = VECTOR<S>, GROUPS = ln_threads(G) / G;
+  using IO = Io<DT>;
+  using C = typename IO::C;
+  using S = typename IO::S;
+  constexpr int V = IO::V, GROUPS = ln_threads(G) / G;
   __shared__ C lds[G > 64 ? G / 64 : 1];
   const int lane = threadIdx.x % G, n = a.g.n, nvec = (n + V - 1) / V;
   const S *gamma = reinterpret_cast<const S *>(a.gamma), *beta = reinterpret_cast<const S *>(a.beta);
-  Vec<S, V> gv[NV], bv[NV];
+  // Every lane loads for every v, a vector past the row as the row's last: a load under a condition is waited for before the next one.
+  int c[NV];
+#pragma unroll
+  for (int v = 0; v < NV; v++) c[v] = v * G + lane < nvec ? v * G + lane : nvec - 1;
+  Words gv[NV], bv[NV];
 #pragma unroll
   for (int v = 0; v < NV; v++) {
-    const int c = v * G + lane;
-    if (c < nvec && gamma) gv[v] = load_part<V, RAGGED>(gamma, c, n, S{});
-    if (c < nvec && beta) bv[v] = load_part<V, RAGGED>(beta, c, n, S{});
+    gv[v] = gamma ? load_part<R>(gamma, c[v], n) : IO::all(1);
+    bv[v] = beta ? load_part<R>(beta, c[v], n) : IO::all(0);
   }
+  // Whether this lane's vector v has element j for itself. Only the row's last vector may not: which v that is is the same for all lanes.
+  const int last = (nvec - 1) / G;
+  auto owns = [&](int v, int j) { return R == WHOLE || v != last || vec_owns<V, R>(c[v], j, n); };
   const C count = (C)n, eps = (C)a.eps;
   for (int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G; row < a.g.rows; row += (int64_t)gridDim.x * GROUPS) {
     int64_t at[LN_OPERANDS];
     row_starts(a.g, (uint32_t)row, a.o, at);
     const S *x = reinterpret_cast<const S *>(a.o[LN_X].base) + at[LN_X];
     S *out = reinterpret_cast<S *>(const_cast<char *>(a.o[LN_OUT].base)) + at[LN_OUT];
-    Vec<S, V> raw[NV];
+    Words raw[NV];
 #pragma unroll
-    for (int v = 0; v < NV; v++)
-      if (v * G + lane < nvec) raw[v] = load_part<V, RAGGED>(x, v * G + lane, n, S{});
+    for (int v = 0; v < NV; v++) raw[v] = load_part<R>(x, c[v], n);
     C t[NV][V], s[1] = {0};
 #pragma unroll
-    for (int v = 0; v < NV; v++)
+    for (int v = 0; v < NV; v++) {
+      IO::widen(raw[v], t[v]);
       if (v * G + lane < nvec)
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-          t[v][j] = TX::ld(raw[v].v[j]);
-          s[0] = s[0] + t[v][j];  // (what is past the row's end was read as zero)
-        }
+        for (int j = 0; j < V; j++) s[0] = s[0] + (owns(v, j) ? t[v][j] : 0);
+    }
     group_combine<G>(s, Sum<C>{}, lds);
     const C mean = s[0] / count;
     s[0] = 0;
 #pragma unroll
-    for (int v = 0; v < NV; v++)
+    for (int v = 0; v < NV; v++) {
+#pragma unroll
+      for (int j = 0; j < V; j++) t[v][j] = t[v][j] - mean;
       if (v * G + lane < nvec)
 #pragma unroll
         for (int j = 0; j < V; j++) {
-          t[v][j] = t[v][j] - mean;
-          if (RAGGED && (v * G + lane) * V + j >= n) t[v][j] = 0;
-          s[0] = fused(t[v][j], t[v][j], s[0]);
+          const C own = owns(v, j) ? t[v][j] : 0;
+          s[0] = fused(own, own, s[0]);
         }
+    }
     group_combine<G>(s, Sum<C>{}, lds);
     const C rstd = reciprocal_root(s[0] / count + eps);
     if (lane == 0) {
@@ -80,19 +86,14 @@ __global__ __launch_bounds__(ln_threads(G)) void layer_norm_kernel(LayerNormArgs
       if (a.o[LN_RSTD].base) reinterpret_cast<C *>(const_cast<char *>(a.o[LN_RSTD].base))[at[LN_RSTD]] = rstd;
     }
 #pragma unroll
-    for (int v = 0; v < NV; v++)
-      if (v * G + lane < nvec) {
-        Vec<S, V> o;
+    for (int v = 0; v < NV; v++) {
+      C w[V], b[V];
+      IO::widen(gv[v], w);
+      IO::widen(bv[v], b);
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-          C y = t[v][j] * rstd;
-          if (gamma && beta) y = fused(y, TX::ld(gv[v].v[j]), TX::ld(bv[v].v[j]));
-          else if (gamma) y = y * TX::ld(gv[v].v[j]);
-          else if (beta) y = y + TX::ld(bv[v].v[j]);
-          o.v[j] = TX::st(y);
-        }
-        store_part<V, RAGGED>(out, v * G + lane, n, o);
-      }
+      for (int j = 0; j < V; j++) t[v][j] = fused(t[v][j] * rstd, w[j], b[j]);
+      if (v * G + lane < nvec) store_part<R>(out, c[v], n, IO::narrow(t[v]));
+    }
   }
 }
 
@@ -100,10 +101,10 @@ __global__ __launch_bounds__(ln_threads(G)) void layer_norm_kernel(LayerNormArgs
 constexpr int LONG_THREADS = 1024;
 template <int DT>
 __global__ __launch_bounds__(LONG_THREADS) void layer_norm_long_kernel(LayerNormArgs a) {
-  using TX = Tr<DT>;
-  using C = typename TX::C;
-  using S = typename TX::S;
-  constexpr int V = VECTOR<S>;
+  using IO = Io<DT>;
+  using C = typename IO::C;
+  using S = typename IO::S;
+  constexpr int V = IO::V;
   __shared__ C lds[LONG_THREADS / 64];
   const int n = a.g.n, nvec = (n + V - 1) / V;
   const S *gamma = reinterpret_cast<const S *>(a.gamma), *beta = reinterpret_cast<const S *>(a.beta);
@@ -113,21 +114,21 @@ __global__ __launch_bounds__(LONG_THREADS) void layer_norm_long_kernel(LayerNorm
     row_starts(a.g, (uint32_t)row, a.o, at);
     const S *x = reinterpret_cast<const S *>(a.o[LN_X].base) + at[LN_X];
     S *out = reinterpret_cast<S *>(const_cast<char *>(a.o[LN_OUT].base)) + at[LN_OUT];
-    C s[1] = {0};
+    C s[1] = {0}, t[V];
     for (int c = threadIdx.x; c < nvec; c += LONG_THREADS) {
-      const Vec<S, V> raw = load_part<V, true>(x, c, n, S{});
+      IO::widen(load_part<RAGGED>(x, c, n), t);
 #pragma unroll
-      for (int j = 0; j < V; j++) s[0] = s[0] + TX::ld(raw.v[j]);
+      for (int j = 0; j < V; j++) s[0] = s[0] + (vec_owns<V, RAGGED>(c, j, n) ? t[j] : 0);
     }
     group_combine<LONG_THREADS>(s, Sum<C>{}, lds);
     const C mean = s[0] / count;
     s[0] = 0;
     for (int c = threadIdx.x; c < nvec; c += LONG_THREADS) {
-      const Vec<S, V> raw = load_part<V, true>(x, c, n, S{});
+      IO::widen(load_part<RAGGED>(x, c, n), t);
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        const C t = c * V + j < n ? TX::ld(raw.v[j]) - mean : 0;
-        s[0] = fused(t, t, s[0]);
+        const C own = vec_owns<V, RAGGED>(c, j, n) ? t[j] - mean : 0;
+        s[0] = fused(own, own, s[0]);
       }
     }
     group_combine<LONG_THREADS>(s, Sum<C>{}, lds);
@@ -137,34 +138,28 @@ __global__ __launch_bounds__(LONG_THREADS) void layer_norm_long_kernel(LayerNorm
       if (a.o[LN_RSTD].base) reinterpret_cast<C *>(const_cast<char *>(a.o[LN_RSTD].base))[at[LN_RSTD]] = rstd;
     }
     for (int c = threadIdx.x; c < nvec; c += LONG_THREADS) {
-      const Vec<S, V> raw = load_part<V, true>(x, c, n, S{});
-      Vec<S, V> gv, bv, o;
-      if (gamma) gv = load_part<V, true>(gamma, c, n, S{});
-      if (beta) bv = load_part<V, true>(beta, c, n, S{});
+      C w[V], b[V];
+      IO::widen(load_part<RAGGED>(x, c, n), t);
+      IO::widen(gamma ? load_part<RAGGED>(gamma, c, n) : IO::all(1), w);
+      IO::widen(beta ? load_part<RAGGED>(beta, c, n) : IO::all(0), b);
 #pragma unroll
-      for (int j = 0; j < V; j++) {
-        C y = (TX::ld(raw.v[j]) - mean) * rstd;
-        if (gamma && beta) y = fused(y, TX::ld(gv.v[j]), TX::ld(bv.v[j]));
-        else if (gamma) y = y * TX::ld(gv.v[j]);
-        else if (beta) y = y + TX::ld(bv.v[j]);
-        o.v[j] = TX::st(y);
-      }
-      store_part<V, true>(out, c, n, o);
+      for (int j = 0; j < V; j++) t[j] = fused((t[j] - mean) * rstd, w[j], b[j]);
+      store_own(out, c, n, IO::narrow(t));
     }
   }
 }
 
 template <int DT, int G, int NV>
 void launch(nxh_context *ctx, const LayerNormArgs &a) {
-  constexpr int V = VECTOR<typename Tr<DT>::S>, GROUPS = ln_threads(G) / G;
+  constexpr int V = Io<DT>::V, GROUPS = ln_threads(G) / G;
   const int64_t most = (int64_t)(ctx->compute_units > 0 ? ctx->compute_units : 256) * (2048 / ln_threads(G));
   const dim3 grid((unsigned)std::min<int64_t>((a.g.rows + GROUPS - 1) / GROUPS, most));
-  if (a.g.n % V == 0) hipLaunchKernelGGL((layer_norm_kernel<DT, G, NV, false>), grid, dim3(ln_threads(G)), 0, ctx->stream, a);
-  else hipLaunchKernelGGL((layer_norm_kernel<DT, G, NV, true>), grid, dim3(ln_threads(G)), 0, ctx->stream, a);
+  if (a.g.n % V == 0) hipLaunchKernelGGL((layer_norm_kernel<DT, G, NV, WHOLE>), grid, dim3(ln_threads(G)), 0, ctx->stream, a);
+  else hipLaunchKernelGGL((layer_norm_kernel<DT, G, NV, G * NV == 1 ? SHORT : RAGGED>), grid, dim3(ln_threads(G)), 0, ctx->stream, a);
 }
 template <int DT>
 void launch_rows(nxh_context *ctx, const LayerNormArgs &a) {
-  constexpr int V = VECTOR<typename Tr<DT>::S>;
+  constexpr int V = Io<DT>::V;
   const int nvec = (a.g.n + V - 1) / V;
 #define X(G, NV) \
   if (nvec <= G * NV) return launch<DT, G, NV>(ctx, a);

@@ -36,23 +36,29 @@ __device__ __forceinline__ C across_groups(C v) {
   return v;
 }
 
-template <int DT, int G, int NV, bool RAGGED>
+template <int DT, int G, int NV, Rows R>
 __global__ __launch_bounds__(ln_threads(G)) void layer_norm_grad_kernel(LayerNormGradArgs a) {
-  using TX = Tr<DT>;
-  using C = typename TX::C;
-  using S = typename TX::S;
-  constexpr int V = VECTOR<S>, T = ln_threads(G), GROUPS = T / G, W = T / 64;
+  using IO = Io<DT>;
+  using C = typename IO::C;
+  using S = typename IO::S;
+  constexpr int V = IO::V, T = ln_threads(G), GROUPS = T / G, W = T / 64;
   __shared__ C lds[G > 64 ? 2 * (G / 64) : 2 * W * G * V];
   const int lane = threadIdx.x % G, n = a.g.n, nvec = (n + V - 1) / V;
   const S *gamma = reinterpret_cast<const S *>(a.gamma);
-  Vec<S, V> gv[NV], xr[NV], gr[NV];
+  // Every lane loads for every v, a vector past the row as the row's last: a load under a condition is waited for before the next one.
+  int c[NV];
+  Words gv[NV], xr[NV], gr[NV];
   C dgamma[NV][V], dbeta[NV][V];
 #pragma unroll
   for (int v = 0; v < NV; v++) {
-    if (v * G + lane < nvec && gamma) gv[v] = load_part<V, RAGGED>(gamma, v * G + lane, n, S{});
+    c[v] = v * G + lane < nvec ? v * G + lane : nvec - 1;
+    gv[v] = gamma ? load_part<R>(gamma, c[v], n) : IO::all(1);
 #pragma unroll
     for (int j = 0; j < V; j++) dgamma[v][j] = dbeta[v][j] = 0;
   }
+  // Whether this lane's vector v has element j for itself. Only the row's last vector may not: which v that is is the same for all lanes.
+  const int last = (nvec - 1) / G;
+  auto owns = [&](int v, int j) { return R == WHOLE || v != last || vec_owns<V, R>(c[v], j, n); };
   const C count = (C)n;
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G, at[LG_OPERANDS];
@@ -64,11 +70,10 @@ __global__ __launch_bounds__(ln_threads(G)) void layer_norm_grad_kernel(LayerNor
     mean = reinterpret_cast<const C *>(a.o[LG_MEAN].base)[at[LG_MEAN]];
     rstd = reinterpret_cast<const C *>(a.o[LG_RSTD].base)[at[LG_RSTD]];
 #pragma unroll
-    for (int v = 0; v < NV; v++)
-      if (v * G + lane < nvec) {
-        xr[v] = load_part<V, RAGGED>(x, v * G + lane, n, S{});
-        gr[v] = load_part<V, RAGGED>(g, v * G + lane, n, S{});
-      }
+    for (int v = 0; v < NV; v++) {
+      xr[v] = load_part<R>(x, c[v], n);
+      gr[v] = load_part<R>(g, c[v], n);
+    }
   };
   if (row < a.g.rows) request(row);
   for (; row < a.g.rows; row += step) {
@@ -76,32 +81,38 @@ __global__ __launch_bounds__(ln_threads(G)) void layer_norm_grad_kernel(LayerNor
     const C mu = mean, rs = rstd;
     C h[NV][V], w[NV][V], s[2] = {0, 0};
 #pragma unroll
-    for (int v = 0; v < NV; v++)
+    for (int v = 0; v < NV; v++) {
+      C x[V], g[V], gain[V];
+      IO::widen(xr[v], x);
+      IO::widen(gr[v], g);
+      IO::widen(gv[v], gain);
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        h[v][j] = (x[j] - mu) * rs;
+        w[v][j] = g[j] * gain[j];
+        dgamma[v][j] = fused(g[j], h[v][j], dgamma[v][j]);  // (of a lane with no vector v: never looked at)
+        dbeta[v][j] = dbeta[v][j] + g[j];
+      }
       if (v * G + lane < nvec)
 #pragma unroll
         for (int j = 0; j < V; j++) {
-          // (past the row's end g was read as zero, which keeps the element out of every sum: h is finite wherever the row is)
-          const C gj = TX::ld(gr[v].v[j]);
-          h[v][j] = (TX::ld(xr[v].v[j]) - mu) * rs;
-          if (RAGGED && (v * G + lane) * V + j >= n) h[v][j] = 0;
-          w[v][j] = gamma ? gj * TX::ld(gv[v].v[j]) : gj;
-          s[0] = s[0] + w[v][j];
-          s[1] = fused(w[v][j], h[v][j], s[1]);
-          dgamma[v][j] = fused(gj, h[v][j], dgamma[v][j]);
-          dbeta[v][j] = dbeta[v][j] + gj;
+          const bool own = owns(v, j);
+          s[0] = s[0] + (own ? w[v][j] : 0);
+          s[1] = fused(own ? w[v][j] : 0, own ? h[v][j] : 0, s[1]);
         }
-    if (row + step < a.g.rows) request(row + step);  // in flight while this row is finished
+    }
+    const int64_t next = row + step < a.g.rows ? row + step : row;  // (a last row is requested twice: no condition here either)
+    request(next);  // in flight while this row is finished
     group_combine<G>(s, Sum<C>{}, lds);
     if (a.o[LG_DX].base) {
       const C c1 = s[0] / count, c2 = s[1] / count;
 #pragma unroll
-      for (int v = 0; v < NV; v++)
-        if (v * G + lane < nvec) {
-          Vec<S, V> o;
+      for (int v = 0; v < NV; v++) {
+        C d[V];
 #pragma unroll
-          for (int j = 0; j < V; j++) o.v[j] = TX::st(rs * fused(-h[v][j], c2, w[v][j] - c1));
-          store_part<V, RAGGED>(dx, v * G + lane, n, o);
-        }
+        for (int j = 0; j < V; j++) d[j] = rs * fused(-h[v][j], c2, w[v][j] - c1);
+        if (v * G + lane < nvec) store_part<R>(dx, c[v], n, IO::narrow(d));
+      }
     }
   }
   if (!a.partials) return;
@@ -111,10 +122,10 @@ __global__ __launch_bounds__(ln_threads(G)) void layer_norm_grad_kernel(LayerNor
     for (int v = 0; v < NV; v++)
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        const int c = (v * G + lane) * V + j;
-        if (c < n) {
-          mine[c] = dgamma[v][j];
-          mine[n + c] = dbeta[v][j];
+        const int c = v * G + lane, column = vec_start<V, R>(c, n) + j;
+        if (c < nvec && vec_owns<V, R>(c, j, n)) {
+          mine[column] = dgamma[v][j];
+          mine[n + column] = dbeta[v][j];
         }
       }
   } else {
@@ -135,8 +146,8 @@ __global__ __launch_bounds__(ln_threads(G)) void layer_norm_grad_kernel(LayerNor
         C s = lds[e];
 #pragma unroll
         for (int k = 1; k < W; k++) s = s + lds[k * 2 * G * V + e];
-        const int c = v * G * V + e % (G * V);
-        if (c < n) mine[(e / (G * V)) * n + c] = s;
+        const int c = v * G + e % (G * V) / V, j = e % V;
+        if (c < nvec && vec_owns<V, R>(c, j, n)) mine[(e / (G * V)) * n + vec_start<V, R>(c, n) + j] = s;
       }
     }
   }
@@ -148,10 +159,10 @@ __global__ __launch_bounds__(ln_threads(G)) void layer_norm_grad_kernel(LayerNor
 constexpr int LONG_THREADS = 1024;
 template <int DT>
 __global__ __launch_bounds__(LONG_THREADS) void layer_norm_grad_long_kernel(LayerNormGradArgs a) {
-  using TX = Tr<DT>;
-  using C = typename TX::C;
-  using S = typename TX::S;
-  constexpr int V = VECTOR<S>;
+  using IO = Io<DT>;
+  using C = typename IO::C;
+  using S = typename IO::S;
+  constexpr int V = IO::V;
   __shared__ C lds[2 * (LONG_THREADS / 64)];
   const int n = a.g.n, nvec = (n + V - 1) / V;
   const S *gamma = reinterpret_cast<const S *>(a.gamma);
@@ -167,41 +178,42 @@ __global__ __launch_bounds__(LONG_THREADS) void layer_norm_grad_long_kernel(Laye
     C s[2] = {0, 0};
     auto walk = [&](auto &&body) {
       for (int c = threadIdx.x; c < nvec; c += LONG_THREADS) {
-        const Vec<S, V> xv = load_part<V, true>(x, c, n, S{}), gv = load_part<V, true>(g, c, n, S{});
-        Vec<S, V> wv;
-        if (gamma) wv = load_part<V, true>(gamma, c, n, S{});
-        C h[V], w[V];
+        C h[V], w[V], gain[V];
+        IO::widen(load_part<RAGGED>(x, c, n), h);
+        IO::widen(load_part<RAGGED>(g, c, n), w);
+        IO::widen(gamma ? load_part<RAGGED>(gamma, c, n) : IO::all(1), gain);
 #pragma unroll
         for (int j = 0; j < V; j++) {
-          h[j] = c * V + j < n ? (TX::ld(xv.v[j]) - mu) * rs : 0;
-          w[j] = gamma ? TX::ld(gv.v[j]) * TX::ld(wv.v[j]) : TX::ld(gv.v[j]);
+          h[j] = (h[j] - mu) * rs;
+          w[j] = w[j] * gain[j];
         }
         body(c, h, w);
       }
     };
-    walk([&](int, const C *h, const C *w) {
+    walk([&](int c, const C *h, const C *w) {
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        s[0] = s[0] + w[j];
-        s[1] = fused(w[j], h[j], s[1]);
+        const bool own = vec_owns<V, RAGGED>(c, j, n);
+        s[0] = s[0] + (own ? w[j] : 0);
+        s[1] = fused(own ? w[j] : 0, own ? h[j] : 0, s[1]);
       }
     });
     group_combine<LONG_THREADS>(s, Sum<C>{}, lds);
     const C c1 = s[0] / count, c2 = s[1] / count;
     walk([&](int c, const C *h, const C *w) {
-      Vec<S, V> o;
+      C d[V];
 #pragma unroll
-      for (int j = 0; j < V; j++) o.v[j] = TX::st(rs * fused(-h[j], c2, w[j] - c1));
-      store_part<V, true>(dx, c, n, o);
+      for (int j = 0; j < V; j++) d[j] = rs * fused(-h[j], c2, w[j] - c1);
+      store_own(dx, c, n, IO::narrow(d));
     });
   }
 }
 template <int DT>
 __global__ __launch_bounds__(256) void layer_norm_columns_kernel(LayerNormGradArgs a, int64_t share) {
-  using TX = Tr<DT>;
-  using C = typename TX::C;
-  using S = typename TX::S;
-  constexpr int V = VECTOR<S>;
+  using IO = Io<DT>;
+  using C = typename IO::C;
+  using S = typename IO::S;
+  constexpr int V = IO::V;
   const int n = a.g.n, c = blockIdx.x * 256 + threadIdx.x;
   if ((int64_t)c * V >= n) return;
   C dgamma[V], dbeta[V];
@@ -212,23 +224,23 @@ __global__ __launch_bounds__(256) void layer_norm_columns_kernel(LayerNormGradAr
   for (int64_t row = first; row < end; row++) {
     int64_t at[LG_OPERANDS];
     row_starts(a.g, (uint32_t)row, a.o, at);
-    const Vec<S, V> xv = load_part<V, true>(reinterpret_cast<const S *>(a.o[LG_X].base) + at[LG_X], c, n, S{});
-    const Vec<S, V> gv = load_part<V, true>(reinterpret_cast<const S *>(a.o[LG_G].base) + at[LG_G], c, n, S{});
+    C x[V], g[V];
+    IO::widen(load_part<RAGGED>(reinterpret_cast<const S *>(a.o[LG_X].base) + at[LG_X], c, n), x);
+    IO::widen(load_part<RAGGED>(reinterpret_cast<const S *>(a.o[LG_G].base) + at[LG_G], c, n), g);
     const C mu = reinterpret_cast<const C *>(a.o[LG_MEAN].base)[at[LG_MEAN]];
     const C rs = reinterpret_cast<const C *>(a.o[LG_RSTD].base)[at[LG_RSTD]];
 #pragma unroll
     for (int j = 0; j < V; j++) {
-      const C gj = TX::ld(gv.v[j]);
-      dgamma[j] = fused(gj, (TX::ld(xv.v[j]) - mu) * rs, dgamma[j]);
-      dbeta[j] = dbeta[j] + gj;
+      dgamma[j] = fused(g[j], (x[j] - mu) * rs, dgamma[j]);
+      dbeta[j] = dbeta[j] + g[j];
     }
   }
   C *mine = reinterpret_cast<C *>(a.partials) + (int64_t)blockIdx.y * 2 * n;
 #pragma unroll
   for (int j = 0; j < V; j++)
-    if (c * V + j < n) {
-      mine[c * V + j] = dgamma[j];
-      mine[n + c * V + j] = dbeta[j];
+    if (vec_owns<V, RAGGED>(c, j, n)) {
+      mine[vec_start<V, RAGGED>(c, n) + j] = dgamma[j];
+      mine[n + vec_start<V, RAGGED>(c, n) + j] = dbeta[j];
     }
 }
 
@@ -243,9 +255,9 @@ struct JoinArgs {
 };
 template <int DT>
 __global__ __launch_bounds__(1024) void layer_norm_join_kernel(JoinArgs a) {
-  using TX = Tr<DT>;
-  using C = typename TX::C;
-  using S = typename TX::S;
+  using IO = Io<DT>;
+  using C = typename IO::C;
+  using S = typename IO::S;
   __shared__ C lds[32][33];
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
   const int64_t column = (int64_t)blockIdx.x * 32 + lane;
@@ -262,7 +274,7 @@ __global__ __launch_bounds__(1024) void layer_norm_join_kernel(JoinArgs a) {
   const int which = column >= a.n;
   char *out = which ? a.out[1] : a.out[0];
   const int64_t stride = which ? a.stride[1] : a.stride[0];
-  if (out) reinterpret_cast<S *>(out)[(column - (which ? a.n : 0)) * stride] = TX::st(s);
+  if (out) reinterpret_cast<S *>(out)[(column - (which ? a.n : 0)) * stride] = IO::st(s);
 }
 
 // ── host side ───────────────────────────────────────────────────────────────
@@ -272,14 +284,14 @@ struct Plan {
 };
 template <int DT, int G, int NV>
 void launch(nxh_context *ctx, const LayerNormGradArgs &a, int64_t blocks) {
-  constexpr int V = VECTOR<typename Tr<DT>::S>;
+  constexpr int V = Io<DT>::V;
   const dim3 grid((unsigned)blocks);
-  if (a.g.n % V == 0) hipLaunchKernelGGL((layer_norm_grad_kernel<DT, G, NV, false>), grid, dim3(ln_threads(G)), 0, ctx->stream, a);
-  else hipLaunchKernelGGL((layer_norm_grad_kernel<DT, G, NV, true>), grid, dim3(ln_threads(G)), 0, ctx->stream, a);
+  if (a.g.n % V == 0) hipLaunchKernelGGL((layer_norm_grad_kernel<DT, G, NV, WHOLE>), grid, dim3(ln_threads(G)), 0, ctx->stream, a);
+  else hipLaunchKernelGGL((layer_norm_grad_kernel<DT, G, NV, G * NV == 1 ? SHORT : RAGGED>), grid, dim3(ln_threads(G)), 0, ctx->stream, a);
 }
 template <int DT>
 void launch_long(nxh_context *ctx, const LayerNormGradArgs &a, int64_t blocks) {
-  constexpr int V = VECTOR<typename Tr<DT>::S>;
+  constexpr int V = Io<DT>::V;
   const int64_t units = ctx->compute_units > 0 ? ctx->compute_units : 256;
   if (a.partials) {  // before dx, which may go where g or x is
     const dim3 grid((unsigned)(((a.g.n + V - 1) / V + 255) / 256), (unsigned)blocks);
@@ -290,7 +302,7 @@ void launch_long(nxh_context *ctx, const LayerNormGradArgs &a, int64_t blocks) {
 }
 template <int DT>
 Plan plan(nxh_context *ctx, int n, int64_t rows) {
-  constexpr int V = VECTOR<typename Tr<DT>::S>;
+  constexpr int V = Io<DT>::V;
   const int64_t units = ctx->compute_units > 0 ? ctx->compute_units : 256;
   const int nvec = (n + V - 1) / V;
 #define X(G, NV)                                                                                                \

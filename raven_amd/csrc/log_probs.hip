@@ -12,13 +12,16 @@
 // have terms of one sign, so nothing cancels, and peak and total are given out apart: x - peak is exact
 // near the peak, where x - log(sum e^x) would round to the step of the logarithm. Memory bounds it: the
 // logits once; the gradient once more in and out.
+//
+// Exponentials are powers of two: with L = log2 e and the reference A = peak L as it rounds, 2^(x L - A) is one
+// fused step and one instruction. What A lost in rounding, r = peak L - A, is a factor 2^r of every term: the
+// sums are freed of it at the end, a quotient of two terms never has it.
 
 #include <type_traits>
 #include <utility>
 
 #include "lane_groups.hpp"
 #include "rows.hpp"
-#include "softmax_math.hpp"
 
 namespace {
 
@@ -37,110 +40,160 @@ __device__ __forceinline__ T *place(const LogProbsArgs &a, const Places &p, int 
   return reinterpret_cast<T *>(const_cast<char *>(a.o[k].base)) + p.at[k];
 }
 
-// e^x for x <= 0. The statistics of 16-bit logits take the hardware's exponential alone: its error, and that of the product
-// in front of it, are some 2^-22 of a term, and no term of the gradient keeps more than 11 bits. float32 logits have both corrected.
-template <int DT>
-struct Exp {
-  __device__ __forceinline__ static float of(float x) { return __builtin_amdgcn_exp2f(x * 0x1.715476p+0f); }
+template <class C> struct Bounds;
+// wide: rows whose largest element is no further from zero have an r below 1 and sums that cannot overflow; others are walked by
+// differences (of finite values near the dtype's ends, or with infinities). low: the least reference, which a lane of
+// lesser elements takes: beside a row's largest they count for nothing. none: 2^none is 0.
+template <> struct Bounds<float> {
+  static constexpr float wide = 0x1p20f, low = -0x1p21f, none = -300.0f, inf = __builtin_inff(), L = 0x1.715476p+0f, ln2 = 0x1.62e43p-1f;
 };
-template <>
-struct Exp<NXH_F32> {
-  __device__ __forceinline__ static float of(float x) { return exp_nonpositive(x); }
+template <> struct Bounds<double> {
+  static constexpr double wide = 0x1p20, low = -0x1p21, none = -2000.0, inf = __builtin_inf(), L = 0x1.71547652b82fep+0, ln2 = 0x1.62e42fefa39efp-1;
 };
-template <>
-struct Exp<NXH_F64> {
-  __device__ __forceinline__ static double of(double x) { return exp(x); }
-};
+__device__ __forceinline__ float power(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ double power(double x) { return exp2(x); }
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_fmaxf(a, b); }  // (a NaN is passed over: the sums have it)
 __device__ __forceinline__ double larger(double a, double b) { return __builtin_fmax(a, b); }
 template <class C>
 struct Larger {
   __device__ __forceinline__ C operator()(C a, C b) const { return larger(a, b); }
 };
-// The lowest finite value, which a lane starts from (differences with it are no NaN), and a difference whose exponential is 0.
-template <class C> struct Bounds;
-template <> struct Bounds<float> { static constexpr float lowest = -0x1.fffffep+127f, far = -200.0f, inf = __builtin_inff(); };
-template <> struct Bounds<double> { static constexpr double lowest = -0x1.fffffffffffffp+1023, far = -2000.0, inf = __builtin_inf(); };
+template <class C>
+__device__ __forceinline__ C reference(C peak) { return larger(peak * Bounds<C>::L, Bounds<C>::low); }
+// Whether a row with this largest element is walked by its reference.
+template <class C>
+__device__ __forceinline__ bool is_near(C peak) { return __builtin_fabs(peak) <= Bounds<C>::wide; }
+
+// body(vector number, vector) over the vectors of a row that a lane has: numbers lane, lane + G, ..., U of them
+// requested before the first is looked at (past the row the last one again: a load under a condition is waited for
+// before the next); then tail(index) for the elements behind the last whole vector, one to a lane.
+template <int G, int U, class S, class B, class E>
+__device__ __forceinline__ void walk(const S *x, int n, int lane, B &&body, E &&tail) {
+  constexpr int V = VECTOR<S>;
+  const int nvec = n / V;
+  for (int c = lane; c < nvec; c += U * G) {
+    Words raw[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) raw[u] = load_words(x + (int64_t)(c + u * G < nvec ? c + u * G : nvec - 1) * V);
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (c + u * G < nvec) body(c + u * G, raw[u]);
+  }
+  if (nvec * V + lane < n) tail(nvec * V + lane);
+}
 
 template <class C>
 struct Statistics {
   C peak, total, log_total, entropy;
 };
 
-// What a lane has seen of its row.
+// What a lane has seen of its row: the largest element, and against the reference a = reference(m) the sums
+// s = sum 2^(x L - a) and t = sum 2^(x L - a) (x L - a).
 template <int DT>
 struct Running {
-  using TX = Tr<DT>;
-  using C = typename TX::C;
-  using S = typename TX::S;
-  C m = Bounds<C>::lowest, s = 0, t = 0;
-  C seen = -Bounds<C>::inf;  // the largest element, which m is not where all are -inf
-  template <int W>
-  __device__ __forceinline__ void take(const Vec<S, W> &raw) {
-    C x[W], top = TX::ld(raw.v[0]);
-    x[0] = top;
+  using IO = Io<DT>;
+  using C = typename IO::C;
+  using S = typename IO::S;
+  C m = -Bounds<C>::inf, a = Bounds<C>::low, s = 0, t = 0;
+  template <int N>
+  __device__ __forceinline__ void take(const C (&x)[N]) {
+    C top = x[0];
 #pragma unroll
-    for (int j = 1; j < W; j++) {
-      x[j] = TX::ld(raw.v[j]);
-      top = larger(top, x[j]);
-    }
-    seen = larger(seen, top);
+    for (int j = 1; j < N; j++) top = larger(top, x[j]);
     raise(larger(m, top));
 #pragma unroll
-    for (int j = 0; j < W; j++) {
-      const C d = x[j] - m, p = Exp<DT>::of(d);
+    for (int j = 0; j < N; j++) {
+      const C d = fused(x[j], Bounds<C>::L, -a), p = power(d);
       s = s + p;
-      t = fused(p, larger(d, Bounds<C>::far), t);  // (0 for -inf, not 0 * -inf)
+      t = fused(p, larger(d, Bounds<C>::none), t);  // (0 for -inf, not 0 * -inf)
     }
   }
-  // the sums against another peak, no lower than m
   __device__ __forceinline__ void raise(C peak) {
-    const C d = larger(m - peak, Bounds<C>::far), k = Exp<DT>::of(d);
+    const C to = reference(peak), d = larger(a - to, Bounds<C>::none), k = power(d);
     t = fused(s, d, t) * k;
     s = s * k;
     m = peak;
+    a = to;
+  }
+  __device__ __forceinline__ void take(Words raw) {
+    C x[IO::V];
+    IO::widen(raw, x);
+    take(x);
+  }
+  __device__ __forceinline__ void take_one(S raw) {
+    const C x[1] = {IO::ld(raw)};
+    take(x);
+  }
+  // joined with the other lanes of a group of N
+  template <int N>
+  __device__ __forceinline__ void join() {
+    raise(lanes_combine<N>(m, Larger<C>{}));
+    s = lanes_combine<N>(s, Sum<C>{});
+    t = lanes_combine<N>(t, Sum<C>{});
   }
 };
 
-// body(vector number) over the vectors of a row that a lane has: numbers lane, lane + G, ... four requested before the first is
-// looked at; then tail(index) for the single elements behind the last whole vector, one to a lane.
-template <int V, int G, class S, class B, class E>
-__device__ __forceinline__ void walk(const S *x, int n, int lane, B &&body, E &&tail) {
-  constexpr int U = 4;
-  const int nvec = n / V;
-  int c = lane;
-  for (; c + (U - 1) * G < nvec; c += U * G) {
-    Vec<S, V> raw[U];
+// The statistics of a row by differences with its largest element, which is given: for rows that are not near.
+template <int DT, int G>
+__device__ __forceinline__ Statistics<typename Tr<DT>::C> far_statistics(const typename Tr<DT>::S *x, int n, int lane, typename Tr<DT>::C peak,
+                                                                         typename Tr<DT>::C *lds) {
+  using IO = Io<DT>;
+  using C = typename IO::C;
+  C sums[2] = {0, 0};
+  auto take = [&](C v) {
+    const C d = v - peak, p = power(d * Bounds<C>::L);
+    sums[0] = sums[0] + p;
+    sums[1] = fused(p, larger(d, Bounds<C>::none), sums[1]);
+  };
+  walk<G, 1>(x, n, lane,
+             [&](int, Words raw) {
+               C v[IO::V];
+               IO::widen(raw, v);
 #pragma unroll
-    for (int u = 0; u < U; u++) raw[u] = load_vec<V>(x + (int64_t)(c + u * G) * V);
-#pragma unroll
-    for (int u = 0; u < U; u++) body(c + u * G, raw[u]);
-  }
-  for (; c < nvec; c += G) body(c, load_vec<V>(x + (int64_t)c * V));
-  if (nvec * V + lane < n) tail(nvec * V + lane);
+               for (int j = 0; j < IO::V; j++) take(v[j]);
+             },
+             [&](int i) { take(IO::ld(x[i])); });
+  group_combine<G>(sums, Sum<C>{}, lds);  // (NaN, from -inf - -inf, where every logit is -inf: there is no distribution)
+  const C log_total = log(sums[0]);
+  return {peak, sums[0], log_total, log_total - sums[1] / sums[0]};
 }
 
-template <int DT, int G>
-__device__ __forceinline__ Statistics<typename Tr<DT>::C> statistics(const typename Tr<DT>::S *x, int n, int lane, typename Tr<DT>::C *lds,
-                                                                     typename Tr<DT>::C &seen) {
+// Shared memory of a group of several waves: the waves' triples, twice, so that one barrier a row will do; sums of rows that are not near.
+template <class C, int G>
+struct Space {
+  C wave[2][G > 64 ? 3 * (G / 64) : 1], sums[G > 64 ? 2 * (G / 64) : 1];
+};
+// The statistics of a row. turn: 0 and 1 from one row of the block to the next; seen(largest element of the lane's own) is called
+// between the walk and the barrier.
+template <int DT, int G, int U, class F>
+__device__ __forceinline__ Statistics<typename Tr<DT>::C> statistics(const typename Tr<DT>::S *x, int n, int lane, int turn,
+                                                                     Space<typename Tr<DT>::C, G> &l, F &&seen) {
   using C = typename Tr<DT>::C;
-  using S = typename Tr<DT>::S;
   Running<DT> r;
-  walk<VECTOR<S>, G>(x, n, lane, [&](int, const Vec<S, VECTOR<S>> &raw) { r.take(raw); }, [&](int i) { r.take(load_vec<1>(x + i)); });
-  seen = r.seen;
-  C m[1] = {r.m};
-  group_combine<G>(m, Larger<C>{}, lds);
-  r.raise(m[0]);
-  C sums[2] = {r.s, r.t};
-  group_combine<G>(sums, Sum<C>{}, lds);
-  Statistics<C> z{m[0], sums[0], 0, 0};
-  if (z.total == 0) {  // every logit is -inf: there is no distribution
-    z.peak = -Bounds<C>::inf;
-    z.total = __builtin_nan("");
+  walk<G, U>(x, n, lane, [&](int, Words raw) { r.take(raw); }, [&](int i) { r.take_one(x[i]); });
+  seen(r.m);
+  r.template join<(G < 64 ? G : 64)>();
+  if constexpr (G > 64) {
+    constexpr int W = G / 64;
+    C *w = l.wave[turn];
+    if ((lane & 63) == 0) {
+      w[lane >> 6] = r.m;
+      w[W + (lane >> 6)] = r.s;
+      w[2 * W + (lane >> 6)] = r.t;
+    }
+    __syncthreads();
+    r.m = w[lane % W];
+    r.a = reference(r.m);
+    r.s = w[W + lane % W];
+    r.t = w[2 * W + lane % W];
+    r.template join<W>();
   }
-  z.log_total = log(z.total);
-  z.entropy = z.log_total - sums[1] / z.total;
-  return z;
+  if (!is_near(r.m)) return far_statistics<DT, G>(x, n, lane, r.m, l.sums);
+  const C lost = fused(r.m, Bounds<C>::L, -r.a);
+  C total = r.s * power(-lost);
+  total = total < 1 ? 1 : total;  // (the peak's own term is 1)
+  const C log_total = log(total), entropy = log_total - Bounds<C>::ln2 * (r.t / r.s - lost);
+  return {r.m, total, log_total, entropy < 0 ? 0 : entropy};
 }
 
 // The log probability of a row's token: one below zero is padding, one past the row names nothing.
@@ -149,7 +202,7 @@ __device__ __forceinline__ typename Tr<DT>::C token_log_p(const typename Tr<DT>:
   using C = typename Tr<DT>::C;
   if (token < 0) return 0;
   if (token >= n) return (C)__builtin_nan("");
-  return Tr<DT>::ld(x[token]) - z.peak - z.log_total;
+  return Io<DT>::ld(x[token]) - z.peak - z.log_total;
 }
 template <int DT>
 __device__ __forceinline__ void give_statistics(const LogProbsArgs &a, const Places &p, const typename Tr<DT>::S *x,
@@ -162,20 +215,21 @@ __device__ __forceinline__ void give_statistics(const LogProbsArgs &a, const Pla
 }
 
 constexpr int group_threads(int g) { return g > 256 ? g : 256; }
+constexpr int AHEAD = 4;  // vectors that a lane requests at once
 
 template <int DT, int G>
 __global__ __launch_bounds__(group_threads(G)) void log_probs_kernel(LogProbsArgs a) {
   using C = typename Tr<DT>::C;
   using S = typename Tr<DT>::S;
   constexpr int GROUPS = group_threads(G) / G;
-  __shared__ C lds[G > 64 ? 2 * (G / 64) : 1];
+  __shared__ Space<C, G> space;
   const int lane = threadIdx.x % G;
-  for (int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G; row < a.g.rows; row += (int64_t)gridDim.x * GROUPS) {
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G; row < a.g.rows; row += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
     Places p;
     row_starts(a.g, (uint32_t)row, a.o, p.at);
     const S *x = place<const S>(a, p, LP_X);
-    C seen;
-    const Statistics<C> z = statistics<DT, G>(x, a.g.n, lane, lds, seen);
+    const Statistics<C> z = statistics<DT, G, AHEAD>(x, a.g.n, lane, turn, space, [](C) {});
     if (lane == 0) give_statistics<DT>(a, p, x, z);
   }
 }
@@ -183,64 +237,74 @@ __global__ __launch_bounds__(group_threads(G)) void log_probs_kernel(LogProbsArg
 // ── the gradient ────────────────────────────────────────────────────────────
 template <int DT>
 struct Gradient {
-  using TX = Tr<DT>;
-  using C = typename TX::C;
-  using S = typename TX::S;
-  Statistics<C> z;
-  C inv_total, g, g_entropy;
+  using IO = Io<DT>;
+  using C = typename IO::C;
+  using S = typename IO::S;
+  C peak, ref, inv_total, g, g_entropy, shift;  // inner = log p + entropy = ln2 d + shift for the exponent d
   int token;
-  bool with_entropy;
-  __device__ __forceinline__ Gradient(const LogProbsArgs &a, const Places &p, const Statistics<C> &s) : z(s) {
-    inv_total = 1 / z.total;
+  bool with_entropy, near;
+  __device__ __forceinline__ Gradient(const LogProbsArgs &a, const Places &p, const Statistics<C> &z) {
+    peak = z.peak;
+    near = is_near(peak);
+    ref = reference(peak);
+    const C lost = near ? fused(peak, Bounds<C>::L, -ref) : 0;
+    inv_total = power(-lost) / z.total;
     token = *place<const int32_t>(a, p, LP_TOKEN);
     g = token < 0 ? 0 : token >= a.g.n ? (C)__builtin_nan("") : *place<const C>(a, p, LP_G);
     with_entropy = a.o[LP_G_ENTROPY].base != nullptr;
     g_entropy = with_entropy ? *place<const C>(a, p, LP_G_ENTROPY) : 0;
+    shift = with_entropy ? z.entropy - z.log_total - Bounds<C>::ln2 * lost : 0;
   }
+  template <bool NEAR, bool ENTROPY>
   __device__ __forceinline__ C at(C x) const {
-    const C d = x - z.peak, p = Exp<DT>::of(d) * inv_total;
-    if (!with_entropy) return -g * p;
-    return -p * fused(g_entropy, larger(d, Bounds<C>::far) - z.log_total + z.entropy, g);
+    const C d = NEAR ? fused(x, Bounds<C>::L, -ref) : (x - peak) * Bounds<C>::L, p = power(d) * inv_total;
+    return ENTROPY ? -p * fused(g_entropy, fused(larger(d, Bounds<C>::none), Bounds<C>::ln2, shift), g) : -g * p;
   }
-  template <int W>
-  __device__ __forceinline__ Vec<S, W> of(const Vec<S, W> &raw, int first) const {
-    C d[W];
+  // The gradient of n elements from x on, the row's from `first` on, by G lanes.
+  template <int G, int U, bool NEAR, bool ENTROPY>
+  __device__ __forceinline__ void write(const S *x, S *out, int n, int first, int lane) const {
+    walk<G, U>(x, n, lane,
+               [&](int c, Words raw) {
+                 C v[IO::V];
+                 IO::widen(raw, v);
 #pragma unroll
-    for (int j = 0; j < W; j++) d[j] = at(TX::ld(raw.v[j]));
-    if ((unsigned)(token - first) < (unsigned)W)
+                 for (int j = 0; j < IO::V; j++) v[j] = at<NEAR, ENTROPY>(v[j]);
+                 const unsigned j = (unsigned)(token - first - c * IO::V);
+                 if (j < (unsigned)IO::V)
 #pragma unroll
-      for (int j = 0; j < W; j++)
-        if (first + j == token) d[j] = d[j] + g;
-    Vec<S, W> o;
-#pragma unroll
-    for (int j = 0; j < W; j++) o.v[j] = TX::st(d[j]);
-    return o;
+                   for (int k = 0; k < IO::V; k++) v[k] = v[k] + ((unsigned)k == j ? g : 0);
+                 store_words(out + (int64_t)c * IO::V, IO::narrow(v));
+               },
+               [&](int i) { out[i] = IO::st(at<NEAR, ENTROPY>(IO::ld(x[i])) + (first + i == token ? g : 0)); });
+  }
+  template <int G, int U>
+  __device__ __forceinline__ void of(const S *x, S *out, int n, int first, int lane) const {
+    if (near && !with_entropy) write<G, U, true, false>(x, out, n, first, lane);
+    else if (near) write<G, U, true, true>(x, out, n, first, lane);
+    else write<G, 1, false, true>(x, out, n, first, lane);
   }
 };
 
-// A row's vectors are dealt out to gridDim.x groups of lanes.
-constexpr int GRAD_VECTORS = 4;  // of a lane
+// A row's vectors are dealt out to gridDim.x groups of lanes, in equal shares.
 template <int DT, int G>
 __global__ __launch_bounds__(256) void log_probs_grad_kernel(LogProbsArgs a) {
   using C = typename Tr<DT>::C;
   using S = typename Tr<DT>::S;
   constexpr int V = VECTOR<S>, GROUPS = 256 / G;
   const int lane = threadIdx.x % G, n = a.g.n;
-  const int first = blockIdx.x * G * GRAD_VECTORS;
-  const int part = n - first * V < G * GRAD_VECTORS * V ? n - first * V : G * GRAD_VECTORS * V;
+  const int nvec = n / V, share = (nvec + (int)gridDim.x - 1) / (int)gridDim.x;
+  const int begin = (int)blockIdx.x * share < nvec ? (int)blockIdx.x * share : nvec, end = begin + share < nvec ? begin + share : nvec;
+  const int first = begin * V, part = (blockIdx.x + 1 == gridDim.x ? n : end * V) - first;
   for (int64_t row = (int64_t)blockIdx.y * GROUPS + threadIdx.x / G; row < a.g.rows; row += (int64_t)gridDim.y * GROUPS) {
     Places p;
     row_starts(a.g, (uint32_t)row, a.o, p.at);
-    const S *x = place<const S>(a, p, LP_X) + (int64_t)first * V;
-    S *out = place<S>(a, p, LP_D) + (int64_t)first * V;
     Statistics<C> z{*place<const C>(a, p, LP_PEAK), *place<const C>(a, p, LP_TOTAL), 0, 0};
     if (a.o[LP_G_ENTROPY].base) {
       z.log_total = log(z.total);
       z.entropy = *place<const C>(a, p, LP_ENTROPY);
     }
-    Gradient<DT> grad(a, p, z);
-    walk<V, G>(x, part, lane, [&](int c, const Vec<S, V> &raw) { store_vec<V>(out + (int64_t)c * V, grad.of(raw, (first + c) * V)); },
-               [&](int i) { store_vec<1>(out + i, grad.of(load_vec<1>(x + i), first * V + i)); });
+    const Gradient<DT> grad(a, p, z);
+    grad.template of<G, AHEAD>(place<const S>(a, p, LP_X) + first, place<S>(a, p, LP_D) + first, part, first, lane);
   }
 }
 
@@ -249,23 +313,25 @@ template <int DT, int G>
 __global__ __launch_bounds__(group_threads(G)) void log_probs_with_grad_kernel(LogProbsArgs a) {
   using C = typename Tr<DT>::C;
   using S = typename Tr<DT>::S;
-  constexpr int V = VECTOR<S>, GROUPS = group_threads(G) / G;
-  __shared__ C lds[G > 64 ? 2 * (G / 64) : 1];
+  constexpr int GROUPS = group_threads(G) / G;
+  __shared__ Space<C, G> space;
   const int lane = threadIdx.x % G, n = a.g.n;
-  for (int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G; row < a.g.rows; row += (int64_t)gridDim.x * GROUPS) {
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G; row < a.g.rows; row += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
     Places p;
     row_starts(a.g, (uint32_t)row, a.o, p.at);
     const S *x = place<const S>(a, p, LP_X);
-    S *out = place<S>(a, p, LP_D);
-    C seen;
-    const Statistics<C> z = statistics<DT, G>(x, n, lane, lds, seen);
-    if (lane == 0) give_statistics<DT>(a, p, x, z);
-    // (the gradient may go where the logits are: the token's logit has been read by then)
-    if constexpr (G > 64) __syncthreads();
-    else __builtin_amdgcn_wave_barrier();
-    Gradient<DT> grad(a, p, z);
-    walk<V, G>(x, n, lane, [&](int c, const Vec<S, V> &raw) { store_vec<V>(out + (int64_t)c * V, grad.of(raw, c * V)); },
-               [&](int i) { store_vec<1>(out + i, grad.of(load_vec<1>(x + i), i)); });
+    // (the gradient may go where the logits are: the token's logit is read before any lane writes)
+    const int token = *place<const int32_t>(a, p, LP_TOKEN);
+    const C picked = Io<DT>::ld(x[token < 0 || token >= n ? 0 : token]);
+    const Statistics<C> z = statistics<DT, G, AHEAD>(x, n, lane, turn, space, [](C) {});
+    if (lane == 0) {
+      if (a.o[LP_LOG_P].base)
+        *place<C>(a, p, LP_LOG_P) = token < 0 ? 0 : token >= n ? (C)__builtin_nan("") : picked - z.peak - z.log_total;
+      if (a.o[LP_ENTROPY].base) *place<C>(a, p, LP_ENTROPY) = z.entropy;
+    }
+    const Gradient<DT> grad(a, p, z);
+    grad.template of<G, AHEAD>(x, place<S>(a, p, LP_D), n, 0, lane);
   }
 }
 
@@ -292,118 +358,119 @@ struct Highest {
   __device__ __forceinline__ T operator()(T a, T b) const { return a > b ? a : b; }
 };
 
-constexpr int TOP_MAX = 64, TOP_CANDIDATES = 1024;
+// alternatives at most; places on the list of candidates (a block's lanes at least); lanes that may hold candidates
+constexpr int TOP_MAX = 64, TOP_CANDIDATES = 1024, TOP_LANES = 5 * TOP_MAX;
 
 template <int DT, int G>
 struct TopSpace {
+  static_assert(G <= TOP_CANDIDATES, "a place for every lane");
   using T = typename KeyOf<typename Tr<DT>::C>::T;
   T key[TOP_CANDIDATES];
   uint32_t index[TOP_CANDIDATES];
-  T low[G / 64], cut;
-  int part[G / 64], count;
+  T lane_key[TOP_LANES];
+  uint32_t lane[TOP_LANES];
+  T low[G / 64];
+  int part[G / 64], lanes, found;
 };
 
 // The k-th largest of the lanes' largest elements bounds the k-th largest of the row from below, and only lanes
-// whose largest reaches it hold candidates: some k of them in a row without order, which walk their elements once more. Ties
-// (a row of equal logits, a vocabulary that is banned but for a few tokens) can make candidates of the whole row: then what lies
-// above the bound is taken, and of what equals it the first in the row. A row whose large elements gather in a few lanes, and one with a
-// NaN, has its k-th largest found bit by bit, a walk for each.
+// whose largest reaches it hold candidates: some k of them in a row without order. All lanes together look through those
+// lanes' elements. Ties (a row of equal logits, a vocabulary that is banned but for a few tokens) can make candidates of the
+// whole row: then what lies above the bound is taken, and of what equals it the first in the row. A row whose large elements
+// gather in a few lanes, and one with a NaN, has its k-th largest found bit by bit, a walk for each.
 template <int DT, int G>
-__device__ __forceinline__ void top_tokens(const typename Tr<DT>::S *x, int n, int k, typename Tr<DT>::C seen, const Statistics<typename Tr<DT>::C> &z,
-                                           TopSpace<DT, G> &l, typename Tr<DT>::C *log_p, int32_t *tokens) {
-  using TX = Tr<DT>;
-  using C = typename TX::C;
-  using S = typename TX::S;
+struct Top {
+  using IO = Io<DT>;
+  using C = typename IO::C;
+  using S = typename IO::S;
   using T = typename KeyOf<C>::T;
-  constexpr int V = VECTOR<S>, W = G / 64;
-  const int lane = threadIdx.x, wave = lane >> 6;
-  const int nvec = n / V;
-  const T mine = lane < nvec || nvec * V + lane < n ? key_of(seen) : 0;
-  // puts what `wanted` says of this lane's elements on the list, which may want more places than it has
-  auto collect = [&](bool look, auto &&wanted) {
-    __syncthreads();
-    if (lane == 0) l.count = 0;
-    __syncthreads();
-    auto offer = [&](S raw, int i) {
-      const T key = key_of(TX::ld(raw));
-      if (wanted(key)) {
-        const int at = atomicAdd(&l.count, 1);
-        if (at < TOP_CANDIDATES) {
-          l.key[at] = key;
-          l.index[at] = (uint32_t)i;
-        }
+  static constexpr int V = IO::V, W = G / 64;
+  const S *x;
+  int n, k;
+  TopSpace<DT, G> &l;
+  const int lane = threadIdx.x, wave = threadIdx.x >> 6;
+  T mine = 0;
+
+  __device__ __forceinline__ Top(const S *row, int length, int top, TopSpace<DT, G> &space) : x(row), n(length), k(top), l(space) {}
+
+  // give(place, key, index), by one lane, for each of the first m entries of the list: a wave takes an entry and its lanes compare it
+  // with 64 others at a time.
+  template <class F>
+  __device__ __forceinline__ void rank(int m, F &&give) const {
+    for (int i = wave; i < m; i += W) {
+      const T key = l.key[i];
+      const uint32_t index = l.index[i];
+      int place = 0;
+      for (int j = 0; j < m; j += 64) {
+        const int other = j + (lane & 63) < m ? j + (lane & 63) : i;
+        place += __popcll(__ballot(l.key[other] > key || (l.key[other] == key && l.index[other] < index)));
       }
-    };
-    if (look)
-      walk<V, G>(x, n, lane,
-                 [&](int c, const Vec<S, V> &raw) {
+      if ((lane & 63) == 0) give(place, key, index);
+    }
+  }
+  __device__ __forceinline__ void offer(S raw, int i, T least) {
+    const T key = key_of(IO::ld(raw));
+    if (key >= least) {
+      const int at = atomicAdd(&l.found, 1);
+      if (at < TOP_CANDIDATES) {
+        l.key[at] = key;
+        l.index[at] = (uint32_t)i;
+      }
+    }
+  }
+  __device__ __forceinline__ void offer(Words raw, int c, T least) {
+    struct Elements { S x[V]; } e = __builtin_bit_cast(Elements, raw);
 #pragma unroll
-                   for (int j = 0; j < V; j++) offer(raw.v[j], c * V + j);
-                 },
-                 [&](int i) { offer(x[i], i); });
-    __syncthreads();
-    return l.count;
-  };
-  T bound = 0;
-  int found = TOP_CANDIDATES + 1;
-  bool by_bits = !(z.total == z.total), ties = by_bits;
-  if (!by_bits) {
-    // Lanes that can be among the k largest: each wave's first k / W, rounded up, already are k.
+    for (int j = 0; j < V; j++) offer(e.x[j], c * V + j, least);
+  }
+  // Before the barrier of the statistics: which of the wave's lanes can be among the k largest of the block: each wave's
+  // first k / W, rounded up, already are k.
+  __device__ __forceinline__ void begin(C seen) {
+    mine = lane < n / V || n / V * V + lane < n ? key_of(seen) : 0;
     const int rounds = (k + W - 1) / W;
-    __syncthreads();
+    T most = 0;
     if (rounds <= 4) {
-      T left = mine, most = 0;
+      T left = mine;
       for (int r = 0; r < rounds; r++) {
         most = lanes_combine<64>(left, Highest<T>{});
         const uint64_t have = __ballot(left == most);
         if ((lane & 63) == __builtin_ctzll(have)) left = 0;
       }
-      if ((lane & 63) == 0) l.low[wave] = most;
-    } else if ((lane & 63) == 0) {
-      l.low[wave] = 0;
     }
-    if (lane == 0) l.count = 0;
-    __syncthreads();
-    T low = l.low[0];
-#pragma unroll
-    for (int w = 1; w < W; w++) low = l.low[w] < low ? l.low[w] : low;
-    if (mine >= low) l.key[atomicAdd(&l.count, 1)] = mine;
-    __syncthreads();
-    const int m = l.count;
-    if (lane < m) {
-      int before = 0;
-      for (int j = 0; j < m; j++) before += l.key[j] > l.key[lane] || (l.key[j] == l.key[lane] && j < lane);
-      if (before == k - 1) l.cut = l.key[lane];
-    }
-    __syncthreads();
-    bound = l.cut;
-    if (__syncthreads_count(mine >= bound) <= 4 * k + 64) found = collect(mine >= bound, [&](T key) { return key >= bound; });
-    if (found > TOP_CANDIDATES) {
-      ties = true;
-      found = collect(mine > bound, [&](T key) { return key > bound; });
-      by_bits = found > TOP_CANDIDATES;
-    }
+    if ((lane & 63) == 0) l.low[wave] = most;
+    if (lane == 0) l.lanes = l.found = 0;
   }
-  if (by_bits) {
-    bound = 0;
+  // Every element of key `least` or more of the row onto the list, which may want more places than it has.
+  __device__ __forceinline__ int collect(T least) {
+    __syncthreads();
+    if (lane == 0) l.found = 0;
+    __syncthreads();
+    walk<G, 1>(x, n, lane, [&](int c, Words raw) { offer(raw, c, least); }, [&](int i) { offer(x[i], i, least); });
+    __syncthreads();
+    return l.found;
+  }
+  // The k-th largest key of the row.
+  __device__ __forceinline__ T by_bits() {
+    T bound = 0;
     for (int bit = 8 * (int)sizeof(T) - 1; bit >= 0; bit--) {
       const T next = bound | (T)1 << bit;
       int count[1] = {0};
-      walk<V, G>(x, n, lane,
-                 [&](int, const Vec<S, V> &raw) {
+      walk<G, 1>(x, n, lane,
+                 [&](int, Words raw) {
+                   struct Elements { S x[V]; } e = __builtin_bit_cast(Elements, raw);
 #pragma unroll
-                   for (int j = 0; j < V; j++) count[0] += key_of(TX::ld(raw.v[j])) >= next;
+                   for (int j = 0; j < V; j++) count[0] += key_of(IO::ld(e.x[j])) >= next;
                  },
-                 [&](int i) { count[0] += key_of(TX::ld(x[i])) >= next; });
+                 [&](int i) { count[0] += key_of(IO::ld(x[i])) >= next; });
       group_combine<G>(count, Sum<int>{}, l.part);
       if (count[0] >= k) bound = next;
     }
-    found = collect(true, [&](T key) { return key > bound; });  // fewer than k
+    return bound;
   }
-  if (ties && found < k) {  // the first of the row's elements that equal the bound
-    int at = found;
+  // The first elements of the row that equal the bound, from place `at` of the list on, up to k.
+  __device__ __forceinline__ void first_equal(T bound, int at) {
     for (int base = 0; at < k && base < n; base += G) {
-      const bool hit = base + lane < n && key_of(TX::ld(x[base + lane])) == bound;
+      const bool hit = base + lane < n && key_of(IO::ld(x[base + lane])) == bound;
       const uint64_t hits = __ballot(hit);
       __syncthreads();
       if ((lane & 63) == 0) l.part[wave] = __popcll(hits);
@@ -419,36 +486,80 @@ __device__ __forceinline__ void top_tokens(const typename Tr<DT>::S *x, int n, i
         l.index[place] = (uint32_t)(base + lane);
       }
     }
-    found = k;
     __syncthreads();
   }
-  for (int i = lane; i < found; i += G) {
-    const T key = l.key[i];
-    const uint32_t index = l.index[i];
-    int before = 0;
-    for (int j = 0; j < found; j++) before += l.key[j] > key || (l.key[j] == key && l.index[j] < index);
-    if (before < k) {
-      log_p[before] = value_of<C>(key) - z.peak - z.log_total;
-      tokens[before] = (int32_t)index;
+  // After the barrier of the statistics: the list holds the k largest elements, and others; how many.
+  __device__ __forceinline__ int candidates(bool ordered) {
+    T bound = 0;
+    int found = TOP_CANDIDATES + 1;
+    if (ordered) {
+      T low = l.low[0];
+#pragma unroll
+      for (int w = 1; w < W; w++) low = l.low[w] < low ? l.low[w] : low;
+      if (mine >= low) {
+        const int at = atomicAdd(&l.lanes, 1);
+        l.key[at] = mine;
+        l.index[at] = (uint32_t)lane;
+      }
+      __syncthreads();
+      const int m = l.lanes;
+      rank(m, [&](int place, T key, uint32_t index) {  // these lanes in their order
+        if (place < TOP_LANES) {
+          l.lane_key[place] = key;
+          l.lane[place] = index;
+        }
+      });
+      __syncthreads();
+      bound = l.lane_key[k - 1];
+      int lanes = k;
+      while (lanes < m && lanes < TOP_LANES && l.lane_key[lanes] == bound) lanes++;
+      if (lanes < TOP_LANES) {
+        const int nvec = n / V, each = (nvec + G - 1) / G;
+        for (int w = lane; w < lanes * each; w += G) {
+          const int c = (w / lanes) * G + (int)l.lane[w % lanes];
+          if (c < nvec) offer(load_words(x + (int64_t)c * V), c, bound);
+        }
+        if (nvec * V + lane < n) offer(x[nvec * V + lane], nvec * V + lane, bound);
+        __syncthreads();
+        found = l.found;
+        if (found <= TOP_CANDIDATES) return found;
+      }
+      found = collect(bound + 1);
     }
+    if (found > TOP_CANDIDATES) {
+      bound = by_bits();
+      found = collect(bound + 1);  // fewer than k
+    }
+    if (found >= k) return found;
+    first_equal(bound, found);
+    return k;
   }
-  __syncthreads();  // the list is free for the next row
-}
+  __device__ __forceinline__ void write(int found, const Statistics<C> &z, C *log_p, int32_t *tokens) const {
+    rank(found, [&](int place, T key, uint32_t index) {
+      if (place < k) {
+        log_p[place] = value_of<C>(key) - z.peak - z.log_total;
+        tokens[place] = (int32_t)index;
+      }
+    });
+  }
+};
 
 template <int DT, int G>
 __global__ __launch_bounds__(G) void log_probs_top_kernel(LogProbsArgs a) {
   using C = typename Tr<DT>::C;
   using S = typename Tr<DT>::S;
-  __shared__ C lds[2 * (G / 64)];
-  __shared__ TopSpace<DT, G> space;
-  for (int64_t row = blockIdx.x; row < a.g.rows; row += gridDim.x) {
+  __shared__ Space<C, G> space;
+  __shared__ TopSpace<DT, G> list;
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.g.rows; row += gridDim.x, turn ^= 1) {
     Places p;
     row_starts(a.g, (uint32_t)row, a.o, p.at);
     const S *x = place<const S>(a, p, LP_X);
-    C seen;
-    const Statistics<C> z = statistics<DT, G>(x, a.g.n, threadIdx.x, lds, seen);
+    Top<DT, G> top(x, a.g.n, a.top, list);
+    const Statistics<C> z = statistics<DT, G, AHEAD>(x, a.g.n, threadIdx.x, turn, space, [&](C s) { top.begin(s); });
     if (threadIdx.x == 0) give_statistics<DT>(a, p, x, z);
-    top_tokens<DT, G>(x, a.g.n, a.top, seen, z, space, place<C>(a, p, LP_TOP_LOG_P), place<int32_t>(a, p, LP_TOP_TOKEN));
+    top.write(top.candidates(z.total == z.total), z, place<C>(a, p, LP_TOP_LOG_P), place<int32_t>(a, p, LP_TOP_TOKEN));
+    __syncthreads();  // the list is free for the next row
   }
 }
 
@@ -492,7 +603,7 @@ void launch_grad(nxh_context *ctx, const LogProbsArgs &a) {
   constexpr int V = VECTOR<typename Tr<DT>::S>;
   auto go = [&](auto group) {
     constexpr int G = decltype(group)::value;
-    const int share = G * GRAD_VECTORS * V, parts = (a.g.n + share - 1) / share;  // (at most 2^14 parts)
+    const int parts = std::max(1, (a.g.n / V + G * AHEAD - 1) / (G * AHEAD));  // (at most 2^14)
     const int64_t rows = (a.g.rows + 256 / G - 1) / (256 / G);
     const dim3 grid((unsigned)parts, (unsigned)std::min(rows, std::min<int64_t>(65535, MOST_LANES / 256 / parts)));
     hipLaunchKernelGGL((log_probs_grad_kernel<DT, G>), grid, dim3(256), 0, ctx->stream, a);

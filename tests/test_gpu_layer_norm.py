@@ -187,7 +187,7 @@ def test_views(hip, oracle, d, n):
         same_bits(logical(odg)[1::2], block.reshape(-1)[:n], "between dgamma's values")
 
 
-@pytest.mark.parametrize("n", [96, 20000])
+@pytest.mark.parametrize("n", [3, 96, 101, 1030, 5001, 20000, 20003])
 def test_results_that_replace_inputs(hip, oracle, n):
     d = dt.float32
     x, g = (drawn((9, n), d, oracle, k) for k in (1, 2))

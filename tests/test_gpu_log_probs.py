@@ -214,7 +214,9 @@ def test_values_that_are_no_numbers(hip, oracle, d, n):
         assert np.all(np.isnan(logical(t)[no])), name
     assert np.all(np.isnan(logical(got[4])[no])) and np.isnan(logical(got[0])[8])
     assert np.array_equal(logical(got[5]), want.top)
-    assert logical(got[1])[3] == 0 and logical(got[3])[3] == 1  # one element that is possible
+    # One element that is possible: its term 2^r, r = peak log2 e - a, and 2^-r have errors of 4 u each (|r| < 2^-22 here), their
+    # product is no less than 1 by the clamp and so at most 8 u + u above it; the entropy is held to its bound above, from zero on.
+    assert 1 <= logical(got[3])[3] <= 1 + 10 * unit(d) and 0 <= logical(got[1])[3] <= want.entropy_err[3]
     g, ge = np.full(9, -1.0), np.full(9, 0.5)
     (hg, _), (hge, _) = values(hip, g, d), values(hip, ge, d)
     dx = [hip.log_probs_grad(hg, hx, ht, got[2], got[3], hge, got[1]), hip.log_probs_with_grad(hg, hx, ht, hge)[2]]
