@@ -74,7 +74,7 @@ __device__ __forceinline__ void walk(const S *x, int n, int lane, B &&body, E &&
   for (int c = lane; c < nvec; c += U * G) {
     Words raw[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) raw[u] = load_words(x + (int64_t)(c + u * G < nvec ? c + u * G : nvec - 1) * V);
+    for (int u = 0; u < U; u++) raw[u] = load_vector(x, c + u * G < nvec ? c + u * G : nvec - 1);
 #pragma unroll
     for (int u = 0; u < U; u++)
       if (c + u * G < nvec) body(c + u * G, raw[u]);
@@ -124,6 +124,22 @@ struct Running {
     const C x[1] = {IO::ld(raw)};
     take(x);
   }
+  // its values as the k-th of count, in shared or device memory
+  __device__ __forceinline__ void store(C *at, int count) const {
+    at[0] = m;
+    at[count] = s;
+    at[2 * count] = t;
+  }
+  __device__ __forceinline__ void load(const C *at, int count) {
+    m = at[0];
+    a = reference(m);
+    s = at[count];
+    t = at[2 * count];
+  }
+  template <int G, int U>
+  __device__ __forceinline__ void take_row(const S *x, int n, int lane) {
+    walk<G, U>(x, n, lane, [&](int, Words raw) { take(raw); }, [&](int i) { take_one(x[i]); });
+  }
   // joined with the other lanes of a group of N
   template <int N>
   __device__ __forceinline__ void join() {
@@ -163,31 +179,24 @@ template <class C, int G>
 struct Space {
   C wave[2][G > 64 ? 3 * (G / 64) : 1], sums[G > 64 ? 2 * (G / 64) : 1];
 };
-// The statistics of a row. turn: 0 and 1 from one row of the block to the next; seen(largest element of the lane's own) is called
-// between the walk and the barrier.
-template <int DT, int G, int U, class F>
-__device__ __forceinline__ Statistics<typename Tr<DT>::C> statistics(const typename Tr<DT>::S *x, int n, int lane, int turn,
-                                                                     Space<typename Tr<DT>::C, G> &l, F &&seen) {
-  using C = typename Tr<DT>::C;
-  Running<DT> r;
-  walk<G, U>(x, n, lane, [&](int, Words raw) { r.take(raw); }, [&](int i) { r.take_one(x[i]); });
-  seen(r.m);
+// The lanes' sums joined: every lane of the group gets them. turn: 0 and 1 from one row of the block to the next.
+template <int DT, int G>
+__device__ __forceinline__ void join_group(Running<DT> &r, int lane, int turn, Space<typename Tr<DT>::C, G> &l) {
   r.template join<(G < 64 ? G : 64)>();
   if constexpr (G > 64) {
     constexpr int W = G / 64;
-    C *w = l.wave[turn];
-    if ((lane & 63) == 0) {
-      w[lane >> 6] = r.m;
-      w[W + (lane >> 6)] = r.s;
-      w[2 * W + (lane >> 6)] = r.t;
-    }
+    auto *w = l.wave[turn];
+    if ((lane & 63) == 0) r.store(w + (lane >> 6), W);
     __syncthreads();
-    r.m = w[lane % W];
-    r.a = reference(r.m);
-    r.s = w[W + lane % W];
-    r.t = w[2 * W + lane % W];
+    r.load(w + lane % W, W);
     r.template join<W>();
   }
+}
+// The statistics of row x from its sums.
+template <int DT, int G>
+__device__ __forceinline__ Statistics<typename Tr<DT>::C> finish(const Running<DT> &r, const typename Tr<DT>::S *x, int n, int lane,
+                                                                 Space<typename Tr<DT>::C, G> &l) {
+  using C = typename Tr<DT>::C;
   if (!is_near(r.m)) return far_statistics<DT, G>(x, n, lane, r.m, l.sums);
   const C lost = fused(r.m, Bounds<C>::L, -r.a);
   C total = r.s * power(-lost);
@@ -229,7 +238,10 @@ __global__ __launch_bounds__(group_threads(G)) void log_probs_kernel(LogProbsArg
     Places p;
     row_starts(a.g, (uint32_t)row, a.o, p.at);
     const S *x = place<const S>(a, p, LP_X);
-    const Statistics<C> z = statistics<DT, G, AHEAD>(x, a.g.n, lane, turn, space, [](C) {});
+    Running<DT> r;
+    r.template take_row<G, AHEAD>(x, a.g.n, lane);
+    join_group<DT, G>(r, lane, turn, space);
+    const Statistics<C> z = finish<DT, G>(r, x, a.g.n, lane, space);
     if (lane == 0) give_statistics<DT>(a, p, x, z);
   }
 }
@@ -260,22 +272,28 @@ struct Gradient {
     const C d = NEAR ? fused(x, Bounds<C>::L, -ref) : (x - peak) * Bounds<C>::L, p = power(d) * inv_total;
     return ENTROPY ? -p * fused(g_entropy, fused(larger(d, Bounds<C>::none), Bounds<C>::ln2, shift), g) : -g * p;
   }
+  // Of the elements from number i of the row on.
+  template <bool NEAR, bool ENTROPY>
+  __device__ __forceinline__ Words vector(Words raw, int i) const {
+    C v[IO::V];
+    IO::widen(raw, v);
+#pragma unroll
+    for (int j = 0; j < IO::V; j++) v[j] = at<NEAR, ENTROPY>(v[j]);
+    const unsigned j = (unsigned)(token - i);
+    if (j < (unsigned)IO::V)
+#pragma unroll
+      for (int k = 0; k < IO::V; k++) v[k] = v[k] + ((unsigned)k == j ? g : 0);
+    return IO::narrow(v);
+  }
+  template <bool NEAR, bool ENTROPY>
+  __device__ __forceinline__ S element(S x, int i) const {
+    return IO::st(at<NEAR, ENTROPY>(IO::ld(x)) + (i == token ? g : 0));
+  }
   // The gradient of n elements from x on, the row's from `first` on, by G lanes.
   template <int G, int U, bool NEAR, bool ENTROPY>
   __device__ __forceinline__ void write(const S *x, S *out, int n, int first, int lane) const {
-    walk<G, U>(x, n, lane,
-               [&](int c, Words raw) {
-                 C v[IO::V];
-                 IO::widen(raw, v);
-#pragma unroll
-                 for (int j = 0; j < IO::V; j++) v[j] = at<NEAR, ENTROPY>(v[j]);
-                 const unsigned j = (unsigned)(token - first - c * IO::V);
-                 if (j < (unsigned)IO::V)
-#pragma unroll
-                   for (int k = 0; k < IO::V; k++) v[k] = v[k] + ((unsigned)k == j ? g : 0);
-                 store_words(out + (int64_t)c * IO::V, IO::narrow(v));
-               },
-               [&](int i) { out[i] = IO::st(at<NEAR, ENTROPY>(IO::ld(x[i])) + (first + i == token ? g : 0)); });
+    walk<G, U>(x, n, lane, [&](int c, Words raw) { store_vector(out, c, vector<NEAR, ENTROPY>(raw, first + c * IO::V)); },
+               [&](int i) { out[i] = element<NEAR, ENTROPY>(x[i], first + i); });
   }
   template <int G, int U>
   __device__ __forceinline__ void of(const S *x, S *out, int n, int first, int lane) const {
@@ -308,28 +326,105 @@ __global__ __launch_bounds__(256) void log_probs_grad_kernel(LogProbsArgs a) {
   }
 }
 
-// Statistics and gradient of a row by the same lanes: the second walk finds the row in the caches.
-template <int DT, int G>
+// Statistics and gradient of a row by the same lanes, whose vectors, at most NV of a lane, stay in registers from the one to the
+// other; as one has been written, the next row's is requested into its place, so that memory works while sums are taken.
+template <int DT, int G, int NV>
 __global__ __launch_bounds__(group_threads(G)) void log_probs_with_grad_kernel(LogProbsArgs a) {
-  using C = typename Tr<DT>::C;
-  using S = typename Tr<DT>::S;
-  constexpr int GROUPS = group_threads(G) / G;
+  using IO = Io<DT>;
+  using C = typename IO::C;
+  using S = typename IO::S;
+  constexpr int GROUPS = group_threads(G) / G, V = IO::V;
   __shared__ Space<C, G> space;
-  const int lane = threadIdx.x % G, n = a.g.n;
+  const int lane = threadIdx.x % G, n = a.g.n, nvec = n / V, last = nvec > 0 ? nvec - 1 : 0;
+  const bool has_behind = nvec * V + lane < n;
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G;
+  if (row >= a.g.rows) return;  // (whole groups; a group of several waves is the block)
+  Places p;
+  const S *x;
+  int token;
+  // The gradient may go where the logits are: the token's is read here, before the lane's others, which the sums are made of that
+  // all lanes wait for.
+  S picked, behind{};
+  auto begin = [&](int64_t r) {
+    row_starts(a.g, (uint32_t)r, a.o, p.at);
+    x = place<const S>(a, p, LP_X);
+    token = *place<const int32_t>(a, p, LP_TOKEN);
+    picked = x[token < 0 || token >= n ? 0 : token];
+  };
+  auto request = [&](int v) { return load_vector(x, v * G + lane < nvec ? v * G + lane : last); };
+  begin(row);
+  Words raw[NV];
+  if (nvec > 0)
+#pragma unroll
+    for (int v = 0; v < NV; v++) raw[v] = request(v);
+  if (has_behind) behind = x[nvec * V + lane];
+  for (int turn = 0; row < a.g.rows; row += step, turn ^= 1) {
+    Running<DT> r;
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+      if (v * G + lane < nvec) r.take(raw[v]);
+      __builtin_amdgcn_sched_barrier(0);  // (one after the other: widened at once they need more registers)
+    }
+    if (has_behind) r.take_one(behind);
+    join_group<DT, G>(r, lane, turn, space);
+    const Statistics<C> z = finish<DT, G>(r, x, n, lane, space);
+    if (lane == 0) {
+      if (a.o[LP_LOG_P].base)
+        *place<C>(a, p, LP_LOG_P) = token < 0 ? 0 : token >= n ? (C)__builtin_nan("") : IO::ld(picked) - z.peak - z.log_total;
+      if (a.o[LP_ENTROPY].base) *place<C>(a, p, LP_ENTROPY) = z.entropy;
+    }
+    if constexpr (G > 64)
+      if (!is_near(z.peak)) __syncthreads();  // (the walk by differences was the last to read the row)
+    const Gradient<DT> grad(a, p, z);
+    S *out = place<S>(a, p, LP_D);
+    begin(row + step < a.g.rows ? row + step : row);  // (behind the last row its own again, for nothing)
+    auto write = [&](auto near, auto entropy) {
+      constexpr bool NEAR = decltype(near)::value, ENTROPY = decltype(entropy)::value;
+      if (nvec > 0)
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+          const Words d = grad.template vector<NEAR, ENTROPY>(raw[v], (v * G + lane) * V);
+          raw[v] = request(v);
+          if (v * G + lane < nvec) store_vector(out, v * G + lane, d);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      if (has_behind) {
+        const S d = grad.template element<NEAR, ENTROPY>(behind, nvec * V + lane);
+        behind = x[nvec * V + lane];
+        out[nvec * V + lane] = d;
+      }
+    };
+    if (grad.near && !grad.with_entropy) write(std::true_type{}, std::false_type{});
+    else if (grad.near) write(std::true_type{}, std::true_type{});
+    else write(std::false_type{}, std::true_type{});
+  }
+}
+// Rows longer than that are read again, out of the caches.
+template <int DT, int G>
+__global__ __launch_bounds__(G) void log_probs_with_grad_long_kernel(LogProbsArgs a) {
+  using IO = Io<DT>;
+  using C = typename IO::C;
+  using S = typename IO::S;
+  __shared__ Space<C, G> space;
+  const int lane = threadIdx.x, n = a.g.n;
   int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G; row < a.g.rows; row += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
+  for (int64_t row = blockIdx.x; row < a.g.rows; row += gridDim.x, turn ^= 1) {
     Places p;
     row_starts(a.g, (uint32_t)row, a.o, p.at);
     const S *x = place<const S>(a, p, LP_X);
-    // (the gradient may go where the logits are: the token's logit is read before any lane writes)
     const int token = *place<const int32_t>(a, p, LP_TOKEN);
-    const C picked = Io<DT>::ld(x[token < 0 || token >= n ? 0 : token]);
-    const Statistics<C> z = statistics<DT, G, AHEAD>(x, n, lane, turn, space, [](C) {});
+    const S picked = x[token < 0 || token >= n ? 0 : token];  // (first, as above)
+    Running<DT> r;
+    r.template take_row<G, AHEAD>(x, n, lane);
+    join_group<DT, G>(r, lane, turn, space);
+    const Statistics<C> z = finish<DT, G>(r, x, n, lane, space);
     if (lane == 0) {
       if (a.o[LP_LOG_P].base)
-        *place<C>(a, p, LP_LOG_P) = token < 0 ? 0 : token >= n ? (C)__builtin_nan("") : picked - z.peak - z.log_total;
+        *place<C>(a, p, LP_LOG_P) = token < 0 ? 0 : token >= n ? (C)__builtin_nan("") : IO::ld(picked) - z.peak - z.log_total;
       if (a.o[LP_ENTROPY].base) *place<C>(a, p, LP_ENTROPY) = z.entropy;
     }
+    if (!is_near(z.peak)) __syncthreads();
     const Gradient<DT> grad(a, p, z);
     grad.template of<G, AHEAD>(x, place<S>(a, p, LP_D), n, 0, lane);
   }
@@ -366,16 +461,14 @@ struct TopSpace {
   static_assert(G <= TOP_CANDIDATES, "a place for every lane");
   using T = typename KeyOf<typename Tr<DT>::C>::T;
   T key[TOP_CANDIDATES];
-  uint32_t index[TOP_CANDIDATES];
-  T lane_key[TOP_LANES];
-  uint32_t lane[TOP_LANES];
-  T low[G / 64];
+  uint32_t index[TOP_CANDIDATES], lane[TOP_LANES], few[64];
+  T lane_key[TOP_LANES], low[G / 64];
   int part[G / 64], lanes, found;
 };
 
-// The k-th largest of the lanes' largest elements bounds the k-th largest of the row from below, and only lanes
-// whose largest reaches it hold candidates: some k of them in a row without order. All lanes together look through those
-// lanes' elements. Ties (a row of equal logits, a vocabulary that is banned but for a few tokens) can make candidates of the
+// Of each wave's lanes the k / W, rounded up, with the largest elements: the least of those k bounds the k-th largest element
+// of the row from below, and only lanes whose largest reaches it hold candidates: one or two times k in a row without
+// order, of which, where they are few, the k largest are found. All lanes together look through those lanes' elements. Ties (a row of equal logits, a vocabulary that is banned but for a few tokens) can make candidates of the
 // whole row: then what lies above the bound is taken, and of what equals it the first in the row. A row whose large elements
 // gather in a few lanes, and one with a NaN, has its k-th largest found bit by bit, a walk for each.
 template <int DT, int G>
@@ -393,19 +486,33 @@ struct Top {
 
   __device__ __forceinline__ Top(const S *row, int length, int top, TopSpace<DT, G> &space) : x(row), n(length), k(top), l(space) {}
 
-  // give(place, key, index), by one lane, for each of the first m entries of the list: a wave takes an entry and its lanes compare it
-  // with 64 others at a time.
+  // give(place, key, index), by one lane, for each of the first m entries of the list: a wave takes an entry and its lanes
+  // compare it with four each, which they hold (read again for each entry, 256 of them took 40 us).
   template <class F>
   __device__ __forceinline__ void rank(int m, F &&give) const {
+    constexpr int Q = 4;
+    auto entry = [&](int j, T &key, uint32_t &index) {
+      key = j < m ? l.key[j] : 0;
+      index = j < m ? l.index[j] : ~0u;  // (before nothing)
+    };
+    T key[Q];
+    uint32_t index[Q];
+#pragma unroll
+    for (int q = 0; q < Q; q++) entry(q * 64 + (lane & 63), key[q], index[q]);
     for (int i = wave; i < m; i += W) {
-      const T key = l.key[i];
-      const uint32_t index = l.index[i];
+      const T mine = l.key[i];
+      const uint32_t at = l.index[i];
       int place = 0;
-      for (int j = 0; j < m; j += 64) {
-        const int other = j + (lane & 63) < m ? j + (lane & 63) : i;
-        place += __popcll(__ballot(l.key[other] > key || (l.key[other] == key && l.index[other] < index)));
+#pragma unroll
+      for (int q = 0; q < Q; q++)
+        if (q * 64 < m) place += __popcll(__ballot(key[q] > mine || (key[q] == mine && index[q] < at)));
+      for (int j = Q * 64; j < m; j += 64) {
+        T k;
+        uint32_t n;
+        entry(j + (lane & 63), k, n);
+        place += __popcll(__ballot(k > mine || (k == mine && n < at)));
       }
-      if ((lane & 63) == 0) give(place, key, index);
+      if ((lane & 63) == 0) give(place, mine, at);
     }
   }
   __device__ __forceinline__ void offer(S raw, int i, T least) {
@@ -423,19 +530,15 @@ struct Top {
 #pragma unroll
     for (int j = 0; j < V; j++) offer(e.x[j], c * V + j, least);
   }
-  // Before the barrier of the statistics: which of the wave's lanes can be among the k largest of the block: each wave's
-  // first k / W, rounded up, already are k.
+  // Before the barrier of the statistics: the wave's part in the bound.
   __device__ __forceinline__ void begin(C seen) {
     mine = lane < n / V || n / V * V + lane < n ? key_of(seen) : 0;
     const int rounds = (k + W - 1) / W;
-    T most = 0;
-    if (rounds <= 4) {
-      T left = mine;
-      for (int r = 0; r < rounds; r++) {
-        most = lanes_combine<64>(left, Highest<T>{});
-        const uint64_t have = __ballot(left == most);
-        if ((lane & 63) == __builtin_ctzll(have)) left = 0;
-      }
+    T most = 0, left = mine;
+    for (int r = 0; r < rounds; r++) {
+      most = lanes_combine<64>(left, Highest<T>{});
+      const uint64_t have = __ballot(left == most);
+      if ((lane & 63) == __builtin_ctzll(have)) left = 0;
     }
     if ((lane & 63) == 0) l.low[wave] = most;
     if (lane == 0) l.lanes = l.found = 0;
@@ -493,31 +596,39 @@ struct Top {
     T bound = 0;
     int found = TOP_CANDIDATES + 1;
     if (ordered) {
-      T low = l.low[0];
+      bound = l.low[0];
 #pragma unroll
-      for (int w = 1; w < W; w++) low = l.low[w] < low ? l.low[w] : low;
-      if (mine >= low) {
+      for (int w = 1; w < W; w++) bound = l.low[w] < bound ? l.low[w] : bound;
+      if (mine >= bound) {
         const int at = atomicAdd(&l.lanes, 1);
-        l.key[at] = mine;
-        l.index[at] = (uint32_t)lane;
+        if (at < TOP_LANES) {
+          l.lane[at] = (uint32_t)lane;
+          l.lane_key[at] = mine;
+        }
       }
       __syncthreads();
-      const int m = l.lanes;
-      rank(m, [&](int place, T key, uint32_t index) {  // these lanes in their order
-        if (place < TOP_LANES) {
-          l.lane_key[place] = key;
-          l.lane[place] = index;
+      int lanes = l.lanes;
+      const uint32_t *which = l.lane;
+      if (lanes <= 64) {  // each wave by itself finds the k-th largest of them, down to the bits that a 16-bit dtype has
+        const int i = lane & 63;
+        const T key = i < lanes ? l.lane_key[i] : 0;
+        bound = 0;
+        constexpr int bits = 8 * (int)sizeof(T);
+#pragma unroll
+        for (int bit = bits - 1; bit >= (sizeof(S) == 2 ? bits - 20 : 0); bit--) {
+          const T next = bound | (T)1 << bit;
+          if (__popcll(__ballot(key >= next)) >= k) bound = next;
         }
-      });
-      __syncthreads();
-      bound = l.lane_key[k - 1];
-      int lanes = k;
-      while (lanes < m && lanes < TOP_LANES && l.lane_key[lanes] == bound) lanes++;
-      if (lanes < TOP_LANES) {
+        const uint64_t reach = __ballot(i < lanes && key >= bound);
+        if (reach >> i & 1) l.few[__popcll(reach & (((uint64_t)1 << i) - 1))] = l.lane[i];  // (the same of every wave)
+        lanes = __popcll(reach);
+        which = l.few;
+      }
+      if (lanes <= TOP_LANES) {
         const int nvec = n / V, each = (nvec + G - 1) / G;
         for (int w = lane; w < lanes * each; w += G) {
-          const int c = (w / lanes) * G + (int)l.lane[w % lanes];
-          if (c < nvec) offer(load_words(x + (int64_t)c * V), c, bound);
+          const int c = (w / lanes) * G + (int)which[w % lanes];
+          if (c < nvec) offer(load_vector(x, c), c, bound);
         }
         if (nvec * V + lane < n) offer(x[nvec * V + lane], nvec * V + lane, bound);
         __syncthreads();
@@ -550,14 +661,19 @@ __global__ __launch_bounds__(G) void log_probs_top_kernel(LogProbsArgs a) {
   using S = typename Tr<DT>::S;
   __shared__ Space<C, G> space;
   __shared__ TopSpace<DT, G> list;
+  const int lane = threadIdx.x, n = a.g.n;
   int turn = 0;
   for (int64_t row = blockIdx.x; row < a.g.rows; row += gridDim.x, turn ^= 1) {
     Places p;
     row_starts(a.g, (uint32_t)row, a.o, p.at);
     const S *x = place<const S>(a, p, LP_X);
-    Top<DT, G> top(x, a.g.n, a.top, list);
-    const Statistics<C> z = statistics<DT, G, AHEAD>(x, a.g.n, threadIdx.x, turn, space, [&](C s) { top.begin(s); });
-    if (threadIdx.x == 0) give_statistics<DT>(a, p, x, z);
+    Top<DT, G> top(x, n, a.top, list);
+    Running<DT> r;
+    r.template take_row<G, AHEAD>(x, n, lane);
+    top.begin(r.m);
+    join_group<DT, G>(r, lane, turn, space);
+    const Statistics<C> z = finish<DT, G>(r, x, n, lane, space);
+    if (lane == 0) give_statistics<DT>(a, p, x, z);
     top.write(top.candidates(z.total == z.total), z, place<C>(a, p, LP_TOP_LOG_P), place<int32_t>(a, p, LP_TOP_TOKEN));
     __syncthreads();  // the list is free for the next row
   }
@@ -566,21 +682,23 @@ __global__ __launch_bounds__(G) void log_probs_top_kernel(LogProbsArgs a) {
 // ── host side ───────────────────────────────────────────────────────────────
 constexpr int64_t MOST_LANES = (int64_t)1 << 31;  // of a launch, which numbers them in 32 bits; groups go on to further rows
 
-// A row's lanes: eight where its vectors are no more, a wave up to four vectors a lane, then a block of four or of sixteen waves.
+// A row's lanes: eight where its vectors are no more, a wave up to four vectors a lane, a block of four waves up to eight, then one
+// of eight waves ([8192,50257] bfloat16: 141 us, 145 with four waves, 211 with sixteen, of which only two blocks are on a unit and
+// wait for each other's phases; five alternatives of [2048,50257] float32: 75, 81 and 97 us).
 template <int DT, class F>
 void by_length(int n, F &&f) {
   constexpr int V = VECTOR<typename Tr<DT>::S>;
   if (n <= 8 * V) f(std::integral_constant<int, 8>{});
   else if (n <= 4 * 64 * V) f(std::integral_constant<int, 64>{});
-  else if (n <= 4 * 256 * V) f(std::integral_constant<int, 256>{});
-  else f(std::integral_constant<int, 1024>{});
+  else if (n <= 8 * 256 * V) f(std::integral_constant<int, 256>{});
+  else f(std::integral_constant<int, 512>{});
 }
 dim3 row_blocks(const LogProbsArgs &a, int threads, int group) {
   const int64_t groups = threads / group;
   return dim3((unsigned)std::min((a.g.rows + groups - 1) / groups, MOST_LANES / threads));
 }
 template <int DT>
-void launch_score(nxh_context *ctx, const LogProbsArgs &a) {
+int launch_score(nxh_context *ctx, const LogProbsArgs &a) {
   by_length<DT>(a.g.n, [&](auto group) {
     constexpr int G = decltype(group)::value;
     if (!a.top) {
@@ -590,16 +708,29 @@ void launch_score(nxh_context *ctx, const LogProbsArgs &a) {
       hipLaunchKernelGGL((log_probs_top_kernel<DT, B>), row_blocks(a, B, B), dim3(B), 0, ctx->stream, a);
     }
   });
+  return NXH_OK;
 }
 template <int DT>
-void launch_with_grad(nxh_context *ctx, const LogProbsArgs &a) {
-  by_length<DT>(a.g.n, [&](auto group) {
-    constexpr int G = decltype(group)::value;
-    hipLaunchKernelGGL((log_probs_with_grad_kernel<DT, G>), row_blocks(a, group_threads(G), G), dim3(group_threads(G)), 0, ctx->stream, a);
-  });
+int launch_with_grad(nxh_context *ctx, const LogProbsArgs &a) {
+  constexpr int V = VECTOR<typename Tr<DT>::S>;
+  const int64_t units = ctx->compute_units > 0 ? ctx->compute_units : 256;
+  auto go = [&](auto group, auto vectors) {
+    constexpr int G = decltype(group)::value, T = group_threads(G), NV = decltype(vectors)::value;
+    // as many blocks as the chip has room for: some 120 registers a lane with eight vectors
+    const int64_t blocks = std::min((a.g.rows + T / G - 1) / (T / G), units * ((NV == 8 ? 1024 : 2048) / T));
+    hipLaunchKernelGGL((log_probs_with_grad_kernel<DT, G, NV>), dim3((unsigned)blocks), dim3(T), 0, ctx->stream, a);
+  };
+  const int nvec = a.g.n / V;
+  if (nvec <= 8) go(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
+  else if (nvec <= 4 * 64) go(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+  else if (DT != NXH_F64 && nvec <= 8 * 256) go(std::integral_constant<int, 256>{}, std::integral_constant<int, 8>{});
+  else if (DT != NXH_F64 && nvec <= 8 * 512) go(std::integral_constant<int, 512>{}, std::integral_constant<int, 8>{});
+  else if (DT != NXH_F64 && nvec <= 8 * 1024) go(std::integral_constant<int, 1024>{}, std::integral_constant<int, 8>{});
+  else hipLaunchKernelGGL((log_probs_with_grad_long_kernel<DT, 1024>), row_blocks(a, 1024, 1024), dim3(1024), 0, ctx->stream, a);
+  return NXH_OK;
 }
 template <int DT>
-void launch_grad(nxh_context *ctx, const LogProbsArgs &a) {
+int launch_grad(nxh_context *ctx, const LogProbsArgs &a) {
   constexpr int V = VECTOR<typename Tr<DT>::S>;
   auto go = [&](auto group) {
     constexpr int G = decltype(group)::value;
@@ -611,6 +742,7 @@ void launch_grad(nxh_context *ctx, const LogProbsArgs &a) {
   if (a.g.n <= 8 * V) go(std::integral_constant<int, 8>{});
   else if (a.g.n <= 4 * 64 * V) go(std::integral_constant<int, 64>{});
   else go(std::integral_constant<int, 256>{});
+  return NXH_OK;
 }
 
 // What the three calls check alike; false in *go where there is nothing to launch.
@@ -653,13 +785,8 @@ int start(nxh_context *ctx, const char *op, const char *path, LogProbsArgs &a) {
   nxh_set_path(path);
   return NXH_OK;
 }
-#define LP_BY_DTYPE(dt, f)                       \
-  do {                                           \
-    if ((dt) == NXH_F32) f<NXH_F32>(ctx, a);     \
-    else if ((dt) == NXH_BF16) f<NXH_BF16>(ctx, a); \
-    else if ((dt) == NXH_F16) f<NXH_F16>(ctx, a);   \
-    else f<NXH_F64>(ctx, a);                     \
-  } while (0)
+#define LP_BY_DTYPE(dt, f)                                                \
+  ((dt) == NXH_F32 ? f<NXH_F32>(ctx, a) : (dt) == NXH_BF16 ? f<NXH_BF16>(ctx, a) : (dt) == NXH_F16 ? f<NXH_F16>(ctx, a) : f<NXH_F64>(ctx, a))
 
 }  // namespace
 
@@ -697,7 +824,7 @@ NXH_EXPORT int nxh_log_probs(nxh_context *ctx, const nxh_tensor *log_p, const nx
   if (!go) return NXH_OK;
   std::lock_guard<std::mutex> guard(ctx->mu);
   if ((rc = start(ctx, op, a.top ? "log_probs_top" : "log_probs", a))) return rc;
-  LP_BY_DTYPE(logits->dtype, launch_score);
+  if ((rc = LP_BY_DTYPE(logits->dtype, launch_score))) return rc;
   NXH_HIP(op, hipGetLastError());
   return NXH_OK;
 }
@@ -721,7 +848,7 @@ NXH_EXPORT int nxh_log_probs_grad(nxh_context *ctx, const nxh_tensor *out, const
   if (!go) return NXH_OK;
   std::lock_guard<std::mutex> guard(ctx->mu);
   if ((rc = start(ctx, op, "log_probs_grad", a))) return rc;
-  LP_BY_DTYPE(logits->dtype, launch_grad);
+  if ((rc = LP_BY_DTYPE(logits->dtype, launch_grad))) return rc;
   NXH_HIP(op, hipGetLastError());
   return NXH_OK;
 }
@@ -744,7 +871,7 @@ NXH_EXPORT int nxh_log_probs_with_grad(nxh_context *ctx, const nxh_tensor *log_p
   if (!go) return NXH_OK;
   std::lock_guard<std::mutex> guard(ctx->mu);
   if ((rc = start(ctx, op, "log_probs_with_grad", a))) return rc;
-  LP_BY_DTYPE(logits->dtype, launch_with_grad);
+  if ((rc = LP_BY_DTYPE(logits->dtype, launch_with_grad))) return rc;
   NXH_HIP(op, hipGetLastError());
   return NXH_OK;
 }

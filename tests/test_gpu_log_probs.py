@@ -144,9 +144,11 @@ def everything(hip, oracle, d, hx, x, tokens, tops=(0,), what=""):
     check_gradient(hip.log_probs_grad(hg, hx, ht, peak, total, hge, entropy), want, g, ge, d, oracle, what + " entropy")
     for entropy_too in (False, True):
         lp, h, dx = hip.log_probs_with_grad(hg, hx, ht, hge if entropy_too else None)
-        same_bits(logical(lp), logical(hip.log_probs(hx, ht)[0]), "log_p beside the gradient")
-        same_bits(logical(h), logical(hip.log_probs(hx, ht)[1]), "entropy beside the gradient")
+        # (a row may have other lanes here than without the gradient, so its sums another order: the bounds above, not bits)
+        check_score((lp, h, peak, total), want, d, oracle, 0, f"{what} beside the gradient")
         check_gradient(dx, want, g, ge if entropy_too else None, d, oracle, what + " at once")
+        for a, b in zip((lp, h, dx), hip.log_probs_with_grad(hg, hx, ht, hge if entropy_too else None)):
+            same_bits(logical(a), logical(b), "equal calls at once")
 
 
 @pytest.mark.parametrize("d", FLOATS, ids=lambda d: d.name)
