@@ -163,7 +163,7 @@ void launch_rows(nxh_context *ctx, const LayerNormArgs &a) {
   const int nvec = (a.g.n + V - 1) / V;
 #define X(G, NV) \
   if (nvec <= G * NV) return launch<DT, G, NV>(ctx, a);
-  LN_GROUPS(X)
+  LN_GROUPS_FORWARD(X)
 #undef X
   const dim3 grid((unsigned)std::min<int64_t>(a.g.rows, ctx->compute_units > 0 ? ctx->compute_units : 256));
   hipLaunchKernelGGL((layer_norm_long_kernel<DT>), grid, dim3(LONG_THREADS), 0, ctx->stream, a);

@@ -36,23 +36,26 @@ __device__ __forceinline__ C across_groups(C v) {
   return v;
 }
 
+// Blocks of eight waves where a row has a wave or less: the block's sums are one row of partial sums, whatever the number of its groups.
+constexpr int lg_threads(int g) { return g > 64 ? g : 512; }
+
 template <int DT, int G, int NV, Rows R>
-__global__ __launch_bounds__(ln_threads(G)) void layer_norm_grad_kernel(LayerNormGradArgs a) {
+__global__ __launch_bounds__(lg_threads(G)) void layer_norm_grad_kernel(LayerNormGradArgs a) {
   using IO = Io<DT>;
   using C = typename IO::C;
   using S = typename IO::S;
-  constexpr int V = IO::V, T = ln_threads(G), GROUPS = T / G, W = T / 64;
+  constexpr int V = IO::V, T = lg_threads(G), GROUPS = T / G, W = T / 64;
   __shared__ C lds[G > 64 ? 2 * (G / 64) : 2 * W * G * V];
   const int lane = threadIdx.x % G, n = a.g.n, nvec = (n + V - 1) / V;
   const S *gamma = reinterpret_cast<const S *>(a.gamma);
   // Every lane loads for every v, a vector past the row as the row's last: a load under a condition is waited for before the next one.
   int c[NV];
-  Words gv[NV], xr[NV], gr[NV];
+  Words gain[NV], xr[NV], gr[NV];
   C dgamma[NV][V], dbeta[NV][V];
 #pragma unroll
   for (int v = 0; v < NV; v++) {
     c[v] = v * G + lane < nvec ? v * G + lane : nvec - 1;
-    gv[v] = gamma ? load_part<R>(gamma, c[v], n) : IO::all(1);
+    gain[v] = gamma ? load_part<R>(gamma, c[v], n) : IO::all(1);
 #pragma unroll
     for (int j = 0; j < V; j++) dgamma[v][j] = dbeta[v][j] = 0;
   }
@@ -63,35 +66,38 @@ __global__ __launch_bounds__(ln_threads(G)) void layer_norm_grad_kernel(LayerNor
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G, at[LG_OPERANDS];
   C mean = 0, rstd = 0;
-  auto request = [&](int64_t r) {  // row r's loads
+  const S *x = nullptr, *g = nullptr;
+  auto begin = [&](int64_t r) {
     row_starts(a.g, (uint32_t)r, a.o, at);
-    const S *x = reinterpret_cast<const S *>(a.o[LG_X].base) + at[LG_X];
-    const S *g = reinterpret_cast<const S *>(a.o[LG_G].base) + at[LG_G];
+    x = reinterpret_cast<const S *>(a.o[LG_X].base) + at[LG_X];
+    g = reinterpret_cast<const S *>(a.o[LG_G].base) + at[LG_G];
     mean = reinterpret_cast<const C *>(a.o[LG_MEAN].base)[at[LG_MEAN]];
     rstd = reinterpret_cast<const C *>(a.o[LG_RSTD].base)[at[LG_RSTD]];
-#pragma unroll
-    for (int v = 0; v < NV; v++) {
-      xr[v] = load_part<R>(x, c[v], n);
-      gr[v] = load_part<R>(g, c[v], n);
-    }
   };
-  if (row < a.g.rows) request(row);
+  auto request = [&](int v) {
+    xr[v] = load_part<R>(x, c[v], n);
+    gr[v] = load_part<R>(g, c[v], n);
+  };
+  if (row < a.g.rows) {
+    begin(row);
+#pragma unroll
+    for (int v = 0; v < NV; v++) request(v);
+  }
   for (; row < a.g.rows; row += step) {
-    S *dx = reinterpret_cast<S *>(const_cast<char *>(a.o[LG_DX].base)) + at[LG_DX];
     const C mu = mean, rs = rstd;
     C h[NV][V], w[NV][V], s[2] = {0, 0};
 #pragma unroll
     for (int v = 0; v < NV; v++) {
-      C x[V], g[V], gain[V];
-      IO::widen(xr[v], x);
-      IO::widen(gr[v], g);
-      IO::widen(gv[v], gain);
+      C gv[V], gw[V];
+      IO::widen(xr[v], h[v]);
+      IO::widen(gr[v], gv);
+      IO::widen(gain[v], gw);
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        h[v][j] = (x[j] - mu) * rs;
-        w[v][j] = g[j] * gain[j];
-        dgamma[v][j] = fused(g[j], h[v][j], dgamma[v][j]);  // (of a lane with no vector v: never looked at)
-        dbeta[v][j] = dbeta[v][j] + g[j];
+        h[v][j] = (h[v][j] - mu) * rs;
+        w[v][j] = gv[j] * gw[j];
+        dgamma[v][j] = fused(gv[j], h[v][j], dgamma[v][j]);  // (of a lane with no vector v: never looked at)
+        dbeta[v][j] = dbeta[v][j] + gv[j];
       }
       if (v * G + lane < nvec)
 #pragma unroll
@@ -101,17 +107,18 @@ __global__ __launch_bounds__(ln_threads(G)) void layer_norm_grad_kernel(LayerNor
           s[1] = fused(own ? w[v][j] : 0, own ? h[v][j] : 0, s[1]);
         }
     }
-    const int64_t next = row + step < a.g.rows ? row + step : row;  // (a last row is requested twice: no condition here either)
-    request(next);  // in flight while this row is finished
+    S *dx = reinterpret_cast<S *>(const_cast<char *>(a.o[LG_DX].base)) + at[LG_DX];
+    begin(row + step < a.g.rows ? row + step : row);  // (behind the last row its own again, for nothing)
+#pragma unroll
+    for (int v = 0; v < NV; v++) request(v);  // in flight while this row is finished
     group_combine<G>(s, Sum<C>{}, lds);
     if (a.o[LG_DX].base) {
       const C c1 = s[0] / count, c2 = s[1] / count;
 #pragma unroll
       for (int v = 0; v < NV; v++) {
-        C d[V];
 #pragma unroll
-        for (int j = 0; j < V; j++) d[j] = rs * fused(-h[v][j], c2, w[v][j] - c1);
-        if (v * G + lane < nvec) store_part<R>(dx, c[v], n, IO::narrow(d));
+        for (int j = 0; j < V; j++) w[v][j] = rs * fused(-h[v][j], c2, w[v][j] - c1);
+        if (v * G + lane < nvec) store_part<R>(dx, c[v], n, IO::narrow(w[v]));
       }
     }
   }
@@ -122,8 +129,8 @@ __global__ __launch_bounds__(ln_threads(G)) void layer_norm_grad_kernel(LayerNor
     for (int v = 0; v < NV; v++)
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        const int c = v * G + lane, column = vec_start<V, R>(c, n) + j;
-        if (c < nvec && vec_owns<V, R>(c, j, n)) {
+        const int i = v * G + lane, column = vec_start<V, R>(i, n) + j;
+        if (i < nvec && vec_owns<V, R>(i, j, n)) {
           mine[column] = dgamma[v][j];
           mine[n + column] = dbeta[v][j];
         }
@@ -132,7 +139,7 @@ __global__ __launch_bounds__(ln_threads(G)) void layer_norm_grad_kernel(LayerNor
     const int wave = threadIdx.x >> 6;
 #pragma unroll
     for (int v = 0; v < NV; v++) {
-      __syncthreads();
+      if (v > 0) __syncthreads();
 #pragma unroll
       for (int j = 0; j < V; j++) {
         const C p = across_groups<G>(dgamma[v][j]), q = across_groups<G>(dbeta[v][j]);
@@ -146,8 +153,8 @@ __global__ __launch_bounds__(ln_threads(G)) void layer_norm_grad_kernel(LayerNor
         C s = lds[e];
 #pragma unroll
         for (int k = 1; k < W; k++) s = s + lds[k * 2 * G * V + e];
-        const int c = v * G + e % (G * V) / V, j = e % V;
-        if (c < nvec && vec_owns<V, R>(c, j, n)) mine[(e / (G * V)) * n + vec_start<V, R>(c, n) + j] = s;
+        const int i = v * G + e % (G * V) / V, j = e % V;
+        if (i < nvec && vec_owns<V, R>(i, j, n)) mine[(e / (G * V)) * n + vec_start<V, R>(i, n) + j] = s;
       }
     }
   }
@@ -245,7 +252,8 @@ __global__ __launch_bounds__(256) void layer_norm_columns_kernel(LayerNormGradAr
 }
 
 // ── the partial sums ────────────────────────────────────────────────────────
-// 32 columns of a block, 32 lanes to each: a lane adds every 32nd partial sum, then the lanes' sums are added in order.
+// 32 columns of a block: a lane adds a vector of them from every 128th partial sum (every 64th of float64), and the lanes' sums are
+// added in order.
 struct JoinArgs {
   const void *partials;
   int64_t blocks;
@@ -258,23 +266,42 @@ __global__ __launch_bounds__(1024) void layer_norm_join_kernel(JoinArgs a) {
   using IO = Io<DT>;
   using C = typename IO::C;
   using S = typename IO::S;
-  __shared__ C lds[32][33];
-  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
-  const int64_t column = (int64_t)blockIdx.x * 32 + lane;
+  constexpr int V = VECTOR<C>, LANES = 32 / V, PARTS = 1024 / LANES, W = 16;
+  __shared__ C lds[W][32];
+  const int lane = threadIdx.x % LANES, part = threadIdx.x / LANES;
+  const int64_t columns = 2 * (int64_t)a.n, first = (int64_t)blockIdx.x * 32 + lane * V;
   const C *p = reinterpret_cast<const C *>(a.partials);
-  C s = 0;
-  if (column < 2 * (int64_t)a.n)
-#pragma unroll 8
-    for (int64_t b = part; b < a.blocks; b += 32) s = s + p[b * 2 * a.n + column];
-  lds[part][lane] = s;
-  __syncthreads();
-  if (part != 0 || column >= 2 * (int64_t)a.n) return;
+  C s[V];
 #pragma unroll
-  for (int k = 1; k < 32; k++) s = s + lds[k][lane];
+  for (int j = 0; j < V; j++) s[j] = 0;
+  if (first + V <= columns) {
+#pragma unroll 4
+    for (int64_t b = part; b < a.blocks; b += PARTS) {
+      struct Elements { C x[V]; } e = __builtin_bit_cast(Elements, load_words(p + b * columns + first));
+#pragma unroll
+      for (int j = 0; j < V; j++) s[j] = s[j] + e.x[j];
+    }
+  } else {
+    for (int64_t b = part; b < a.blocks; b += PARTS)
+#pragma unroll
+      for (int j = 0; j < V; j++)
+        if (first + j < columns) s[j] = s[j] + p[b * columns + first + j];
+  }
+#pragma unroll
+  for (int j = 0; j < V; j++) {
+    s[j] = across_groups<LANES>(s[j]);
+    if ((threadIdx.x & 63) < LANES) lds[threadIdx.x >> 6][lane * V + j] = s[j];
+  }
+  __syncthreads();
+  const int64_t column = (int64_t)blockIdx.x * 32 + threadIdx.x;
+  if (threadIdx.x >= 32 || column >= columns) return;
+  C sum = lds[0][threadIdx.x];
+#pragma unroll
+  for (int w = 1; w < W; w++) sum = sum + lds[w][threadIdx.x];
   const int which = column >= a.n;
   char *out = which ? a.out[1] : a.out[0];
   const int64_t stride = which ? a.stride[1] : a.stride[0];
-  if (out) reinterpret_cast<S *>(out)[(column - (which ? a.n : 0)) * stride] = IO::st(s);
+  if (out) reinterpret_cast<S *>(out)[(column - (which ? a.n : 0)) * stride] = IO::st(sum);
 }
 
 // ── host side ───────────────────────────────────────────────────────────────
@@ -286,8 +313,8 @@ template <int DT, int G, int NV>
 void launch(nxh_context *ctx, const LayerNormGradArgs &a, int64_t blocks) {
   constexpr int V = Io<DT>::V;
   const dim3 grid((unsigned)blocks);
-  if (a.g.n % V == 0) hipLaunchKernelGGL((layer_norm_grad_kernel<DT, G, NV, WHOLE>), grid, dim3(ln_threads(G)), 0, ctx->stream, a);
-  else hipLaunchKernelGGL((layer_norm_grad_kernel<DT, G, NV, G * NV == 1 ? SHORT : RAGGED>), grid, dim3(ln_threads(G)), 0, ctx->stream, a);
+  if (a.g.n % V == 0) hipLaunchKernelGGL((layer_norm_grad_kernel<DT, G, NV, WHOLE>), grid, dim3(lg_threads(G)), 0, ctx->stream, a);
+  else hipLaunchKernelGGL((layer_norm_grad_kernel<DT, G, NV, G * NV == 1 ? SHORT : RAGGED>), grid, dim3(lg_threads(G)), 0, ctx->stream, a);
 }
 template <int DT>
 void launch_long(nxh_context *ctx, const LayerNormGradArgs &a, int64_t blocks) {
@@ -307,7 +334,7 @@ Plan plan(nxh_context *ctx, int n, int64_t rows) {
   const int nvec = (n + V - 1) / V;
 #define X(G, NV)                                                                                                \
   if (nvec <= G * NV)                                                                                           \
-    return {launch<DT, G, NV>, std::min((rows + ln_threads(G) / G - 1) / (ln_threads(G) / G), 2 * units)};
+    return {launch<DT, G, NV>, std::min((rows + lg_threads(G) / G - 1) / (lg_threads(G) / G), units * (G == 256 ? 2 : 1))};
   LN_GROUPS(X)
 #undef X
   const int64_t tiles = (nvec + 255) / 256;
@@ -354,7 +381,7 @@ NXH_EXPORT int nxh_layer_norm_grad(nxh_context *ctx, const nxh_tensor *dx, const
   std::lock_guard<std::mutex> guard(ctx->mu);
   NXH_HIP(op, hipSetDevice(ctx->device));
   const bool weights = dgamma || dbeta;
-  nxh_set_path(a.g.n > LN_VECTORS * (16 / es) ? "layer_norm_grad_long" : "layer_norm_grad");
+  nxh_set_path(a.g.n > LN_VECTORS_GRAD * (16 / es) ? "layer_norm_grad_long" : "layer_norm_grad");
   Plan p{nullptr, 0};  // no rows: sums of nothing
   if (a.g.rows > 0)
     p = dt == NXH_F32 ? plan<NXH_F32>(ctx, a.g.n, a.g.rows) : dt == NXH_BF16 ? plan<NXH_BF16>(ctx, a.g.n, a.g.rows)

@@ -721,12 +721,22 @@ int launch_with_grad(nxh_context *ctx, const LogProbsArgs &a) {
     hipLaunchKernelGGL((log_probs_with_grad_kernel<DT, G, NV>), dim3((unsigned)blocks), dim3(T), 0, ctx->stream, a);
   };
   const int nvec = a.g.n / V;
-  if (nvec <= 8) go(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
-  else if (nvec <= 4 * 64) go(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
-  else if (DT != NXH_F64 && nvec <= 8 * 256) go(std::integral_constant<int, 256>{}, std::integral_constant<int, 8>{});
-  else if (DT != NXH_F64 && nvec <= 8 * 512) go(std::integral_constant<int, 512>{}, std::integral_constant<int, 8>{});
-  else if (DT != NXH_F64 && nvec <= 8 * 1024) go(std::integral_constant<int, 1024>{}, std::integral_constant<int, 8>{});
-  else hipLaunchKernelGGL((log_probs_with_grad_long_kernel<DT, 1024>), row_blocks(a, 1024, 1024), dim3(1024), 0, ctx->stream, a);
+  if (nvec <= 8) {
+    go(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
+    return NXH_OK;
+  }
+  if (nvec <= 4 * 64) {
+    go(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+    return NXH_OK;
+  }
+  if constexpr (DT != NXH_F64) {  // (float64 has no registers for more)
+    std::integral_constant<int, 8> eight;
+    if (nvec <= 8 * 256) go(std::integral_constant<int, 256>{}, eight);
+    else if (nvec <= 8 * 512) go(std::integral_constant<int, 512>{}, eight);
+    else if (nvec <= 8 * 1024) go(std::integral_constant<int, 1024>{}, eight);
+    if (nvec <= 8 * 1024) return NXH_OK;
+  }
+  hipLaunchKernelGGL((log_probs_with_grad_long_kernel<DT, 1024>), row_blocks(a, 1024, 1024), dim3(1024), 0, ctx->stream, a);
   return NXH_OK;
 }
 template <int DT>
