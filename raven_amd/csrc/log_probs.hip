@@ -453,20 +453,19 @@ struct Highest {
   __device__ __forceinline__ T operator()(T a, T b) const { return a > b ? a : b; }
 };
 
-// alternatives at most; places on the list of candidates (a block's lanes at least); lanes that may hold candidates
-constexpr int TOP_MAX = 64, TOP_CANDIDATES = 1024, TOP_LANES = 5 * TOP_MAX;
+constexpr int TOP_MAX = 64;  // alternatives
 
 template <int DT, int G>
 struct TopSpace {
-  static_assert(G <= TOP_CANDIDATES, "a place for every lane");
   using T = typename KeyOf<typename Tr<DT>::C>::T;
-  T key[TOP_CANDIDATES];
-  uint32_t index[TOP_CANDIDATES], lane[TOP_LANES], few[64];
-  T lane_key[TOP_LANES], low[G / 64];
+  static constexpr int PLACES = G > 64 ? 1024 : 512, LANES = G > 64 ? 5 * TOP_MAX : 64;  // of candidates; of lanes that may hold them
+  T key[PLACES];
+  uint32_t index[PLACES], lane[LANES], few[64];
+  T lane_key[LANES], few_key[64], low[G / 64];
   int part[G / 64], lanes, found;
 };
 
-// Of each wave's lanes the k / W, rounded up, with the largest elements: the least of those k bounds the k-th largest element
+// Of each of W waves' lanes the k / W, rounded up, with the largest elements: the least of those k bounds the k-th largest element
 // of the row from below, and only lanes whose largest reaches it hold candidates: one or two times k in a row without
 // order, of which, where they are few, the k largest are found. All lanes together look through those lanes' elements. Ties (a row of equal logits, a vocabulary that is banned but for a few tokens) can make candidates of the
 // whole row: then what lies above the bound is taken, and of what equals it the first in the row. A row whose large elements
@@ -477,7 +476,7 @@ struct Top {
   using C = typename IO::C;
   using S = typename IO::S;
   using T = typename KeyOf<C>::T;
-  static constexpr int V = IO::V, W = G / 64;
+  static constexpr int V = IO::V, W = G / 64, PLACES = TopSpace<DT, G>::PLACES, LANES = TopSpace<DT, G>::LANES;
   const S *x;
   int n, k;
   TopSpace<DT, G> &l;
@@ -486,40 +485,93 @@ struct Top {
 
   __device__ __forceinline__ Top(const S *row, int length, int top, TopSpace<DT, G> &space) : x(row), n(length), k(top), l(space) {}
 
-  // give(place, key, index), by one lane, for each of the first m entries of the list: a wave takes an entry and its lanes
-  // compare it with four each, which they hold (read again for each entry, 256 of them took 40 us).
+  // give(place, key, index) for the k largest of the first m entries of the list. A wave's lanes hold an entry each and count the
+  // larger ones. Of 65 to 256 entries each wave takes its share, an entry at a time, against four that each lane holds. Of more, the k-th
+  // is found first, bit by bit of key and index (all of 256 against all others, read again for each, took 40 us).
   template <class F>
   __device__ __forceinline__ void rank(int m, F &&give) const {
-    constexpr int Q = 4;
-    auto entry = [&](int j, T &key, uint32_t &index) {
-      key = j < m ? l.key[j] : 0;
-      index = j < m ? l.index[j] : ~0u;  // (before nothing)
-    };
-    T key[Q];
-    uint32_t index[Q];
+    if (W > 1 && m > 64 && m <= 256) {
+      constexpr int Q = 4;
+      T key[Q];
+      uint32_t index[Q];
 #pragma unroll
-    for (int q = 0; q < Q; q++) entry(q * 64 + (lane & 63), key[q], index[q]);
-    for (int i = wave; i < m; i += W) {
-      const T mine = l.key[i];
-      const uint32_t at = l.index[i];
-      int place = 0;
-#pragma unroll
-      for (int q = 0; q < Q; q++)
-        if (q * 64 < m) place += __popcll(__ballot(key[q] > mine || (key[q] == mine && index[q] < at)));
-      for (int j = Q * 64; j < m; j += 64) {
-        T k;
-        uint32_t n;
-        entry(j + (lane & 63), k, n);
-        place += __popcll(__ballot(k > mine || (k == mine && n < at)));
+      for (int q = 0; q < Q; q++) {
+        const int j = q * 64 + (lane & 63);
+        key[q] = j < m ? l.key[j] : 0;
+        index[q] = j < m ? l.index[j] : ~0u;  // (before nothing)
       }
-      if ((lane & 63) == 0) give(place, mine, at);
+      for (int i = wave; i < m; i += W) {
+        const T mine = l.key[i];
+        const uint32_t at = l.index[i];
+        int place = 0;
+#pragma unroll
+        for (int q = 0; q < Q; q++)
+          if (q * 64 < m) place += __popcll(__ballot(key[q] > mine || (key[q] == mine && index[q] < at)));
+        if ((lane & 63) == 0 && place < k) give(place, mine, at);
+      }
+      return;
     }
+    if (wave != 0) return;
+    T key = 0;
+    uint32_t index = 0;
+    int count = m;
+    if (m <= 64) {
+      if (lane < m) {
+        key = l.key[lane];
+        index = l.index[lane];
+      }
+    } else {
+      auto number = [&](auto &&is) {
+        int c = 0;
+        for (int j = lane; j - lane < m; j += 64) c += __popcll(__ballot(j < m && is(l.key[j], l.index[j])));
+        return c;
+      };
+      T bound = 0;
+      for (int bit = 8 * (int)sizeof(T) - 1; bit >= 0; bit--) {
+        const T next = bound | (T)1 << bit;
+        if (number([&](T e, uint32_t) { return e >= next; }) >= k) bound = next;
+      }
+      const int equal = k - number([&](T e, uint32_t) { return e > bound; });  // so many of those at the bound, the first ones
+      uint32_t last = 0;
+      for (int bit = 23; bit >= 0; bit--) {
+        const uint32_t next = last | 1u << bit;
+        if (number([&](T e, uint32_t i) { return e == bound && i < next; }) < equal) last = next;
+      }
+      count = 0;
+      for (int j = lane; j - lane < m; j += 64) {
+        const T e = j < m ? l.key[j] : 0;
+        const uint32_t i = j < m ? l.index[j] : ~0u;
+        const bool is = e > bound || (e == bound && i <= last);
+        const uint64_t all = __ballot(is);
+        if (is) {
+          const int place = count + __popcll(all & (((uint64_t)1 << lane) - 1));
+          l.few_key[place] = e;
+          l.few[place] = i;
+        }
+        count += __popcll(all);
+      }
+      __builtin_amdgcn_wave_barrier();
+      if (lane < count) {
+        key = l.few_key[lane];
+        index = l.few[lane];
+      }
+    }
+    int place = 0;
+    for (int j = 0; j < count; j++) {
+      const T other = lane_value(key, j);
+      place += other > key || (other == key && (uint32_t)__builtin_amdgcn_readlane((int)index, j) < index);
+    }
+    if (lane < count && place < k) give(place, key, index);
+  }
+  __device__ __forceinline__ static uint32_t lane_value(uint32_t v, int j) { return (uint32_t)__builtin_amdgcn_readlane((int)v, j); }
+  __device__ __forceinline__ static uint64_t lane_value(uint64_t v, int j) {
+    return (uint64_t)lane_value((uint32_t)(v >> 32), j) << 32 | lane_value((uint32_t)v, j);
   }
   __device__ __forceinline__ void offer(S raw, int i, T least) {
     const T key = key_of(IO::ld(raw));
     if (key >= least) {
       const int at = atomicAdd(&l.found, 1);
-      if (at < TOP_CANDIDATES) {
+      if (at < PLACES) {
         l.key[at] = key;
         l.index[at] = (uint32_t)i;
       }
@@ -530,15 +582,19 @@ struct Top {
 #pragma unroll
     for (int j = 0; j < V; j++) offer(e.x[j], c * V + j, least);
   }
-  // Before the barrier of the statistics: the wave's part in the bound.
+  // Before the barrier of the statistics: the wave's part in the bound. Waves that are not full of vectors take no part in it; of a
+  // row that one wave holds every lane with an element is looked at.
   __device__ __forceinline__ void begin(C seen) {
-    mine = lane < n / V || n / V * V + lane < n ? key_of(seen) : 0;
-    const int rounds = (k + W - 1) / W;
-    T most = 0, left = mine;
-    for (int r = 0; r < rounds; r++) {
-      most = lanes_combine<64>(left, Highest<T>{});
-      const uint64_t have = __ballot(left == most);
-      if ((lane & 63) == __builtin_ctzll(have)) left = 0;
+    const int nvec = n / V, full = nvec <= 64 ? 0 : nvec / 64 < W ? nvec / 64 : W;
+    mine = lane < nvec || nvec * V + lane < n ? key_of(seen) : 0;
+    T most = full ? ~(T)0 : 1;
+    if (wave < full) {
+      T left = mine;
+      for (int r = 0; r * full < k; r++) {
+        most = lanes_combine<64>(left, Highest<T>{});
+        const uint64_t have = __ballot(left == most);
+        if ((lane & 63) == __builtin_ctzll(have)) left = 0;
+      }
     }
     if ((lane & 63) == 0) l.low[wave] = most;
     if (lane == 0) l.lanes = l.found = 0;
@@ -594,14 +650,14 @@ struct Top {
   // After the barrier of the statistics: the list holds the k largest elements, and others; how many.
   __device__ __forceinline__ int candidates(bool ordered) {
     T bound = 0;
-    int found = TOP_CANDIDATES + 1;
+    int found = PLACES + 1;
     if (ordered) {
       bound = l.low[0];
 #pragma unroll
       for (int w = 1; w < W; w++) bound = l.low[w] < bound ? l.low[w] : bound;
       if (mine >= bound) {
         const int at = atomicAdd(&l.lanes, 1);
-        if (at < TOP_LANES) {
+        if (at < LANES) {
           l.lane[at] = (uint32_t)lane;
           l.lane_key[at] = mine;
         }
@@ -610,21 +666,22 @@ struct Top {
       int lanes = l.lanes;
       const uint32_t *which = l.lane;
       if (lanes <= 64) {  // each wave by itself finds the k-th largest of them, down to the bits that a 16-bit dtype has
+        constexpr int bits = 8 * (int)sizeof(T);
         const int i = lane & 63;
         const T key = i < lanes ? l.lane_key[i] : 0;
-        bound = 0;
-        constexpr int bits = 8 * (int)sizeof(T);
+        T kth = 0;
 #pragma unroll
         for (int bit = bits - 1; bit >= (sizeof(S) == 2 ? bits - 20 : 0); bit--) {
-          const T next = bound | (T)1 << bit;
-          if (__popcll(__ballot(key >= next)) >= k) bound = next;
+          const T next = kth | (T)1 << bit;
+          if (__popcll(__ballot(key >= next)) >= k) kth = next;
         }
+        if (kth > bound) bound = kth;
         const uint64_t reach = __ballot(i < lanes && key >= bound);
         if (reach >> i & 1) l.few[__popcll(reach & (((uint64_t)1 << i) - 1))] = l.lane[i];  // (the same of every wave)
         lanes = __popcll(reach);
         which = l.few;
       }
-      if (lanes <= TOP_LANES) {
+      if (lanes <= LANES) {
         const int nvec = n / V, each = (nvec + G - 1) / G;
         for (int w = lane; w < lanes * each; w += G) {
           const int c = (w / lanes) * G + (int)which[w % lanes];
@@ -633,11 +690,11 @@ struct Top {
         if (nvec * V + lane < n) offer(x[nvec * V + lane], nvec * V + lane, bound);
         __syncthreads();
         found = l.found;
-        if (found <= TOP_CANDIDATES) return found;
+        if (found <= PLACES) return found;
       }
       found = collect(bound + 1);
     }
-    if (found > TOP_CANDIDATES) {
+    if (found > PLACES) {
       bound = by_bits();
       found = collect(bound + 1);  // fewer than k
     }
@@ -647,10 +704,8 @@ struct Top {
   }
   __device__ __forceinline__ void write(int found, const Statistics<C> &z, C *log_p, int32_t *tokens) const {
     rank(found, [&](int place, T key, uint32_t index) {
-      if (place < k) {
-        log_p[place] = value_of<C>(key) - z.peak - z.log_total;
-        tokens[place] = (int32_t)index;
-      }
+      log_p[place] = value_of<C>(key) - z.peak - z.log_total;
+      tokens[place] = (int32_t)index;
     });
   }
 };
@@ -672,6 +727,7 @@ __global__ __launch_bounds__(G) void log_probs_top_kernel(LogProbsArgs a) {
     r.template take_row<G, AHEAD>(x, n, lane);
     top.begin(r.m);
     join_group<DT, G>(r, lane, turn, space);
+    if constexpr (G == 64) __syncthreads();  // (what begin wrote is there)
     const Statistics<C> z = finish<DT, G>(r, x, n, lane, space);
     if (lane == 0) give_statistics<DT>(a, p, x, z);
     top.write(top.candidates(z.total == z.total), z, place<C>(a, p, LP_TOP_LOG_P), place<int32_t>(a, p, LP_TOP_TOKEN));
@@ -679,7 +735,92 @@ __global__ __launch_bounds__(G) void log_probs_top_kernel(LogProbsArgs a) {
   }
 }
 
+// ── few long rows ───────────────────────────────────────────────────────────
+// Rows that would leave most of the chip idle are cut into parts, a block to each: a part's sums and its own most likely tokens, in their
+// order, go to memory, and a block for each row joins them.
+constexpr int PART_LANES = 256, JOIN_LANES = 1024, PARTS_MAX = 16;
+struct Parts {
+  void *sums;       // [rows][3][parts]
+  void *keys;       // [rows][parts][top]
+  uint32_t *index;  // [rows][parts][top]
+  void *values;     // [3][rows]: peak, total and entropy for the gradient; null: not wanted
+  int parts, share;  // vectors of a part; the last has the elements behind the last vector too
+};
+template <int DT>
+__global__ __launch_bounds__(PART_LANES) void log_probs_parts_kernel(LogProbsArgs a, Parts q) {
+  using C = typename Tr<DT>::C;
+  using S = typename Tr<DT>::S;
+  using T = typename KeyOf<C>::T;
+  constexpr int G = PART_LANES, V = VECTOR<S>;
+  __shared__ Space<C, G> space;
+  __shared__ TopSpace<DT, G> list;
+  const int lane = threadIdx.x, part = blockIdx.x;
+  const int64_t row = blockIdx.y;
+  Places p;
+  row_starts(a.g, (uint32_t)row, a.o, p.at);
+  const int first = part * q.share * V, n = part + 1 == q.parts ? a.g.n - first : q.share * V;
+  const S *x = place<const S>(a, p, LP_X) + first;
+  Top<DT, G> top(x, n, a.top, list);
+  Running<DT> r;
+  r.template take_row<G, AHEAD>(x, n, lane);
+  if (a.top) top.begin(r.m);
+  join_group<DT, G>(r, lane, 0, space);
+  if (lane == 0) r.store(reinterpret_cast<C *>(q.sums) + row * 3 * q.parts + part, q.parts);
+  if (!a.top) return;
+  const int64_t at = (row * q.parts + part) * a.top;
+  top.rank(top.candidates(r.s == r.s), [&](int place, T key, uint32_t index) {
+    reinterpret_cast<T *>(q.keys)[at + place] = key;
+    q.index[at + place] = index + (uint32_t)first;
+  });
+}
+template <int DT>
+__global__ __launch_bounds__(JOIN_LANES) void log_probs_join_kernel(LogProbsArgs a, Parts q) {
+  using C = typename Tr<DT>::C;
+  using S = typename Tr<DT>::S;
+  using T = typename KeyOf<C>::T;
+  constexpr int G = JOIN_LANES;
+  __shared__ Space<C, G> space;
+  __shared__ TopSpace<DT, G> list;
+  const int lane = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  Places p;
+  row_starts(a.g, (uint32_t)row, a.o, p.at);
+  const S *x = place<const S>(a, p, LP_X);
+  // The row's k-th is bounded from below by any part's k-th, and by the least of the parts' k / parts-th, rounded up.
+  const T *keys = reinterpret_cast<const T *>(q.keys) + row * q.parts * a.top;
+  const int offered = q.parts * a.top, part = lane % PARTS_MAX;
+  T bound = 0;
+  if (a.top) {
+    const bool has = part < q.parts;
+    const T kth = lanes_combine<PARTS_MAX>(has ? keys[(part + 1) * a.top - 1] : 0, Highest<T>{});
+    const T share = ~lanes_combine<PARTS_MAX>(has ? ~keys[part * a.top + (a.top - 1) / q.parts] : 0, Highest<T>{});
+    bound = kth > share ? kth : share;
+  }
+  if (lane == 0) list.found = 0;
+  __syncthreads();
+  if (lane < offered && keys[lane] >= bound) {  // (at most 16 * 64 = JOIN_LANES, and as many places)
+    const int at = atomicAdd(&list.found, 1);
+    list.key[at] = keys[lane];
+    list.index[at] = q.index[row * offered + lane];
+  }
+  Running<DT> r;
+  if (part < q.parts) r.load(reinterpret_cast<const C *>(q.sums) + row * 3 * q.parts + part, q.parts);
+  r.template join<PARTS_MAX>();
+  const Statistics<C> z = finish<DT, G>(r, x, a.g.n, lane, space);
+  if (lane == 0) {
+    give_statistics<DT>(a, p, x, z);
+    if (C *v = reinterpret_cast<C *>(q.values)) {
+      v[row] = z.peak;
+      v[a.g.rows + row] = z.total;
+      v[2 * a.g.rows + row] = z.entropy;
+    }
+  }
+  __syncthreads();
+  Top<DT, G>(x, a.g.n, a.top, list).write(list.found, z, place<C>(a, p, LP_TOP_LOG_P), place<int32_t>(a, p, LP_TOP_TOKEN));
+}
+
 // ── host side ───────────────────────────────────────────────────────────────
+constexpr int PART_VECTORS = 16 * 512;  // of rows that are not cut
 constexpr int64_t MOST_LANES = (int64_t)1 << 31;  // of a launch, which numbers them in 32 bits; groups go on to further rows
 
 // A row's lanes: eight where its vectors are no more, a wave up to four vectors a lane, a block of four waves up to eight, then one
@@ -697,22 +838,88 @@ dim3 row_blocks(const LogProbsArgs &a, int threads, int group) {
   const int64_t groups = threads / group;
   return dim3((unsigned)std::min((a.g.rows + groups - 1) / groups, MOST_LANES / threads));
 }
+// How many parts a row is cut into; 1: not at all. A block of 512 lanes for a row of 2^16 bfloat16 elements has the time of two more
+// launches left in it.
+template <int DT>
+int parts_of(nxh_context *ctx, const LogProbsArgs &a) {
+  const int64_t units = ctx->compute_units > 0 ? ctx->compute_units : 256, nvec = a.g.n / VECTOR<typename Tr<DT>::S>;
+  if (nvec <= PART_VECTORS || a.g.rows * 4 > units) return 1;
+  return (int)std::min<int64_t>(std::min<int64_t>(PARTS_MAX, 2 * units / a.g.rows), nvec / (2 * PART_LANES));
+}
+// The statistics and most likely tokens of rows in parts. values: room for [3][rows], or null.
+template <int DT>
+int launch_parts(nxh_context *ctx, const LogProbsArgs &a, int parts, void *values) {
+  using C = typename Tr<DT>::C;
+  const int nvec = a.g.n / VECTOR<typename Tr<DT>::S>;
+  Parts q;
+  q.share = (nvec + parts - 1) / parts;
+  q.parts = (nvec + q.share - 1) / q.share;
+  q.values = values;
+  const size_t sums = (size_t)a.g.rows * 3 * q.parts * sizeof(C), list = (size_t)a.g.rows * q.parts * a.top;
+  void *space = nullptr;
+  if (int rc = nxh_alloc_locked(ctx, sums + list * (sizeof(typename KeyOf<C>::T) + 4), &space)) return rc;
+  q.sums = space;
+  q.keys = (char *)space + sums;
+  q.index = (uint32_t *)((char *)q.keys + list * sizeof(typename KeyOf<C>::T));
+  hipLaunchKernelGGL((log_probs_parts_kernel<DT>), dim3((unsigned)q.parts, (unsigned)a.g.rows), dim3(PART_LANES), 0, ctx->stream, a, q);
+  hipLaunchKernelGGL((log_probs_join_kernel<DT>), dim3((unsigned)a.g.rows), dim3(JOIN_LANES), 0, ctx->stream, a, q);
+  nxh_free_locked(ctx, space);  // (the stream orders its next use behind these launches)
+  return NXH_OK;
+}
 template <int DT>
 int launch_score(nxh_context *ctx, const LogProbsArgs &a) {
+  if (const int parts = parts_of<DT>(ctx, a); parts > 1) return launch_parts<DT>(ctx, a, parts, nullptr);
   by_length<DT>(a.g.n, [&](auto group) {
     constexpr int G = decltype(group)::value;
     if (!a.top) {
       hipLaunchKernelGGL((log_probs_kernel<DT, G>), row_blocks(a, group_threads(G), G), dim3(group_threads(G)), 0, ctx->stream, a);
     } else {
-      constexpr int B = group_threads(G);
+      constexpr int B = G > 64 ? G : 64;
       hipLaunchKernelGGL((log_probs_top_kernel<DT, B>), row_blocks(a, B, B), dim3(B), 0, ctx->stream, a);
     }
   });
   return NXH_OK;
 }
 template <int DT>
-int launch_with_grad(nxh_context *ctx, const LogProbsArgs &a) {
+int launch_grad(nxh_context *ctx, const LogProbsArgs &a) {
   constexpr int V = VECTOR<typename Tr<DT>::S>;
+  auto go = [&](auto group) {
+    constexpr int G = decltype(group)::value;
+    const int parts = std::max(1, (a.g.n / V + G * AHEAD - 1) / (G * AHEAD));  // (at most 2^14)
+    const int64_t rows = (a.g.rows + 256 / G - 1) / (256 / G);
+    const dim3 grid((unsigned)parts, (unsigned)std::min(rows, std::min<int64_t>(65535, MOST_LANES / 256 / parts)));
+    hipLaunchKernelGGL((log_probs_grad_kernel<DT, G>), grid, dim3(256), 0, ctx->stream, a);
+  };
+  if (a.g.n <= 8 * V) go(std::integral_constant<int, 8>{});
+  else if (a.g.n <= 4 * 64 * V) go(std::integral_constant<int, 64>{});
+  else go(std::integral_constant<int, 256>{});
+  return NXH_OK;
+}
+
+template <int DT>
+int launch_with_grad(nxh_context *ctx, const LogProbsArgs &a) {
+  using C = typename Tr<DT>::C;
+  constexpr int V = VECTOR<typename Tr<DT>::S>;
+  if (const int parts = parts_of<DT>(ctx, a); parts > 1) {
+    void *values = nullptr;
+    if (int rc = nxh_alloc_locked(ctx, (size_t)a.g.rows * 3 * sizeof(C), &values)) return rc;
+    int rc = launch_parts<DT>(ctx, a, parts, values);
+    if (!rc) {
+      LogProbsArgs b = a;
+      for (int k = 0; k < 3; k++) {
+        RowOperand &o = b.o[k == 2 ? LP_ENTROPY : LP_PEAK + k];
+        o.base = (const char *)values + (size_t)k * a.g.rows * sizeof(C);
+        int64_t stride = 1;
+        for (int d = a.g.nouter - 1; d >= 0; d--) {
+          o.stride[d] = stride;
+          stride *= a.g.oshape[d];
+        }
+      }
+      rc = launch_grad<DT>(ctx, b);
+    }
+    nxh_free_locked(ctx, values);
+    return rc;
+  }
   const int64_t units = ctx->compute_units > 0 ? ctx->compute_units : 256;
   auto go = [&](auto group, auto vectors) {
     constexpr int G = decltype(group)::value, T = group_threads(G), NV = decltype(vectors)::value;
@@ -739,22 +946,6 @@ int launch_with_grad(nxh_context *ctx, const LogProbsArgs &a) {
   hipLaunchKernelGGL((log_probs_with_grad_long_kernel<DT, 1024>), row_blocks(a, 1024, 1024), dim3(1024), 0, ctx->stream, a);
   return NXH_OK;
 }
-template <int DT>
-int launch_grad(nxh_context *ctx, const LogProbsArgs &a) {
-  constexpr int V = VECTOR<typename Tr<DT>::S>;
-  auto go = [&](auto group) {
-    constexpr int G = decltype(group)::value;
-    const int parts = std::max(1, (a.g.n / V + G * AHEAD - 1) / (G * AHEAD));  // (at most 2^14)
-    const int64_t rows = (a.g.rows + 256 / G - 1) / (256 / G);
-    const dim3 grid((unsigned)parts, (unsigned)std::min(rows, std::min<int64_t>(65535, MOST_LANES / 256 / parts)));
-    hipLaunchKernelGGL((log_probs_grad_kernel<DT, G>), grid, dim3(256), 0, ctx->stream, a);
-  };
-  if (a.g.n <= 8 * V) go(std::integral_constant<int, 8>{});
-  else if (a.g.n <= 4 * 64 * V) go(std::integral_constant<int, 64>{});
-  else go(std::integral_constant<int, 256>{});
-  return NXH_OK;
-}
-
 // What the three calls check alike; false in *go where there is nothing to launch.
 int prepare(const char *op, LogProbsArgs &a, const nxh_tensor *logits, const nxh_tensor *tokens, bool *go) {
   int rc = NXH_OK;

@@ -455,3 +455,64 @@ def test_refusals(hip):
     many = B.expand(B.reshape(x, (1, 1, 4, 8)), (1 << 20, 1 << 20, 4, 8))
     with pytest.raises(RuntimeError, match="too many rows"):
         B.log_probs(many, B.expand(B.reshape(t, (1, 1, 4)), (1 << 20, 1 << 20, 4)), out=(None,) * 6)
+
+
+@pytest.mark.parametrize("d, n", [(dt.float32, 40000), (dt.bfloat16, 70001), (dt.float64, 17001), (dt.float16, 200000)], ids=lambda v: v.name if hasattr(v, "name") else str(v))
+def test_few_long_rows(hip, oracle, d, n):
+    """Rows that are cut into parts, with the rows that are hard for what finds the most likely tokens: large elements in one part, in
+    one lane, ties within and across parts, parts of -inf, NaNs and infinities."""
+    rng = np.random.default_rng(n)
+    x = rng.standard_normal((10, n)) * 2
+    x[1] = 0.0
+    x[2] = np.arange(n) / n
+    x[3, : n // 2] = -np.inf
+    x[4] = -np.inf
+    x[4, n - 1] = x[4, n // 3] = 2.0
+    x[5] = np.where(np.arange(n) % 1000 == 7, 4.0, 0.0)
+    x[6] = np.where(np.arange(n) // (16 // d.itemsize) % 256 == 5, 3.0, 0.0)
+    x[7, n // 2] = np.nan
+    x[8, 5] = np.inf
+    x[9] = np.finfo(d.np_storage if d is not dt.bfloat16 else np.float32).min / 2
+    xs = encode(x, d, oracle)
+    x = decode(xs, d, oracle)
+    tokens = rng.integers(0, n, 10)
+    tokens[0], tokens[4], tokens[2] = n - 1, n - 1, -1
+    hx, ht = tensor(hip, xs, d), tensor(hip, tokens.astype(np.int32), dt.int32)
+    ok = [0, 1, 2, 3, 4, 5, 6, 9]
+    g, ge = rng.standard_normal(10), rng.standard_normal(10)
+    (hg, g), (hge, ge) = values(hip, g, d), values(hip, ge, d)
+    for k in (0, 1, 20, 64):
+        want, got = Want(x, tokens, d, k), hip.log_probs(hx, ht, k)
+        some = Want(x[ok], tokens[ok], d, k)
+        for t, w, err in zip(got, (some.log_p, some.entropy, some.peak, some.total), (some.log_p_err, some.entropy_err, 0 * some.e, some.e * some.total)):
+            within(logical(t)[ok].astype(np.float64), w, err, HALF[stats(d).name], 0, f"top {k} of {d.name}")
+        assert np.all(np.isnan(logical(got[0])[[7, 8]])) and np.all(np.isnan(logical(got[3])[[7, 8]]))
+        if k:
+            assert np.array_equal(logical(got[5]), want.top), f"top {k}"
+            within(logical(got[4])[ok].astype(np.float64), some.top_log_p, some.top_err, HALF[stats(d).name], 0, f"their log probabilities, {k}")
+    for e in (None, hge):
+        w, err = want.gradient(g, None if e is None else ge)
+        lp, h, dx = hip.log_probs_with_grad(hg, hx, ht, e)
+        over = tensor(hip, xs, d)
+        again = hip.log_probs_with_grad(hg, over, ht, e, out=(lp, h, over))[2]
+        same_bits(logical(again), logical(dx), "in place")
+        alone = hip.log_probs_grad(hg, hx, ht, got[2], got[3], e, None if e is None else got[1])
+        for t in (dx, alone):
+            v = decode(logical(t), d, oracle)
+            within(v[ok], w[ok], err[ok], HALF[d.name], TINY[d.name], "gradient")
+            assert np.all(np.isnan(v[[7, 8]]))
+    view = hip.flip(hip.expand(hip.reshape(hip.shrink(hx, [(0, 1), (3, n)]), (1, 1, n - 3)), (2, 3, n - 3)), (True, False, False))
+    got = hip.log_probs(view, hip.full(dt.int32, (2, 3), 4), 5)
+    check_score(got, Want(np.broadcast_to(x[:1, 3:], (2, 3, n - 3)), np.full((2, 3), 4), d, 5), d, oracle, 5, "a view")
+    hip.capture_begin()
+    try:
+        out = (*hip.log_probs(hx, ht, 20), *hip.log_probs_with_grad(hg, hx, ht, hge))
+    finally:
+        graph = hip.capture_end()
+    try:
+        for _ in range(3):
+            graph.launch()
+            for a, b in zip(out, (*hip.log_probs(hx, ht, 20), *hip.log_probs_with_grad(hg, hx, ht, hge))):
+                same_bits(logical(a), logical(b), "replay")
+    finally:
+        graph.destroy()
