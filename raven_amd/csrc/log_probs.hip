@@ -64,22 +64,46 @@ __device__ __forceinline__ C reference(C peak) { return larger(peak * Bounds<C>:
 template <class C>
 __device__ __forceinline__ bool is_near(C peak) { return __builtin_fabs(peak) <= Bounds<C>::wide; }
 
-// body(vector number, vector) over the vectors of a row that a lane has: numbers lane, lane + G, ..., U of them
-// requested before the first is looked at (past the row the last one again: a load under a condition is waited for
-// before the next); then tail(index) for the elements behind the last whole vector, one to a lane.
-template <int G, int U, class S, class B, class E>
-__device__ __forceinline__ void walk(const S *x, int n, int lane, B &&body, E &&tail) {
-  constexpr int V = VECTOR<S>;
-  const int nvec = n / V;
-  for (int c = lane; c < nvec; c += U * G) {
+// How a row of n elements is cut: vectors that lie on 16 bytes, and single elements in front of the first and behind the last of them
+// (of [8192,50257] contiguous bfloat16 logits seven rows in eight begin off 16 bytes: 173 us by vectors from their first
+// element on, 141 by vectors that lie on 16 bytes). A group of eight lanes, whose rows are short, takes them from the first element on.
+template <int G, class S>
+struct Cut {
+  static constexpr int V = VECTOR<S>;
+  int head, nvec, singles;
+  __device__ __forceinline__ Cut(const S *x, int n) {
+    head = G < 16 ? 0 : (int)((0 - (uintptr_t)x / sizeof(S)) % V);
+    head = head < n ? head : n;
+    nvec = (n - head) / V;
+    singles = n - nvec * V;
+  }
+  __device__ __forceinline__ int vector(int c) const { return head + c * V; }
+  __device__ __forceinline__ int single(int i) const { return i < head ? i : nvec * V + i; }
+};
+template <class S>
+__device__ __forceinline__ void store_at(S *row, int i, Words w) {
+  store_words(reinterpret_cast<S *>(reinterpret_cast<char *>(row) + (uint32_t)i * (uint32_t)sizeof(S)), w);
+}
+// body(number of its first element, vector) over those of a row's vectors begin to end that a lane has, U of them requested before the
+// first is looked at (past the last that one again: a load under a condition is waited for before the next).
+template <int G, int U, class S, class B>
+__device__ __forceinline__ void vectors(const Cut<G, S> &cut, const S *x, int begin, int end, int lane, B &&body) {
+  const S *v = x + cut.head;
+  for (int c = begin + lane; c < end; c += U * G) {
     Words raw[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) raw[u] = load_vector(x, c + u * G < nvec ? c + u * G : nvec - 1);
+    for (int u = 0; u < U; u++) raw[u] = load_vector(v, c + u * G < end ? c + u * G : end - 1);
 #pragma unroll
     for (int u = 0; u < U; u++)
-      if (c + u * G < nvec) body(c + u * G, raw[u]);
+      if (c + u * G < end) body(cut.vector(c + u * G), raw[u]);
   }
-  if (nvec * V + lane < n) tail(nvec * V + lane);
+}
+// ... and one(number) over the single elements.
+template <int G, int U, class S, class B, class E>
+__device__ __forceinline__ void walk(const S *x, int n, int lane, B &&body, E &&one) {
+  const Cut<G, S> cut(x, n);
+  vectors<G, U>(cut, x, 0, cut.nvec, lane, body);
+  for (int i = lane; i < cut.singles; i += G) one(cut.single(i));
 }
 
 template <class C>
@@ -289,17 +313,18 @@ struct Gradient {
   __device__ __forceinline__ S element(S x, int i) const {
     return IO::st(at<NEAR, ENTROPY>(IO::ld(x)) + (i == token ? g : 0));
   }
-  // The gradient of n elements from x on, the row's from `first` on, by G lanes.
+  // The gradient of the row's vectors begin to end, by G lanes, and of its single elements.
   template <int G, int U, bool NEAR, bool ENTROPY>
-  __device__ __forceinline__ void write(const S *x, S *out, int n, int first, int lane) const {
-    walk<G, U>(x, n, lane, [&](int c, Words raw) { store_vector(out, c, vector<NEAR, ENTROPY>(raw, first + c * IO::V)); },
-               [&](int i) { out[i] = element<NEAR, ENTROPY>(x[i], first + i); });
+  __device__ __forceinline__ void write(const Cut<G, S> &cut, const S *x, S *out, int begin, int end, bool singles, int lane) const {
+    vectors<G, U>(cut, x, begin, end, lane, [&](int i, Words raw) { store_at(out, i, vector<NEAR, ENTROPY>(raw, i)); });
+    if (singles)
+      for (int i = lane; i < cut.singles; i += G) out[cut.single(i)] = element<NEAR, ENTROPY>(x[cut.single(i)], cut.single(i));
   }
   template <int G, int U>
-  __device__ __forceinline__ void of(const S *x, S *out, int n, int first, int lane) const {
-    if (near && !with_entropy) write<G, U, true, false>(x, out, n, first, lane);
-    else if (near) write<G, U, true, true>(x, out, n, first, lane);
-    else write<G, 1, false, true>(x, out, n, first, lane);
+  __device__ __forceinline__ void of(const Cut<G, S> &cut, const S *x, S *out, int begin, int end, bool singles, int lane) const {
+    if (near && !with_entropy) write<G, U, true, false>(cut, x, out, begin, end, singles, lane);
+    else if (near) write<G, U, true, true>(cut, x, out, begin, end, singles, lane);
+    else write<G, 1, false, true>(cut, x, out, begin, end, singles, lane);
   }
 };
 
@@ -308,11 +333,8 @@ template <int DT, int G>
 __global__ __launch_bounds__(256) void log_probs_grad_kernel(LogProbsArgs a) {
   using C = typename Tr<DT>::C;
   using S = typename Tr<DT>::S;
-  constexpr int V = VECTOR<S>, GROUPS = 256 / G;
-  const int lane = threadIdx.x % G, n = a.g.n;
-  const int nvec = n / V, share = (nvec + (int)gridDim.x - 1) / (int)gridDim.x;
-  const int begin = (int)blockIdx.x * share < nvec ? (int)blockIdx.x * share : nvec, end = begin + share < nvec ? begin + share : nvec;
-  const int first = begin * V, part = (blockIdx.x + 1 == gridDim.x ? n : end * V) - first;
+  constexpr int GROUPS = 256 / G;
+  const int lane = threadIdx.x % G;
   for (int64_t row = (int64_t)blockIdx.y * GROUPS + threadIdx.x / G; row < a.g.rows; row += (int64_t)gridDim.y * GROUPS) {
     Places p;
     row_starts(a.g, (uint32_t)row, a.o, p.at);
@@ -322,7 +344,10 @@ __global__ __launch_bounds__(256) void log_probs_grad_kernel(LogProbsArgs a) {
       z.entropy = *place<const C>(a, p, LP_ENTROPY);
     }
     const Gradient<DT> grad(a, p, z);
-    grad.template of<G, AHEAD>(place<const S>(a, p, LP_X) + first, place<S>(a, p, LP_D) + first, part, first, lane);
+    const S *x = place<const S>(a, p, LP_X);
+    const Cut<G, S> cut(x, a.g.n);
+    const int share = (cut.nvec + (int)gridDim.x - 1) / (int)gridDim.x, begin = (int)blockIdx.x * share;
+    grad.template of<G, AHEAD>(cut, x, place<S>(a, p, LP_D), begin, begin + share < cut.nvec ? begin + share : cut.nvec, blockIdx.x == 0, lane);
   }
 }
 
@@ -333,10 +358,9 @@ __global__ __launch_bounds__(group_threads(G)) void log_probs_with_grad_kernel(L
   using IO = Io<DT>;
   using C = typename IO::C;
   using S = typename IO::S;
-  constexpr int GROUPS = group_threads(G) / G, V = IO::V;
+  constexpr int GROUPS = group_threads(G) / G;
   __shared__ Space<C, G> space;
-  const int lane = threadIdx.x % G, n = a.g.n, nvec = n / V, last = nvec > 0 ? nvec - 1 : 0;
-  const bool has_behind = nvec * V + lane < n;
+  const int lane = threadIdx.x % G, n = a.g.n;
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G;
   if (row >= a.g.rows) return;  // (whole groups; a group of several waves is the block)
@@ -345,28 +369,33 @@ __global__ __launch_bounds__(group_threads(G)) void log_probs_with_grad_kernel(L
   int token;
   // The gradient may go where the logits are: the token's is read here, before the lane's others, which the sums are made of that
   // all lanes wait for.
-  S picked, behind{};
+  S picked, alone{};
   auto begin = [&](int64_t r) {
     row_starts(a.g, (uint32_t)r, a.o, p.at);
     x = place<const S>(a, p, LP_X);
     token = *place<const int32_t>(a, p, LP_TOKEN);
     picked = x[token < 0 || token >= n ? 0 : token];
   };
-  auto request = [&](int v) { return load_vector(x, v * G + lane < nvec ? v * G + lane : last); };
   begin(row);
+  Cut<G, S> cut(x, n);  // (at most one of its single elements is a lane's)
+  auto request = [&](const Cut<G, S> &of, int v) {
+    return load_vector(x + of.head, v * G + lane < of.nvec ? v * G + lane : of.nvec > 0 ? of.nvec - 1 : 0);
+  };
+  // (a row without a vector has fewer elements than one and is not read by vectors: then none has)
+  const bool has = cut.nvec > 0;
   Words raw[NV];
-  if (nvec > 0)
+  if (has)
 #pragma unroll
-    for (int v = 0; v < NV; v++) raw[v] = request(v);
-  if (has_behind) behind = x[nvec * V + lane];
+    for (int v = 0; v < NV; v++) raw[v] = request(cut, v);
+  if (lane < cut.singles) alone = x[cut.single(lane)];
   for (int turn = 0; row < a.g.rows; row += step, turn ^= 1) {
     Running<DT> r;
 #pragma unroll
     for (int v = 0; v < NV; v++) {
-      if (v * G + lane < nvec) r.take(raw[v]);
+      if (v * G + lane < cut.nvec) r.take(raw[v]);
       __builtin_amdgcn_sched_barrier(0);  // (one after the other: widened at once they need more registers)
     }
-    if (has_behind) r.take_one(behind);
+    if (lane < cut.singles) r.take_one(alone);
     join_group<DT, G>(r, lane, turn, space);
     const Statistics<C> z = finish<DT, G>(r, x, n, lane, space);
     if (lane == 0) {
@@ -379,25 +408,27 @@ __global__ __launch_bounds__(group_threads(G)) void log_probs_with_grad_kernel(L
     const Gradient<DT> grad(a, p, z);
     S *out = place<S>(a, p, LP_D);
     begin(row + step < a.g.rows ? row + step : row);  // (behind the last row its own again, for nothing)
+    const Cut<G, S> next(x, n);
     auto write = [&](auto near, auto entropy) {
       constexpr bool NEAR = decltype(near)::value, ENTROPY = decltype(entropy)::value;
-      if (nvec > 0)
+      if (has)
 #pragma unroll
         for (int v = 0; v < NV; v++) {
-          const Words d = grad.template vector<NEAR, ENTROPY>(raw[v], (v * G + lane) * V);
-          raw[v] = request(v);
-          if (v * G + lane < nvec) store_vector(out, v * G + lane, d);
+          const Words d = grad.template vector<NEAR, ENTROPY>(raw[v], cut.vector(v * G + lane));
+          raw[v] = request(next, v);
+          if (v * G + lane < cut.nvec) store_at(out, cut.vector(v * G + lane), d);
           __builtin_amdgcn_sched_barrier(0);
         }
-      if (has_behind) {
-        const S d = grad.template element<NEAR, ENTROPY>(behind, nvec * V + lane);
-        behind = x[nvec * V + lane];
-        out[nvec * V + lane] = d;
+      if (lane < cut.singles) {
+        const S d = grad.template element<NEAR, ENTROPY>(alone, cut.single(lane));
+        out[cut.single(lane)] = d;
       }
+      if (lane < next.singles) alone = x[next.single(lane)];
     };
     if (grad.near && !grad.with_entropy) write(std::true_type{}, std::false_type{});
     else if (grad.near) write(std::true_type{}, std::true_type{});
     else write(std::false_type{}, std::true_type{});
+    cut = next;
   }
 }
 // Rows longer than that are read again, out of the caches.
@@ -426,7 +457,8 @@ __global__ __launch_bounds__(G) void log_probs_with_grad_long_kernel(LogProbsArg
     }
     if (!is_near(z.peak)) __syncthreads();
     const Gradient<DT> grad(a, p, z);
-    grad.template of<G, AHEAD>(x, place<S>(a, p, LP_D), n, 0, lane);
+    const Cut<G, S> cut(x, n);
+    grad.template of<G, AHEAD>(cut, x, place<S>(a, p, LP_D), 0, cut.nvec, true, lane);
   }
 }
 
@@ -479,11 +511,12 @@ struct Top {
   static constexpr int V = IO::V, W = G / 64, PLACES = TopSpace<DT, G>::PLACES, LANES = TopSpace<DT, G>::LANES;
   const S *x;
   int n, k;
+  const Cut<G, S> cut;
   TopSpace<DT, G> &l;
   const int lane = threadIdx.x, wave = threadIdx.x >> 6;
   T mine = 0;
 
-  __device__ __forceinline__ Top(const S *row, int length, int top, TopSpace<DT, G> &space) : x(row), n(length), k(top), l(space) {}
+  __device__ __forceinline__ Top(const S *row, int length, int top, TopSpace<DT, G> &space) : x(row), n(length), k(top), cut(row, length), l(space) {}
 
   // give(place, key, index) for the k largest of the first m entries of the list. A wave's lanes hold an entry each and count the
   // larger ones. Of 65 to 256 entries each wave takes its share, an entry at a time, against four that each lane holds. Of more, the k-th
@@ -577,16 +610,16 @@ struct Top {
       }
     }
   }
-  __device__ __forceinline__ void offer(Words raw, int c, T least) {
+  __device__ __forceinline__ void offer(Words raw, int i, T least) {
     struct Elements { S x[V]; } e = __builtin_bit_cast(Elements, raw);
 #pragma unroll
-    for (int j = 0; j < V; j++) offer(e.x[j], c * V + j, least);
+    for (int j = 0; j < V; j++) offer(e.x[j], i + j, least);
   }
   // Before the barrier of the statistics: the wave's part in the bound. Waves that are not full of vectors take no part in it; of a
   // row that one wave holds every lane with an element is looked at.
   __device__ __forceinline__ void begin(C seen) {
-    const int nvec = n / V, full = nvec <= 64 ? 0 : nvec / 64 < W ? nvec / 64 : W;
-    mine = lane < nvec || nvec * V + lane < n ? key_of(seen) : 0;
+    const int nvec = cut.nvec, full = nvec <= 64 ? 0 : nvec / 64 < W ? nvec / 64 : W;
+    mine = lane < nvec || lane < cut.singles ? key_of(seen) : 0;
     T most = full ? ~(T)0 : 1;
     if (wave < full) {
       T left = mine;
@@ -604,7 +637,7 @@ struct Top {
     __syncthreads();
     if (lane == 0) l.found = 0;
     __syncthreads();
-    walk<G, 1>(x, n, lane, [&](int c, Words raw) { offer(raw, c, least); }, [&](int i) { offer(x[i], i, least); });
+    walk<G, 1>(x, n, lane, [&](int i, Words raw) { offer(raw, i, least); }, [&](int i) { offer(x[i], i, least); });
     __syncthreads();
     return l.found;
   }
@@ -682,12 +715,12 @@ struct Top {
         which = l.few;
       }
       if (lanes <= LANES) {
-        const int nvec = n / V, each = (nvec + G - 1) / G;
+        const int each = (cut.nvec + G - 1) / G;
         for (int w = lane; w < lanes * each; w += G) {
           const int c = (w / lanes) * G + (int)which[w % lanes];
-          if (c < nvec) offer(load_vector(x, c), c, bound);
+          if (c < cut.nvec) offer(load_vector(x + cut.head, c), cut.vector(c), bound);
         }
-        if (nvec * V + lane < n) offer(x[nvec * V + lane], nvec * V + lane, bound);
+        if (lane < cut.singles) offer(x[cut.single(lane)], cut.single(lane), bound);
         __syncthreads();
         found = l.found;
         if (found <= PLACES) return found;
