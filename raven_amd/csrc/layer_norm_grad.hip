@@ -45,7 +45,8 @@ __global__ __launch_bounds__(lg_threads(G)) void layer_norm_grad_kernel(LayerNor
   using C = typename IO::C;
   using S = typename IO::S;
   constexpr int V = IO::V, T = lg_threads(G), GROUPS = T / G, W = T / 64;
-  __shared__ C lds[G > 64 ? 2 * (G / 64) : 2 * W * G * V];
+  constexpr int HALF = 2 * W * G * V;
+  __shared__ __align__(16) C lds[G > 64 ? 2 * (G / 64) : 2 * HALF];
   const int lane = threadIdx.x % G, n = a.g.n, nvec = (n + V - 1) / V;
   const S *gamma = reinterpret_cast<const S *>(a.gamma);
   // Every lane loads for every v, a vector past the row as the row's last: a load under a condition is waited for before the next one.
@@ -139,20 +140,22 @@ __global__ __launch_bounds__(lg_threads(G)) void layer_norm_grad_kernel(LayerNor
     const int wave = threadIdx.x >> 6;
 #pragma unroll
     for (int v = 0; v < NV; v++) {
-      if (v > 0) __syncthreads();
+      C *now = lds + (v & 1) * HALF;  // (in turn, so that one barrier a vector will do)
+      struct alignas(16) Sums { C s[V]; } p, q;
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        const C p = across_groups<G>(dgamma[v][j]), q = across_groups<G>(dbeta[v][j]);
-        if ((threadIdx.x & 63) < G) {
-          lds[(wave * 2 + 0) * G * V + lane * V + j] = p;
-          lds[(wave * 2 + 1) * G * V + lane * V + j] = q;
-        }
+        p.s[j] = across_groups<G>(dgamma[v][j]);
+        q.s[j] = across_groups<G>(dbeta[v][j]);
+      }
+      if ((threadIdx.x & 63) < G) {
+        *reinterpret_cast<Sums *>(now + ((wave * 2 + 0) * G + lane) * V) = p;
+        *reinterpret_cast<Sums *>(now + ((wave * 2 + 1) * G + lane) * V) = q;
       }
       __syncthreads();
       for (int e = threadIdx.x; e < 2 * G * V; e += T) {
-        C s = lds[e];
+        C s = now[e];
 #pragma unroll
-        for (int k = 1; k < W; k++) s = s + lds[k * 2 * G * V + e];
+        for (int k = 1; k < W; k++) s = s + now[k * 2 * G * V + e];
         const int i = v * G + e % (G * V) / V, j = e % V;
         if (i < nvec && vec_owns<V, R>(i, j, n)) mine[(e / (G * V)) * n + vec_start<V, R>(i, n) + j] = s;
       }
