@@ -271,6 +271,16 @@ __global__ __launch_bounds__(group_threads(G)) void log_probs_kernel(LogProbsArg
 }
 
 // ── the gradient ────────────────────────────────────────────────────────────
+// What a row's gradient is made for.
+template <class C>
+struct Upstream {
+  C g, g_entropy;
+  int token;
+};
+template <class C>
+__device__ __forceinline__ Upstream<C> upstream(const LogProbsArgs &a, const Places &p) {
+  return {*place<const C>(a, p, LP_G), a.o[LP_G_ENTROPY].base ? *place<const C>(a, p, LP_G_ENTROPY) : 0, *place<const int32_t>(a, p, LP_TOKEN)};
+}
 template <int DT>
 struct Gradient {
   using IO = Io<DT>;
@@ -279,16 +289,16 @@ struct Gradient {
   C peak, ref, inv_total, g, g_entropy, shift;  // inner = log p + entropy = ln2 d + shift for the exponent d
   int token;
   bool with_entropy, near;
-  __device__ __forceinline__ Gradient(const LogProbsArgs &a, const Places &p, const Statistics<C> &z) {
+  __device__ __forceinline__ Gradient(const LogProbsArgs &a, const Upstream<C> &up, const Statistics<C> &z) {
     peak = z.peak;
     near = is_near(peak);
     ref = reference(peak);
     const C lost = near ? fused(peak, Bounds<C>::L, -ref) : 0;
     inv_total = power(-lost) / z.total;
-    token = *place<const int32_t>(a, p, LP_TOKEN);
-    g = token < 0 ? 0 : token >= a.g.n ? (C)__builtin_nan("") : *place<const C>(a, p, LP_G);
+    token = up.token;
+    g = token < 0 ? 0 : token >= a.g.n ? (C)__builtin_nan("") : up.g;
     with_entropy = a.o[LP_G_ENTROPY].base != nullptr;
-    g_entropy = with_entropy ? *place<const C>(a, p, LP_G_ENTROPY) : 0;
+    g_entropy = up.g_entropy;
     shift = with_entropy ? z.entropy - z.log_total - Bounds<C>::ln2 * lost : 0;
   }
   template <bool NEAR, bool ENTROPY>
@@ -343,7 +353,7 @@ __global__ __launch_bounds__(256) void log_probs_grad_kernel(LogProbsArgs a) {
       z.log_total = log(z.total);
       z.entropy = *place<const C>(a, p, LP_ENTROPY);
     }
-    const Gradient<DT> grad(a, p, z);
+    const Gradient<DT> grad(a, upstream<C>(a, p), z);
     const S *x = place<const S>(a, p, LP_X);
     const Cut<G, S> cut(x, a.g.n);
     const int share = (cut.nvec + (int)gridDim.x - 1) / (int)gridDim.x, begin = (int)blockIdx.x * share;
@@ -366,15 +376,15 @@ __global__ __launch_bounds__(group_threads(G)) void log_probs_with_grad_kernel(L
   if (row >= a.g.rows) return;  // (whole groups; a group of several waves is the block)
   Places p;
   const S *x;
-  int token;
-  // The gradient may go where the logits are: the token's is read here, before the lane's others, which the sums are made of that
-  // all lanes wait for.
+  // The gradient may go where the logits are, log_p and entropy where g and g_entropy are: the token's logit and the row's own
+  // values are read here, before the lane's other logits, which the sums are made of that all lanes wait for.
   S picked, alone{};
+  Upstream<C> up;
   auto begin = [&](int64_t r) {
     row_starts(a.g, (uint32_t)r, a.o, p.at);
     x = place<const S>(a, p, LP_X);
-    token = *place<const int32_t>(a, p, LP_TOKEN);
-    picked = x[token < 0 || token >= n ? 0 : token];
+    up = upstream<C>(a, p);
+    picked = x[up.token < 0 || up.token >= n ? 0 : up.token];
   };
   begin(row);
   Cut<G, S> cut(x, n);  // (at most one of its single elements is a lane's)
@@ -400,12 +410,12 @@ __global__ __launch_bounds__(group_threads(G)) void log_probs_with_grad_kernel(L
     const Statistics<C> z = finish<DT, G>(r, x, n, lane, space);
     if (lane == 0) {
       if (a.o[LP_LOG_P].base)
-        *place<C>(a, p, LP_LOG_P) = token < 0 ? 0 : token >= n ? (C)__builtin_nan("") : IO::ld(picked) - z.peak - z.log_total;
+        *place<C>(a, p, LP_LOG_P) = up.token < 0 ? 0 : up.token >= n ? (C)__builtin_nan("") : IO::ld(picked) - z.peak - z.log_total;
       if (a.o[LP_ENTROPY].base) *place<C>(a, p, LP_ENTROPY) = z.entropy;
     }
     if constexpr (G > 64)
       if (!is_near(z.peak)) __syncthreads();  // (the walk by differences was the last to read the row)
-    const Gradient<DT> grad(a, p, z);
+    const Gradient<DT> grad(a, up, z);
     S *out = place<S>(a, p, LP_D);
     begin(row + step < a.g.rows ? row + step : row);  // (behind the last row its own again, for nothing)
     const Cut<G, S> next(x, n);
@@ -444,19 +454,19 @@ __global__ __launch_bounds__(G) void log_probs_with_grad_long_kernel(LogProbsArg
     Places p;
     row_starts(a.g, (uint32_t)row, a.o, p.at);
     const S *x = place<const S>(a, p, LP_X);
-    const int token = *place<const int32_t>(a, p, LP_TOKEN);
-    const S picked = x[token < 0 || token >= n ? 0 : token];  // (first, as above)
+    const Upstream<C> up = upstream<C>(a, p);
+    const S picked = x[up.token < 0 || up.token >= n ? 0 : up.token];  // (first, as above)
     Running<DT> r;
     r.template take_row<G, AHEAD>(x, n, lane);
     join_group<DT, G>(r, lane, turn, space);
     const Statistics<C> z = finish<DT, G>(r, x, n, lane, space);
     if (lane == 0) {
       if (a.o[LP_LOG_P].base)
-        *place<C>(a, p, LP_LOG_P) = token < 0 ? 0 : token >= n ? (C)__builtin_nan("") : IO::ld(picked) - z.peak - z.log_total;
+        *place<C>(a, p, LP_LOG_P) = up.token < 0 ? 0 : up.token >= n ? (C)__builtin_nan("") : IO::ld(picked) - z.peak - z.log_total;
       if (a.o[LP_ENTROPY].base) *place<C>(a, p, LP_ENTROPY) = z.entropy;
     }
     if (!is_near(z.peak)) __syncthreads();
-    const Gradient<DT> grad(a, p, z);
+    const Gradient<DT> grad(a, up, z);
     const Cut<G, S> cut(x, n);
     grad.template of<G, AHEAD>(cut, x, place<S>(a, p, LP_D), 0, cut.nvec, true, lane);
   }
@@ -776,7 +786,7 @@ struct Parts {
   void *sums;       // [rows][3][parts]
   void *keys;       // [rows][parts][top]
   uint32_t *index;  // [rows][parts][top]
-  void *values;     // [3][rows]: peak, total and entropy for the gradient; null: not wanted
+  void *values;     // [5][rows]: peak, total, entropy, g and g_entropy for the gradient; null: not wanted
   int parts, share;  // vectors of a part; the last has the elements behind the last vector too
 };
 template <int DT>
@@ -841,12 +851,15 @@ __global__ __launch_bounds__(JOIN_LANES) void log_probs_join_kernel(LogProbsArgs
   r.template join<PARTS_MAX>();
   const Statistics<C> z = finish<DT, G>(r, x, a.g.n, lane, space);
   if (lane == 0) {
-    give_statistics<DT>(a, p, x, z);
     if (C *v = reinterpret_cast<C *>(q.values)) {
+      const Upstream<C> up = upstream<C>(a, p);  // (log_p and entropy may go where they are)
       v[row] = z.peak;
       v[a.g.rows + row] = z.total;
       v[2 * a.g.rows + row] = z.entropy;
+      v[3 * a.g.rows + row] = up.g;
+      v[4 * a.g.rows + row] = up.g_entropy;
     }
+    give_statistics<DT>(a, p, x, z);
   }
   __syncthreads();
   Top<DT, G>(x, a.g.n, a.top, list).write(list.found, z, place<C>(a, p, LP_TOP_LOG_P), place<int32_t>(a, p, LP_TOP_TOKEN));
@@ -879,7 +892,7 @@ int parts_of(nxh_context *ctx, const LogProbsArgs &a) {
   if (nvec <= PART_VECTORS || a.g.rows * 4 > units) return 1;
   return (int)std::min<int64_t>(std::min<int64_t>(PARTS_MAX, 2 * units / a.g.rows), nvec / (2 * PART_LANES));
 }
-// The statistics and most likely tokens of rows in parts. values: room for [3][rows], or null.
+// The statistics and most likely tokens of rows in parts. values: room for [5][rows], or null.
 template <int DT>
 int launch_parts(nxh_context *ctx, const LogProbsArgs &a, int parts, void *values) {
   using C = typename Tr<DT>::C;
@@ -935,12 +948,13 @@ int launch_with_grad(nxh_context *ctx, const LogProbsArgs &a) {
   constexpr int V = VECTOR<typename Tr<DT>::S>;
   if (const int parts = parts_of<DT>(ctx, a); parts > 1) {
     void *values = nullptr;
-    if (int rc = nxh_alloc_locked(ctx, (size_t)a.g.rows * 3 * sizeof(C), &values)) return rc;
+    if (int rc = nxh_alloc_locked(ctx, (size_t)a.g.rows * 5 * sizeof(C), &values)) return rc;
     int rc = launch_parts<DT>(ctx, a, parts, values);
     if (!rc) {
       LogProbsArgs b = a;
-      for (int k = 0; k < 3; k++) {
-        RowOperand &o = b.o[k == 2 ? LP_ENTROPY : LP_PEAK + k];
+      constexpr int which[] = {LP_PEAK, LP_TOTAL, LP_ENTROPY, LP_G, LP_G_ENTROPY};
+      for (int k = 0; k < (a.o[LP_G_ENTROPY].base ? 5 : 4); k++) {
+        RowOperand &o = b.o[which[k]];
         o.base = (const char *)values + (size_t)k * a.g.rows * sizeof(C);
         int64_t stride = 1;
         for (int d = a.g.nouter - 1; d >= 0; d--) {

@@ -291,6 +291,22 @@ def test_gradients_that_replace_logits(hip, oracle, n):
         same_bits(logical(p), q, "at once and in place")
 
 
+@pytest.mark.parametrize("rows, n", [(70, 5), (7, 700), (5, 5001), (3, 30000), (66, 33000), (3, 40000)])
+def test_results_that_replace_their_gradients(hip, oracle, rows, n):
+    """log_p and entropy written where g and g_entropy are, every length's kernel."""
+    d = dt.float32
+    xs, _ = drawn((rows, n), d, oracle, n)
+    rng = np.random.default_rng(n)
+    hx, ht = tensor(hip, xs, d), tensor(hip, rng.integers(-1, n, rows).astype(np.int32), dt.int32)
+    g, ge = rng.standard_normal(rows), rng.standard_normal(rows)
+    want = [logical(t) for t in hip.log_probs_with_grad(values(hip, g, d)[0], hx, ht, values(hip, ge, d)[0])]
+    for first in (0, 1):
+        both = values(hip, g, d)[0], values(hip, ge, d)[0]
+        out = (both[first], both[1 - first], hip.buffer(d, (rows, n)))
+        for p, q in zip(hip.log_probs_with_grad(both[0], hx, ht, both[1], out=out), want):
+            same_bits(logical(p), q, f"over {first}")
+
+
 def test_differences(hip, oracle):
     """The gradient against differences of the forward pass in float64 (steps of 1e-6)."""
     rng = np.random.default_rng(3)
