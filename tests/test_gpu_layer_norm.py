@@ -320,6 +320,28 @@ def test_behind_deferred_work(hip, oracle):
         same_bits(p, q, "behind deferred work")
 
 
+@pytest.mark.parametrize("n", [5, 1001, 6001, 20003])
+def test_one_row_whose_results_replace_what_has_its_shape(hip, oracle, n):
+    """With no outer axis the weights, their gradients and the row are of one shape: each result in the place of each of them."""
+    d = dt.float32
+    held = {k: drawn((n,), d, oracle, n + i)[0] for i, k in enumerate(("x", "gamma", "beta", "g"))}
+
+    def fresh():
+        return {k: tensor(hip, v, d) for k, v in held.items()}
+
+    t = fresh()
+    y, mean, rstd = hip.layer_norm(t["x"], t["gamma"], t["beta"], EPS)
+    want = [logical(v) for v in hip.layer_norm_grad(t["g"], t["x"], mean, rstd, t["gamma"])]
+    for name in ("x", "gamma", "beta"):
+        t = fresh()
+        same_bits(logical(hip.layer_norm(t["x"], t["gamma"], t["beta"], EPS, out=(t[name], None, None))[0]), logical(y), f"over {name}")
+    for names in (("x", "gamma", "g"), ("g", "x", "gamma"), ("gamma", "g", "x")):
+        t = fresh()
+        got = hip.layer_norm_grad(t["g"], t["x"], mean, rstd, t["gamma"], out=tuple(t[k] for k in names))
+        for a, b in zip(got, want):
+            same_bits(logical(a), b, f"gradients over {names}")
+
+
 def test_refusals(hip):
     B, f32 = hip, dt.float32
     x, v, s = B.full(f32, (4, 8), 1.0), B.full(f32, (8,), 1.0), B.full(f32, (4,), 1.0)
