@@ -148,28 +148,39 @@ __global__ __launch_bounds__(lg_threads(G, NV * Io<DT>::V)) void layer_norm_grad
         }
       }
   } else {
+    // A wave's sums lie in planes of 16 bytes a lane: [wave][dgamma, dbeta][plane][lane][element of the plane].
+    constexpr int E = 16 / (int)sizeof(C), P = (V + E - 1) / E, WAVE = 2 * P * G * E;
     const int wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int v = 0; v < NV; v++) {
-      C *now = lds + (v & 1) * HALF;  // (in turn, so that one barrier a vector will do)
-      struct alignas(16) Sums { C s[V]; } p, q;
+    for (int first = 0; first < NV; first += 2) {  // two vectors a barrier, as there is room
+      if (first > 0) __syncthreads();
 #pragma unroll
-      for (int j = 0; j < V; j++) {
-        p.s[j] = across_groups<G>(dgamma[v][j]);
-        q.s[j] = across_groups<G>(dbeta[v][j]);
-      }
-      if ((threadIdx.x & 63) < G) {
-        *reinterpret_cast<Sums *>(now + ((wave * 2 + 0) * G + lane) * V) = p;
-        *reinterpret_cast<Sums *>(now + ((wave * 2 + 1) * G + lane) * V) = q;
-      }
+      for (int v = first; v < NV && v < first + 2; v++)
+#pragma unroll
+        for (int q = 0; q < P; q++) {
+          struct alignas(16) Plane { C s[E]; } p, r;
+#pragma unroll
+          for (int j = 0; j < E; j++) {
+            p.s[j] = across_groups<G>(dgamma[v][q * E + j]);
+            r.s[j] = across_groups<G>(dbeta[v][q * E + j]);
+          }
+          if ((threadIdx.x & 63) < G) {
+            C *at = lds + (v - first) * HALF + wave * WAVE + (q * G + lane) * E;
+            *reinterpret_cast<Plane *>(at) = p;
+            *reinterpret_cast<Plane *>(at + P * G * E) = r;
+          }
+        }
       __syncthreads();
-      for (int e = threadIdx.x; e < 2 * G * V; e += T) {
-        C s = now[e];
 #pragma unroll
-        for (int k = 1; k < W; k++) s = s + now[k * 2 * G * V + e];
-        const int i = v * G + e % (G * V) / V, j = e % V;
-        if (i < nvec && vec_owns<V, R>(i, j, n)) mine[(e / (G * V)) * n + vec_start<V, R>(i, n) + j] = s;
-      }
+      for (int v = first; v < NV && v < first + 2; v++)
+        for (int e = threadIdx.x; e < WAVE; e += T) {
+          const C *at = lds + (v - first) * HALF + e;
+          C s = at[0];
+#pragma unroll
+          for (int k = 1; k < W; k++) s = s + at[k * WAVE];
+          const int which = e / (P * G * E), i = v * G + e / E % G, j = e / (G * E) % P * E + e % E;
+          if (i < nvec && vec_owns<V, R>(i, j, n)) mine[which * n + vec_start<V, R>(i, n) + j] = s;
+        }
     }
   }
 }

@@ -28,16 +28,14 @@ __device__ __forceinline__ void row_starts(const RowGeom &g, uint32_t row, const
 #pragma unroll
   for (int k = 0; k < K; k++) at[k] = 0;
   uint32_t r = row;
-  for (int d = g.nouter - 1; d >= 0; d--) {  // (the host has merged what composes: usually one dim and no division)
-    uint32_t i = r;
-    if (d > 0) {
-      const uint32_t q = r / g.oshape[d];
-      i = r - q * g.oshape[d];
-      r = q;
-    }
+  for (int d = g.nouter - 1; d > 0; d--) {  // (the host has merged what composes: usually one dim and no division)
+    const uint32_t q = r / g.oshape[d], i = r - q * g.oshape[d];
+    r = q;
 #pragma unroll
     for (int k = 0; k < K; k++) at[k] += (int64_t)i * operands[k].stride[d];
   }
+#pragma unroll
+  for (int k = 0; k < K; k++) at[k] += (int64_t)r * operands[k].stride[0];  // (no outer dim: the strides are 0)
 }
 
 // ── host side ───────────────────────────────────────────────────────────────
