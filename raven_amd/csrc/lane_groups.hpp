@@ -32,10 +32,6 @@ template <class S>
 __device__ __forceinline__ Words load_vector(const S *row, int c) {
   return load_words(reinterpret_cast<const S *>(reinterpret_cast<const char *>(row) + (uint32_t)c * 16u));
 }
-template <class S>
-__device__ __forceinline__ void store_vector(S *row, int c, Words w) {
-  store_words(reinterpret_cast<S *>(reinterpret_cast<char *>(row) + (uint32_t)c * 16u), w);
-}
 
 // What elements are computed as, and back, one or a vector at a time. float16 and bfloat16 take the hardware's conversions, which
 // round to nearest, ties to even, and keep a NaN a NaN; the primitives' keep its payload too, at some ten instructions an

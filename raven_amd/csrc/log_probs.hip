@@ -11,7 +11,8 @@
 // rescaled where a vector of 16 bytes brings a larger one; the lanes' triples are then joined. Both sums
 // have terms of one sign, so nothing cancels, and peak and total are given out apart: x - peak is exact
 // near the peak, where x - log(sum e^x) would round to the step of the logarithm. Memory bounds it: the
-// logits once; the gradient once more in and out.
+// logits once; the gradient once more in and out. Five alternatives of [2048,50257] float32 75 us (5.5 TB/s);
+// [8192,50257] bfloat16 statistics 141 us (5.8 TB/s), both at once 317 us (5.2 TB/s), the gradient by itself 279.
 //
 // Exponentials are powers of two: with L = log2 e and the reference A = peak L as it rounds, 2^(x L - A) is one
 // fused step and one instruction. What A lost in rounding, r = peak L - A, is a factor 2^r of every term: the
@@ -780,7 +781,8 @@ __global__ __launch_bounds__(G) void log_probs_top_kernel(LogProbsArgs a) {
 
 // ── few long rows ───────────────────────────────────────────────────────────
 // Rows that would leave most of the chip idle are cut into parts, a block to each: a part's sums and its own most likely tokens, in their
-// order, go to memory, and a block for each row joins them.
+// order, go to memory, and a block for each row joins them. (A row of 200000 float32 logits 17.1 us whole, 7.1 in parts; statistics and
+// gradient of [20,150000] 26 and 15 us.)
 constexpr int PART_LANES = 256, JOIN_LANES = 1024, PARTS_MAX = 16;
 struct Parts {
   void *sums;       // [rows][3][parts]
@@ -866,7 +868,8 @@ __global__ __launch_bounds__(JOIN_LANES) void log_probs_join_kernel(LogProbsArgs
 }
 
 // ── host side ───────────────────────────────────────────────────────────────
-constexpr int PART_VECTORS = 16 * 512;  // of rows that are not cut
+// Of rows that are not cut: vectors, and, with alternatives, whose search goes by the element, elements.
+constexpr int WHOLE_VECTORS = 8192, WHOLE_TOP = 72 << 10;
 constexpr int64_t MOST_LANES = (int64_t)1 << 31;  // of a launch, which numbers them in 32 bits; groups go on to further rows
 
 // A row's lanes: eight where its vectors are no more, a wave up to four vectors a lane, a block of four waves up to eight, then one
@@ -884,12 +887,14 @@ dim3 row_blocks(const LogProbsArgs &a, int threads, int group) {
   const int64_t groups = threads / group;
   return dim3((unsigned)std::min((a.g.rows + groups - 1) / groups, MOST_LANES / threads));
 }
-// How many parts a row is cut into; 1: not at all. A block of 512 lanes for a row of 2^16 bfloat16 elements has the time of two more
-// launches left in it.
+// How many parts a row is cut into; 1: not at all. Two launches more and what the parts pass on have to pay (eight rows of bfloat16, whole
+// and in parts: statistics of 50257 elements 6.5 and 7.0 us, of 80000 8.6 and 6.8; with their gradient 11.7 and 10.7, 14.5 and 10.6;
+// with 20 alternatives 11.3 and 15.6, 14.0 and 13.3, of 131000 17.7 and 14.9; of 50257 float32 12.2 and 14.2, of a row of 200000 22.9
+// and 14.4), and a block for every row has to leave units idle.
 template <int DT>
 int parts_of(nxh_context *ctx, const LogProbsArgs &a) {
   const int64_t units = ctx->compute_units > 0 ? ctx->compute_units : 256, nvec = a.g.n / VECTOR<typename Tr<DT>::S>;
-  if (nvec <= PART_VECTORS || a.g.rows * 4 > units) return 1;
+  if (nvec <= WHOLE_VECTORS || (a.top && a.g.n <= WHOLE_TOP) || a.g.rows * 4 > units) return 1;
   return (int)std::min<int64_t>(std::min<int64_t>(PARTS_MAX, 2 * units / a.g.rows), nvec / (2 * PART_LANES));
 }
 // The statistics and most likely tokens of rows in parts. values: room for [5][rows], or null.

@@ -473,7 +473,7 @@ def test_refusals(hip):
         B.log_probs(many, B.expand(B.reshape(t, (1, 1, 4)), (1 << 20, 1 << 20, 4)), out=(None,) * 6)
 
 
-@pytest.mark.parametrize("d, n", [(dt.float32, 40000), (dt.bfloat16, 70001), (dt.float64, 17001), (dt.float16, 200000)], ids=lambda v: v.name if hasattr(v, "name") else str(v))
+@pytest.mark.parametrize("d, n", [(dt.float32, 40000), (dt.bfloat16, 70001), (dt.float64, 17001), (dt.float16, 200000), (dt.float32, 80000), (dt.float64, 75001)], ids=lambda v: v.name if hasattr(v, "name") else str(v))
 def test_few_long_rows(hip, oracle, d, n):
     """Rows that are cut into parts, with the rows that are hard for what finds the most likely tokens: large elements in one part, in
     one lane, ties within and across parts, parts of -inf, NaNs and infinities."""
