@@ -209,6 +209,15 @@ __device__ __forceinline__ void group_combine(C (&v)[K], F f, C *lds) {
   }
 }
 
+// Which of a block's T / G groups a lane belongs to. Groups of whole waves have it, and the addresses that follow from it, in
+// scalar registers.
+template <int G, int T>
+__device__ __forceinline__ int group_number() {
+  if constexpr (G == T) return 0;
+  else if constexpr (G >= 64) return __builtin_amdgcn_readfirstlane((int)threadIdx.x / G);
+  else return (int)threadIdx.x / G;
+}
+
 template <class C>
 struct Sum {
   __device__ __forceinline__ C operator()(C a, C b) const { return a + b; }

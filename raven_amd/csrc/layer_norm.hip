@@ -50,7 +50,7 @@ __global__ __launch_bounds__(ln_threads(G)) void layer_norm_kernel(LayerNormArgs
   const int last = (nvec - 1) / G;
   auto owns = [&](int v, int j) { return R == WHOLE || v != last || vec_owns<V, R>(c[v], j, n); };
   const C count = (C)n, eps = (C)a.eps;
-  for (int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G; row < a.g.rows; row += (int64_t)gridDim.x * GROUPS) {
+  for (int64_t row = (int64_t)blockIdx.x * GROUPS + group_number<G, ln_threads(G)>(); row < a.g.rows; row += (int64_t)gridDim.x * GROUPS) {
     int64_t at[LN_OPERANDS];
     row_starts(a.g, (uint32_t)row, a.o, at);
     const S *x = reinterpret_cast<const S *>(a.o[LN_X].base) + at[LN_X];
@@ -89,6 +89,7 @@ __global__ __launch_bounds__(ln_threads(G)) void layer_norm_kernel(LayerNormArgs
 #pragma unroll
     for (int v = 0; v < NV; v++) {
       C w[V], b[V];
+      if constexpr (G * NV * V >= 1024 * 32) asm("" : "+v"(gv[v]), "+v"(bv[v]));  // (widened once for all rows they would take registers that there are not)
       IO::widen(gv[v], w);
       IO::widen(bv[v], b);
 #pragma unroll

@@ -41,14 +41,16 @@ __device__ __forceinline__ C across_groups(C v) {
 // groups. Sixteen waves where a lane's 16 elements leave them the registers: those together keep the memory at work. Eight of them
 // where it has more, each with its next row on the way while it finishes one. ([98304,64] float16 12.8 us with eight, 12.3 with
 // sixteen; [65536,128] bfloat16 14.5 and 13.5; 24 elements of sixteen waves go to scratch memory: [8192,1536] bfloat16 18 and 54.)
-constexpr int lg_threads(int g, int elements) { return g > 64 ? g : elements <= 16 ? 1024 : 512; }
+// (float64 needs some three registers an element more.)
+template <int DT, int G, int NV>
+constexpr int lg_threads = G > 64 ? G : NV * Io<DT>::V * (DT == NXH_F64 ? 3 : 1) <= 16 ? 1024 : 512;
 
 template <int DT, int G, int NV, Rows R>
-__global__ __launch_bounds__(lg_threads(G, NV * Io<DT>::V)) void layer_norm_grad_kernel(LayerNormGradArgs a) {
+__global__ __launch_bounds__((lg_threads<DT, G, NV>)) void layer_norm_grad_kernel(LayerNormGradArgs a) {
   using IO = Io<DT>;
   using C = typename IO::C;
   using S = typename IO::S;
-  constexpr int V = IO::V, T = lg_threads(G, NV * Io<DT>::V), GROUPS = T / G, W = T / 64;
+  constexpr int V = IO::V, T = lg_threads<DT, G, NV>, GROUPS = T / G, W = T / 64;
   constexpr int HALF = 2 * W * G * V;
   __shared__ __align__(16) C lds[G > 64 ? 2 * (G / 64) : 2 * HALF];
   const int lane = threadIdx.x % G, n = a.g.n, nvec = (n + V - 1) / V;
@@ -69,7 +71,7 @@ __global__ __launch_bounds__(lg_threads(G, NV * Io<DT>::V)) void layer_norm_grad
   auto owns = [&](int v, int j) { return R == WHOLE || v != last || vec_owns<V, R>(c[v], j, n); };
   const C count = (C)n;
   const int64_t step = (int64_t)gridDim.x * GROUPS;
-  int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G, at[LG_OPERANDS];
+  int64_t row = (int64_t)blockIdx.x * GROUPS + group_number<G, T>(), at[LG_OPERANDS];
   C mean = 0, rstd = 0;
   const S *x = nullptr, *g = nullptr;
   auto begin = [&](int64_t r) {
@@ -100,6 +102,7 @@ __global__ __launch_bounds__(lg_threads(G, NV * Io<DT>::V)) void layer_norm_grad
 #pragma unroll
     for (int v = 0; v < NV; v++) {
       C gv[V], gw[V];
+      if constexpr (NV * V >= 32) asm("" : "+v"(gain[v]));  // (widened once for all rows it would take registers that there are not)
       IO::widen(xr[v], h[v]);
       IO::widen(gr[v], gv);
       IO::widen(gain[v], gw);
@@ -339,8 +342,8 @@ template <int DT, int G, int NV>
 void launch(nxh_context *ctx, const LayerNormGradArgs &a, int64_t blocks) {
   constexpr int V = Io<DT>::V;
   const dim3 grid((unsigned)blocks);
-  if (a.g.n % V == 0) hipLaunchKernelGGL((layer_norm_grad_kernel<DT, G, NV, WHOLE>), grid, dim3(lg_threads(G, NV * Io<DT>::V)), 0, ctx->stream, a);
-  else hipLaunchKernelGGL((layer_norm_grad_kernel<DT, G, NV, G * NV == 1 ? SHORT : RAGGED>), grid, dim3(lg_threads(G, NV * Io<DT>::V)), 0, ctx->stream, a);
+  if (a.g.n % V == 0) hipLaunchKernelGGL((layer_norm_grad_kernel<DT, G, NV, WHOLE>), grid, dim3((lg_threads<DT, G, NV>)), 0, ctx->stream, a);
+  else hipLaunchKernelGGL((layer_norm_grad_kernel<DT, G, NV, G * NV == 1 ? SHORT : RAGGED>), grid, dim3((lg_threads<DT, G, NV>)), 0, ctx->stream, a);
 }
 template <int DT>
 void launch_long(nxh_context *ctx, const LayerNormGradArgs &a, int64_t blocks) {
@@ -360,7 +363,7 @@ Plan plan(nxh_context *ctx, int n, int64_t rows) {
   const int nvec = (n + V - 1) / V;
 #define X(G, NV)                                                                                                \
   if (nvec <= G * NV)                                                                                           \
-    return {launch<DT, G, NV>, std::min((rows + lg_threads(G, NV * Io<DT>::V) / G - 1) / (lg_threads(G, NV * Io<DT>::V) / G), units * (G == 256 ? 2 : 1))};
+    return {launch<DT, G, NV>, std::min((rows + lg_threads<DT, G, NV> / G - 1) / (lg_threads<DT, G, NV> / G), units * (G == 256 ? 2 : 1))};
   LN_GROUPS_GRAD(X)
 #undef X
   const int64_t tiles = (nvec + 255) / 256;

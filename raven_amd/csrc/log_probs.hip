@@ -259,7 +259,7 @@ __global__ __launch_bounds__(group_threads(G)) void log_probs_kernel(LogProbsArg
   __shared__ Space<C, G> space;
   const int lane = threadIdx.x % G;
   int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G; row < a.g.rows; row += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
+  for (int64_t row = (int64_t)blockIdx.x * GROUPS + group_number<G, group_threads(G)>(); row < a.g.rows; row += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
     Places p;
     row_starts(a.g, (uint32_t)row, a.o, p.at);
     const S *x = place<const S>(a, p, LP_X);
@@ -373,7 +373,7 @@ __global__ __launch_bounds__(group_threads(G)) void log_probs_with_grad_kernel(L
   __shared__ Space<C, G> space;
   const int lane = threadIdx.x % G, n = a.g.n;
   const int64_t step = (int64_t)gridDim.x * GROUPS;
-  int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G;
+  int64_t row = (int64_t)blockIdx.x * GROUPS + group_number<G, group_threads(G)>();
   if (row >= a.g.rows) return;  // (whole groups; a group of several waves is the block)
   Places p;
   const S *x;
