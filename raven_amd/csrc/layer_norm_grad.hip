@@ -37,6 +37,21 @@ __device__ __forceinline__ C across_groups(C v) {
   return v;
 }
 
+// A lane's sums of a vector of columns, as words. (Of a row's last vector those that it shares with the one before are made of the same
+// elements in the same order there: equal bits.)
+template <int DT>
+__device__ __forceinline__ void store_sums(typename Tr<DT>::C *at, const typename Tr<DT>::C (&sums)[Io<DT>::V]) {
+  using C = typename Tr<DT>::C;
+  constexpr int E = VECTOR<C>;
+#pragma unroll
+  for (int k = 0; k < Io<DT>::V; k += E) {
+    struct Plane { C s[E]; } p;
+#pragma unroll
+    for (int j = 0; j < E; j++) p.s[j] = sums[k + j];
+    store_words(at + k, __builtin_bit_cast(Words, p));
+  }
+}
+
 // Blocks of many waves where a row has a wave or less: the block's sums are one row of partial sums, whatever the number of its
 // groups. Sixteen waves where a lane's 16 elements leave them the registers: those together keep the memory at work. Eight of them
 // where it has more, each with its next row on the way while it finishes one. ([98304,64] float16 12.8 us with eight, 12.3 with
@@ -143,13 +158,9 @@ __global__ __launch_bounds__((lg_threads<DT, G, NV>)) void layer_norm_grad_kerne
   if constexpr (G > 64) {  // the block's only group
 #pragma unroll
     for (int v = 0; v < NV; v++)
-#pragma unroll
-      for (int j = 0; j < V; j++) {
-        const int i = v * G + lane, column = vec_start<V, R>(i, n) + j;
-        if (i < nvec && vec_owns<V, R>(i, j, n)) {
-          mine[column] = dgamma[v][j];
-          mine[n + column] = dbeta[v][j];
-        }
+      if (v * G + lane < nvec) {
+        store_sums<DT>(mine + vec_start<V, R>(c[v], n), dgamma[v]);
+        store_sums<DT>(mine + n + vec_start<V, R>(c[v], n), dbeta[v]);
       }
   } else {
     // A wave's sums lie in planes of 16 bytes a lane: [wave][dgamma, dbeta][plane][lane][element of the plane].
@@ -271,13 +282,9 @@ __global__ __launch_bounds__(256) void layer_norm_columns_kernel(LayerNormGradAr
       dbeta[j] = dbeta[j] + g[j];
     }
   }
-  C *mine = reinterpret_cast<C *>(a.partials) + (int64_t)blockIdx.y * 2 * n;
-#pragma unroll
-  for (int j = 0; j < V; j++)
-    if (vec_owns<V, RAGGED>(c, j, n)) {
-      mine[vec_start<V, RAGGED>(c, n) + j] = dgamma[j];
-      mine[n + vec_start<V, RAGGED>(c, n) + j] = dbeta[j];
-    }
+  C *mine = reinterpret_cast<C *>(a.partials) + (int64_t)blockIdx.y * 2 * n + vec_start<V, RAGGED>(c, n);
+  store_sums<DT>(mine, dgamma);
+  store_sums<DT>(mine + n, dbeta);
 }
 
 // ── the partial sums ────────────────────────────────────────────────────────
