@@ -4,6 +4,8 @@
 // bytes at whatever alignment the row has.
 #pragma once
 
+#include <type_traits>
+
 #include "nxh_common.hpp"
 
 namespace {
@@ -27,10 +29,18 @@ __device__ __forceinline__ void store_words(S *p, Words w) {
   __builtin_memcpy(p, &w, sizeof w);
 }
 
-// Vector c of a row, by an offset of 32 bits (a row has at most 2^27 bytes): beside a row that all lanes share it is one register.
+// Element i of a row, by an offset of 32 bits (a row has at most 2^27 bytes): beside a row that all lanes share it is one register, for
+// every operand the same.
+template <class S>
+__device__ __forceinline__ S *element_at(S *row, int i) {
+  using Byte = std::conditional_t<std::is_const<S>::value, const char, char>;
+  return reinterpret_cast<S *>(reinterpret_cast<Byte *>(row) + (uint32_t)i * (uint32_t)sizeof(S));
+}
+
+// Vector c of a row.
 template <class S>
 __device__ __forceinline__ Words load_vector(const S *row, int c) {
-  return load_words(reinterpret_cast<const S *>(reinterpret_cast<const char *>(row) + (uint32_t)c * 16u));
+  return load_words(element_at(row, c * VECTOR<S>));
 }
 
 // What elements are computed as, and back, one or a vector at a time. float16 and bfloat16 take the hardware's conversions, which
@@ -111,7 +121,7 @@ __device__ __forceinline__ bool vec_owns(int c, int j, int n) {
 template <Rows R, class S>
 __device__ __forceinline__ Words load_part(const S *row, int c, int n) {
   constexpr int V = VECTOR<S>;
-  if constexpr (R != SHORT) return load_words(row + vec_start<V, R>(c, n));
+  if constexpr (R != SHORT) return load_words(element_at(row, vec_start<V, R>(c, n)));
   struct Elements { S x[V]; } e;
 #pragma unroll
   for (int j = 0; j < V; j++) e.x[j] = row[j < n ? j : 0];
@@ -121,7 +131,7 @@ template <Rows R, class S>
 __device__ __forceinline__ void store_part(S *row, int c, int n, Words w) {
   constexpr int V = VECTOR<S>;
   if constexpr (R != SHORT) {
-    store_words(row + vec_start<V, R>(c, n), w);
+    store_words(element_at(row, vec_start<V, R>(c, n)), w);
   } else {
     struct Elements { S x[V]; } e = __builtin_bit_cast(Elements, w);
 #pragma unroll
@@ -134,7 +144,7 @@ template <class S>
 __device__ __forceinline__ void store_own(S *row, int c, int n, Words w) {
   constexpr int V = VECTOR<S>;
   if ((c + 1) * V <= n) {
-    store_words(row + c * V, w);
+    store_words(element_at(row, c * V), w);
     return;
   }
   struct Elements { S x[V]; } e = __builtin_bit_cast(Elements, w);
@@ -186,8 +196,8 @@ __device__ __forceinline__ C lanes_combine(C v, F f) {
   if constexpr (G >= 64) v = combine_step<32>(v, f);
   return v;
 }
-// f over K values of each of a group's lanes at once. A group of several waves is the whole block and meets in
-// `lds` (K * G / 64 values); the waves' results are taken in order, so every lane has the same bits.
+// f over K values of each of a group's lanes at once; every lane gets the same bits. A group of several waves is the whole block and
+// meets in `lds` (K * G / 64 values), of which each lane reads one wave's: all of sixteen waves' would be as many registers.
 template <int G, int K, class C, class F>
 __device__ __forceinline__ void group_combine(C (&v)[K], F f, C *lds) {
 #pragma unroll
@@ -200,12 +210,7 @@ __device__ __forceinline__ void group_combine(C (&v)[K], F f, C *lds) {
       for (int k = 0; k < K; k++) lds[(threadIdx.x >> 6) * K + k] = v[k];
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < K; k++) {
-      C s = lds[k];
-#pragma unroll
-      for (int w = 1; w < W; w++) s = f(s, lds[w * K + k]);
-      v[k] = s;
-    }
+    for (int k = 0; k < K; k++) v[k] = lanes_combine<W>(lds[(threadIdx.x % W) * K + k], f);
   }
 }
 

@@ -70,6 +70,8 @@ __global__ __launch_bounds__((lg_threads<DT, G, NV>)) void layer_norm_grad_kerne
   __shared__ __align__(16) C lds[G > 64 ? 2 * (G / 64) : 2 * HALF];
   const int lane = threadIdx.x % G, n = a.g.n, nvec = (n + V - 1) / V;
   const S *gamma = reinterpret_cast<const S *>(a.gamma);
+  // Sixteen waves have registers for a row at a time, and for gamma, which the caches have, while its row is read.
+  constexpr bool AHEAD = T < 1024, HELD = G < 1024;
   // Every lane loads for every v, a vector past the row as the row's last: a load under a condition is waited for before the next one.
   int c[NV];
   Words gain[NV], xr[NV], gr[NV];
@@ -77,7 +79,7 @@ __global__ __launch_bounds__((lg_threads<DT, G, NV>)) void layer_norm_grad_kerne
 #pragma unroll
   for (int v = 0; v < NV; v++) {
     c[v] = v * G + lane < nvec ? v * G + lane : nvec - 1;
-    gain[v] = gamma ? load_part<R>(gamma, c[v], n) : IO::all(1);
+    if (HELD) gain[v] = gamma ? load_part<R>(gamma, c[v], n) : IO::all(1);
 #pragma unroll
     for (int j = 0; j < V; j++) dgamma[v][j] = dbeta[v][j] = 0;
   }
@@ -99,8 +101,8 @@ __global__ __launch_bounds__((lg_threads<DT, G, NV>)) void layer_norm_grad_kerne
   auto request = [&](int v) {
     xr[v] = load_part<R>(x, c[v], n);
     gr[v] = load_part<R>(g, c[v], n);
+    if (!HELD) gain[v] = gamma ? load_part<R>(gamma, c[v], n) : IO::all(1);
   };
-  constexpr bool AHEAD = T < 1024;
   if (AHEAD && row < a.g.rows) {
     begin(row);
 #pragma unroll
@@ -372,6 +374,9 @@ Plan plan(nxh_context *ctx, int n, int64_t rows) {
   if (nvec <= G * NV)                                                                                           \
     return {launch<DT, G, NV>, std::min((rows + lg_threads<DT, G, NV> / G - 1) / (lg_threads<DT, G, NV> / G), units * (G == 256 ? 2 : 1))};
   LN_GROUPS_GRAD(X)
+  if constexpr (V < 8) {
+    LN_GROUPS_GRAD_WORDS(X)
+  }
 #undef X
   const int64_t tiles = (nvec + 255) / 256;
   return {launch_long<DT>, std::max<int64_t>(1, std::min(rows / 8, 2 * units / tiles))};
@@ -417,7 +422,7 @@ NXH_EXPORT int nxh_layer_norm_grad(nxh_context *ctx, const nxh_tensor *dx, const
   std::lock_guard<std::mutex> guard(ctx->mu);
   NXH_HIP(op, hipSetDevice(ctx->device));
   const bool weights = dgamma || dbeta;
-  nxh_set_path(a.g.n > LN_VECTORS_GRAD * (16 / es) ? "layer_norm_grad_long" : "layer_norm_grad");
+  nxh_set_path(a.g.n > ln_vectors_grad((int)es) * (16 / es) ? "layer_norm_grad_long" : "layer_norm_grad");
   Plan p{nullptr, 0};  // no rows: sums of nothing
   if (a.g.rows > 0)
     p = dt == NXH_F32 ? plan<NXH_F32>(ctx, a.g.n, a.g.rows) : dt == NXH_BF16 ? plan<NXH_BF16>(ctx, a.g.n, a.g.rows)

@@ -16,9 +16,12 @@ namespace {
 #define LN_GROUPS_FORWARD(X) LN_GROUPS_SHORT(X) X(32, 3) LN_GROUPS_LONG(X) X(1024, 4)
 // The gradient has not the registers: three vectors leave room for half of the waves (12.7 us, 12.2 with two of a wave).
 #define LN_GROUPS_GRAD(X) LN_GROUPS_SHORT(X) LN_GROUPS_LONG(X)
-// The most vectors that registers hold; longer rows are walked again. (With four of 1024 lanes, of which a unit
-// has registers for 128 each, the gradient keeps values in scratch memory: [2000,20000] bfloat16 454 us, 97 by walking.)
-constexpr int LN_VECTORS = 4096, LN_VECTORS_GRAD = 2048;
+#define LN_GROUPS_GRAD_WORDS(X) X(1024, 3) X(1024, 4)  // of dtypes whose vectors have at most four elements
+// The most vectors that registers hold; longer rows are walked again. In sixteen waves a lane has 128 registers: rows of float32 and
+// float64 stay in them ([2013,16000] float32 150 us by walking, 89), with 24 or 32 elements of a 16-bit dtype values would go
+// to scratch memory ([2000,20000] bfloat16 95 by walking, 111).
+constexpr int LN_VECTORS = 4096;
+constexpr int ln_vectors_grad(int element_size) { return element_size < 4 ? 2048 : 4096; }
 
 constexpr int ln_threads(int g) { return g > 256 ? g : 256; }
 

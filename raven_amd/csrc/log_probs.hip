@@ -81,10 +81,6 @@ struct Cut {
   __device__ __forceinline__ int vector(int c) const { return head + c * V; }
   __device__ __forceinline__ int single(int i) const { return i < head ? i : nvec * V + i; }
 };
-template <class S>
-__device__ __forceinline__ void store_at(S *row, int i, Words w) {
-  store_words(reinterpret_cast<S *>(reinterpret_cast<char *>(row) + (uint32_t)i * (uint32_t)sizeof(S)), w);
-}
 // body(number of its first element, vector) over those of a row's vectors begin to end that a lane has, U of them requested before the
 // first is looked at (past the last that one again: a load under a condition is waited for before the next).
 template <int G, int U, class S, class B>
@@ -327,7 +323,7 @@ struct Gradient {
   // The gradient of the row's vectors begin to end, by G lanes, and of its single elements.
   template <int G, int U, bool NEAR, bool ENTROPY>
   __device__ __forceinline__ void write(const Cut<G, S> &cut, const S *x, S *out, int begin, int end, bool singles, int lane) const {
-    vectors<G, U>(cut, x, begin, end, lane, [&](int i, Words raw) { store_at(out, i, vector<NEAR, ENTROPY>(raw, i)); });
+    vectors<G, U>(cut, x, begin, end, lane, [&](int i, Words raw) { store_words(element_at(out, i), vector<NEAR, ENTROPY>(raw, i)); });
     if (singles)
       for (int i = lane; i < cut.singles; i += G) out[cut.single(i)] = element<NEAR, ENTROPY>(x[cut.single(i)], cut.single(i));
   }
@@ -427,7 +423,7 @@ __global__ __launch_bounds__(group_threads(G)) void log_probs_with_grad_kernel(L
         for (int v = 0; v < NV; v++) {
           const Words d = grad.template vector<NEAR, ENTROPY>(raw[v], cut.vector(v * G + lane));
           raw[v] = request(next, v);
-          if (v * G + lane < cut.nvec) store_at(out, cut.vector(v * G + lane), d);
+          if (v * G + lane < cut.nvec) store_words(element_at(out, cut.vector(v * G + lane)), d);
           __builtin_amdgcn_sched_barrier(0);
         }
       if (lane < cut.singles) {

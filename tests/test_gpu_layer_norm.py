@@ -118,7 +118,7 @@ def test_lengths(hip, oracle, d, n):
     assert hip.last_path() == ("layer_norm_long" if n > longest else "layer_norm")
     m, r = ((t, decode(logical(t), stats(d), oracle)) for t in (mean, rstd))
     got = check_backward(hip, oracle, d, (hg, g[1]), (hx, x[1]), m, r, (hgamma, gamma[1]))
-    assert hip.last_path() == ("layer_norm_grad_long" if n > longest // 2 else "layer_norm_grad")
+    assert hip.last_path() == ("layer_norm_grad_long" if n > (longest // 2 if d.itemsize == 2 else longest) else "layer_norm_grad")
     for a, b in zip(got, hip.layer_norm_grad(hg, hx, mean, rstd, hgamma)):
         same_bits(logical(a), logical(b), "equal calls")
     check_forward(hip, oracle, d, (hx, x[1]))
@@ -137,6 +137,20 @@ def test_numbers_of_rows(hip, oracle, d, rows, n):
     _, mean, rstd = check_forward(hip, oracle, d, (hx, x[1]), (hgamma, gamma[1]))
     m, r = ((t, decode(logical(t), stats(d), oracle)) for t in (mean, rstd))
     check_backward(hip, oracle, d, (hg, g[1]), (hx, x[1]), m, r, (hgamma, gamma[1]))
+
+
+@pytest.mark.parametrize("d, n", [(dt.float32, 9001), (dt.float32, 12300), (dt.float32, 16384), (dt.float64, 5003), (dt.float64, 8191), (dt.bfloat16, 5001),
+                                  (dt.bfloat16, 16381), (dt.float16, 20001)], ids=lambda v: v.name if hasattr(v, "name") else str(v))
+def test_many_wide_rows(hip, oracle, d, n):
+    """Several rows to a block, some blocks one fewer."""
+    x, g = (drawn((523, n), d, oracle, n + k, 1.5, 0.4) for k in (0, 1))
+    gamma = drawn((n,), d, oracle, n, 0.3, 1.0)
+    hx, hg, hgamma = (tensor(hip, v[0], d) for v in (x, g, gamma))
+    _, mean, rstd = check_forward(hip, oracle, d, (hx, x[1]), (hgamma, gamma[1]))
+    m, r = ((t, decode(logical(t), stats(d), oracle)) for t in (mean, rstd))
+    got = check_backward(hip, oracle, d, (hg, g[1]), (hx, x[1]), m, r, (hgamma, gamma[1]))
+    over = hip.layer_norm_grad(hg, hx, mean, rstd, hgamma, out=(hx, got[1], got[2]))
+    same_bits(logical(over[0]), logical(got[0]), "in place")
 
 
 def views(B, n):
