@@ -516,6 +516,8 @@ struct Top {
   using S = typename IO::S;
   using T = typename KeyOf<C>::T;
   static constexpr int V = IO::V, W = G / 64, PLACES = TopSpace<DT, G>::PLACES, LANES = TopSpace<DT, G>::LANES;
+  // A key has so many bits that tell elements apart, above some that do not (float16 has 19, bfloat16 16).
+  static constexpr int BITS = sizeof(S) == 2 ? 20 : 8 * (int)sizeof(T), SPARE = 8 * (int)sizeof(T) - BITS;
   const S *x;
   int n, k;
   const Cut<G, S> cut;
@@ -526,8 +528,9 @@ struct Top {
   __device__ __forceinline__ Top(const S *row, int length, int top, TopSpace<DT, G> &space) : x(row), n(length), k(top), cut(row, length), l(space) {}
 
   // give(place, key, index) for the k largest of the first m entries of the list. A wave's lanes hold an entry each and count the
-  // larger ones. Of 65 to 256 entries each wave takes its share, an entry at a time, against four that each lane holds. Of more, the k-th
-  // is found first, bit by bit of key and index (all of 256 against all others, read again for each, took 40 us).
+  // larger ones. Of 65 to 256 entries each of several waves takes its share, an entry at a time, against four that each lane holds (one
+  // wave by itself: 59 us for 64 of [20,260] float32, 20 as follows). Of more, the k-th is found first, bit by bit of the key, and
+  // of the index where entries tie there.
   template <class F>
   __device__ __forceinline__ void rank(int m, F &&give) const {
     if (W > 1 && m > 64 && m <= 256) {
@@ -563,25 +566,34 @@ struct Top {
     } else {
       auto number = [&](auto &&is) {
         int c = 0;
-        for (int j = lane; j - lane < m; j += 64) c += __popcll(__ballot(j < m && is(l.key[j], l.index[j])));
+        for (int j = lane; j - lane < m; j += 256) {
+          T e[4];
+#pragma unroll
+          for (int q = 0; q < 4; q++) e[q] = l.key[j + q * 64 < m ? j + q * 64 : m - 1] >> SPARE;
+#pragma unroll
+          for (int q = 0; q < 4; q++) c += __popcll(__ballot(j + q * 64 < m && is(e[q], j + q * 64)));
+        }
         return c;
       };
       T bound = 0;
-      for (int bit = 8 * (int)sizeof(T) - 1; bit >= 0; bit--) {
+      for (int bit = BITS - 1; bit >= 0; bit--) {
         const T next = bound | (T)1 << bit;
-        if (number([&](T e, uint32_t) { return e >= next; }) >= k) bound = next;
+        if (number([&](T e, int) { return e >= next; }) >= k) bound = next;
       }
-      const int equal = k - number([&](T e, uint32_t) { return e > bound; });  // so many of those at the bound, the first ones
-      uint32_t last = 0;
-      for (int bit = 23; bit >= 0; bit--) {
-        const uint32_t next = last | 1u << bit;
-        if (number([&](T e, uint32_t i) { return e == bound && i < next; }) < equal) last = next;
+      const int above = number([&](T e, int) { return e > bound; }), least = number([&](T e, int) { return e >= bound; });
+      uint32_t last = ~0u;  // of those at the bound the first ones, up to this index
+      if (least > k) {
+        last = 0;
+        for (int bit = 31 - __builtin_clz(n); bit >= 0; bit--) {
+          const uint32_t next = last | 1u << bit;
+          if (above + number([&](T e, int j) { return e == bound && l.index[j] < next; }) < k) last = next;
+        }
       }
       count = 0;
       for (int j = lane; j - lane < m; j += 64) {
         const T e = j < m ? l.key[j] : 0;
         const uint32_t i = j < m ? l.index[j] : ~0u;
-        const bool is = e > bound || (e == bound && i <= last);
+        const bool is = j < m && (e >> SPARE > bound || (e >> SPARE == bound && i <= last));
         const uint64_t all = __ballot(is);
         if (is) {
           const int place = count + __popcll(all & (((uint64_t)1 << lane) - 1));
@@ -622,6 +634,16 @@ struct Top {
 #pragma unroll
     for (int j = 0; j < V; j++) offer(e.x[j], i + j, least);
   }
+  // The k-th largest of the keys of a wave's lanes, down to the bits that tell them apart.
+  __device__ __forceinline__ static T wave_kth(T key, int k) {
+    T kth = 0;
+#pragma unroll
+    for (int bit = BITS + SPARE - 1; bit >= SPARE; bit--) {
+      const T next = kth | (T)1 << bit;
+      if (__popcll(__ballot(key >= next)) >= k) kth = next;
+    }
+    return kth;
+  }
   // Before the barrier of the statistics: the wave's part in the bound. Waves that are not full of vectors take no part in it; of a
   // row that one wave holds every lane with an element is looked at.
   __device__ __forceinline__ void begin(C seen) {
@@ -629,11 +651,16 @@ struct Top {
     mine = lane < nvec || lane < cut.singles ? key_of(seen) : 0;
     T most = full ? ~(T)0 : 1;
     if (wave < full) {
-      T left = mine;
-      for (int r = 0; r * full < k; r++) {
-        most = lanes_combine<64>(left, Highest<T>{});
-        const uint64_t have = __ballot(left == most);
-        if ((lane & 63) == __builtin_ctzll(have)) left = 0;
+      const int share = (k + full - 1) / full;
+      if (share > 8) {
+        most = wave_kth(mine, share);
+      } else {
+        T left = mine;
+        for (int r = 0; r < share; r++) {
+          most = lanes_combine<64>(left, Highest<T>{});
+          const uint64_t have = __ballot(left == most);
+          if ((lane & 63) == __builtin_ctzll(have)) left = 0;
+        }
       }
     }
     if ((lane & 63) == 0) l.low[wave] = most;
@@ -706,15 +733,9 @@ struct Top {
       int lanes = l.lanes;
       const uint32_t *which = l.lane;
       if (lanes <= 64) {  // each wave by itself finds the k-th largest of them, down to the bits that a 16-bit dtype has
-        constexpr int bits = 8 * (int)sizeof(T);
         const int i = lane & 63;
         const T key = i < lanes ? l.lane_key[i] : 0;
-        T kth = 0;
-#pragma unroll
-        for (int bit = bits - 1; bit >= (sizeof(S) == 2 ? bits - 20 : 0); bit--) {
-          const T next = kth | (T)1 << bit;
-          if (__popcll(__ballot(key >= next)) >= k) kth = next;
-        }
+        const T kth = wave_kth(key, k);
         if (kth > bound) bound = kth;
         const uint64_t reach = __ballot(i < lanes && key >= bound);
         if (reach >> i & 1) l.few[__popcll(reach & (((uint64_t)1 << i) - 1))] = l.lane[i];  // (the same of every wave)
