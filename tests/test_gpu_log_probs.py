@@ -192,6 +192,25 @@ def test_orders_and_ties(hip, oracle, d, n):
 
 
 @pytest.mark.parametrize("d", FLOATS, ids=lambda d: d.name)
+@pytest.mark.parametrize("n", [64, 65, 98, 130, 257, 511, 700, 1000, 2900, 40000])
+def test_many_alternatives_that_tie(hip, oracle, d, n):
+    """Rows of few values, of both signs, so that many an entry ties with the last alternative; of them some with NaNs, which come last,
+    infinities, and elements that are banned."""
+    rng = np.random.default_rng(n)
+    x = np.stack([rng.integers(-m, m + 1, n) / 8 for m in (1, 2, 5, 12, 30, 100, 400)] * 4)
+    x[7:14] = np.where(rng.random((7, n)) < 0.5, -np.inf, x[7:14])
+    x[14:21] = -np.abs(x[14:21]) - 1
+    x[21:28, rng.integers(0, n, n // 2)] = np.nan
+    x[24:28, rng.integers(0, n, 3)] = np.inf
+    xs = encode(x, d, oracle)
+    x = decode(xs, d, oracle)
+    hx, ht = tensor(hip, xs, d), hip.full(dt.int32, (28,), 0)
+    for k in (1, 7, 9, 33, 64):
+        want = np.argsort(-x, -1, kind="stable")[:, :k]
+        assert np.array_equal(logical(hip.log_probs(hx, ht, k)[5]), want), k
+
+
+@pytest.mark.parametrize("d", FLOATS, ids=lambda d: d.name)
 @pytest.mark.parametrize("n", [6, 40, 700, 9000])
 def test_values_that_are_no_numbers(hip, oracle, d, n):
     rng = np.random.default_rng(n)
