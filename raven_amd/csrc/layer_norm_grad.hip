@@ -9,8 +9,8 @@
 // Nothing is added by atomics, so equal calls give equal bits. All sums are float32 (float64 for float64).
 //
 // Memory bounds it: g and x in, dx out; the partial sums are held to some percent of that by the
-// number of blocks. [65536,1024] bfloat16 79 us (5.1 TB/s), [16384,4096] 86. Of [8192,768], 11.7 us, a half does not go by the
-// rows: 3.7 us from the launch to the end of a first row, 1.5 for the blocks' sums, 2.2 for the second launch.
+// number of blocks. [65536,1024] bfloat16 79 us (5.1 TB/s), [16384,4096] 81 (5.0), [16384,16384] 311 (5.2). Of [8192,768], 11.5 us, a
+// half does not go by the rows: 3.7 us from the launch to the end of a first row, 1.5 for the blocks' sums, 2.2 for the second launch.
 
 #include "layer_norm_train.hpp"
 
@@ -365,6 +365,9 @@ void launch_long(nxh_context *ctx, const LayerNormGradArgs &a, int64_t blocks) {
   if (a.o[LG_DX].base)
     hipLaunchKernelGGL((layer_norm_grad_long_kernel<DT>), dim3((unsigned)std::min(a.g.rows, units)), dim3(LONG_THREADS), 0, ctx->stream, a);
 }
+// A block for each unit: another one has partial sums of its own, which are to be written and read. It pays where blocks of four waves keep
+// too little on its way, with many rows ([30000,3600] bfloat16 157 us with one, 127 with two; [16384,8192], twice the vectors a lane, 161 and
+// 164; [1024,4096] 15 and 19).
 template <int DT>
 Plan plan(nxh_context *ctx, int n, int64_t rows) {
   constexpr int V = Io<DT>::V;
@@ -372,7 +375,7 @@ Plan plan(nxh_context *ctx, int n, int64_t rows) {
   const int nvec = (n + V - 1) / V;
 #define X(G, NV)                                                                                                \
   if (nvec <= G * NV)                                                                                           \
-    return {launch<DT, G, NV>, std::min((rows + lg_threads<DT, G, NV> / G - 1) / (lg_threads<DT, G, NV> / G), units * (G == 256 ? 2 : 1))};
+    return {launch<DT, G, NV>, std::min((rows + lg_threads<DT, G, NV> / G - 1) / (lg_threads<DT, G, NV> / G), units * (G == 256 && NV == 2 && rows > 16 * units ? 2 : 1))};
   LN_GROUPS_GRAD(X)
   if constexpr (V < 8) {
     LN_GROUPS_GRAD_WORDS(X)
