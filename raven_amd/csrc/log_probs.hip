@@ -12,7 +12,7 @@
 // have terms of one sign, so nothing cancels, and peak and total are given out apart: x - peak is exact
 // near the peak, where x - log(sum e^x) would round to the step of the logarithm. Memory bounds it: the
 // logits once; the gradient once more in and out. Five alternatives of [2048,50257] float32 75 us (5.5 TB/s);
-// [8192,50257] bfloat16 statistics 141 us (5.8 TB/s), both at once 317 us (5.2 TB/s), the gradient by itself 279.
+// [8192,50257] bfloat16 statistics 141 us (5.8 TB/s), both at once 315 us (5.2 TB/s), the gradient by itself 290 (5.7).
 //
 // Exponentials are powers of two: with L = log2 e and the reference A = peak L as it rounds, 2^(x L - A) is one
 // fused step and one instruction. What A lost in rounding, r = peak L - A, is a factor 2^r of every term: the
