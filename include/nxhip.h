@@ -359,7 +359,9 @@ int nxh_linear_gelu_tanh(nxh_context *ctx, const nxh_tensor *out, const nxh_tens
 
 /* out = (x - mean) * rstd [* gamma] [+ beta] over the last axis, mean = sum x / n,
    rstd = 1 / sqrt (sum (x - mean)^2 / n + eps). mean and rstd are what the gradient
-   takes, each may be NULL; gamma and beta (rank 1, the row's length, x's dtype) too. */
+   takes, each may be NULL; gamma and beta (rank 1, the row's length, x's dtype) too. All rows
+   are made with gamma and beta: mean and rstd of several rows cannot replace them
+   (Invalid_argument). */
 int nxh_layer_norm(nxh_context *ctx, const nxh_tensor *out, const nxh_tensor *mean, const nxh_tensor *rstd,
                    const nxh_tensor *x, const nxh_tensor *gamma, const nxh_tensor *beta, double eps);
 /* The gradients of nxh_layer_norm for g, what flows back into its out; x, gamma as there,

@@ -191,6 +191,11 @@ NXH_EXPORT int nxh_layer_norm(nxh_context *ctx, const nxh_tensor *out, const nxh
     if (t && ((rc = row_values_ok(op, t, x, statistics_dtype(dx))) || (rc = out_rows_ok(op, t)))) return rc;
   for (const nxh_tensor *t : {gamma, beta})
     if (t && (rc = row_vector_ok(op, t, a.g.n))) return rc;
+  // With as many rows as columns statistics have the shape of the weights, which blocks read at their start, while others already write.
+  for (const nxh_tensor *t : {mean, rstd})
+    for (const nxh_tensor *w : {gamma, beta})
+      if (t && w && a.g.rows > 1 && same_view(t, w))
+        return nxh_fail(NXH_INVALID_ARGUMENT, op, "mean and rstd must not replace gamma or beta");
   if (a.g.rows == 0) return NXH_OK;
   if (a.g.n == 0) return nxh_fail(NXH_INVALID_ARGUMENT, op, NXH_ERR_EMPTY_REDUCE);
   if (!unit_stride(x) || !unit_stride(out)) return nxh_fail(NXH_FAILURE, op, "rows must be contiguous");

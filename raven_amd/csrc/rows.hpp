@@ -142,6 +142,15 @@ int row_vector_ok(const char *op, const nxh_tensor *t, int n) {
   if (n > 1 && t->strides[0] != 1) return nxh_fail(NXH_FAILURE, op, "rows must be contiguous");
   return NXH_OK;
 }
+// Whether two tensors are one view: the same elements in the same order.
+bool same_view(const nxh_tensor *a, const nxh_tensor *b) {
+  if (a->dtype != b->dtype || a->ndim != b->ndim) return false;
+  const int64_t es = (int64_t)nxh_elem_size(a->dtype);
+  if ((const char *)a->data + a->offset * es != (const char *)b->data + b->offset * es) return false;
+  for (int d = 0; d < a->ndim; d++)
+    if (a->shape[d] != b->shape[d] || (a->shape[d] > 1 && a->strides[d] != b->strides[d])) return false;
+  return true;
+}
 bool unit_stride(const nxh_tensor *t) { return t->shape[t->ndim - 1] <= 1 || t->strides[t->ndim - 1] == 1; }
 
 }  // namespace

@@ -1,0 +1,55 @@
+"""Results of the training operators in the place of inputs that have their shape."""
+
+import numpy as np
+import pytest
+
+from helpers import logical, same_bits
+from raven_amd import dtype as dt
+
+pytestmark = pytest.mark.gpu
+
+
+def square(hip, d, n):
+    rng = np.random.default_rng(n)
+    x, gamma, beta = (rng.standard_normal(s).astype(d.np_storage) for s in ((n, n), (n,), (n,)))
+    return hip.reshape(hip.from_host(x, d), (n, n)), hip.from_host(gamma, d), hip.from_host(beta, d)
+
+
+@pytest.mark.parametrize("d", [dt.float32, dt.float64], ids=lambda d: d.name)
+@pytest.mark.parametrize("n", [2, 300, 700])
+def test_statistics_never_replace_weights(hip, d, n):
+    """With as many rows as columns mean and rstd have the shape of gamma and beta, which every row is made with: rows that are done would
+    write what others have yet to read."""
+    x, gamma, beta = square(hip, d, n)
+    y = hip.buffer(d, (n, n))
+    held = logical(gamma), logical(beta)
+    for out in ((y, gamma, None), (y, None, gamma), (y, beta, None), (y, None, beta), (y, gamma, beta), (x, hip.shrink(beta, [(0, n)]), None)):
+        with pytest.raises(ValueError, match="layer_norm: mean and rstd must not replace gamma or beta"):
+            hip.layer_norm(x, gamma, beta, out=out)
+    same_bits(logical(gamma), held[0], "gamma")
+    same_bits(logical(beta), held[1], "beta")
+    # weights that the call does not have may be replaced, and a view beside the weights may be written
+    want = [logical(t) for t in hip.layer_norm(x, gamma)]
+    both = hip.from_host(np.concatenate([held[0], held[1]]), d)
+    first, second = hip.shrink(both, [(0, n)]), hip.shrink(both, [(n, 2 * n)])
+    for a, b in zip(hip.layer_norm(x, first, out=(y, second, beta)), want):
+        same_bits(logical(a), b, "beside gamma")
+    same_bits(logical(first), held[0], "gamma beside its statistics")
+
+
+def test_gradients_of_weights_may_replace_statistics(hip):
+    n, d = 300, dt.float32
+    x, gamma, g = square(hip, d, n)
+    g = hip.reshape(hip.from_host(np.random.default_rng(1).standard_normal((n, n)).astype(np.float32), d), (n, n))
+    _, mean, rstd = hip.layer_norm(x, gamma)
+    want = [logical(t) for t in hip.layer_norm_grad(g, x, mean, rstd, gamma)]
+    for a, b in zip(hip.layer_norm_grad(g, x, mean, rstd, gamma, out=(hip.buffer(d, (n, n)), mean, rstd)), want):
+        same_bits(logical(a), b, "over the statistics")
+
+
+def test_a_single_row_of_one(hip):
+    """One row: its statistics are written when the weights have been read."""
+    d = dt.float32
+    x, gamma, beta = (hip.reshape(hip.from_host(np.array([v], np.float32), d), s) for v, s in ((3.0, (1, 1)), (2.0, (1,)), (0.5, (1,))))
+    y, mean, rstd = hip.layer_norm(x, gamma, beta, out=(hip.buffer(d, (1, 1)), gamma, beta))
+    assert logical(y)[0, 0] == 0.5 and logical(mean)[0] == 3 and logical(rstd)[0] == np.float32(1) / np.sqrt(np.float32(1e-5))
