@@ -389,7 +389,7 @@ int nxh_dropout(nxh_context *ctx, const nxh_tensor *out, const nxh_tensor *x, co
    probabilities, in descending order, equal logits by index, NaNs last: top_log_p, top_tokens
    (int32), logits' shape with 0 to 64 as last extent, rows contiguous. Each result may be NULL, the
    last two together. A logit of -inf has probability 0; a row with a NaN or +inf, or of -inf
-   alone, has NaN for all values but peak (the largest that is a number). */
+   alone, has NaN for all values but peak (the largest that is a number) and log_p of padding. */
 int nxh_log_probs(nxh_context *ctx, const nxh_tensor *log_p, const nxh_tensor *entropy, const nxh_tensor *peak,
                   const nxh_tensor *total, const nxh_tensor *top_log_p, const nxh_tensor *top_tokens,
                   const nxh_tensor *logits, const nxh_tensor *tokens);
@@ -397,7 +397,8 @@ int nxh_log_probs(nxh_context *ctx, const nxh_tensor *log_p, const nxh_tensor *e
    what flows back into entropy (values of rows, broadcasts among them):
      g (1[token] - p) - g_entropy p (log p + entropy)
    peak, total and entropy as nxh_log_probs gave them; entropy is NULL where g_entropy is. The
-   first term is left out for padding; a token past the row makes its row NaN. */
+   first term is left out for padding: without g_entropy its row is zeros, whatever the logits
+   are. A token past the row makes its row NaN. */
 int nxh_log_probs_grad(nxh_context *ctx, const nxh_tensor *out, const nxh_tensor *g, const nxh_tensor *logits,
                        const nxh_tensor *tokens, const nxh_tensor *peak, const nxh_tensor *total,
                        const nxh_tensor *g_entropy, const nxh_tensor *entropy);

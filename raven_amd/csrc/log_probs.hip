@@ -286,6 +286,7 @@ struct Gradient {
   C peak, ref, inv_total, g, g_entropy, shift;  // inner = log p + entropy = ln2 d + shift for the exponent d
   int token;
   bool with_entropy, near;
+  uint32_t there;  // all bits; none for padding without an entropy's gradient, which has zeros whatever its logits are: NaNs among them
   __device__ __forceinline__ Gradient(const LogProbsArgs &a, const Upstream<C> &up, const Statistics<C> &z) {
     peak = z.peak;
     near = is_near(peak);
@@ -295,6 +296,7 @@ struct Gradient {
     token = up.token;
     g = token < 0 ? 0 : token >= a.g.n ? (C)__builtin_nan("") : up.g;
     with_entropy = a.o[LP_G_ENTROPY].base != nullptr;
+    there = token < 0 && !with_entropy ? 0 : ~0u;
     g_entropy = up.g_entropy;
     shift = with_entropy ? z.entropy - z.log_total - Bounds<C>::ln2 * lost : 0;
   }
@@ -314,11 +316,11 @@ struct Gradient {
     if (j < (unsigned)IO::V)
 #pragma unroll
       for (int k = 0; k < IO::V; k++) v[k] = v[k] + ((unsigned)k == j ? g : 0);
-    return IO::narrow(v);
+    return IO::narrow(v) & there;
   }
   template <bool NEAR, bool ENTROPY>
   __device__ __forceinline__ S element(S x, int i) const {
-    return IO::st(at<NEAR, ENTROPY>(IO::ld(x)) + (i == token ? g : 0));
+    return there ? IO::st(at<NEAR, ENTROPY>(IO::ld(x)) + (i == token ? g : 0)) : S{};
   }
   // The gradient of the row's vectors begin to end, by G lanes, and of its single elements.
   template <int G, int U, bool NEAR, bool ENTROPY>
