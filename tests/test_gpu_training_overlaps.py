@@ -53,3 +53,19 @@ def test_a_single_row_of_one(hip):
     x, gamma, beta = (hip.reshape(hip.from_host(np.array([v], np.float32), d), s) for v, s in ((3.0, (1, 1)), (2.0, (1,)), (0.5, (1,))))
     y, mean, rstd = hip.layer_norm(x, gamma, beta, out=(hip.buffer(d, (1, 1)), gamma, beta))
     assert logical(y)[0, 0] == 0.5 and logical(mean)[0] == 3 and logical(rstd)[0] == np.float32(1) / np.sqrt(np.float32(1e-5))
+
+
+@pytest.mark.parametrize("d", [dt.float32, dt.float64], ids=lambda d: d.name)
+@pytest.mark.parametrize("rows, n", [(1, 1), (700, 5), (70, 33), (9, 64)])
+def test_alternatives_that_replace_logits(hip, d, rows, n):
+    """Where all of a row is listed its log probabilities have the shape of the logits."""
+    rng = np.random.default_rng(n)
+    x = rng.standard_normal((rows, n)).astype(d.np_storage)
+    x[0] = 3e6  # (far from zero: walked twice)
+    logits = lambda: hip.reshape(hip.from_host(x, d), (rows, n))  # noqa: E731
+    tokens = hip.from_host(rng.integers(0, n, rows).astype(np.int32), dt.int32)
+    want = [logical(t) for t in hip.log_probs(logits(), tokens, n)]
+    over = logits()
+    out = tuple(hip.buffer(d, (rows,)) for _ in range(4)) + (over, hip.buffer(dt.int32, (rows, n)))
+    for a, b in zip(hip.log_probs(over, tokens, n, out=out), want):
+        same_bits(logical(a), b, "over the logits")
