@@ -376,8 +376,9 @@ int nxh_layer_norm_grad(nxh_context *ctx, const nxh_tensor *dx, const nxh_tensor
    graph uses what it holds at each replay) and of an element's row-major position i in x's
    shape: block i / 4 of nxh_threefry (counter words: low 32 bits, high 32 bits) gives two words,
    whose four halves (low, high, low, high) are the numbers u of the block's four elements; kept
-   is u >= cut, cut = floor (65536 rate + 1/2), scale = 65536 / (65536 - cut). rate 1 keeps
-   nothing. The gradient of x for g is nxh_dropout of g with the same key and rate, the
+   is u >= cut, cut = floor (65536 rate + 1/2), scale = 65536 / (65536 - cut). A rate is thereby
+   rounded to a whole number of 65536ths: below 2^-17 nothing is dropped (scale 1), and from
+   1 - 2^-17 on nothing is kept. The gradient of x for g is nxh_dropout of g with the same key and rate, the
    residual's is g itself. */
 int nxh_dropout(nxh_context *ctx, const nxh_tensor *out, const nxh_tensor *x, const nxh_tensor *residual,
                 const nxh_tensor *key, double rate);
@@ -403,7 +404,9 @@ int nxh_log_probs_grad(nxh_context *ctx, const nxh_tensor *out, const nxh_tensor
                        const nxh_tensor *tokens, const nxh_tensor *peak, const nxh_tensor *total,
                        const nxh_tensor *g_entropy, const nxh_tensor *entropy);
 /* Both at once, for losses whose g and g_entropy do not depend on log_p and entropy (a mean of
-   them, with weights): reads the logits from memory once. log_p, entropy, g_entropy may be NULL. */
+   them, with weights). Logits are read once where a row has at most 8192 vectors of 16 bytes (in
+   float64 256); longer rows are read again, from the caches where those hold them. log_p, entropy,
+   g_entropy may be NULL. */
 int nxh_log_probs_with_grad(nxh_context *ctx, const nxh_tensor *log_p, const nxh_tensor *entropy, const nxh_tensor *out,
                             const nxh_tensor *g, const nxh_tensor *logits, const nxh_tensor *tokens,
                             const nxh_tensor *g_entropy);

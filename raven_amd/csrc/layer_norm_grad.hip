@@ -70,7 +70,9 @@ __global__ __launch_bounds__((lg_threads<DT, G, NV>)) void layer_norm_grad_kerne
   __shared__ __align__(16) C lds[G > 64 ? 2 * (G / 64) : 2 * HALF];
   const int lane = threadIdx.x % G, n = a.g.n, nvec = (n + V - 1) / V;
   const S *gamma = reinterpret_cast<const S *>(a.gamma);
-  // Sixteen waves have registers for a row at a time, and for gamma, which the caches have, while its row is read.
+  // A lane of sixteen waves has 128 registers. Two vectors of a 16-bit dtype take 111 of them, four of float32 116, with one row at a time; one
+  // vector takes 34 to 68 (float64 too) and would have room for the next row's, which has not been tried. Where a row is all sixteen waves'
+  // gamma, which the caches have, is read with it.
   constexpr bool AHEAD = T < 1024, HELD = G < 1024;
   // Every lane loads for every v, a vector past the row as the row's last: a load under a condition is waited for before the next one.
   int c[NV];

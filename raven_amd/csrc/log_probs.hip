@@ -12,7 +12,8 @@
 // have terms of one sign, so nothing cancels, and peak and total are given out apart: x - peak is exact
 // near the peak, where x - log(sum e^x) would round to the step of the logarithm. Memory bounds it: the
 // logits once; the gradient once more in and out. Five alternatives of [2048,50257] float32 75 us (5.5 TB/s);
-// [8192,50257] bfloat16 statistics 141 us (5.8 TB/s), both at once 315 us (5.2 TB/s), the gradient by itself 290 (5.7).
+// [8192,50257] bfloat16 statistics 152 to 159 us (5.2 to 5.4 TB/s, on three inputs in turn; 141 on one), both at once 318
+// (5.2), the gradient by itself 290 (5.7).
 //
 // Exponentials are powers of two: with L = log2 e and the reference A = peak L as it rounds, 2^(x L - A) is one
 // fused step and one instruction. What A lost in rounding, r = peak L - A, is a factor 2^r of every term: the
@@ -440,7 +441,8 @@ __global__ __launch_bounds__(group_threads(G)) void log_probs_with_grad_kernel(L
     cut = next;
   }
 }
-// Rows longer than that are read again, out of the caches.
+// Rows longer than that are read again, out of the caches: those of float64 from 257 vectors on, which then have 1024 lanes each, many of them
+// with no vector ([8192,512] float64 22 us by the kernel above, [8192,600] 156 by this one, [4096,1500] 97, [2048,4000] 70).
 template <int DT, int G>
 __global__ __launch_bounds__(G) void log_probs_with_grad_long_kernel(LogProbsArgs a) {
   using IO = Io<DT>;
@@ -909,7 +911,9 @@ dim3 row_blocks(const LogProbsArgs &a, int threads, int group) {
 // How many parts a row is cut into; 1: not at all. Two launches more and what the parts pass on have to pay (eight rows of bfloat16, whole
 // and in parts: statistics of 50257 elements 6.5 and 7.0 us, of 80000 8.6 and 6.8; with their gradient 11.7 and 10.7, 14.5 and 10.6;
 // with 20 alternatives 11.3 and 15.6, 14.0 and 13.3, of 131000 17.7 and 14.9; of 50257 float32 12.2 and 14.2, of a row of 200000 22.9
-// and 14.4), and a block for every row has to leave units idle.
+// and 14.4), and a block for every row has to leave three quarters of the units idle. At that border of 64 and 65 rows the two are even at
+// 80000 float32 (statistics 10.1 in parts, 10.3 whole; with their gradient 18.0, 17.3; with 20 alternatives 19.1, 17.2); longer rows would gain
+// from parts beyond it (150000: 11.7 and 16.9; 24.7 and 30.4; 22.0 and 28.1).
 template <int DT>
 int parts_of(nxh_context *ctx, const LogProbsArgs &a) {
   const int64_t units = ctx->compute_units > 0 ? ctx->compute_units : 256, nvec = a.g.n / VECTOR<typename Tr<DT>::S>;
@@ -994,7 +998,8 @@ int launch_with_grad(nxh_context *ctx, const LogProbsArgs &a) {
   const int64_t units = ctx->compute_units > 0 ? ctx->compute_units : 256;
   auto go = [&](auto group, auto vectors) {
     constexpr int G = decltype(group)::value, T = group_threads(G), NV = decltype(vectors)::value;
-    // as many blocks as the chip has room for: some 120 registers a lane with eight vectors
+    // As many blocks as the chip has room for, but for 256 lanes with eight vectors: their 84 registers (float32; 16-bit dtypes 94) leave
+    // a unit room for five blocks, of which it gets four. (512 lanes: two; 1024: one.)
     const int64_t blocks = std::min((a.g.rows + T / G - 1) / (T / G), units * ((NV == 8 ? 1024 : 2048) / T));
     hipLaunchKernelGGL((log_probs_with_grad_kernel<DT, G, NV>), dim3((unsigned)blocks), dim3(T), 0, ctx->stream, a);
   };

@@ -583,7 +583,8 @@ class Backend(Calls):
         return out
 
     def dropout(self, x: Tensor, key: Tensor, rate: float, residual: Tensor | None = None, out: Tensor | None = None) -> Tensor:
-        """``residual +`` what of ``x`` a mask keeps, scaled by what it drops. The mask is a function of ``key`` (two
+        """``residual +`` what of ``x`` a mask keeps, scaled by what it drops. ``rate`` counts in 65536ths, to the nearest (one
+        below 2^-17 drops nothing). The mask is a function of ``key`` (two
         int32) and an element's position and is never stored: the gradient of ``x`` for ``g`` is
         ``dropout(g, key, rate)``. Calls that are to drop independently take keys of their own."""
         if out is None:
@@ -626,7 +627,7 @@ class Backend(Calls):
 
     def log_probs_with_grad(self, g: Tensor, logits: Tensor, tokens: Tensor, g_entropy: Tensor | None = None, out=None):
         """``(log_p, entropy, d_logits)`` in one call, for losses whose ``g`` and ``g_entropy`` are known before it (means,
-        weighted sums): the logits are read from memory once."""
+        weighted sums): the logits are read once where a row has at most 8192 vectors of 16 bytes (float64: 256)."""
         if out is None:
             stats = self._statistics_dtype(logits.dtype)
             out = self.buffer(stats, logits.shape[:-1]), self.buffer(stats, logits.shape[:-1]), self.buffer(logits.dtype, logits.shape)
