@@ -411,6 +411,29 @@ int nxh_log_probs_with_grad(nxh_context *ctx, const nxh_tensor *log_p, const nxh
                             const nxh_tensor *g, const nxh_tensor *logits, const nxh_tensor *tokens,
                             const nxh_tensor *g_entropy);
 
+/* Attention that is differentiated. q, out: [batch, heads, queries, dim]; k, v: [batch, kv_heads, keys,
+   dim], heads a multiple of kv_heads: query head h reads the keys of head h kv_heads / heads.
+   f16/bf16/f32, dim 1 to 128, rows contiguous and following each other within 2^23 elements, other
+   strides any (heads split from a projection's rows; zero for inputs). Query i sees key j if
+   j < lengths[its batch] (int32 [batch]; NULL: all), if mask (bool [batch, heads, queries, keys], any
+   strides; NULL: all) is true there, and with causal != 0 if j <= i + keys - queries. Over what it sees,
+   s_j = scale q_i . k_j (0 < scale <= 1e30):
+     lse_i = log sum e^(s_j)  (float32 [batch, heads, queries], any strides),  out_i = sum e^(s_j - lse_i) v_j
+   A query that sees no key has out 0 and lse -inf. Keys from a sequence's length on are not read. A key
+   hidden by the mask or by causal has probability 0, which multiplies its v like any other: an infinity
+   or a NaN there may reach queries that do not see it. Sums are float32, with one rounding on the way out; f16 and bf16
+   round the exponentials for their product with v. */
+int nxh_attention_train(nxh_context *ctx, const nxh_tensor *out, const nxh_tensor *lse, const nxh_tensor *q, const nxh_tensor *k,
+                        const nxh_tensor *v, const nxh_tensor *lengths, const nxh_tensor *mask, double scale, int causal);
+/* The gradients of q, k and v for g, what flows back into out; out and lse as nxh_attention_train gave
+   them, the other arguments as it took them. dk and dv are summed over the query heads that share them, zeros from a
+   sequence's length on; a query that sees no key has dq 0. f16 and bf16 round the probabilities and the scores'
+   gradients for their products. A gradient never replaces an input (Invalid_argument where both begin
+   at one element; other overlaps are undefined). No atomics: equal calls give equal bits. */
+int nxh_attention_grad(nxh_context *ctx, const nxh_tensor *dq, const nxh_tensor *dk, const nxh_tensor *dv, const nxh_tensor *g,
+                       const nxh_tensor *q, const nxh_tensor *k, const nxh_tensor *v, const nxh_tensor *out, const nxh_tensor *lse,
+                       const nxh_tensor *lengths, const nxh_tensor *mask, double scale, int causal);
+
 /* ── Fourier transforms ──────────────────────────────────────────────────── */
 
 /* fft / ifft (backend_intf.ml:594-598; nx_backend.ml:507-528; nx_c_fft.c:940-956,

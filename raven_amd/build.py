@@ -37,6 +37,7 @@ FLAGS = [
 # VGPR form of MFMA removes the copies: 152 registers, 3 waves per SIMD.
 PER_SOURCE_FLAGS = {
     "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "attention_train.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],  # (the same rescale)
 }
 
 

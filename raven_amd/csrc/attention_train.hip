@@ -1,0 +1,181 @@
+// attention_train.hip — nxh_attention_train: attention whose gradient follows. For a query i and the keys j it
+// sees (below its sequence's length, j <= i + keys - queries where causal, and where the mask has it)
+//   s_j = scale q . k_j,  lse = log sum e^(s_j),  out = sum e^(s_j - lse) v_j
+// A query that sees none has out 0 and lse -inf. lse is what attention_grad.hip makes the probabilities from again.
+//
+// One pass over the keys. Scores stay unscaled, e^(scale (s - m)) = 2^(c s - c m), c = scale log2(e): one fused
+// step and one power each. The reference m follows the largest score only once that is 2^8 above it, so that most
+// tiles scale no results; what an exponential has too much, its sum has too. Sums, lse and results are float32; an
+// exponential is rounded to 16 bits for the product with v, which then is the instruction's own (float32 operands: as it is).
+
+#include "attention_tiles.hpp"
+
+namespace {
+
+// Blocks of four waves. KW = 1: each has 32 queries of 128. KW = 2: two share 32 queries, each takes every other 32 keys
+// of a tile, and their results are joined at the end: twice the blocks.
+template <class EL, int DP, int KW>
+__global__ __launch_bounds__(256) void attention_train_kernel(AttentionArgs a) {
+  using S = typename EL::S;
+  constexpr int KEYS = EL::F32 ? 32 * KW : 64, QUERIES = 128 / KW, OT = DP / 32;
+  using T = Tile<EL, DP, KEYS>;
+  constexpr int STAGE = 2 * T::SIZE;
+  __shared__ __attribute__((aligned(16))) S stages[2 * STAGE];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31;
+  const int pair = wave / KW, part = wave % KW;
+  const uint32_t heads = (uint32_t)a.batch * (uint32_t)a.heads;
+  const int tile = a.tiles - 1 - (int)(blockIdx.x / heads);  // the last queries first: under a causal mask they see most
+  const int bh = (int)(blockIdx.x % heads), b = bh / a.heads, h = bh % a.heads, hk = h / (a.heads / a.kv_heads);
+  const int keys = keys_of(a, b);
+  const int q0 = tile * QUERIES + pair * 32, qi = q0 + c32;
+  const S *K = rows_of<EL>(a.k, b, hk), *V = rows_of<EL>(a.v, b, hk);
+  const uint8_t *mask = a.mask.base ? reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)b * a.mask.batch + (int64_t)h * a.mask.head : nullptr;
+  Column<EL, DP> q;
+  q.load(rows_of<EL>(a.q, b, h) + (int64_t)qi * a.q.row, qi < a.sq, a.dim);
+
+  int seen = keys;  // by the block's last query
+  if (a.causal) seen = min(seen, max(0, min((tile + 1) * QUERIES, a.sq) + a.shift));
+  const int steps = (seen + KEYS - 1) / KEYS;
+
+  T kt, vt;
+  kt.begin(a.k.row);
+  vt.begin(a.v.row);
+  auto fetch = [&](int t) {
+    kt.fetch(K, a.k.row, t * KEYS, keys, a.dim);
+    vt.fetch(V, a.v.row, t * KEYS, keys, a.dim);
+  };
+  auto lay = [&](int t) {
+    kt.lay(stages + (t & 1) * STAGE);
+    vt.lay(stages + (t & 1) * STAGE + T::SIZE);
+  };
+  if (steps > 0) {
+    fetch(0);
+    lay(0);
+    if (steps > 1) fetch(1);
+  }
+  f32x16 out[OT];
+#pragma unroll
+  for (int t = 0; t < OT; t++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) out[t][e] = 0.0f;
+  float m = -INF, sum = 0.0f;
+  float mc = 0.0f, lim = INF;  // -c m, and +inf before the first score, where exponentials take 0
+  for (int t = 0; t < steps; t++) {
+    __syncthreads();  // this tile is there, and the one before has been used
+    if (t + 1 < steps) {
+      lay(t + 1);
+      if (t + 2 < steps) fetch(t + 2);
+    }
+    const S *stage = stages + (t & 1) * STAGE;
+#pragma unroll
+    for (int sub = 0; sub < KEYS / 32; sub += KW) {
+      const int r0 = (sub + part) * 32, j0 = t * KEYS + r0;
+      if (j0 >= keys || (a.causal && j0 > q0 + 31 + a.shift)) continue;  // nothing of it is seen
+      f32x16 s;
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[e] = 0.0f;
+      rows_by_columns<EL, DP, T::PITCH>(s, stage + r0 * T::PITCH, q);
+      if (mask || j0 + 32 > keys || (a.causal && j0 + 31 > q0 + a.shift)) {
+        const uint32_t see = keys_seen(a, mask, qi, j0, keys);
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[e] = (see >> e) & 1 ? s[e] : -INF;
+      }
+      float most = s[0];
+#pragma unroll
+      for (int e = 1; e < 16; e++) most = __builtin_fmaxf(most, s[e]);
+      most = __builtin_fmaxf(most, other_half(most));
+      const bool grow = most > m && __builtin_fmaf(most, a.c2, lim) > 8.0f;
+      if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+        const float mc_new = -most * a.c2;
+        const float alpha = grow ? __builtin_amdgcn_exp2f(__builtin_fmaf(m, a.c2, mc_new)) : 1.0f;
+        m = grow ? most : m;
+        mc = grow ? mc_new : mc;
+        lim = grow ? mc_new : lim;
+        sum = sum * alpha;
+#pragma unroll
+        for (int o = 0; o < OT; o++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) out[o][e] = out[o][e] * alpha;
+      }
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.c2, mc));
+      float add = s[0];
+#pragma unroll
+      for (int e = 1; e < 16; e++) add = add + s[e];
+      sum = sum + add;
+      Weights<EL> p;
+      p.set(s);
+      add_weighted_rows<EL, DP, T::PITCH>(out, stage + T::SIZE + r0 * T::PITCH, p);
+    }
+  }
+  if constexpr (KW == 2) {  // the odd wave of a pair hands over
+    static_assert(sizeof(float) * 2 * (OT * 16 + 2) * 64 <= sizeof(stages), "results of two waves fit the stages");
+    float(*over)[OT * 16 + 2][64] = reinterpret_cast<float(*)[OT * 16 + 2][64]>(stages);
+    __syncthreads();
+    if (part == 1) {
+#pragma unroll
+      for (int o = 0; o < OT; o++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) over[pair][o * 16 + e][lane] = out[o][e];
+      over[pair][OT * 16][lane] = m;
+      over[pair][OT * 16 + 1][lane] = sum;
+    }
+    __syncthreads();
+    if (part == 1) return;
+    const float m1 = over[pair][OT * 16][lane], top = __builtin_fmaxf(m, m1), ref = top == -INF ? 0.0f : top;
+    // (a wave that saw nothing has m -inf, and its factor is 0)
+    const float f0 = __builtin_amdgcn_exp2f((m - ref) * a.c2), f1 = __builtin_amdgcn_exp2f((m1 - ref) * a.c2);
+    sum = sum * f0 + over[pair][OT * 16 + 1][lane] * f1;
+#pragma unroll
+    for (int o = 0; o < OT; o++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) out[o][e] = out[o][e] * f0 + over[pair][o * 16 + e][lane] * f1;
+    m = top;
+  }
+  sum = sum + other_half(sum);
+  if (qi >= a.sq) return;
+  store_column<EL, DP>(const_cast<S *>(rows_of<EL>(a.out, b, h)) + (int64_t)qi * a.out.row, out, sum == 0.0f ? 0.0f : 1.0f / sum, a.dim);
+  if (lane < 32) {
+    float *lse = reinterpret_cast<float *>(const_cast<char *>(a.lse.base)) + (int64_t)b * a.lse.batch + (int64_t)h * a.lse.head + (int64_t)qi * a.lse.row;
+    *lse = sum == 0.0f ? -INF : __builtin_fmaf(m, a.scale, __builtin_amdgcn_logf(sum) * LN2);
+  }
+}
+
+template <class EL, int DP, int KW>
+void launch(nxh_context *ctx, AttentionArgs a) {
+  a.tiles = (a.sq + 128 / KW - 1) / (128 / KW);
+  hipLaunchKernelGGL((attention_train_kernel<EL, DP, KW>), dim3((unsigned)(a.batch * a.heads * a.tiles)), dim3(256), 0, ctx->stream, a);
+}
+template <class EL, int KW>
+void launch_dim(nxh_context *ctx, const AttentionArgs &a) {
+  if (a.dim <= 32) launch<EL, 32, KW>(ctx, a);
+  else if (a.dim <= 64) launch<EL, 64, KW>(ctx, a);
+  else if (a.dim <= 96) launch<EL, 96, KW>(ctx, a);
+  else launch<EL, 128, KW>(ctx, a);
+}
+
+}  // namespace
+
+NXH_EXPORT int nxh_attention_train(nxh_context *ctx, const nxh_tensor *out, const nxh_tensor *lse, const nxh_tensor *q, const nxh_tensor *k,
+                                   const nxh_tensor *v, const nxh_tensor *lengths, const nxh_tensor *mask, double scale, int causal) {
+  NXH_DEFER_TOUCH(ctx, 2, out, lse, q, k, v, lengths, mask);
+  const char *op = "attention_train";
+  if (!ctx || !out || !lse || !q || !k || !v) return nxh_fail(NXH_INVALID_ARGUMENT, op, "null argument");
+  int rc;
+  for (const nxh_tensor *t : {out, lse, q, k, v, lengths, mask})
+    if (t && (rc = nxh_check_tensor(op, t))) return rc;
+  AttentionArgs a;
+  if ((rc = attention_arguments(op, a, q, k, v, out, lse, lengths, mask, scale, causal, false))) return rc;
+  if (a.batch == 0 || a.heads == 0 || a.sq == 0) return NXH_OK;
+  for (const nxh_tensor *i : {q, k, v})
+    if (same_start(out, i)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "out must not replace an input");
+  std::lock_guard<std::mutex> guard(ctx->mu);
+  NXH_HIP(op, hipSetDevice(ctx->device));
+  nxh_set_path("attention_train");
+  if (q->dtype == NXH_F32) launch_dim<gemm_tile::ElF32, 1>(ctx, a);
+  else if (q->dtype == NXH_BF16) launch_dim<gemm_tile::ElBF16, 2>(ctx, a);
+  else launch_dim<gemm_tile::ElF16, 2>(ctx, a);
+  NXH_HIP(op, hipGetLastError());
+  return NXH_OK;
+}

@@ -638,6 +638,32 @@ class Backend(Calls):
             self._check(rc)
         return out
 
+    def attention_train(self, q: Tensor, k: Tensor, v: Tensor, scale: float, causal: bool = False, lengths: Tensor | None = None,
+                        mask: Tensor | None = None, out=None):
+        """``(y, lse)``: attention of ``[batch, heads, length, dim]`` operands (fewer heads of ``k`` and ``v`` are shared) over the
+        keys below ``lengths`` (int32 ``[batch]``), where ``mask`` is true and, causal, up to a query's own; and the logarithm of
+        each row's sum, which ``attention_grad`` takes (``attention`` rounds as the primitives do and keeps none)."""
+        if out is None:
+            out = self.buffer(q.dtype, q.shape), self.buffer(dt.float32, q.shape[:-1])
+        y, lse = out
+        rc = self._lib.nxh_attention_train(self._h, y._desc(), lse._desc(), q._desc(), k._desc(), v._desc(), lengths and lengths._desc(),
+                                           mask and mask._desc(), float(scale), int(causal))
+        if rc:
+            self._check(rc)
+        return out
+
+    def attention_grad(self, g: Tensor, q: Tensor, k: Tensor, v: Tensor, y: Tensor, lse: Tensor, scale: float, causal: bool = False,
+                       lengths: Tensor | None = None, mask: Tensor | None = None, out=None):
+        """``(dq, dk, dv)``: the gradients of ``attention_train`` for ``g``, what flows back into its ``y``."""
+        if out is None:
+            out = self.buffer(q.dtype, q.shape), self.buffer(k.dtype, k.shape), self.buffer(v.dtype, v.shape)
+        dq, dk, dv = out
+        rc = self._lib.nxh_attention_grad(self._h, dq._desc(), dk._desc(), dv._desc(), g._desc(), q._desc(), k._desc(), v._desc(),
+                                          y._desc(), lse._desc(), lengths and lengths._desc(), mask and mask._desc(), float(scale), int(causal))
+        if rc:
+            self._check(rc)
+        return out
+
     # ── fold family (nx_backend.ml:266-307) ─────────────────────────────────
     def _reduce_general(self, op: str, axes: Sequence[int], x: Tensor) -> Tensor:
         """``reduce`` of any axes: out of order, empty extents, errors."""

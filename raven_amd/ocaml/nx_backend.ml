@@ -618,6 +618,26 @@ module Train = struct
     let log_p, entropy = (values (), values ()) in
     let out = create_tensor logits.context logits.dtype logits.shape in
     caml_log_probs_with_grad (Some log_p) (Some entropy) out g logits tokens g_entropy; (log_p, entropy, out)
+
+  external caml_attention_train :
+    ('a, 'b) t -> (float, Dtype.float32_elt) t -> ('a, 'b) t -> ('a, 'b) t -> ('a, 'b) t -> (int32, Dtype.int32_elt) t option ->
+    (bool, Dtype.bool_elt) t option -> float -> bool -> unit = "caml_nx_hip_attention_train_bc" "caml_nx_hip_attention_train"
+  external caml_attention_grad :
+    ('a, 'b) t -> ('a, 'b) t -> ('a, 'b) t -> ('a, 'b) t -> ('a, 'b) t -> ('a, 'b) t -> ('a, 'b) t -> ('a, 'b) t ->
+    (float, Dtype.float32_elt) t -> (int32, Dtype.int32_elt) t option -> (bool, Dtype.bool_elt) t option -> float -> bool -> unit
+    = "caml_nx_hip_attention_grad_bc" "caml_nx_hip_attention_grad"
+
+  (* [batch; heads; length; dim] operands: the result, and the logarithm of each row's sum *)
+  let attention ?lengths ?mask ?(causal = false) ~scale q k v =
+    let out = create_tensor q.context q.dtype q.shape in
+    let lse = create_tensor q.context Dtype.Float32 (row_values q) in
+    caml_attention_train out lse q k v lengths mask scale causal; (out, lse)
+
+  (* dq, dk, dv for [g], what flows back into [out] *)
+  let attention_grad ?lengths ?mask ?(causal = false) ~scale ~out ~lse q k v g =
+    let like x = create_tensor x.context x.dtype x.shape in
+    let dq, dk, dv = (like q, like k, like v) in
+    caml_attention_grad dq dk dv g q k v out lse lengths mask scale causal; (dq, dk, dv)
 end
 
 (* Recorded sequences: every operation between [capture_begin] and [capture_end]

@@ -40,6 +40,7 @@
   X(gelu_tanh) X(attention) X(linear) X(linear_gelu_tanh) X(set_deferred) X(deferred_stats)        \
   X(layer_norm) X(layer_norm_grad) X(dropout)                                  \
   X(log_probs) X(log_probs_grad) X(log_probs_with_grad)                        \
+  X(attention_train) X(attention_grad)                                         \
   X(set_cache_policy) X(cache_policy_stats)                                    \
   X(capture_begin) X(capture_end) X(graph_launch) X(graph_destroy)             \
   X(timer_start) X(timer_stop) X(last_path)
@@ -831,6 +832,48 @@ CAMLprim value caml_nx_hip_log_probs_with_grad(value vlog_p, value ventropy, val
 CAMLprim value caml_nx_hip_log_probs_with_grad_bc(value *argv, int argn) {
   (void)argn;
   return caml_nx_hip_log_probs_with_grad(argv[0], argv[1], argv[2], argv[3], argv[4], argv[5], argv[6]);
+}
+
+CAMLprim value caml_nx_hip_attention_train(value vout, value vlse, value vq, value vk, value vv, value vlengths, value vmask,
+                                           value vscale, value vcausal) {
+  CAMLparam5(vout, vlse, vq, vk, vv);
+  CAMLxparam4(vlengths, vmask, vscale, vcausal);
+  nxh_tensor o, l, q, k, v, n, m;
+  nxh_context *c = extract(vout, &o);
+  extract(vlse, &l);
+  extract(vq, &q);
+  extract(vk, &k);
+  extract(vv, &v);
+  check(c, L.attention_train(c, &o, &l, &q, &k, &v, optional(vlengths, &n), optional(vmask, &m), Double_val(vscale), Bool_val(vcausal)));
+  CAMLreturn(Val_unit);
+}
+CAMLprim value caml_nx_hip_attention_train_bc(value *argv, int argn) {
+  (void)argn;
+  return caml_nx_hip_attention_train(argv[0], argv[1], argv[2], argv[3], argv[4], argv[5], argv[6], argv[7], argv[8]);
+}
+CAMLprim value caml_nx_hip_attention_grad(value vdq, value vdk, value vdv, value vg, value vq, value vk, value vv, value vout,
+                                          value vlse, value vlengths, value vmask, value vscale, value vcausal) {
+  CAMLparam5(vdq, vdk, vdv, vg, vq);
+  CAMLxparam5(vk, vv, vout, vlse, vlengths);
+  CAMLxparam3(vmask, vscale, vcausal);
+  nxh_tensor dq, dk, dv, g, q, k, v, o, l, n, m;
+  nxh_context *c = extract(vdq, &dq);
+  extract(vdk, &dk);
+  extract(vdv, &dv);
+  extract(vg, &g);
+  extract(vq, &q);
+  extract(vk, &k);
+  extract(vv, &v);
+  extract(vout, &o);
+  extract(vlse, &l);
+  check(c, L.attention_grad(c, &dq, &dk, &dv, &g, &q, &k, &v, &o, &l, optional(vlengths, &n), optional(vmask, &m), Double_val(vscale),
+                            Bool_val(vcausal)));
+  CAMLreturn(Val_unit);
+}
+CAMLprim value caml_nx_hip_attention_grad_bc(value *argv, int argn) {
+  (void)argn;
+  return caml_nx_hip_attention_grad(argv[0], argv[1], argv[2], argv[3], argv[4], argv[5], argv[6], argv[7], argv[8], argv[9], argv[10],
+                                    argv[11], argv[12]);
 }
 
 CAMLprim value caml_nx_hip_set_deferred(value vctx, value von) {
