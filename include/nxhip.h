@@ -434,6 +434,35 @@ int nxh_attention_grad(nxh_context *ctx, const nxh_tensor *dq, const nxh_tensor 
                        const nxh_tensor *q, const nxh_tensor *k, const nxh_tensor *v, const nxh_tensor *out, const nxh_tensor *lse,
                        const nxh_tensor *lengths, const nxh_tensor *mask, double scale, int causal);
 
+/* Positions as rotations: the first 2 n dimensions of each row of q and k ([batch, heads, length, dim],
+   k with heads of its own number, or NULL with k_out) are n pairs, n the length of frequencies (float64
+   [n], 2 n <= dim, in radians); pair i at position s (positions: int32 [batch, length], any strides) becomes
+     (a, b) -> amplitude (a cos(s f_i) - b sin(s f_i), a sin(s f_i) + b cos(s f_i))
+   and the other dimensions are copied. flags: bit 0, pairs are neighbours (2 i, 2 i + 1), else halves
+   (i, i + n); bit 1, angles negated, which is the gradient. f16/bf16/f32/f64, rows contiguous, other strides any.
+   Angles are float64, sine and cosine float32 (float64 for float64), one rounding on the way out. A result may be its own
+   operand (the same view); other overlaps are undefined. */
+int nxh_rotary(nxh_context *ctx, const nxh_tensor *q_out, const nxh_tensor *k_out, const nxh_tensor *q, const nxh_tensor *k,
+               const nxh_tensor *positions, const nxh_tensor *frequencies, double amplitude, int flags);
+
+/* A step of AdamW over `count` tensors at once, in place; tensor i of each list has one shape, all are
+   contiguous. params (f16/bf16/f32, all of one dtype), grads (of that dtype), masters (NULL, or float32:
+   what 16-bit params are the rounding of; then params are only written). With f = factor (float32, one
+   element; NULL: 1), t = step (int32, one element, from 1 on), lr = rate (float32, one element), all three device memory that a recorded
+   graph reads at each replay:
+     m = beta1 m + (1 - beta1) f g,  v = beta2 v + (1 - beta2) (f g)^2
+     p = p (1 - lr decay) - lr / (1 - beta1^t) m / (sqrt v / sqrt (1 - beta2^t) + eps)
+   m and v are float32, or, with m_scales and v_scales (float32 [ceil (elements / 256)] each) and key
+   (int32 [2], device memory), float8_e4m3: elements 256 b .. 256 b + 255 of m are their codes times m_scales[b], those of
+   sqrt v likewise, and each is rounded to one of its two neighbours by random bits (nxh_threefry of key; another
+   key each step), sqrt v that is not 0 not to 0. A gradient that is not finite leaves its element (8 bits: its block of 256) not
+   finite. The same tensor twice among those that are written: Invalid_argument. */
+int nxh_adamw(nxh_context *ctx, int count, const nxh_tensor *const *params, const nxh_tensor *const *grads,
+              const nxh_tensor *const *m, const nxh_tensor *const *v, const nxh_tensor *const *masters,
+              const nxh_tensor *const *m_scales, const nxh_tensor *const *v_scales, const nxh_tensor *rate,
+              const nxh_tensor *step, const nxh_tensor *factor, const nxh_tensor *key, double beta1, double beta2,
+              double eps, double decay);
+
 /* ── Fourier transforms ──────────────────────────────────────────────────── */
 
 /* fft / ifft (backend_intf.ml:594-598; nx_backend.ml:507-528; nx_c_fft.c:940-956,

@@ -134,6 +134,8 @@ SIGNATURES = {
     "nxh_log_probs_with_grad": (C.c_int, [_CTX] + [_T] * 7),
     "nxh_attention_train": (C.c_int, [_CTX] + [_T] * 7 + [C.c_double, C.c_int]),
     "nxh_attention_grad": (C.c_int, [_CTX] + [_T] * 11 + [C.c_double, C.c_int]),
+    "nxh_rotary": (C.c_int, [_CTX] + [_T] * 6 + [C.c_double, C.c_int]),
+    "nxh_adamw": (C.c_int, [_CTX, C.c_int] + [_P(_T)] * 7 + [_T] * 4 + [C.c_double] * 4),
     "nxh_set_deferred": (C.c_int, [_CTX, C.c_int]),
     "nxh_deferred_stats": (C.c_int, [_CTX, _P(C.c_uint64), C.c_int]),
     "nxh_set_cache_policy": (C.c_int, [_CTX, C.c_int]),

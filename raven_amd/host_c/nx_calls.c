@@ -11,7 +11,8 @@
  *   Tensor        buffer, view, dtype, context (nx_backend.ml:36-43)
  *   Calls         the base class of Backend: unary, binary, compare, where, cast, copy, assign, full,
  *                 reduce, matmul; and what the frontend makes of them over operands that broadcast:
- *                 broadcast_binary, broadcast_where, reduce_keep. A call whose arguments are out of the ordinary (axes that are no
+ *                 broadcast_binary, broadcast_where, reduce_keep; adamw, whose lists of a model's tensors are a thousand
+ *                 descriptors a call. A call whose arguments are out of the ordinary (axes that are no
  *                 plain integers, batches that broadcast, ...) goes to the Python method of the same
  *                 name with `_general` behind it.
  */
@@ -36,6 +37,7 @@ static struct {
   int (*copy)(nxh_context *, const nxh_tensor *, const nxh_tensor *);
   int (*reduce)(nxh_context *, int, const nxh_tensor *, const nxh_tensor *, const int32_t *, int);
   int (*matmul)(nxh_context *, const nxh_tensor *, const nxh_tensor *, const nxh_tensor *);
+  __typeof__(nxh_adamw) *adamw;
 } L;
 
 /* what setup() hands over from Python */
@@ -763,6 +765,87 @@ static PyObject *calls_matmul(Calls *self, Args args, Py_ssize_t n, PyObject *kw
   return general(self, "_matmul_general", a, 2);
 }
 
+/* A step of AdamW. Descriptors lie in memory that is kept from call to call (fresh pages would cost more than filling them);
+   a call that finds it taken by another thread's makes its own. */
+static nxh_tensor *adamw_space;
+static size_t adamw_room;
+static PyObject *calls_adamw(Calls *self, PyObject *args, PyObject *kw) {
+  static char *names[] = {"params", "grads", "m", "v", "rate", "step", "beta1", "beta2", "eps", "decay", "factor", "masters", "m_scales", "v_scales", "key", NULL};
+  enum { LISTS = 7, ONES = 4 };
+  PyObject *lists[LISTS] = {NULL}, *ones[ONES] = {NULL}, *seq[LISTS] = {NULL};
+  double beta1 = 0.9, beta2 = 0.999, eps = 1e-8, decay = 0.0;
+  if (!PyArg_ParseTupleAndKeywords(args, kw, "OOOOOO|ddddOOOOO", names, &lists[0], &lists[1], &lists[2], &lists[3], &ones[0], &ones[1], &beta1, &beta2, &eps,
+                                   &decay, &ones[2], &lists[4], &lists[5], &lists[6], &ones[3]))
+    return NULL;
+  nxh_tensor *d = NULL;
+  const nxh_tensor **p = NULL;
+  Py_ssize_t count = 0;
+  int bad = 0, rc = 0;
+  size_t room = 0;
+  for (int l = 0; l < LISTS && !bad; l++) {
+    if (!lists[l] || lists[l] == Py_None) continue;
+    if (!(seq[l] = PySequence_Fast(lists[l], "adamw: tensors come in lists"))) bad = 1;
+    else if (l == 0) count = PySequence_Fast_GET_SIZE(seq[0]);
+    else if (PySequence_Fast_GET_SIZE(seq[l]) != count) {
+      PyErr_SetString(PyExc_ValueError, "adamw: the lists have different lengths");
+      bad = 1;
+    }
+  }
+  if (!bad && count > INT32_MAX / (2 * LISTS)) {
+    PyErr_SetString(PyExc_ValueError, "adamw: too many tensors");
+    bad = 1;
+  }
+  const size_t all = (size_t)count * LISTS + ONES;
+  if (!bad) {
+    if (adamw_room >= all) d = adamw_space, room = adamw_room;
+    else if ((d = PyMem_RawMalloc(all * sizeof *d))) {
+      PyMem_RawFree(adamw_space);
+      room = all;
+    }
+    if (d) adamw_space = NULL, adamw_room = 0;
+    p = PyMem_RawMalloc(all * sizeof *p);
+    if (!d || !p) PyErr_NoMemory(), bad = 1;
+  }
+  for (int l = 0; l < LISTS && !bad; l++)
+    for (Py_ssize_t i = 0; i < count && seq[l] && !bad; i++) {
+      const size_t at = (size_t)l * (size_t)count + (size_t)i;
+      p[at] = &d[at];
+      PyObject *o = i < PySequence_Fast_GET_SIZE(seq[l]) ? PySequence_Fast_GET_ITEM(seq[l], i) : NULL; /* (describing one may run code that cuts a list) */
+      if (!o) PyErr_SetString(PyExc_ValueError, "adamw: the lists have different lengths"), bad = 1;
+      else {
+        Py_INCREF(o);
+        bad = describe(&d[at], o);
+        Py_DECREF(o);
+      }
+    }
+  const nxh_tensor *one[ONES] = {NULL};
+  for (int k = 0; k < ONES && !bad; k++)
+    if (ones[k] && ones[k] != Py_None) {
+      one[k] = &d[all - ONES + (size_t)k];
+      bad = describe(&d[all - ONES + (size_t)k], ones[k]);
+    }
+  if (!bad) {
+    const nxh_tensor *const *of[LISTS];
+    for (int l = 0; l < LISTS; l++) of[l] = seq[l] ? p + (size_t)l * (size_t)count : NULL;
+    nxh_context *h = self->h;
+    Py_BEGIN_ALLOW_THREADS
+    rc = L.adamw(h, (int)count, of[0], of[1], of[2], of[3], of[4], of[5], of[6], one[0], one[1], one[2], one[3], beta1, beta2, eps, decay);
+    Py_END_ALLOW_THREADS
+  }
+  PyMem_RawFree(p);
+  if (d && room > adamw_room) {
+    PyMem_RawFree(adamw_space);
+    adamw_space = d;
+    adamw_room = room;
+  } else {
+    PyMem_RawFree(d);
+  }
+  for (int l = 0; l < LISTS; l++) Py_XDECREF(seq[l]);
+  if (bad) return NULL;
+  if (rc) return raise_status((PyObject *)self, rc);
+  Py_RETURN_NONE;
+}
+
 #define FAST METH_FASTCALL | METH_KEYWORDS
 static PyMethodDef calls_methods[] = {
     {"unary", (PyCFunction)(void (*)(void))calls_unary, FAST, "unary($self, op, x)\n--\n\n"},
@@ -783,6 +866,12 @@ static PyMethodDef calls_methods[] = {
      "broadcast_where($self, cond, if_true, if_false)\n--\n\nwhere, likewise."},
     {"reduce_keep", (PyCFunction)(void (*)(void))calls_reduce_keep, FAST,
      "reduce_keep($self, op, axes, x)\n--\n\nreduce whose reduced axes (ascending) stay as dims of extent 1; NotImplemented likewise."},
+    {"adamw", (PyCFunction)(void (*)(void))calls_adamw, METH_VARARGS | METH_KEYWORDS,
+     "adamw($self, params, grads, m, v, rate, step, beta1=0.9, beta2=0.999, eps=1e-08, decay=0.0, factor=None, masters=None, "
+     "m_scales=None, v_scales=None, key=None)\n--\n\n"
+     "One step of AdamW over lists of tensors, in place. ``rate``, ``step`` (from 1 on) and ``factor`` of the gradients are one element\n"
+     "each on the device. ``masters``: float32 copies that 16-bit ``params`` are the roundings of. ``m``, ``v`` are float32, or\n"
+     "float8_e4m3 of m and of v's root, with a scale for each 256 elements in ``m_scales`` and ``v_scales``, rounded by random bits of ``key``."},
     {NULL, NULL, 0, NULL}};
 static PyGetSetDef calls_getset[] = {{"_h", (getter)calls_get_h, (setter)calls_set_h, NULL, NULL}, {NULL, NULL, NULL, NULL, NULL}};
 static PyTypeObject CallsType = {
@@ -804,7 +893,7 @@ static PyObject *bind(PyObject *m, PyObject *d) {
   } e[] = {{"nxh_alloc", (void **)&L.alloc},     {"nxh_free", (void **)&L.free},       {"nxh_fill", (void **)&L.fill},
            {"nxh_unary", (void **)&L.unary},     {"nxh_binary", (void **)&L.binary},   {"nxh_compare", (void **)&L.compare},
            {"nxh_where", (void **)&L.where},     {"nxh_cast", (void **)&L.cast},       {"nxh_copy", (void **)&L.copy},
-           {"nxh_reduce", (void **)&L.reduce},   {"nxh_matmul", (void **)&L.matmul}};
+           {"nxh_reduce", (void **)&L.reduce},   {"nxh_matmul", (void **)&L.matmul}, {"nxh_adamw", (void **)&L.adamw}};
   for (size_t i = 0; i < sizeof e / sizeof *e; i++) {
     PyObject *v = PyMapping_GetItemString(d, e[i].name);
     if (!v) return NULL;

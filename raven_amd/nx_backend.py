@@ -94,7 +94,7 @@ setup(_CONTIGUOUS, View.create, view_image, stamp, encode_scalar, np.ndarray, dt
 class Backend(Calls):
     """An execution context (``create_context``, nx_backend.mli:32-39) plus the
     operations of ``Backend_intf.S``. unary, binary, compare, where, cast, copy,
-    assign, full, reduce and matmul are ``Calls``' (host_c/nx_calls.c)."""
+    assign, full, reduce and matmul are ``Calls``' (host_c/nx_calls.c), and so is adamw."""
 
     def __init__(self):
         self._lib = _ffi.load()
@@ -660,6 +660,32 @@ class Backend(Calls):
         dq, dk, dv = out
         rc = self._lib.nxh_attention_grad(self._h, dq._desc(), dk._desc(), dv._desc(), g._desc(), q._desc(), k._desc(), v._desc(),
                                           y._desc(), lse._desc(), lengths and lengths._desc(), mask and mask._desc(), float(scale), int(causal))
+        if rc:
+            self._check(rc)
+        return out
+
+    @staticmethod
+    def rotary_frequencies(pairs: int, base: float = 10000.0, factor: float = 1.0, context: int | None = None,
+                           fast: float = 32.0, slow: float = 1.0) -> np.ndarray:
+        """Radians a position for each pair, ``base ** (-i / pairs)``, as ``rotary`` takes them (float64). For contexts
+        ``factor`` times as long as those a model was trained on: all divided by it, or, with ``context`` (that length), those
+        that turn at most ``slow`` times in it, none of those that turn ``fast`` times or more, and shares in between."""
+        f = float(base) ** (-np.arange(pairs, dtype=np.float64) / max(pairs, 1))
+        if context is None:
+            return f / factor
+        keep = np.clip((context * f / (2 * np.pi) - slow) / (fast - slow), 0.0, 1.0)
+        return f * (keep + (1 - keep) / factor)
+
+    def rotary(self, q: Tensor, k: Tensor | None, positions: Tensor, frequencies: Tensor, interleaved: bool = False, inverse: bool = False,
+               amplitude: float = 1.0, out=None):
+        """``(q, k)`` (``[batch, heads, length, dim]`` each, ``k`` may be None) with the first ``2 n`` dimensions of each row turned
+        as ``n`` pairs by ``positions`` (int32 ``[batch, length]``) times ``frequencies`` (float64 ``[n]``): neighbours where
+        ``interleaved``, else halves. ``inverse`` turns back: the gradient. ``out`` may be the operands themselves."""
+        if out is None:
+            out = self.buffer(q.dtype, q.shape), k and self.buffer(k.dtype, k.shape)
+        q_out, k_out = out
+        rc = self._lib.nxh_rotary(self._h, q_out._desc(), k_out and k_out._desc(), q._desc(), k and k._desc(), positions._desc(),
+                                  frequencies._desc(), float(amplitude), int(bool(interleaved)) | int(bool(inverse)) << 1)
         if rc:
             self._check(rc)
         return out

@@ -638,6 +638,29 @@ module Train = struct
     let like x = create_tensor x.context x.dtype x.shape in
     let dq, dk, dv = (like q, like k, like v) in
     caml_attention_grad dq dk dv g q k v out lse lengths mask scale causal; (dq, dk, dv)
+
+  external caml_rotary :
+    ('a, 'b) t -> ('a, 'b) t option -> ('a, 'b) t -> ('a, 'b) t option -> (int32, Dtype.int32_elt) t -> (float, Dtype.float64_elt) t ->
+    float -> int -> unit = "caml_nx_hip_rotary_bc" "caml_nx_hip_rotary"
+
+  (* queries and keys, their first dimensions turned by position * frequency; the gradient is the [inverse] *)
+  let rotary ?(interleaved = false) ?(inverse = false) ?(amplitude = 1.0) ~positions ~frequencies q k =
+    let like x = create_tensor x.context x.dtype x.shape in
+    let q_out, k_out = (like q, Option.map like k) in
+    caml_rotary q_out k_out q k positions frequencies amplitude ((if interleaved then 1 else 0) lor if inverse then 2 else 0);
+    (q_out, k_out)
+
+  (* [any] tensors: the lists of a step hold different types *)
+  type any = Any : ('a, 'b) t -> any [@@unboxed]
+  external caml_adamw :
+    any array array -> (float, Dtype.float32_elt) t -> (int32, Dtype.int32_elt) t -> (float, Dtype.float32_elt) t option ->
+    (int32, Dtype.int32_elt) t option -> floatarray -> unit = "caml_nx_hip_adamw_bc" "caml_nx_hip_adamw"
+
+  (* a step over all of [params], in place; with [scales] (of m and of v's root) and [key], [m] and [v] are of 8 bits *)
+  let adamw ?(beta1 = 0.9) ?(beta2 = 0.999) ?(eps = 1e-8) ?(decay = 0.0) ?factor ?(masters = [||]) ?(scales = ([||], [||])) ?key ~rate ~step
+      ~params ~grads ~m ~v () =
+    caml_adamw [| params; grads; m; v; masters; fst scales; snd scales |] rate step factor key
+      (Float.Array.of_list [ beta1; beta2; eps; decay ])
 end
 
 (* Recorded sequences: every operation between [capture_begin] and [capture_end]

@@ -40,7 +40,7 @@
   X(gelu_tanh) X(attention) X(linear) X(linear_gelu_tanh) X(set_deferred) X(deferred_stats)        \
   X(layer_norm) X(layer_norm_grad) X(dropout)                                  \
   X(log_probs) X(log_probs_grad) X(log_probs_with_grad)                        \
-  X(attention_train) X(attention_grad)                                         \
+  X(attention_train) X(attention_grad) X(rotary) X(adamw)                      \
   X(set_cache_policy) X(cache_policy_stats)                                    \
   X(capture_begin) X(capture_end) X(graph_launch) X(graph_destroy)             \
   X(timer_start) X(timer_stop) X(last_path)
@@ -874,6 +874,59 @@ CAMLprim value caml_nx_hip_attention_grad_bc(value *argv, int argn) {
   (void)argn;
   return caml_nx_hip_attention_grad(argv[0], argv[1], argv[2], argv[3], argv[4], argv[5], argv[6], argv[7], argv[8], argv[9], argv[10],
                                     argv[11], argv[12]);
+}
+
+CAMLprim value caml_nx_hip_rotary(value vq_out, value vk_out, value vq, value vk, value vpositions, value vfrequencies, value vamplitude,
+                                  value vflags) {
+  CAMLparam5(vq_out, vk_out, vq, vk, vpositions);
+  CAMLxparam3(vfrequencies, vamplitude, vflags);
+  nxh_tensor qo, ko, q, k, p, f;
+  nxh_context *c = extract(vq_out, &qo);
+  extract(vq, &q);
+  extract(vpositions, &p);
+  extract(vfrequencies, &f);
+  check(c, L.rotary(c, &qo, optional(vk_out, &ko), &q, optional(vk, &k), &p, &f, Double_val(vamplitude), Int_val(vflags)));
+  CAMLreturn(Val_unit);
+}
+CAMLprim value caml_nx_hip_rotary_bc(value *argv, int argn) {
+  (void)argn;
+  return caml_nx_hip_rotary(argv[0], argv[1], argv[2], argv[3], argv[4], argv[5], argv[6], argv[7]);
+}
+
+/* lists: seven arrays (params, grads, m, v, masters, m_scales, v_scales), the last three empty where there are none; settings: beta1, beta2, eps, decay */
+CAMLprim value caml_nx_hip_adamw(value vlists, value vrate, value vstep, value vfactor, value vkey, value vsettings) {
+  CAMLparam5(vlists, vrate, vstep, vfactor, vkey);
+  CAMLxparam1(vsettings);
+  nxh_tensor r, s, f, k;
+  nxh_context *c = extract(vrate, &r);
+  extract(vstep, &s);
+  const size_t n = Wosize_val(Field(vlists, 0));
+  nxh_tensor *d = (nxh_tensor *)caml_stat_alloc(sizeof(nxh_tensor) * (7 * n + 1));
+  const nxh_tensor **p = (const nxh_tensor **)caml_stat_alloc(sizeof(nxh_tensor *) * (7 * n + 1));
+  const nxh_tensor *const *lists[7];
+  int equal = 1;
+  for (size_t l = 0; l < 7; l++) {
+    const size_t m = Wosize_val(Field(vlists, l));
+    lists[l] = m || l < 4 ? p + l * n : NULL;
+    if (m != n && (m || l < 4)) equal = 0;
+    for (size_t i = 0; i < n && m == n; i++) {
+      extract(Field(Field(vlists, l), i), &d[l * n + i]);
+      p[l * n + i] = &d[l * n + i];
+    }
+  }
+  const int rc = equal ? L.adamw(c, (int)n, lists[0], lists[1], lists[2], lists[3], lists[4], lists[5], lists[6], &r, &s, optional(vfactor, &f),
+                                 optional(vkey, &k), Double_flat_field(vsettings, 0), Double_flat_field(vsettings, 1),
+                                 Double_flat_field(vsettings, 2), Double_flat_field(vsettings, 3))
+                       : 0;
+  caml_stat_free(p);
+  caml_stat_free(d);
+  if (!equal) caml_invalid_argument("adamw: the lists have different lengths");
+  check(c, rc);
+  CAMLreturn(Val_unit);
+}
+CAMLprim value caml_nx_hip_adamw_bc(value *argv, int argn) {
+  (void)argn;
+  return caml_nx_hip_adamw(argv[0], argv[1], argv[2], argv[3], argv[4], argv[5]);
 }
 
 CAMLprim value caml_nx_hip_set_deferred(value vctx, value von) {

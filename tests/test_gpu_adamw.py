@@ -1,0 +1,366 @@
+"""adamw against its formula: float64 with bounds, and float32 bit for bit, which every operation of the step is.
+
+How far float64's results may be away, derived before the first run; u = 2^-24. x = f g is a rounding, beta and 1 - beta are roundings, so are
+the two products and the sum:
+  m  5 u (|b1 m| + |c1 x|),  v  relative 6 u (its terms are positive)
+  the denominator: root of v 3 u + u, its factor u, product and sum 2 u, eps's rounding u: relative 8 u
+  the quotient's error (m's, 9 u of it) times lr / (1 - b1^t) (2 u and a product), w (1 - lr decay): 2 u, their sum u."""
+
+import numpy as np
+import pytest
+
+from helpers import decode, encode, logical, same_bits
+from raven_amd import dtype as dt
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+HALF = {"float32": 2.0 ** -24, "float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}
+TINY = {"float32": 2.0 ** -149, "float16": 2.0 ** -25, "bfloat16": 2.0 ** -133}
+F32, F16, BF16, E4M3, I32 = dt.float32, dt.float16, dt.bfloat16, dt.float8_e4m3, dt.int32
+SHAPES = [(3,), (1,), (256,), (257,), (5, 100), (64, 64), (4095,), (4097,), (9000,), (2, 3, 7)]
+CODES = np.concatenate([np.arange(8) * 2.0 ** -9] + [2.0 ** (e - 7) * (1 + np.arange(8) / 8) for e in range(1, 16)])[:127]
+
+
+def tensor(hip, storage, d):
+    storage = np.asarray(storage)
+    return hip.reshape(hip.from_host(np.ascontiguousarray(storage), d), storage.shape)
+
+
+def read(t):
+    """A copy: storage that is stepped in place is read again later."""
+    return logical(t).copy()
+
+
+def one(hip, x, d):
+    return tensor(hip, np.array([x], d.np_storage), d)
+
+
+class Model:
+    """Tensors of some shapes, with the host's copy of what they hold."""
+
+    def __init__(self, hip, oracle, d, shapes, masters=False, bits=32, seed=0, spread=1e-3, views=False):
+        rng = np.random.default_rng(seed)
+        self.hip, self.d, self.shapes, self.bits = hip, d, shapes, bits
+        self.w = [rng.standard_normal(s).astype(np.float32) * np.float32(0.1) for s in shapes]
+        self.p_s = [encode(w, d, oracle) for w in self.w]
+        if not masters:
+            self.w = [decode(p, d, oracle).astype(np.float32) for p in self.p_s]
+        self.g_s = [encode(rng.standard_normal(s) * spread * np.exp(rng.standard_normal()), d, oracle) for s in shapes]
+        self.g = [decode(g, d, oracle).astype(np.float32) for g in self.g_s]
+        place = self.inside if views else lambda s, k: tensor(hip, s, k)
+        self.p, self.grads = [place(s, d) for s in self.p_s], [place(s, d) for s in self.g_s]
+        self.masters = [place(w, F32) for w in self.w] if masters else None
+        m = [rng.standard_normal(s) * spread / 3 for s in shapes]
+        v = [(rng.standard_normal(s) * spread) ** 2 for s in shapes]
+        if bits == 32:
+            self.m0, self.v0 = [x.astype(np.float32) for x in m], [x.astype(np.float32) for x in v]
+            self.m, self.v, self.ms, self.vs, self.key = [place(x, F32) for x in self.m0], [place(x, F32) for x in self.v0], None, None, None
+        else:
+            blocks = [-(-int(np.prod(s)) // 256) for s in shapes]
+            self.mc, self.vc = [rng.integers(0, 256, s).astype(np.uint8) for s in shapes], [rng.integers(0, 127, s).astype(np.uint8) for s in shapes]
+            for c in self.mc:
+                c[(c & 127) == 127] = 5
+            self.ms0 = [(rng.random(b) * spread / 400).astype(np.float32) for b in blocks]
+            self.vs0 = [(rng.random(b) * spread / 400).astype(np.float32) for b in blocks]
+            self.m, self.v = [place(x, E4M3) for x in self.mc], [place(x, E4M3) for x in self.vc]
+            self.ms, self.vs = [place(x, F32) for x in self.ms0], [place(x, F32) for x in self.vs0]
+            self.key_words = rng.integers(-2**31, 2**31, 2).astype(np.int32)
+            self.key = tensor(hip, self.key_words, I32)
+            self.m0 = [self.spread(decode_codes(c), s) for c, s in zip(self.mc, self.ms0)]
+            self.v0 = [self.spread(decode_codes(c), s) ** 2 for c, s in zip(self.vc, self.vs0)]
+
+    def inside(self, storage, d):
+        """A tensor in the middle of memory, one element off any alignment."""
+        flat = np.concatenate([np.zeros(3, storage.dtype), storage.reshape(-1), np.zeros(5, storage.dtype)])
+        n = storage.size
+        return self.hip.reshape(self.hip.shrink(tensor(self.hip, flat, d), [(3, 3 + n)]), storage.shape)
+
+    @staticmethod
+    def spread(x, scales):
+        return (x.reshape(-1) * np.repeat(scales, 256)[:x.size]).reshape(x.shape).astype(np.float32)
+
+    def step(self, rate=1e-2, step=3, factor=None, **kw):
+        self.hip.adamw(self.p, self.grads, self.m, self.v, one(self.hip, rate, F32), one(self.hip, step, I32), masters=self.masters,
+                       factor=None if factor is None else one(self.hip, factor, F32), m_scales=self.ms, v_scales=self.vs, key=self.key, **kw)
+
+
+def decode_codes(c):
+    return np.where(c & 128, -1, 1).astype(np.float32) * CODES.astype(np.float32)[c & 127]
+
+
+def exact(w, g, m, v, rate, step, factor=1.0, beta1=0.9, beta2=0.999, eps=1e-8, decay=0.0):
+    """(w, m, v) in float64, and how far each may be off."""
+    w, m, v, x = (np.asarray(a, np.float64) for a in (w, m, v, g))
+    rate, x = float(np.float32(rate)), x * float(np.float32(factor))
+    m_err = 5 * U * (beta1 * np.abs(m) + (1 - beta1) * np.abs(x))
+    m, v = beta1 * m + (1 - beta1) * x, beta2 * v + (1 - beta2) * x * x
+    size, root = rate / (1 - beta1 ** step), 1 / np.sqrt(1 - beta2 ** step)
+    below = np.sqrt(v) * root + eps
+    with np.errstate(divide="ignore", invalid="ignore"):
+        quotient, q_err = m / below, m_err / below
+    w_new = w * (1 - rate * decay) - quotient * size
+    w_err = 3 * U * np.abs(w) + size * (q_err * (1 + 10 * U) + 13 * U * np.abs(quotient)) + U * np.abs(w_new)
+    return (w_new, m, v), (w_err, m_err, 6 * U * v + 2.0 ** -148)
+
+
+def single(w, g, m, v, rate, step, factor=1.0, beta1=0.9, beta2=0.999, eps=1e-8, decay=0.0):
+    """The step in float32, operation by operation: (w, m, v, root of v)."""
+    f = np.float32
+    x = g * f(factor)
+    m = m * f(beta1) + x * f(1 - beta1)
+    v = v * f(beta2) + x * x * f(1 - beta2)
+    r = np.sqrt(v)
+    size, root, shrink = f(float(f(rate)) / (1 - beta1 ** step)), f(1 / np.sqrt(1 - beta2 ** step)), f(1 - float(f(rate)) * decay)
+    return w * shrink - m / (r * root + f(eps)) * size, m, v, r
+
+
+def check32(hip, oracle, d, shapes=SHAPES, masters=False, seed=0, views=False, **kw):
+    model = Model(hip, oracle, d, shapes, masters, 32, seed, views=views)
+    model.step(**kw)
+    args = {"rate": 1e-2, "step": 3, **kw}
+    for i in range(len(shapes)):
+        want, err = exact(model.w[i], model.g[i], model.m0[i], model.v0[i], **args)
+        p = decode(read(model.p[i]), d, oracle)
+        lim = err[0] + HALF[d.name] * (np.abs(want[0]) + err[0]) + TINY[d.name]
+        assert np.all(np.abs(p - want[0]) <= lim), shapes[i]
+        for t, w, e in zip((model.m[i], model.v[i]), want[1:], err[1:]):
+            assert np.all(np.abs(read(t) - w) <= e), shapes[i]
+        w32, m32, v32, _ = single(model.w[i], model.g[i], model.m0[i], model.v0[i], **args)
+        same_bits(read(model.m[i]), m32)
+        same_bits(read(model.v[i]), v32)
+        if masters:
+            same_bits(read(model.masters[i]), w32)
+        same_bits(read(model.p[i]), encode(w32, d, oracle), shapes[i])
+
+
+@pytest.mark.parametrize("d, masters", [(F32, False), (BF16, True), (F16, True), (BF16, False), (F16, False)])
+@pytest.mark.parametrize("views", [False, True])
+def test_states_of_32_bits(hip, oracle, d, masters, views):
+    check32(hip, oracle, d, masters=masters, views=views)
+
+
+@pytest.mark.parametrize("kw", [{"step": 1}, {"step": 100000}, {"decay": 0.1}, {"factor": 0.25}, {"beta1": 0.0, "beta2": 0.0}, {"eps": 1e-3, "rate": 0.0},
+                                {"beta1": 0.95, "beta2": 0.98, "decay": 0.01, "factor": 3.0, "step": 17}])
+def test_settings(hip, oracle, kw):
+    check32(hip, oracle, F32, **kw)
+
+
+def test_many_tensors(hip, oracle):
+    """More than a launch takes, with none of an element among them."""
+    check32(hip, oracle, F32, shapes=[(1 + 37 * i % 300,) for i in range(150)] + [(0,), (3, 0), (1000,)], seed=5)
+    check8(hip, oracle, BF16, shapes=[(1 + 37 * i % 300,) for i in range(150)] + [(0,), (3, 0), (1000,)], masters=True, seed=5)
+
+
+def test_large_tensor(hip, oracle):
+    check32(hip, oracle, BF16, shapes=[(3_000_001,)], masters=True)
+    check8(hip, oracle, F32, shapes=[(3_000_001,)])
+
+
+# ── states of 8 bits ────────────────────────────────────────────────────────────────────────────
+
+def numbers(hip, key, n):
+    """Sixteen bits of the generator for each of n elements."""
+    blocks = -(-n // 4)
+    counter = np.stack([np.arange(blocks), np.zeros(blocks)], 1).astype(np.int32)
+    words = logical(hip.threefry(tensor(hip, np.broadcast_to(key, (blocks, 2)), I32), tensor(hip, counter, I32))).view(np.uint32)
+    return np.stack([words[:, 0] & 0xFFFF, words[:, 0] >> 16, words[:, 1] & 0xFFFF, words[:, 1] >> 16], 1).reshape(-1)[:n]
+
+
+def rounded(x, u, never_zero):
+    """(codes, scales) of a tensor, in float32."""
+    n = x.size
+    blocks = -(-n // 256)
+    wide = np.zeros(blocks * 256, np.float32)
+    wide[:n] = x.reshape(-1)
+    most = np.abs(wide).reshape(-1, 256).max(1) if n else np.zeros(0, np.float32)
+    some = most >= 2.0 ** -100
+    inverse = np.where(some, np.float32(1) / np.where(some, most, np.float32(1)) * np.float32(448), np.float32(0)).astype(np.float32)
+    y = np.abs(wide) * np.repeat(inverse, 256)
+    low = y < np.float32(2.0 ** -6)
+    bits = np.where(low, y + np.float32(2.0 ** -6), y).astype(np.float32).view(np.uint32) + (np.pad(u, (0, wide.size - n)).astype(np.uint32) << 4)
+    codes = np.minimum((bits >> 20) - np.where(low, 968, 960), 126)
+    if never_zero:
+        codes = np.where((y > 0) & (codes == 0), 1, codes)
+    codes = codes | np.signbit(wide) * 128
+    return codes[:n].reshape(x.shape).astype(np.uint8), np.where(some, most * np.float32(1 / 448), 0).astype(np.float32)
+
+
+def check8(hip, oracle, d, shapes=SHAPES, masters=False, seed=0, views=False, **kw):
+    model = Model(hip, oracle, d, shapes, masters, 8, seed, views=views)
+    model.step(**kw)
+    args = {"rate": 1e-2, "step": 3, **kw}
+    sizes = [int(np.prod(s)) for s in shapes]
+    starts = np.cumsum([0] + [-(-n // 256) * 256 for n in sizes])
+    u = numbers(hip, model.key_words, int(starts[-1]))
+    for i, n in enumerate(sizes):
+        w32, m32, v32, r32 = single(model.w[i], model.g[i], model.m0[i], model.v0[i], **args)
+        same_bits(read(model.p[i]), encode(w32, d, oracle), shapes[i])
+        mine = u[starts[i]:starts[i] + n]
+        for t, s, x, bits, root in ((model.m[i], model.ms[i], m32, mine, False), (model.v[i], model.vs[i], r32, (mine << 8 | mine >> 8) & 0xFFFF, True)):
+            codes, scales = rounded(x, bits, root)
+            same_bits(read(s), scales, (shapes[i], root))
+            same_bits(read(t), codes, (shapes[i], root))
+            # and from the definition: no further from the value than the codes around it lie apart
+            if not n:
+                continue
+            per = np.repeat(scales, 256)[:n].reshape(x.shape).astype(np.float64)
+            back, true = decode_codes(codes).astype(np.float64) * per, x.astype(np.float64)
+            gap = per * np.maximum(2.0 ** -9, 2.0 ** (np.floor(np.log2(np.maximum(np.abs(true) / np.where(per > 0, per, 1), 2.0 ** -9))) - 3))
+            assert np.all(np.abs(back - true) <= gap * 1.001), shapes[i]
+            if root:
+                assert np.all((back > 0) == (true > 0))
+
+
+@pytest.mark.parametrize("d, masters", [(F32, False), (BF16, True), (F16, False)])
+@pytest.mark.parametrize("views", [False, True])
+def test_states_of_8_bits(hip, oracle, d, masters, views):
+    check8(hip, oracle, d, masters=masters, views=views, decay=0.1, factor=0.5)
+
+
+def test_a_small_change_moves_the_mean(hip):
+    """v falls by 0.1 % a step where gradients are zero; codes are 6 % apart. Their mean falls all the same."""
+    n = 1 << 18
+    codes = np.full(n, 100, np.uint8)  # 100: 2^5 1.5
+    codes[::256] = 126  # what the scale is made from
+    p, g = tensor(hip, np.zeros(n, np.float32), F32), tensor(hip, np.zeros(n, np.float32), F32)
+    scales = tensor(hip, np.full(n // 256, 1e-4, np.float32), F32)
+    m, v = tensor(hip, codes, E4M3), tensor(hip, codes, E4M3)
+    hip.adamw([p], [g], [m], [v], one(hip, 0.0, F32), one(hip, 5, I32), m_scales=[tensor(hip, np.full(n // 256, 1e-4, np.float32), F32)],
+              v_scales=[scales], key=tensor(hip, np.array([1, 2], np.int32), I32))
+    got = decode_codes(read(v)).reshape(-1, 256).astype(np.float64) * read(scales)[:, None]
+    rest = got[:, 1:]
+    want = 48e-4 * np.sqrt(0.999)
+    # the value lies between codes 44 and 48 of the shrunk scale, which falls as the value does: 48 again, off by the last bits
+    assert np.all(np.abs(rest - want) <= 4.001e-4) and abs(rest.mean() - want) <= 1e-6 * want + 5 * 2e-4 / np.sqrt(rest.size)
+
+
+def test_zeros_stay_and_roots_never_become_zero(hip):
+    n = 1024
+    g = np.zeros(n, np.float32)
+    g[0], g[1], g[300] = 1.0, 1e-7, 1e-30
+    codes = lambda: tensor(hip, np.zeros(n, np.uint8), E4M3)  # noqa: E731
+    scales = lambda: tensor(hip, np.zeros(4, np.float32), F32)  # noqa: E731
+    p, m, v, ms, vs = tensor(hip, np.zeros(n, np.float32), F32), codes(), codes(), scales(), scales()
+    hip.adamw([p], [tensor(hip, g, F32)], [m], [v], one(hip, 0.1, F32), one(hip, 1, I32), m_scales=[ms], v_scales=[vs],
+              key=tensor(hip, np.array([3, 4], np.int32), I32))
+    c = read(v)
+    assert c[0] == 126 and c[1] == 1 and np.all(c[2:300] == 0) and np.all(read(p)[2:300] == 0)
+    # (1e-30)^2 is no float32: its root is zero, as the value is
+    assert c[300] == 0 and np.isfinite(read(p)).all() and np.all(read(vs)[2:] == 0)
+
+
+def test_gradients_that_are_no_numbers(hip):
+    n = 600
+    g = np.full(n, 1e-3, np.float32)
+    g[5] = np.nan
+    for bits in (32, 8):
+        p = tensor(hip, np.ones(n, np.float32), F32)
+        if bits == 32:
+            m, v, kw = tensor(hip, np.zeros(n, np.float32), F32), tensor(hip, np.zeros(n, np.float32), F32), {}
+        else:
+            m, v = tensor(hip, np.zeros(n, np.uint8), E4M3), tensor(hip, np.zeros(n, np.uint8), E4M3)
+            kw = {"m_scales": [tensor(hip, np.zeros(3, np.float32), F32)], "v_scales": [tensor(hip, np.zeros(3, np.float32), F32)],
+                  "key": tensor(hip, np.array([3, 4], np.int32), I32)}
+        for _ in range(2):
+            hip.adamw([p], [tensor(hip, g, F32)], [m], [v], one(hip, 0.1, F32), one(hip, 1, I32), **kw)
+        bad = ~np.isfinite(read(p))
+        assert bad[5] and bad.sum() == 1
+
+
+# ── calls ───────────────────────────────────────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_recorded_steps_go_on_counting(hip, oracle, bits):
+    a, b = (Model(hip, oracle, BF16, SHAPES, True, bits, seed=9) for _ in range(2))
+    rate, step = one(hip, 1e-2, F32), one(hip, 1, I32)
+
+    def call(model):
+        hip.adamw(model.p, model.grads, model.m, model.v, rate, step, masters=model.masters, m_scales=model.ms, v_scales=model.vs, key=model.key, decay=0.1)
+
+    call(a)
+    call(b)
+    hip.capture_begin()
+    call(a)
+    graph = hip.capture_end()
+    for t in range(2, 6):
+        hip.assign(step, one(hip, t, I32))
+        hip.assign(rate, one(hip, 1e-2 / t, F32))
+        if bits == 8:
+            for model in (a, b):
+                hip.assign(model.key, tensor(hip, np.array([t, 7], np.int32), I32))
+        graph.launch()
+        call(b)
+        hip.synchronize()
+        for x, y in zip(a.p + a.m + a.v + a.masters + (a.ms or []), b.p + b.m + b.v + b.masters + (b.ms or [])):
+            same_bits(read(x), read(y), f"step {t}")
+    graph.destroy()
+
+
+def test_deferred_gradients(hip, oracle):
+    g = tensor(hip, np.random.default_rng(1).standard_normal(300).astype(np.float32), F32)
+    results = []
+    for deferred in (False, True):
+        p, m, v = (tensor(hip, np.zeros(300, np.float32), F32) for _ in range(3))
+        hip.set_deferred(deferred)
+        try:
+            hip.adamw([p], [hip.binary("add", g, g)], [m], [v], one(hip, 0.1, F32), one(hip, 1, I32))
+            results.append([read(t) for t in (p, m, v)])
+        finally:
+            hip.set_deferred(False)
+    for x, y in zip(*results):
+        same_bits(x, y)
+
+
+def test_nothing(hip):
+    hip.adamw([], [], [], [], one(hip, 0.1, F32), one(hip, 1, I32))
+    hip.adamw((), (), (), (), one(hip, 0.1, F32), one(hip, 1, I32), masters=None)
+
+
+def test_refusals(hip):
+    t = lambda *s, d=F32: hip.buffer(d, s)  # noqa: E731
+    r, s = one(hip, 0.1, F32), one(hip, 1, I32)
+    p = t(4, 5)
+    lists = lambda: ([p], [t(4, 5)], [t(4, 5)], [t(4, 5)])  # noqa: E731
+    hip.adamw(*lists(), r, s)
+    with pytest.raises(ValueError, match="lengths"):
+        hip.adamw([p], [], [], [], r, s)
+    with pytest.raises(ValueError, match="shape"):
+        hip.adamw([p], [t(4, 6)], [t(4, 5)], [t(4, 5)], r, s)
+    with pytest.raises(RuntimeError, match="dtype"):
+        hip.adamw([p], [t(4, 5, d=BF16)], [t(4, 5)], [t(4, 5)], r, s)
+    with pytest.raises(RuntimeError, match="dtype"):
+        hip.adamw([p, t(3, d=BF16)], [t(4, 5), t(3, d=BF16)], [t(4, 5), t(3)], [t(4, 5), t(3)], r, s)
+    with pytest.raises(RuntimeError, match="dtype"):
+        hip.adamw([t(3, d=dt.float64)], [t(3, d=dt.float64)], [t(3)], [t(3)], r, s)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        hip.adamw([p], [hip.permute(t(5, 4), (1, 0))], [t(4, 5)], [t(4, 5)], r, s)
+    with pytest.raises(ValueError, match="twice"):
+        hip.adamw([p, p], [t(4, 5)] * 2, [t(4, 5), t(4, 5)], [t(4, 5), t(4, 5)], r, s)
+    x = t(4, 5)
+    with pytest.raises(ValueError, match="twice"):
+        hip.adamw([p], [t(4, 5)], [x], [x], r, s)
+    with pytest.raises(ValueError, match="masters"):
+        hip.adamw(*lists(), r, s, masters=[t(4, 5)])
+    with pytest.raises(ValueError, match="float32"):
+        hip.adamw(*lists(), t(2), s)
+    with pytest.raises(ValueError, match="int32"):
+        hip.adamw(*lists(), r, r)
+    for kw in ({"beta1": 1.0}, {"beta2": -0.1}, {"eps": -1.0}, {"decay": float("nan")}):
+        with pytest.raises(ValueError):
+            hip.adamw(*lists(), r, s, **kw)
+    key = t(2, d=I32)
+    eight = ([p], [t(4, 5)], [t(4, 5, d=E4M3)], [t(4, 5, d=E4M3)], r, s)
+    hip.adamw(*eight, m_scales=[t(1)], v_scales=[t(1)], key=key)
+    with pytest.raises(ValueError, match="null"):
+        hip.adamw(*eight, m_scales=[t(1)], v_scales=[t(1)])
+    with pytest.raises(ValueError, match="null"):
+        hip.adamw(*eight, m_scales=[t(1)], key=key)
+    with pytest.raises(ValueError, match="shape"):
+        hip.adamw(*eight, m_scales=[t(2)], v_scales=[t(1)], key=key)
+    with pytest.raises(ValueError, match="key"):
+        hip.adamw(*eight, m_scales=[t(1)], v_scales=[t(1)], key=t(3, d=I32))
+    with pytest.raises(RuntimeError, match="dtype"):
+        hip.adamw(*lists(), r, s, m_scales=[t(1)], v_scales=[t(1)], key=key)
+    with pytest.raises(TypeError):
+        hip.adamw(5, [], [], [], r, s)
