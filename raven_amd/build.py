@@ -38,6 +38,7 @@ FLAGS = [
 PER_SOURCE_FLAGS = {
     "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attention_train.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],  # (the same rescale)
+    "attention_grad.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],  # (scores and their gradients are worked on between two products)
 }
 
 

@@ -32,7 +32,7 @@ __device__ __forceinline__ float exponent_of(float lse) {
 template <class EL, int DP>
 __global__ __launch_bounds__(256) void attention_grad_queries_kernel(AttentionArgs a) {
   using S = typename EL::S;
-  constexpr int KEYS = EL::F32 ? 32 : 64, QUERIES = 128, OT = DP / 32;
+  constexpr int KEYS = EL::F32 || DP > 64 ? 32 : 64, QUERIES = 128, OT = DP / 32;
   using T = Tile<EL, DP, KEYS>;
   constexpr int STAGE = 2 * T::SIZE;
   __shared__ __attribute__((aligned(16))) S stages[2 * STAGE];
@@ -54,8 +54,8 @@ __global__ __launch_bounds__(256) void attention_grad_queries_kernel(AttentionAr
   kt.begin(a.k.row);
   vt.begin(a.v.row);
   auto fetch = [&](int t) {
-    kt.fetch(K, a.k.row, t * KEYS, keys, a.dim);
-    vt.fetch(V, a.v.row, t * KEYS, keys, a.dim);
+    kt.fetch(K + (int64_t)t * KEYS * a.k.row, keys - t * KEYS, a.dim);
+    vt.fetch(V + (int64_t)t * KEYS * a.v.row, keys - t * KEYS, a.dim);
   };
   auto lay = [&](int t) {
     kt.lay(stages + (t & 1) * STAGE);
@@ -89,25 +89,45 @@ __global__ __launch_bounds__(256) void attention_grad_queries_kernel(AttentionAr
       if (t + 2 < steps) fetch(t + 2);
     }
     const S *stage = stages + (t & 1) * STAGE;
-#pragma unroll
-    for (int sub = 0; sub < KEYS / 32; sub++) {
-      const int r0 = sub * 32, j0 = t * KEYS + r0;
-      if (j0 >= keys || (a.causal && j0 > q0 + 31 + a.shift)) continue;  // nothing of it is seen
-      f32x16 p, ds;
+    auto products = [&](int r0, f32x16 &p, f32x16 &ds) {
 #pragma unroll
       for (int e = 0; e < 16; e++) p[e] = 0.0f, ds[e] = -delta;
       rows_by_columns<EL, DP, T::PITCH>(p, stage + r0 * T::PITCH, q);
       rows_by_columns<EL, DP, T::PITCH>(ds, stage + T::SIZE + r0 * T::PITCH, g);
+    };
+    auto differences = [&](const f32x16 &p, f32x16 &ds) {
 #pragma unroll
       for (int e = 0; e < 16; e++) ds[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[e], a.c2, power)) * ds[e];
+    };
+    auto add = [&](int r0, const f32x16 &ds) {
+      Weights<EL> w;
+      w.set(ds);
+      add_weighted_rows<EL, DP, T::PITCH>(dq, stage + r0 * T::PITCH, w);
+    };
+    if (KEYS == 64 && !mask && (t + 1) * KEYS <= keys && !(a.causal && (t + 1) * KEYS - 1 > q0 + a.shift)) {
+      // All of it is seen: both halves' products first, so that one's exponentials run beside the other's matrix instructions.
+      f32x16 p0, ds0, p1, ds1;
+      products(0, p0, ds0);
+      products(32, p1, ds1);
+      differences(p0, ds0);
+      add(0, ds0);
+      differences(p1, ds1);
+      add(32, ds1);
+      continue;
+    }
+#pragma unroll 1
+    for (int r0 = 0; r0 < KEYS; r0 += 32) {
+      const int j0 = t * KEYS + r0;
+      if (j0 >= keys || (a.causal && j0 > q0 + 31 + a.shift)) break;  // nothing from there on is seen
+      f32x16 p, ds;
+      products(r0, p, ds);
+      differences(p, ds);
       if (mask || j0 + 32 > keys || (a.causal && j0 + 31 > q0 + a.shift)) {
         const uint32_t see = keys_seen(a, mask, qi, j0, keys);
 #pragma unroll
         for (int e = 0; e < 16; e++) ds[e] = (see >> e) & 1 ? ds[e] : 0.0f;
       }
-      Weights<EL> w;
-      w.set(ds);
-      add_weighted_rows<EL, DP, T::PITCH>(dq, stage + r0 * T::PITCH, w);
+      add(r0, ds);
     }
   }
   if (there) store_column<EL, DP>(const_cast<S *>(rows_of<EL>(a.dq, b, h)) + (int64_t)qi * a.dq.row, dq, a.scale * UNLIFT<EL>, a.dim);
@@ -130,140 +150,311 @@ __device__ __forceinline__ uint32_t queries_seeing(const AttentionArgs &a, const
   return seeing & kept;
 }
 
-// Blocks of four waves with 32 keys each. What a block walks over, the query tiles of all heads that share its keys, is cut into
-// a.parts, a block each, where there would be few blocks; their sums are joined by another launch.
+// Where a block of the second launch is: its keys, and its part of what they are seen by, the query tiles of all heads that share
+// them, one head after the other.
+template <class EL, int QUERIES>
+struct KeysWalk {
+  int b, hk, keys, first;  // batch, head, the sequence's keys, the block's first
+  int part, steps;
+  int tiles, before;  // a head's query tiles, and how many of them see none of the block's keys
+  int at, head;       // tile and head of a step
+  __device__ __forceinline__ KeysWalk(const AttentionArgs &a) {
+    const uint32_t heads = (uint32_t)a.batch * (uint32_t)a.kv_heads, rest = blockIdx.x / heads;
+    const int bh = (int)(blockIdx.x % heads), group = a.heads / a.kv_heads;
+    b = bh / a.kv_heads;
+    hk = bh % a.kv_heads;
+    keys = keys_of(a, b);
+    first = (int)(rest / (uint32_t)a.parts) * 128;  // the first keys first: under a causal mask most queries see them
+    part = (int)(rest % (uint32_t)a.parts);
+    tiles = (a.sq + QUERIES - 1) / QUERIES;
+    before = a.causal ? min(tiles, max(0, first - a.shift) / QUERIES) : 0;
+    const int64_t all = first < keys ? (int64_t)group * (tiles - before) : 0;
+    const int64_t from = all * part / a.parts, to = all * (part + 1) / a.parts;
+    steps = (int)(to - from);
+    at = before, head = hk * group;
+    if (steps > 0) {
+      at += (int)(from % (tiles - before));
+      head += (int)(from / (tiles - before));
+    }
+  }
+  // Whether the next step is in another head.
+  __device__ __forceinline__ bool next() {
+    if (++at < tiles) return false;
+    at = before;
+    head++;
+    return true;
+  }
+};
+
+// What a thread brings of each step: rows of an operand, and in the first threads a row's lse and delta.
+template <class EL, int QUERIES, class T>
+struct KeysFetch {
+  const typename EL::S *rows;
+  const float *lse, *delta;
+  float power, less;
+  __device__ __forceinline__ void begin(const AttentionArgs &a, const HeadOperand &o, const KeysWalk<EL, QUERIES> &w) {
+    const int64_t i = (int64_t)w.at * QUERIES;
+    rows = rows_of<EL>(o, w.b, w.head) + i * o.row;
+    lse = reinterpret_cast<const float *>(a.lse.base) + (int64_t)w.b * a.lse.batch + (int64_t)w.head * a.lse.head + (i + threadIdx.x) * a.lse.row;
+    delta = a.delta + ((int64_t)w.b * a.heads + w.head) * a.sq + i + threadIdx.x;
+  }
+  __device__ __forceinline__ void fetch(const AttentionArgs &a, const HeadOperand &o, KeysWalk<EL, QUERIES> &w, T &tile) {
+    const int left = a.sq - w.at * QUERIES;
+    tile.fetch(rows, left, a.dim);
+    values(left);
+    if (w.next()) {
+      begin(a, o, w);
+    } else {
+      rows += (int64_t)QUERIES * o.row;
+      lse += (int64_t)QUERIES * a.lse.row;
+      delta += QUERIES;
+    }
+  }
+  __device__ __forceinline__ void values(int left) {
+    if (threadIdx.x < QUERIES) {
+      power = -INF, less = 0.0f;
+      if ((int)threadIdx.x < left) power = *lse, less = -*delta;
+    }
+  }
+  __device__ __forceinline__ void lay(float *powers, float *deltas) const {
+    if (threadIdx.x < QUERIES) {
+      powers[threadIdx.x] = exponent_of<EL>(power);
+      deltas[threadIdx.x] = less;
+    }
+  }
+};
+
+__device__ __forceinline__ void row_values(const float *values, f32x16 &x) {
+  const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int e = 0; e < 16; e += 4) {
+    const gemm_tile::f32x4 v = *reinterpret_cast<const gemm_tile::f32x4 *>(values + e * 2 + half * 4);
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[e + j] = v[j];
+  }
+}
+
+// A column's sums: a key's dk or dv.
+template <class EL, int DP, class W>
+__device__ __forceinline__ void store_key(const AttentionArgs &a, const W &w, int kj, bool is_k, f32x16 (&acc)[DP / 32]) {
+  if (kj >= w.keys) {  // a key that its sequence does not have saw zeros in its place: its gradients are zeros
+#pragma unroll
+    for (int t = 0; t < DP / 32; t++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) acc[t][e] = 0.0f;
+  }
+  const float factor = is_k ? a.scale * UNLIFT<EL> : UNLIFT<EL>;
+  if (a.partial) {
+    float *to = a.partial + ((((int64_t)w.part * a.batch + w.b) * a.kv_heads + w.hk) * a.sk + kj) * 2 * a.dim;
+    store_column<gemm_tile::ElF32, DP>(is_k ? to : to + a.dim, acc, factor, a.dim);
+  } else {
+    const HeadOperand &o = is_k ? a.dk : a.dv;
+    store_column<EL, DP>(const_cast<typename EL::S *>(rows_of<EL>(o, w.b, w.hk)) + (int64_t)kj * o.row, acc, factor, a.dim);
+  }
+}
+
+// Blocks of four waves with 32 keys each, for heads of up to 64. What a block walks over is cut into a.parts, a block each, where
+// there would be few blocks; their sums are joined by another launch.
 template <class EL, int DP>
 __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs a) {
   using S = typename EL::S;
-  constexpr int QUERIES = EL::F32 || DP > 96 ? 32 : 64, KEYS = 128, OT = DP / 32;
+  constexpr int QUERIES = EL::F32 ? 32 : 64, OT = DP / 32;
   using T = Tile<EL, DP, QUERIES>;
   constexpr int STAGE = 2 * T::SIZE;
   __shared__ __attribute__((aligned(16))) S stages[2 * STAGE];
   __shared__ __attribute__((aligned(16))) float powers[2][QUERIES], deltas[2][QUERIES];
 
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, half = lane >> 5;
-  const uint32_t heads = (uint32_t)a.batch * (uint32_t)a.kv_heads;
-  const uint32_t rest = blockIdx.x / heads;
-  const int tile = (int)(rest / (uint32_t)a.parts), part = (int)(rest % (uint32_t)a.parts);  // the first keys first: under a causal mask most see them
-  const int bh = (int)(blockIdx.x % heads), b = bh / a.kv_heads, hk = bh % a.kv_heads, group = a.heads / a.kv_heads;
-  const int keys = keys_of(a, b);
-  const int k0 = tile * KEYS + wave * 32, kj = k0 + c32;
-  const bool there = kj < a.sk;
+  KeysWalk<EL, QUERIES> w(a);
+  const int k0 = w.first + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32, kj = k0 + (threadIdx.x & 31);
   Column<EL, DP> k, v;
-  k.load(rows_of<EL>(a.k, b, hk) + (int64_t)kj * a.k.row, kj < keys, a.dim);
-  v.load(rows_of<EL>(a.v, b, hk) + (int64_t)kj * a.v.row, kj < keys, a.dim);
-
-  const int tiles = (a.sq + QUERIES - 1) / QUERIES;
-  const int before = a.causal ? min(tiles, max(0, tile * KEYS - a.shift) / QUERIES) : 0;  // tiles whose queries see none of the block's keys
-  const int64_t all = tile * KEYS < keys ? (int64_t)group * (tiles - before) : 0;
-  const int64_t from = all * part / a.parts, to = all * (part + 1) / a.parts;
-  const int steps = (int)(to - from);
-  // where the walk is: query tile and head of the step that is fetched next
-  int at = steps > 0 ? before + (int)(from % (tiles - before)) : 0, head = hk * group + (steps > 0 ? (int)(from / (tiles - before)) : 0);
-
+  k.load(rows_of<EL>(a.k, w.b, w.hk) + (int64_t)kj * a.k.row, kj < w.keys, a.dim);
+  v.load(rows_of<EL>(a.v, w.b, w.hk) + (int64_t)kj * a.v.row, kj < w.keys, a.dim);
   T qt, gt;
   qt.begin(a.q.row);
   gt.begin(a.g.row);
-  float power = -INF, delta = 0.0f;
-  int i0_now = 0, head_now = 0, i0_next = 0, head_next = 0;  // of the tile that is worked on, and of the one that was fetched last
-  auto fetch = [&]() {
-    const int i0 = at * QUERIES;
-    qt.fetch(rows_of<EL>(a.q, b, head), a.q.row, i0, a.sq, a.dim);
-    gt.fetch(rows_of<EL>(a.g, b, head), a.g.row, i0, a.sq, a.dim);
-    if (threadIdx.x < QUERIES) {
-      const int i = i0 + threadIdx.x;
-      power = -INF, delta = 0.0f;
-      if (i < a.sq) {
-        power = reinterpret_cast<const float *>(a.lse.base)[(int64_t)b * a.lse.batch + (int64_t)head * a.lse.head + (int64_t)i * a.lse.row];
-        delta = a.delta[((int64_t)b * a.heads + head) * a.sq + i];
-      }
-    }
-    i0_next = i0, head_next = head;
-    if (++at == tiles) at = before, head++;
+  KeysFetch<EL, QUERIES, T> from;
+  const S *g_rows;
+  int at = w.at, head = w.head;  // of the step that is worked on
+  auto begin = [&]() {
+    from.begin(a, a.q, w);
+    g_rows = rows_of<EL>(a.g, w.b, w.head) + (int64_t)w.at * QUERIES * a.g.row;
   };
-  auto lay = [&](int t) {
-    qt.lay(stages + (t & 1) * STAGE);
-    gt.lay(stages + (t & 1) * STAGE + T::SIZE);
-    if (threadIdx.x < QUERIES) {
-      powers[t & 1][threadIdx.x] = exponent_of<EL>(power);
-      deltas[t & 1][threadIdx.x] = -delta;
-    }
+  auto fetch = [&]() {
+    gt.fetch(g_rows, a.sq - w.at * QUERIES, a.dim);
+    const int h = w.head;
+    from.fetch(a, a.q, w, qt);
+    g_rows = w.head == h ? g_rows + (int64_t)QUERIES * a.g.row : rows_of<EL>(a.g, w.b, w.head) + (int64_t)w.at * QUERIES * a.g.row;
+  };
+  auto lay = [&](int s) {
+    qt.lay(stages + s * STAGE);
+    gt.lay(stages + s * STAGE + T::SIZE);
+    from.lay(powers[s], deltas[s]);
   };
   f32x16 dk[OT], dv[OT];
 #pragma unroll
   for (int t = 0; t < OT; t++)
 #pragma unroll
     for (int e = 0; e < 16; e++) dk[t][e] = dv[t][e] = 0.0f;
-  if (steps > 0) {
+  if (w.steps > 0) {
+    begin();
     fetch();
-    i0_now = i0_next, head_now = head_next;
     lay(0);
-    if (steps > 1) fetch();
+    if (w.steps > 1) fetch();
   }
-  for (int t = 0; t < steps; t++) {
+  for (int t = 0; t < w.steps; t++) {
     __syncthreads();  // this tile is there, and the one before has been used
-    const int i0_t = i0_now, head_t = head_now;
-    if (t + 1 < steps) {
-      lay(t + 1);
-      i0_now = i0_next, head_now = head_next;
-      if (t + 2 < steps) fetch();
+    if (t + 1 < w.steps) {
+      lay((t + 1) & 1);
+      if (t + 2 < w.steps) fetch();
     }
     const S *stage = stages + (t & 1) * STAGE;
-    const uint8_t *mask = a.mask.base ? reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)b * a.mask.batch + (int64_t)head_t * a.mask.head : nullptr;
+    const float *power = powers[t & 1], *delta = deltas[t & 1];
+    const int i0 = at * QUERIES;
+    auto products = [&](int r0, f32x16 &p, f32x16 &ds) {
 #pragma unroll
-    for (int sub = 0; sub < QUERIES / 32; sub++) {
-      const int r0 = sub * 32, i0 = i0_t + r0;
-      if (i0 >= a.sq || k0 >= keys || (a.causal && k0 > i0 + 31 + a.shift)) continue;  // nothing of it sees these keys
-      f32x16 p, ds;
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const gemm_tile::f32x4 d = *reinterpret_cast<const gemm_tile::f32x4 *>(&deltas[t & 1][r0 + e * 2 + half * 4]);
-#pragma unroll
-        for (int j = 0; j < 4; j++) p[e + j] = 0.0f, ds[e + j] = d[j];
-      }
+      for (int e = 0; e < 16; e++) p[e] = 0.0f;
+      row_values(delta + r0, ds);
       rows_by_columns<EL, DP, T::PITCH>(p, stage + r0 * T::PITCH, k);
       rows_by_columns<EL, DP, T::PITCH>(ds, stage + T::SIZE + r0 * T::PITCH, v);
+    };
+    auto differences = [&](int r0, f32x16 &p, f32x16 &ds) {
+      f32x16 l;
+      row_values(power + r0, l);
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const gemm_tile::f32x4 w = *reinterpret_cast<const gemm_tile::f32x4 *>(&powers[t & 1][r0 + e * 2 + half * 4]);
-#pragma unroll
-        for (int j = 0; j < 4; j++) p[e + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[e + j], a.c2, w[j]));
+      for (int e = 0; e < 16; e++) {
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[e], a.c2, l[e]));
+        ds[e] = p[e] * ds[e];
       }
+      if (!a.mask.base && !(a.causal && k0 + 31 > i0 + r0 + a.shift)) return;
+      const uint8_t *mask = a.mask.base ? reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)w.b * a.mask.batch + (int64_t)head * a.mask.head : nullptr;
+      const uint32_t seeing = queries_seeing(a, mask, kj, i0 + r0);
 #pragma unroll
-      for (int e = 0; e < 16; e++) ds[e] = p[e] * ds[e];
-      if (mask || (a.causal && k0 + 31 > i0 + a.shift)) {
-        const uint32_t seeing = queries_seeing(a, mask, kj, i0);
+      for (int e = 0; e < 16; e++) {
+        const bool keep = (seeing >> e) & 1;
+        p[e] = keep ? p[e] : 0.0f;
+        ds[e] = keep ? ds[e] : 0.0f;
+      }
+    };
+    auto add = [&](int r0, const Weights<EL> &p, const Weights<EL> &ds) {
+      add_weighted_rows<EL, DP, T::PITCH>(dv, stage + T::SIZE + r0 * T::PITCH, p);
+      add_weighted_rows<EL, DP, T::PITCH>(dk, stage + r0 * T::PITCH, ds);
+    };
+    if (k0 < w.keys && !(a.causal && k0 > i0 + QUERIES - 1 + a.shift)) {  // (else nothing of the tile sees these keys)
+      f32x16 p, ds;
+      Weights<EL> pw, dsw;
+      products(0, p, ds);
+      differences(0, p, ds);
+      pw.set(p);
+      dsw.set(ds);
+      if constexpr (QUERIES == 64) {  // the second half's scores are on their way while the first half's sums are added to
+        products(32, p, ds);
+        add(0, pw, dsw);
+        differences(32, p, ds);
+        pw.set(p);
+        dsw.set(ds);
+      }
+      add(QUERIES - 32, pw, dsw);
+    }
+    if (++at == w.tiles) at = w.before, head++;
+  }
+  if (kj >= a.sk) return;
+  store_key<EL, DP>(a, w, kj, true, dk);
+  store_key<EL, DP>(a, w, kj, false, dv);
+}
+
+// The same for heads of more than 64. Blocks of eight waves, of which two have the same 32 keys: one makes the scores, p and dv,
+// the other g . v, ds and dk, one tile of queries behind the first, whose p it takes from LDS. So a wave holds the vectors and the
+// sums of one operand, not of two, which for heads of 128 are more registers than two waves of a unit's may have.
+template <class EL, int DP>
+__global__ __launch_bounds__(512) void attention_grad_wide_keys_kernel(AttentionArgs a) {
+  using S = typename EL::S;
+  constexpr int QUERIES = 32, OT = DP / 32;
+  using T = Tile<EL, DP, QUERIES>;  // (each half of the threads brings one operand's)
+  constexpr int STAGE = 2 * T::SIZE;
+  __shared__ __attribute__((aligned(16))) S stages[3 * STAGE];
+  __shared__ __attribute__((aligned(16))) float powers[3][QUERIES], deltas[3][QUERIES];
+  __shared__ __attribute__((aligned(16))) float over[2][4][4][64][4];  // p, for the other wave: [tile][pair][e / 4][lane][e % 4]
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = wave & 3;
+  const bool second = wave >= 4;  // dk
+  KeysWalk<EL, QUERIES> w(a);
+  const int k0 = w.first + pair * 32, kj = k0 + (lane & 31);
+  const HeadOperand &mine = second ? a.v : a.k, &brought = second ? a.g : a.q;
+  Column<EL, DP> own;
+  own.load(rows_of<EL>(mine, w.b, w.hk) + (int64_t)kj * mine.row, kj < w.keys, a.dim);
+  T tile;
+  tile.begin(brought.row);
+  KeysFetch<EL, QUERIES, T> from;
+  int at = w.at, head = w.head;  // of the step that this wave works on
+  auto lay = [&](int s) {
+    tile.lay(stages + s * STAGE + (second ? T::SIZE : 0));
+    from.lay(powers[s], deltas[s]);
+  };
+  f32x16 acc[OT];  // of dv, in the second wave of dk
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const bool keep = (seeing >> e) & 1;
-          p[e] = keep ? p[e] : 0.0f;
-          ds[e] = keep ? ds[e] : 0.0f;
+  for (int t = 0; t < OT; t++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) acc[t][e] = 0.0f;
+  if (w.steps > 0) {
+    from.begin(a, brought, w);
+    from.fetch(a, brought, w, tile);
+    lay(0);
+    if (w.steps > 1) from.fetch(a, brought, w, tile);
+  }
+  int now = 0, next = 1;  // the stages of what this wave works on, and of what is laid
+  for (int t = 0; w.steps > 0 && t <= w.steps; t++) {
+    __syncthreads();  // tile t is there, p of the tile before too, and what is laid now is no longer used
+    if (t + 1 < w.steps) {
+      lay(next);
+      if (t + 2 < w.steps) from.fetch(a, brought, w, tile);
+    }
+    next = next == 2 ? 0 : next + 1;
+    if (second ? t == 0 : t == w.steps) continue;
+    const S *rows = stages + now * STAGE;
+    const int i0 = at * QUERIES;
+    float(*between)[64][4] = over[(second ? t - 1 : t) & 1][pair];
+    if (k0 < w.keys && !(a.causal && k0 > i0 + 31 + a.shift)) {  // (else nothing of the tile sees these keys)
+      const bool inner = !a.mask.base && !(a.causal && k0 + 31 > i0 + a.shift);
+      f32x16 x;
+      if (second) {
+        row_values(deltas[now], x);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[e] = 0.0f;
+      }
+      rows_by_columns<EL, DP, T::PITCH>(x, rows + (second ? T::SIZE : 0), own);
+      if (!second) {
+        f32x16 l;
+        row_values(powers[now], l);
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.c2, l[e]));
+        if (!inner) {
+          const uint8_t *mask = a.mask.base ? reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)w.b * a.mask.batch + (int64_t)head * a.mask.head : nullptr;
+          const uint32_t seeing = queries_seeing(a, mask, kj, i0);
+#pragma unroll
+          for (int e = 0; e < 16; e++) x[e] = (seeing >> e) & 1 ? x[e] : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) *reinterpret_cast<gemm_tile::f32x4 *>(between[e >> 2][lane]) = gemm_tile::f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const gemm_tile::f32x4 p = *reinterpret_cast<const gemm_tile::f32x4 *>(between[e >> 2][lane]);
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float ds = p[j] * x[e + j];
+            x[e + j] = inner || p[j] != 0.0f ? ds : 0.0f;  // (what a query does not see may be no number)
+          }
         }
       }
-      Weights<EL> w;
-      w.set(p);
-      add_weighted_rows<EL, DP, T::PITCH>(dv, stage + T::SIZE + r0 * T::PITCH, w);
-      w.set(ds);
-      add_weighted_rows<EL, DP, T::PITCH>(dk, stage + r0 * T::PITCH, w);
+      Weights<EL> y;
+      y.set(x);
+      add_weighted_rows<EL, DP, T::PITCH>(acc, rows + (second ? 0 : T::SIZE), y);
     }
+    now = now == 2 ? 0 : now + 1;
+    if (++at == w.tiles) at = w.before, head++;
   }
-  if (!there) return;
-  // a key that its sequence does not have saw zeros in its place: its gradients are zeros
-  const float one = kj < keys ? UNLIFT<EL> : 0.0f;
-  if (kj >= keys) {
-#pragma unroll
-    for (int t = 0; t < OT; t++)
-#pragma unroll
-      for (int e = 0; e < 16; e++) dk[t][e] = dv[t][e] = 0.0f;
-  }
-  if (a.partial) {
-    float *to_k = a.partial + ((((int64_t)part * a.batch + b) * a.kv_heads + hk) * a.sk + kj) * 2 * a.dim;
-    store_column<gemm_tile::ElF32, DP>(to_k, dk, a.scale * one, a.dim);
-    store_column<gemm_tile::ElF32, DP>(to_k + a.dim, dv, one, a.dim);
-  } else {
-    store_column<EL, DP>(const_cast<S *>(rows_of<EL>(a.dk, b, hk)) + (int64_t)kj * a.dk.row, dk, a.scale * one, a.dim);
-    store_column<EL, DP>(const_cast<S *>(rows_of<EL>(a.dv, b, hk)) + (int64_t)kj * a.dv.row, dv, one, a.dim);
-  }
+  if (kj < a.sk) store_key<EL, DP>(a, w, kj, second, acc);
 }
 
 // The parts' sums, in order.
@@ -292,7 +483,9 @@ void launch(nxh_context *ctx, AttentionArgs a) {
   }
   if (a.sk == 0) return;
   a.tiles = (a.sk + 127) / 128;
-  hipLaunchKernelGGL((attention_grad_keys_kernel<EL, DP>), dim3((unsigned)(a.batch * a.kv_heads * a.tiles * a.parts)), dim3(256), 0, ctx->stream, a);
+  const dim3 grid((unsigned)(a.batch * a.kv_heads * a.tiles * a.parts));
+  if constexpr (DP <= 64) hipLaunchKernelGGL((attention_grad_keys_kernel<EL, DP>), grid, dim3(256), 0, ctx->stream, a);
+  else hipLaunchKernelGGL((attention_grad_wide_keys_kernel<EL, DP>), grid, dim3(512), 0, ctx->stream, a);
   if (!a.partial) return;
   const int64_t size = (int64_t)a.batch * a.kv_heads * a.sk * 2 * a.dim;
   hipLaunchKernelGGL((attention_grad_join_kernel<EL>), dim3((unsigned)std::min<int64_t>((size + 255) / 256, 1 << 16)), dim3(256), 0, ctx->stream, a);
@@ -328,10 +521,10 @@ NXH_EXPORT int nxh_attention_grad(nxh_context *ctx, const nxh_tensor *dq, const 
     for (const nxh_tensor *i : inputs)
       if (same_start(r, i)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "a gradient must not replace an input");
   // A block has 128 keys of a head and walks over all queries that see them: cut into parts where that leaves units
-  // without work, down to parts of two tiles.
+  // without work, down to parts of four tiles.
   const int units = ctx->compute_units > 0 ? ctx->compute_units : 256;
-  const int64_t blocks = (int64_t)a.batch * a.kv_heads * ((a.sk + 127) / 128), walk = (int64_t)(a.heads / a.kv_heads) * ((a.sq + 63) / 64);
-  a.parts = blocks > 0 && walk > 0 ? (int)std::max<int64_t>(1, std::min<int64_t>({16, 2 * units / blocks, walk / 2})) : 1;
+  const int64_t blocks = (int64_t)a.batch * a.kv_heads * ((a.sk + 127) / 128), walk = (int64_t)(a.heads / a.kv_heads) * ((a.sq + 31) / 32);
+  a.parts = blocks > 0 && walk > 0 ? (int)std::max<int64_t>(1, std::min<int64_t>({16, 2 * units / blocks, walk / 4})) : 1;
   if ((double)blocks * a.parts > 2147483647.0) return nxh_fail(NXH_FAILURE, op, "too many rows for one launch");
   std::lock_guard<std::mutex> guard(ctx->mu);
   NXH_HIP(op, hipSetDevice(ctx->device));

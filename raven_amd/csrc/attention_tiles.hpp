@@ -101,42 +101,47 @@ __device__ __forceinline__ V16 load_part(const typename EL::S *p, int left) {
   return w;
 }
 
-// A tile of ROWS rows of DP elements (the head's, and zeros) in LDS, brought by 256 threads through registers. Rows are 16 bytes
-// further apart than they are long: eight rows' vectors at one place, and the four rows of a transposing load, lie in different banks.
+// A tile of ROWS rows of DP elements (the head's, and zeros) in LDS, brought by 256 threads (as many of them as divide its
+// vectors) through registers. Rows are 16 bytes (128 elements of 16 bits: 48) further apart than they are long: sixteen rows'
+// vectors at one place lie in different banks, and of the four rows of a transposing load no more than two in one.
 template <class EL, int DP, int ROWS>
 struct Tile {
   using S = typename EL::S;
-  static constexpr int PITCH = DP + EL::VE, SIZE = ROWS * PITCH, VPR = DP / EL::VE, NV = ROWS * VPR / 256;
-  static_assert(NV * 256 == ROWS * VPR, "whole vectors a thread");
+  static constexpr int PITCH = DP + EL::VE * (!EL::F32 && DP == 128 ? 3 : 1), SIZE = ROWS * PITCH, VPR = DP / EL::VE, ALL = ROWS * VPR;
+  static constexpr int THREADS = ALL % 256 == 0 ? 256 : ALL % 192 == 0 ? 192 : ALL, NV = ALL / THREADS;
+  static_assert(THREADS <= 256 && NV * THREADS == ALL, "whole vectors a thread");
   V16 pre[NV];
   uint32_t off[NV];  // bytes from the tile's first row
 
+  __device__ __forceinline__ static bool brings() { return THREADS == 256 || (threadIdx.x & 255) < THREADS; }
   __device__ __forceinline__ void begin(int64_t row) {
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const int v = threadIdx.x + i * 256;
+      const int v = (int)(threadIdx.x & 255) + i * THREADS;
       off[i] = ((uint32_t)(v / VPR) * (uint32_t)row + (uint32_t)(v % VPR) * EL::VE) * (uint32_t)sizeof(S);
     }
   }
-  // Rows from `first` on; `limit` rows exist.
-  __device__ __forceinline__ void fetch(const S *rows, int64_t row, int first, int limit, int dim) {
-    const char *at = reinterpret_cast<const char *>(rows + (int64_t)first * row);
-    if (first + ROWS <= limit && dim == DP) {
+  // The rows from `first` on, of which `left` exist.
+  __device__ __forceinline__ void fetch(const S *first, int left, int dim) {
+    if (!brings()) return;
+    const char *at = reinterpret_cast<const char *>(first);
+    if (left >= ROWS && dim == DP) {
 #pragma unroll
       for (int i = 0; i < NV; i++) __builtin_memcpy(&pre[i], at + off[i], 16);
       return;
     }
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const int v = threadIdx.x + i * 256, c = (v % VPR) * EL::VE;
+      const int v = (int)(threadIdx.x & 255) + i * THREADS, c = (v % VPR) * EL::VE;
       pre[i] = V16{0, 0, 0, 0};
-      if (first + v / VPR < limit && c < dim) pre[i] = load_part<EL>(reinterpret_cast<const S *>(at + off[i]), dim - c);
+      if (v / VPR < left && c < dim) pre[i] = load_part<EL>(reinterpret_cast<const S *>(at + off[i]), dim - c);
     }
   }
   __device__ __forceinline__ void lay(S *tile) const {
+    if (!brings()) return;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const int v = threadIdx.x + i * 256;
+      const int v = (int)(threadIdx.x & 255) + i * THREADS;
       *reinterpret_cast<V16 *>(tile + (v / VPR) * PITCH + (v % VPR) * EL::VE) = pre[i];
     }
   }

@@ -42,8 +42,8 @@ __global__ __launch_bounds__(256) void attention_train_kernel(AttentionArgs a) {
   kt.begin(a.k.row);
   vt.begin(a.v.row);
   auto fetch = [&](int t) {
-    kt.fetch(K, a.k.row, t * KEYS, keys, a.dim);
-    vt.fetch(V, a.v.row, t * KEYS, keys, a.dim);
+    kt.fetch(K + (int64_t)t * KEYS * a.k.row, keys - t * KEYS, a.dim);
+    vt.fetch(V + (int64_t)t * KEYS * a.v.row, keys - t * KEYS, a.dim);
   };
   auto lay = [&](int t) {
     kt.lay(stages + (t & 1) * STAGE);
