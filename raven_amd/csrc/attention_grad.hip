@@ -33,9 +33,9 @@ template <class EL, int DP>
 __global__ __launch_bounds__(256) void attention_grad_queries_kernel(AttentionArgs a) {
   using S = typename EL::S;
   constexpr int KEYS = EL::F32 || DP > 64 ? 32 : 64, QUERIES = 128, OT = DP / 32;
-  using T = Tile<EL, DP, KEYS>;
-  constexpr int STAGE = 2 * T::SIZE;
-  __shared__ __attribute__((aligned(16))) S stages[2 * STAGE];
+  using T = Tile<EL, DP, KEYS, 4>;
+  constexpr int STAGE = 2 * T::SIZE, RING = 3;
+  __shared__ __attribute__((aligned(1024))) unsigned char stages[RING * STAGE];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31;
   const uint32_t heads = (uint32_t)a.batch * (uint32_t)a.heads;
@@ -50,22 +50,24 @@ __global__ __launch_bounds__(256) void attention_grad_queries_kernel(AttentionAr
   if (a.causal) seen = min(seen, max(0, min((tile + 1) * QUERIES, a.sq) + a.shift));
   const int steps = (seen + KEYS - 1) / KEYS;
 
+  const uint32_t lds = lds_address(stages);
   T kt, vt;
-  kt.begin(a.k.row);
-  vt.begin(a.v.row);
-  auto fetch = [&](int t) {
-    kt.fetch(K + (int64_t)t * KEYS * a.k.row, keys - t * KEYS, a.dim);
-    vt.fetch(V + (int64_t)t * KEYS * a.v.row, keys - t * KEYS, a.dim);
-  };
-  auto lay = [&](int t) {
-    kt.lay(stages + (t & 1) * STAGE);
-    vt.lay(stages + (t & 1) * STAGE + T::SIZE);
-  };
-  if (steps > 0) {
-    fetch(0);
-    lay(0);
-    if (steps > 1) fetch(1);
+  kt.begin(wave, a.k.row);
+  vt.begin(wave, a.v.row);
+  if (a.dim != DP) {
+    for (int s = 0; s < RING; s++) {
+      kt.clear(lds + s * STAGE, a.dim);
+      vt.clear(lds + s * STAGE + T::SIZE, a.dim);
+    }
+    __syncthreads();
   }
+  auto whole = [&](int t) { return (t + 1) * KEYS <= keys && a.k.direct && a.v.direct; };
+  auto fetch = [&](int t, uint32_t to) {
+    kt.fetch(K + (int64_t)t * KEYS * a.k.row, keys - t * KEYS, a.k, a.dim, to);
+    vt.fetch(V + (int64_t)t * KEYS * a.v.row, keys - t * KEYS, a.v, a.dim, to + T::SIZE);
+  };
+  if (steps > 0) fetch(0, lds);
+  if (steps > 1) fetch(1, lds + STAGE);
   Column<EL, DP> q, g;
   g.load(rows_of<EL>(a.g, b, h) + (int64_t)qi * a.g.row, there, a.dim);
   q.load(rows_of<EL>(a.out, b, h) + (int64_t)qi * a.out.row, there, a.dim);
@@ -73,62 +75,58 @@ __global__ __launch_bounds__(256) void attention_grad_queries_kernel(AttentionAr
   delta = delta + other_half(delta);
   q.load(rows_of<EL>(a.q, b, h) + (int64_t)qi * a.q.row, there, a.dim);
   float power = -INF;
-  if (there) {
-    power = exponent_of<EL>(reinterpret_cast<const float *>(a.lse.base)[(int64_t)b * a.lse.batch + (int64_t)h * a.lse.head + (int64_t)qi * a.lse.row]);
-    if (lane < 32) a.delta[(int64_t)bh * a.sq + qi] = delta;
+  if (there) power = exponent_of<EL>(reinterpret_cast<const float *>(a.lse.base)[(int64_t)b * a.lse.batch + (int64_t)h * a.lse.head + (int64_t)qi * a.lse.row]);
+  if (qi < a.rows_pitch) {  // for the second launch, 32 rows' powers and then their differences' starts; past the end -inf and 0
+    float *to = a.rows + ((int64_t)bh * a.rows_pitch + q0) * 2;
+    to[lane] = lane < 32 ? power : there ? -delta : 0.0f;
   }
   f32x16 dq[OT];
 #pragma unroll
   for (int t = 0; t < OT; t++)
 #pragma unroll
     for (int e = 0; e < 16; e++) dq[t][e] = 0.0f;
+  uint32_t stage = lds, ahead = lds + 2 * STAGE;
   for (int t = 0; t < steps; t++) {
-    __syncthreads();  // this tile is there, and the one before has been used
-    if (t + 1 < steps) {
-      lay(t + 1);
-      if (t + 2 < steps) fetch(t + 2);
-    }
-    const S *stage = stages + (t & 1) * STAGE;
+    // this tile has come, and the stage that is filled next has been used
+    if (t > 0 && t + 1 < steps && whole(t + 1)) meet<2 * T::LPW>();
+    else meet<0>();
+    if (t + 2 < steps) fetch(t + 2, ahead);
+    const uint32_t rows = stage;
+    stage = stage == lds + 2 * STAGE ? lds : stage + STAGE;
+    ahead = ahead == lds + 2 * STAGE ? lds : ahead + STAGE;
     auto products = [&](int r0, f32x16 &p, f32x16 &ds) {
 #pragma unroll
       for (int e = 0; e < 16; e++) p[e] = 0.0f, ds[e] = -delta;
-      rows_by_columns<EL, DP, T::PITCH>(p, stage + r0 * T::PITCH, q);
-      rows_by_columns<EL, DP, T::PITCH>(ds, stage + T::SIZE + r0 * T::PITCH, g);
+      two_scores<T>(p, q, ds, g, rows + r0 * T::ROW);
     };
-    auto differences = [&](const f32x16 &p, f32x16 &ds) {
+    auto differences = [&](int r0, const f32x16 &p, f32x16 &ds) {
 #pragma unroll
       for (int e = 0; e < 16; e++) ds[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[e], a.c2, power)) * ds[e];
-    };
-    auto add = [&](int r0, const f32x16 &ds) {
-      Weights<EL> w;
-      w.set(ds);
-      add_weighted_rows<EL, DP, T::PITCH>(dq, stage + r0 * T::PITCH, w);
-    };
-    if (KEYS == 64 && !mask && (t + 1) * KEYS <= keys && !(a.causal && (t + 1) * KEYS - 1 > q0 + a.shift)) {
-      // All of it is seen: both halves' products first, so that one's exponentials run beside the other's matrix instructions.
-      f32x16 p0, ds0, p1, ds1;
-      products(0, p0, ds0);
-      products(32, p1, ds1);
-      differences(p0, ds0);
-      add(0, ds0);
-      differences(p1, ds1);
-      add(32, ds1);
-      continue;
-    }
-#pragma unroll 1
-    for (int r0 = 0; r0 < KEYS; r0 += 32) {
       const int j0 = t * KEYS + r0;
-      if (j0 >= keys || (a.causal && j0 > q0 + 31 + a.shift)) break;  // nothing from there on is seen
-      f32x16 p, ds;
-      products(r0, p, ds);
-      differences(p, ds);
-      if (mask || j0 + 32 > keys || (a.causal && j0 + 31 > q0 + a.shift)) {
-        const uint32_t see = keys_seen(a, mask, qi, j0, keys);
+      if (!mask && j0 + 32 <= keys && !(a.causal && j0 + 31 > q0 + a.shift)) return;
+      const uint32_t see = keys_seen(a, mask, qi, j0, keys);
 #pragma unroll
-        for (int e = 0; e < 16; e++) ds[e] = (see >> e) & 1 ? ds[e] : 0.0f;
-      }
-      add(r0, ds);
+      for (int e = 0; e < 16; e++) ds[e] = (see >> e) & 1 ? ds[e] : 0.0f;
+    };
+    if (a.causal && t * KEYS > q0 + 31 + a.shift) continue;  // nothing of it is seen
+    f32x16 p, ds;
+    Weights<EL> w;
+    RowElements<T, EL, OT> k;  // (on their way during the exponentials; those of heads of 128 would be more registers than there are)
+    products(0, p, ds);
+    if constexpr (DP <= 96) k.load(rows);
+    if constexpr (!EL::F32) in_order();
+    differences(0, p, ds);
+    if constexpr (DP > 96) k.load(rows);
+    w.set(ds);
+    if constexpr (KEYS == 64) {
+      k.add(dq, w);
+      products(32, p, ds);
+      k.load(rows + 32 * T::ROW);
+      in_order();
+      differences(32, p, ds);
+      w.set(ds);
     }
+    k.add(dq, w);
   }
   if (there) store_column<EL, DP>(const_cast<S *>(rows_of<EL>(a.dq, b, h)) + (int64_t)qi * a.dq.row, dq, a.scale * UNLIFT<EL>, a.dim);
 }
@@ -186,49 +184,12 @@ struct KeysWalk {
   }
 };
 
-// What a thread brings of each step: rows of an operand, and in the first threads a row's lse and delta.
-template <class EL, int QUERIES, class T>
-struct KeysFetch {
-  const typename EL::S *rows;
-  const float *lse, *delta;
-  float power, less;
-  __device__ __forceinline__ void begin(const AttentionArgs &a, const HeadOperand &o, const KeysWalk<EL, QUERIES> &w) {
-    const int64_t i = (int64_t)w.at * QUERIES;
-    rows = rows_of<EL>(o, w.b, w.head) + i * o.row;
-    lse = reinterpret_cast<const float *>(a.lse.base) + (int64_t)w.b * a.lse.batch + (int64_t)w.head * a.lse.head + (i + threadIdx.x) * a.lse.row;
-    delta = a.delta + ((int64_t)w.b * a.heads + w.head) * a.sq + i + threadIdx.x;
-  }
-  __device__ __forceinline__ void fetch(const AttentionArgs &a, const HeadOperand &o, KeysWalk<EL, QUERIES> &w, T &tile) {
-    const int left = a.sq - w.at * QUERIES;
-    tile.fetch(rows, left, a.dim);
-    values(left);
-    if (w.next()) {
-      begin(a, o, w);
-    } else {
-      rows += (int64_t)QUERIES * o.row;
-      lse += (int64_t)QUERIES * a.lse.row;
-      delta += QUERIES;
-    }
-  }
-  __device__ __forceinline__ void values(int left) {
-    if (threadIdx.x < QUERIES) {
-      power = -INF, less = 0.0f;
-      if ((int)threadIdx.x < left) power = *lse, less = -*delta;
-    }
-  }
-  __device__ __forceinline__ void lay(float *powers, float *deltas) const {
-    if (threadIdx.x < QUERIES) {
-      powers[threadIdx.x] = exponent_of<EL>(power);
-      deltas[threadIdx.x] = less;
-    }
-  }
-};
-
-__device__ __forceinline__ void row_values(const float *values, f32x16 &x) {
-  const int half = (threadIdx.x >> 5) & 1;
+// A value of each of 32 rows, as the scores lie.
+__device__ __forceinline__ void row_values(uint32_t values, f32x16 &x) {
+  const uint32_t at = values + ((threadIdx.x >> 5) & 1) * 16;
 #pragma unroll
   for (int e = 0; e < 16; e += 4) {
-    const gemm_tile::f32x4 v = *reinterpret_cast<const gemm_tile::f32x4 *>(values + e * 2 + half * 4);
+    const gemm_tile::f32x4 v = *at_lds<const lds_f32x4>(at + e * 8);
 #pragma unroll
     for (int j = 0; j < 4; j++) x[e + j] = v[j];
   }
@@ -257,76 +218,78 @@ __device__ __forceinline__ void store_key(const AttentionArgs &a, const W &w, in
 // there would be few blocks; their sums are joined by another launch.
 template <class EL, int DP>
 __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs a) {
-  using S = typename EL::S;
   constexpr int QUERIES = EL::F32 ? 32 : 64, OT = DP / 32;
-  using T = Tile<EL, DP, QUERIES>;
-  constexpr int STAGE = 2 * T::SIZE;
-  __shared__ __attribute__((aligned(16))) S stages[2 * STAGE];
-  __shared__ __attribute__((aligned(16))) float powers[2][QUERIES], deltas[2][QUERIES];
+  using T = Tile<EL, DP, QUERIES, 4>;
+  constexpr int STAGE = 2 * T::SIZE + 1024, RING = 3, VALUES = 2 * T::SIZE;  // queries, their gradients, and each row's values
+  __shared__ __attribute__((aligned(1024))) unsigned char stages[RING * STAGE];
 
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   KeysWalk<EL, QUERIES> w(a);
-  const int k0 = w.first + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32, kj = k0 + (threadIdx.x & 31);
+  const int k0 = w.first + wave * 32, kj = k0 + (threadIdx.x & 31);
+  const uint32_t lds = lds_address(stages);
+  T qt, gt;
+  qt.begin(wave, a.q.row);
+  gt.begin(wave, a.g.row);
+  if (a.dim != DP) {
+    for (int s = 0; s < RING; s++) {
+      qt.clear(lds + s * STAGE, a.dim);
+      gt.clear(lds + s * STAGE + T::SIZE, a.dim);
+    }
+    __syncthreads();
+  }
+  const bool direct = a.q.direct && a.g.direct;
+  int at = w.at, head = w.head;  // of the step that is worked on (the walk's are of the one that is fetched)
+  // The walk's step, and on; whether all of it is on its way past the registers.
+  auto fetch = [&](uint32_t to) {
+    const int64_t i0 = (int64_t)w.at * QUERIES;
+    const int left = a.sq - w.at * QUERIES;
+    qt.fetch(rows_of<EL>(a.q, w.b, w.head) + i0 * a.q.row, left, a.q, a.dim, to);
+    gt.fetch(rows_of<EL>(a.g, w.b, w.head) + i0 * a.g.row, left, a.g, a.dim, to + T::SIZE);
+    if (wave < QUERIES / 32)
+      load_to_lds4(a.rows + (((int64_t)w.b * a.heads + w.head) * a.rows_pitch + i0 + wave * 32) * 2, (threadIdx.x & 63) * 4, to + VALUES + wave * 256);
+    w.next();
+    return direct && left >= QUERIES;
+  };
+  bool whole = false;  // of the step after the one that is worked on
+  if (w.steps > 0) fetch(lds);
+  if (w.steps > 1) whole = fetch(lds + STAGE);
   Column<EL, DP> k, v;
   k.load(rows_of<EL>(a.k, w.b, w.hk) + (int64_t)kj * a.k.row, kj < w.keys, a.dim);
   v.load(rows_of<EL>(a.v, w.b, w.hk) + (int64_t)kj * a.v.row, kj < w.keys, a.dim);
-  T qt, gt;
-  qt.begin(a.q.row);
-  gt.begin(a.g.row);
-  KeysFetch<EL, QUERIES, T> from;
-  const S *g_rows;
-  int at = w.at, head = w.head;  // of the step that is worked on
-  auto begin = [&]() {
-    from.begin(a, a.q, w);
-    g_rows = rows_of<EL>(a.g, w.b, w.head) + (int64_t)w.at * QUERIES * a.g.row;
-  };
-  auto fetch = [&]() {
-    gt.fetch(g_rows, a.sq - w.at * QUERIES, a.dim);
-    const int h = w.head;
-    from.fetch(a, a.q, w, qt);
-    g_rows = w.head == h ? g_rows + (int64_t)QUERIES * a.g.row : rows_of<EL>(a.g, w.b, w.head) + (int64_t)w.at * QUERIES * a.g.row;
-  };
-  auto lay = [&](int s) {
-    qt.lay(stages + s * STAGE);
-    gt.lay(stages + s * STAGE + T::SIZE);
-    from.lay(powers[s], deltas[s]);
-  };
   f32x16 dk[OT], dv[OT];
 #pragma unroll
   for (int t = 0; t < OT; t++)
 #pragma unroll
     for (int e = 0; e < 16; e++) dk[t][e] = dv[t][e] = 0.0f;
-  if (w.steps > 0) {
-    begin();
-    fetch();
-    lay(0);
-    if (w.steps > 1) fetch();
-  }
+  uint32_t stage = lds, ahead = lds + 2 * STAGE;
   for (int t = 0; t < w.steps; t++) {
-    __syncthreads();  // this tile is there, and the one before has been used
-    if (t + 1 < w.steps) {
-      lay((t + 1) & 1);
-      if (t + 2 < w.steps) fetch();
-    }
-    const S *stage = stages + (t & 1) * STAGE;
-    const float *power = powers[t & 1], *delta = deltas[t & 1];
-    const int i0 = at * QUERIES;
+    // this tile has come, and the stage that is filled next has been used
+    if (t == 0 || !whole) meet<0>();
+    else if (wave < QUERIES / 32) meet<2 * T::LPW + 1>();
+    else meet<2 * T::LPW>();
+    whole = false;
+    if (t + 2 < w.steps) whole = fetch(ahead);
+    const uint32_t rows = stage;
+    stage = stage == lds + 2 * STAGE ? lds : stage + STAGE;
+    ahead = ahead == lds + 2 * STAGE ? lds : ahead + STAGE;
+    const int i0 = at * QUERIES, head_now = head;
+    if (++at == w.tiles) at = w.before, head++;
     auto products = [&](int r0, f32x16 &p, f32x16 &ds) {
 #pragma unroll
       for (int e = 0; e < 16; e++) p[e] = 0.0f;
-      row_values(delta + r0, ds);
-      rows_by_columns<EL, DP, T::PITCH>(p, stage + r0 * T::PITCH, k);
-      rows_by_columns<EL, DP, T::PITCH>(ds, stage + T::SIZE + r0 * T::PITCH, v);
+      row_values(rows + VALUES + r0 * 8 + 128, ds);
+      two_scores<T>(p, k, ds, v, rows + r0 * T::ROW);
     };
     auto differences = [&](int r0, f32x16 &p, f32x16 &ds) {
       f32x16 l;
-      row_values(power + r0, l);
+      row_values(rows + VALUES + r0 * 8, l);
 #pragma unroll
       for (int e = 0; e < 16; e++) {
         p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[e], a.c2, l[e]));
         ds[e] = p[e] * ds[e];
       }
       if (!a.mask.base && !(a.causal && k0 + 31 > i0 + r0 + a.shift)) return;
-      const uint8_t *mask = a.mask.base ? reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)w.b * a.mask.batch + (int64_t)head * a.mask.head : nullptr;
+      const uint8_t *mask = a.mask.base ? reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)w.b * a.mask.batch + (int64_t)head_now * a.mask.head : nullptr;
       const uint32_t seeing = queries_seeing(a, mask, kj, i0 + r0);
 #pragma unroll
       for (int e = 0; e < 16; e++) {
@@ -335,27 +298,30 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
         ds[e] = keep ? ds[e] : 0.0f;
       }
     };
-    auto add = [&](int r0, const Weights<EL> &p, const Weights<EL> &ds) {
-      add_weighted_rows<EL, DP, T::PITCH>(dv, stage + T::SIZE + r0 * T::PITCH, p);
-      add_weighted_rows<EL, DP, T::PITCH>(dk, stage + r0 * T::PITCH, ds);
-    };
-    if (k0 < w.keys && !(a.causal && k0 > i0 + QUERIES - 1 + a.shift)) {  // (else nothing of the tile sees these keys)
-      f32x16 p, ds;
-      Weights<EL> pw, dsw;
-      products(0, p, ds);
-      differences(0, p, ds);
+    if (k0 >= w.keys || (a.causal && k0 > i0 + QUERIES - 1 + a.shift)) continue;  // nothing of the tile sees these keys
+    f32x16 p, ds;
+    Weights<EL> pw, dsw;
+    RowElements<T, EL, OT> g, q;  // (on their way during the exponentials)
+    products(0, p, ds);
+    g.load(rows + T::SIZE);
+    q.load(rows);
+    if constexpr (!EL::F32) in_order();
+    differences(0, p, ds);
+    pw.set(p);
+    dsw.set(ds);
+    if constexpr (QUERIES == 64) {
+      g.add(dv, pw);
+      q.add(dk, dsw);
+      products(32, p, ds);
+      g.load(rows + T::SIZE + 32 * T::ROW);
+      q.load(rows + 32 * T::ROW);
+      in_order();
+      differences(32, p, ds);
       pw.set(p);
       dsw.set(ds);
-      if constexpr (QUERIES == 64) {  // the second half's scores are on their way while the first half's sums are added to
-        products(32, p, ds);
-        add(0, pw, dsw);
-        differences(32, p, ds);
-        pw.set(p);
-        dsw.set(ds);
-      }
-      add(QUERIES - 32, pw, dsw);
     }
-    if (++at == w.tiles) at = w.before, head++;
+    g.add(dv, pw);
+    q.add(dk, dsw);
   }
   if (kj >= a.sk) return;
   store_key<EL, DP>(a, w, kj, true, dk);
@@ -367,12 +333,11 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
 // sums of one operand, not of two, which for heads of 128 are more registers than two waves of a unit's may have.
 template <class EL, int DP>
 __global__ __launch_bounds__(512) void attention_grad_wide_keys_kernel(AttentionArgs a) {
-  using S = typename EL::S;
   constexpr int QUERIES = 32, OT = DP / 32;
-  using T = Tile<EL, DP, QUERIES>;  // (each half of the threads brings one operand's)
-  constexpr int STAGE = 2 * T::SIZE;
-  __shared__ __attribute__((aligned(16))) S stages[3 * STAGE];
-  __shared__ __attribute__((aligned(16))) float powers[3][QUERIES], deltas[3][QUERIES];
+  using T = Tile<EL, DP, QUERIES, 4>;  // (four waves bring each operand's)
+  constexpr int STAGE = 2 * T::SIZE + 1024, RING = EL::F32 ? 3 : 4, VALUES = 2 * T::SIZE;
+  constexpr int AHEAD = RING - 2;  // tiles on their way
+  __shared__ __attribute__((aligned(1024))) unsigned char stages[RING * STAGE];
   __shared__ __attribute__((aligned(16))) float over[2][4][4][64][4];  // p, for the other wave: [tile][pair][e / 4][lane][e % 4]
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = wave & 3;
@@ -380,79 +345,93 @@ __global__ __launch_bounds__(512) void attention_grad_wide_keys_kernel(Attention
   KeysWalk<EL, QUERIES> w(a);
   const int k0 = w.first + pair * 32, kj = k0 + (lane & 31);
   const HeadOperand &mine = second ? a.v : a.k, &brought = second ? a.g : a.q;
+  const uint32_t lds = lds_address(stages);
+  T tile;
+  tile.begin(pair, brought.row);
+  if (a.dim != DP) {
+    for (int s = 0; s < RING; s++) tile.clear(lds + s * STAGE + (second ? T::SIZE : 0), a.dim);
+    __syncthreads();
+  }
+  int at = w.at, head = w.head;  // of the step that this wave works on (the walk's are of the one that is fetched)
+  auto fetch = [&](uint32_t to) {
+    const int64_t i0 = (int64_t)w.at * QUERIES;
+    const int left = a.sq - w.at * QUERIES;
+    tile.fetch(rows_of<EL>(brought, w.b, w.head) + i0 * brought.row, left, brought, a.dim, to + (second ? T::SIZE : 0));
+    if (wave == 0) load_to_lds4(a.rows + (((int64_t)w.b * a.heads + w.head) * a.rows_pitch + i0) * 2, lane * 4, to + VALUES);
+    w.next();
+    return brought.direct && left >= QUERIES;
+  };
+  bool whole = false;  // what is on its way for the step after this one
+  if (w.steps > 0) fetch(lds);
+  if (AHEAD == 2 && w.steps > 1) whole = fetch(lds + STAGE);
   Column<EL, DP> own;
   own.load(rows_of<EL>(mine, w.b, w.hk) + (int64_t)kj * mine.row, kj < w.keys, a.dim);
-  T tile;
-  tile.begin(brought.row);
-  KeysFetch<EL, QUERIES, T> from;
-  int at = w.at, head = w.head;  // of the step that this wave works on
-  auto lay = [&](int s) {
-    tile.lay(stages + s * STAGE + (second ? T::SIZE : 0));
-    from.lay(powers[s], deltas[s]);
-  };
   f32x16 acc[OT];  // of dv, in the second wave of dk
 #pragma unroll
   for (int t = 0; t < OT; t++)
 #pragma unroll
     for (int e = 0; e < 16; e++) acc[t][e] = 0.0f;
-  if (w.steps > 0) {
-    from.begin(a, brought, w);
-    from.fetch(a, brought, w, tile);
-    lay(0);
-    if (w.steps > 1) from.fetch(a, brought, w, tile);
-  }
-  int now = 0, next = 1;  // the stages of what this wave works on, and of what is laid
+  uint32_t stage = lds, ahead = lds + AHEAD * STAGE;
   for (int t = 0; w.steps > 0 && t <= w.steps; t++) {
-    __syncthreads();  // tile t is there, p of the tile before too, and what is laid now is no longer used
-    if (t + 1 < w.steps) {
-      lay(next);
-      if (t + 2 < w.steps) from.fetch(a, brought, w, tile);
+    // tile t has come, p of the tile before it too, and what is filled next has been used
+    if (t == 0 || !whole) meet<0>();
+    else if (wave == 0) meet<T::LPW + 1>();
+    else meet<T::LPW>();
+    whole = false;
+    if (t + AHEAD < w.steps) {
+      const bool is = fetch(ahead);
+      if (AHEAD == 2) whole = is;
     }
-    next = next == 2 ? 0 : next + 1;
+    ahead = ahead == lds + (RING - 1) * STAGE ? lds : ahead + STAGE;
     if (second ? t == 0 : t == w.steps) continue;
-    const S *rows = stages + now * STAGE;
-    const int i0 = at * QUERIES;
-    float(*between)[64][4] = over[(second ? t - 1 : t) & 1][pair];
-    if (k0 < w.keys && !(a.causal && k0 > i0 + 31 + a.shift)) {  // (else nothing of the tile sees these keys)
-      const bool inner = !a.mask.base && !(a.causal && k0 + 31 > i0 + a.shift);
-      f32x16 x;
-      if (second) {
-        row_values(deltas[now], x);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; e++) x[e] = 0.0f;
-      }
-      rows_by_columns<EL, DP, T::PITCH>(x, rows + (second ? T::SIZE : 0), own);
-      if (!second) {
-        f32x16 l;
-        row_values(powers[now], l);
-#pragma unroll
-        for (int e = 0; e < 16; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.c2, l[e]));
-        if (!inner) {
-          const uint8_t *mask = a.mask.base ? reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)w.b * a.mask.batch + (int64_t)head * a.mask.head : nullptr;
-          const uint32_t seeing = queries_seeing(a, mask, kj, i0);
-#pragma unroll
-          for (int e = 0; e < 16; e++) x[e] = (seeing >> e) & 1 ? x[e] : 0.0f;
-        }
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) *reinterpret_cast<gemm_tile::f32x4 *>(between[e >> 2][lane]) = gemm_tile::f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const gemm_tile::f32x4 p = *reinterpret_cast<const gemm_tile::f32x4 *>(between[e >> 2][lane]);
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const float ds = p[j] * x[e + j];
-            x[e + j] = inner || p[j] != 0.0f ? ds : 0.0f;  // (what a query does not see may be no number)
-          }
-        }
-      }
-      Weights<EL> y;
-      y.set(x);
-      add_weighted_rows<EL, DP, T::PITCH>(acc, rows + (second ? 0 : T::SIZE), y);
-    }
-    now = now == 2 ? 0 : now + 1;
+    const uint32_t rows = stage;
+    stage = stage == lds + (RING - 1) * STAGE ? lds : stage + STAGE;
+    const int i0 = at * QUERIES, head_now = head;
     if (++at == w.tiles) at = w.before, head++;
+    if (k0 >= w.keys || (a.causal && k0 > i0 + 31 + a.shift)) continue;  // nothing of the tile sees these keys
+    float(*between)[64][4] = over[(second ? t - 1 : t) & 1][pair];
+    const bool inner = !a.mask.base && !(a.causal && k0 + 31 > i0 + a.shift);
+    f32x16 x;
+    if (second) {
+      row_values(rows + VALUES + 128, x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; e++) x[e] = 0.0f;
+    }
+    RowVectors<T, EL, DP> vectors;
+    vectors.load(rows + (second ? T::SIZE : 0));
+    if constexpr (!EL::F32) in_order();
+    vectors.scores(x, own);
+    RowElements<T, EL, OT> elements;  // (on their way during the exponentials)
+    elements.load(rows + (second ? 0 : T::SIZE));
+    if constexpr (!EL::F32) in_order();
+    if (!second) {
+      f32x16 l;
+      row_values(rows + VALUES, l);
+#pragma unroll
+      for (int e = 0; e < 16; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.c2, l[e]));
+      if (!inner) {
+        const uint8_t *mask = a.mask.base ? reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)w.b * a.mask.batch + (int64_t)head_now * a.mask.head : nullptr;
+        const uint32_t seeing = queries_seeing(a, mask, kj, i0);
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[e] = (seeing >> e) & 1 ? x[e] : 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) *reinterpret_cast<gemm_tile::f32x4 *>(between[e >> 2][lane]) = gemm_tile::f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const gemm_tile::f32x4 p = *reinterpret_cast<const gemm_tile::f32x4 *>(between[e >> 2][lane]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float ds = p[j] * x[e + j];
+          x[e + j] = inner || p[j] != 0.0f ? ds : 0.0f;  // (what a query does not see may be no number)
+        }
+      }
+    }
+    Weights<EL> y;
+    y.set(x);
+    elements.add(acc, y);
   }
   if (kj < a.sk) store_key<EL, DP>(a, w, kj, second, acc);
 }
@@ -528,11 +507,12 @@ NXH_EXPORT int nxh_attention_grad(nxh_context *ctx, const nxh_tensor *dq, const 
   if ((double)blocks * a.parts > 2147483647.0) return nxh_fail(NXH_FAILURE, op, "too many rows for one launch");
   std::lock_guard<std::mutex> guard(ctx->mu);
   NXH_HIP(op, hipSetDevice(ctx->device));
-  const size_t rows = ((size_t)a.batch * a.heads * a.sq * 4 + 255) / 256 * 256;
+  a.rows_pitch = (a.sq + 63) / 64 * 64;
+  const size_t rows = (size_t)a.batch * a.heads * a.rows_pitch * 8;
   const size_t sums = a.parts > 1 ? (size_t)a.parts * a.batch * a.kv_heads * a.sk * 2 * a.dim * 4 : 0;
   void *space = nullptr;
   if ((rc = nxh_alloc_locked(ctx, rows + sums, &space))) return rc;
-  a.delta = (float *)space;
+  a.rows = (float *)space;
   a.partial = sums ? (float *)((char *)space + rows) : nullptr;
   nxh_set_path("attention_grad");
   if (dt == NXH_F32) launch_dim<gemm_tile::ElF32>(ctx, a);

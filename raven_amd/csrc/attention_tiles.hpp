@@ -30,6 +30,7 @@ constexpr float INF = __builtin_inff();
 struct HeadOperand {
   const char *base;
   int64_t batch, head, row;  // strides, elements
+  int direct;                // rows are whole 16-byte units on 16-byte addresses: they may go to LDS past the registers
 };
 struct AttentionArgs {
   HeadOperand q, k, v, out, g, dq, dk, dv;
@@ -38,7 +39,8 @@ struct AttentionArgs {
   HeadOperand lse;       // row: of one value each
   const int32_t *lengths;  // null: none
   int64_t lengths_step;
-  float *delta;    // [batch, heads, sq]
+  float *rows;     // what each row's exponents and differences take, [batch, heads][rows_pitch][2]
+  int rows_pitch;
   float *partial;  // parts' dk and dv, [parts][batch, kv_heads, sk][2][dim]; null: one part
   int parts;
   int batch, heads, kv_heads, sq, sk, dim, tiles;
@@ -101,48 +103,89 @@ __device__ __forceinline__ V16 load_part(const typename EL::S *p, int left) {
   return w;
 }
 
-// A tile of ROWS rows of DP elements (the head's, and zeros) in LDS, brought by 256 threads (as many of them as divide its
-// vectors) through registers. Rows are 16 bytes (128 elements of 16 bits: 48) further apart than they are long: sixteen rows'
-// vectors at one place lie in different banks, and of the four rows of a transposing load no more than two in one.
-template <class EL, int DP, int ROWS>
+// ── tiles in LDS ────────────────────────────────────────────────────────────
+typedef __attribute__((address_space(3))) V16 lds_V16;
+typedef __attribute__((address_space(3))) float lds_float;
+typedef __attribute__((address_space(3))) gemm_tile::f32x4 lds_f32x4;
+// What lies at an LDS address.
+template <class P>
+__device__ __forceinline__ P *at_lds(uint32_t address) {
+  return reinterpret_cast<P *>((uintptr_t)address);
+}
+__device__ __forceinline__ uint32_t lds_address(void *p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)p; }
+
+// Each lane's 16 (4) bytes at `base` + its offset go to consecutive LDS addresses from `lds` on. m0 carries the LDS address; the
+// compiler treats it as reserved and writes it in front of each of its own uses.
+__device__ __forceinline__ void load_to_lds16(const void *base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_to_lds4(const void *base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+}
+// Waits for all loads of this wave but the last N, and for its LDS accesses, then for the block's other waves.
+template <int N>
+__device__ __forceinline__ void meet() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// ROWS rows of DP elements (the head's, and zeros), brought by WAVES waves. A load to LDS fills 1 KiB without gaps, so conflicts of
+// banks are avoided by choosing which 16 bytes of a row lie where: unit u of row r at u ^ turn(r). Sixteen rows' units at one
+// place, and four rows' four units that half a wave of a transposing load reads, then lie in all 64 banks.
+template <class EL, int DP, int ROWS, int WAVES>
 struct Tile {
   using S = typename EL::S;
-  static constexpr int PITCH = DP + EL::VE * (!EL::F32 && DP == 128 ? 3 : 1), SIZE = ROWS * PITCH, VPR = DP / EL::VE, ALL = ROWS * VPR;
-  static constexpr int THREADS = ALL % 256 == 0 ? 256 : ALL % 192 == 0 ? 192 : ALL, NV = ALL / THREADS;
-  static_assert(THREADS <= 256 && NV * THREADS == ALL, "whole vectors a thread");
-  V16 pre[NV];
-  uint32_t off[NV];  // bytes from the tile's first row
+  static constexpr int UNITS = DP / EL::VE, ROW = DP * (int)sizeof(S), SIZE = ROWS * ROW;  // units of a row; bytes
+  static constexpr int LOADS = ROWS * UNITS / 64, LPW = (LOADS + WAVES - 1) / WAVES;       // of a tile, and of a wave that has any
+  static_assert(LOADS * 64 == ROWS * UNITS && LOADS % LPW == 0, "whole loads, the same number each");
+  uint32_t off[LPW];  // bytes from the tile's first row
+  int wave;           // of those that bring this tile; none where it is LOADS / LPW or more
 
-  __device__ __forceinline__ static bool brings() { return THREADS == 256 || (threadIdx.x & 255) < THREADS; }
-  __device__ __forceinline__ void begin(int64_t row) {
+  __device__ __forceinline__ static int turn(int r) {
+    if constexpr (UNITS % 16 == 0 && !(EL::F32 && UNITS == 32)) return ((r & 3) << 2) | ((r >> 2) & 3);
+    else if constexpr (UNITS == 32) return r & 15;
+    else if constexpr (UNITS == 24) return (r >> 1) & 7;
+    else if constexpr (UNITS == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    else return (r >> 2) & 3;
+  }
+  __device__ __forceinline__ void begin(int w, int64_t row) {
+    wave = w;
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const int v = (int)(threadIdx.x & 255) + i * THREADS;
-      off[i] = ((uint32_t)(v / VPR) * (uint32_t)row + (uint32_t)(v % VPR) * EL::VE) * (uint32_t)sizeof(S);
+    for (int i = 0; i < LPW; i++) {
+      const int u = (wave * LPW + i) * 64 + lane, r = u / UNITS;
+      off[i] = (uint32_t)r * (uint32_t)row * (uint32_t)sizeof(S) + (uint32_t)((u % UNITS) ^ turn(r)) * 16u;
     }
   }
-  // The rows from `first` on, of which `left` exist.
-  __device__ __forceinline__ void fetch(const S *first, int left, int dim) {
-    if (!brings()) return;
-    const char *at = reinterpret_cast<const char *>(first);
-    if (left >= ROWS && dim == DP) {
+  // Units past the head's end, which loads leave as they are, in all of a tile's memory.
+  __device__ __forceinline__ void clear(uint32_t tile, int dim) const {
+    if (dim == DP || wave >= LOADS / LPW) return;
 #pragma unroll
-      for (int i = 0; i < NV; i++) __builtin_memcpy(&pre[i], at + off[i], 16);
+    for (int i = 0; i < LPW; i++) *at_lds<lds_V16>(tile + ((wave * LPW + i) * 64 + (threadIdx.x & 63)) * 16) = V16{0, 0, 0, 0};
+  }
+  // The rows from `first` on, of which `left` exist. Whole tiles go past the registers and arrive by meet(); others are there once
+  // this returns.
+  __device__ __forceinline__ void fetch(const S *first, int left, const HeadOperand &o, int dim, uint32_t tile) const {
+    if (wave >= LOADS / LPW) return;
+    const int lane = threadIdx.x & 63;
+    const uint32_t to = tile + (uint32_t)wave * LPW * 1024u;
+    if (left >= ROWS && o.direct) {
+#pragma unroll
+      for (int i = 0; i < LPW; i++) {
+        if (dim == DP) {
+          load_to_lds16(first, off[i], to + i * 1024);
+        } else {
+          const int u = (wave * LPW + i) * 64 + lane;
+          if (((u % UNITS) ^ turn(u / UNITS)) * EL::VE < dim) load_to_lds16(first, off[i], to + i * 1024);
+        }
+      }
       return;
     }
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const int v = (int)(threadIdx.x & 255) + i * THREADS, c = (v % VPR) * EL::VE;
-      pre[i] = V16{0, 0, 0, 0};
-      if (v / VPR < left && c < dim) pre[i] = load_part<EL>(reinterpret_cast<const S *>(at + off[i]), dim - c);
-    }
-  }
-  __device__ __forceinline__ void lay(S *tile) const {
-    if (!brings()) return;
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const int v = (int)(threadIdx.x & 255) + i * THREADS;
-      *reinterpret_cast<V16 *>(tile + (v / VPR) * PITCH + (v % VPR) * EL::VE) = pre[i];
+    for (int i = 0; i < LPW; i++) {
+      const int u = (wave * LPW + i) * 64 + lane, r = u / UNITS, c = ((u % UNITS) ^ turn(r)) * EL::VE;
+      V16 w = {0, 0, 0, 0};
+      if (r < left && c < dim) w = load_part<EL>(reinterpret_cast<const S *>(reinterpret_cast<const char *>(first) + off[i]), dim - c);
+      *at_lds<lds_V16>(to + (i * 64 + lane) * 16) = w;
     }
   }
 };
@@ -181,15 +224,37 @@ struct Column {
   }
 };
 
-// acc[e] += row (e / 4) * 8 + g * 4 + e % 4 of 32 . this lane's column.
-template <class EL, int DP, int PITCH>
-__device__ __forceinline__ void rows_by_columns(f32x16 &acc, const typename EL::S *rows, const Column<EL, DP> &column) {
-  const typename EL::S *at = rows + (threadIdx.x & 31) * PITCH + ((threadIdx.x >> 5) & 1) * EL::VE;
+// What stands before it is issued before what stands behind. The compiler keeps registers free by reading from LDS right in front of
+// each use, and each matrix instruction then waits out a read's latency: all of a product's reads are issued first.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
+// Elements of 32 rows as scores() takes them, steps FROM to TO of the dim: row lane % 32. `rows`: where the first row lies, a
+// multiple of 32 of a tile.
+template <class T, class EL, int DP, int FROM = 0, int TO = DP / (2 * EL::VE)>
+struct RowVectors {
+  V16 f[TO - FROM];
+  __device__ __forceinline__ void load(uint32_t rows) {
+    const int r = threadIdx.x & 31, g = (threadIdx.x >> 5) & 1, x = g ^ T::turn(r);
+    const uint32_t at = rows + (uint32_t)(r * T::ROW);
 #pragma unroll
-  for (int s = 0; s < Column<EL, DP>::STEPS; s++) {
-    const V16 r = *reinterpret_cast<const V16 *>(at + s * 2 * EL::VE);
-    gemm_tile::mfma_step<EL>(acc, r, column.f[s]);
+    for (int s = FROM; s < TO; s++) {
+      // (turns stay inside groups of four, eight or sixteen units: what lies above is a constant)
+      constexpr int GROUP = T::UNITS % 16 == 0 ? 16 : T::UNITS % 8 == 0 ? 8 : 4;
+      f[s - FROM] = *at_lds<const lds_V16>(at + (uint32_t)(x ^ ((2 * s) % GROUP)) * 16 + (uint32_t)((2 * s) / GROUP * GROUP * 16));
+    }
   }
+  // acc[e] += row (e / 4) * 8 + g * 4 + e % 4 . this lane's column
+  __device__ __forceinline__ void scores(f32x16 &acc, const Column<EL, DP> &column) const {
+#pragma unroll
+    for (int s = FROM; s < TO; s++) gemm_tile::mfma_step<EL>(acc, f[s - FROM], column.f[s]);
+  }
+};
+// The same in one, for float32, whose instructions take longer than a read.
+template <class T, class EL, int DP>
+__device__ __forceinline__ void rows_by_columns(f32x16 &acc, uint32_t rows, const Column<EL, DP> &column) {
+  RowVectors<T, EL, DP> v;
+  v.load(rows);
+  v.scores(acc, column);
 }
 
 // Weights of 32 rows and this lane's column, as the second product takes them: rounded to the operands' type, which its
@@ -208,29 +273,87 @@ struct Weights<gemm_tile::ElF32> {
   __device__ __forceinline__ void set(const f32x16 &x) { w = x; }
 };
 
-// acc[t][e] += sum over 32 rows of element 32 t + (e / 4) * 8 + g * 4 + e % 4 of a row times its weight for this lane's column.
-template <class EL, int DP, int PITCH>
-__device__ __forceinline__ void add_weighted_rows(f32x16 (&acc)[DP / 32], const typename EL::S *rows, const Weights<EL> &p) {
-  const int lane = threadIdx.x & 63, g = lane >> 5;
-  if constexpr (EL::F32) {
-    const float *at = rows + 4 * g * PITCH + (lane & 31);
-#pragma unroll
-    for (int e = 0; e < 16; e++)
-#pragma unroll
-      for (int t = 0; t < DP / 32; t++)
-        acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(at[((e >> 2) * 8 + (e & 3)) * PITCH + t * 32], p.w[e], acc[t], 0, 0, 0);
-  } else {
-    const uint16_t *at = rows + (4 * g + ((lane & 15) >> 2)) * PITCH + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+// Elements of 32 rows as the second product takes them: acc[t][e] += sum over the rows of element 32 t + (e / 4) * 8 + g * 4 +
+// e % 4 of a row times its weight for this lane's column. 16-bit elements are read ahead.
+template <class T, class EL, int OT>
+struct RowElements {
+  V16 f[2 * OT];
+  __device__ __forceinline__ void load(uint32_t rows) {
+    // the transposing load: sixteen lanes read 4 rows of 16 elements, lane i eight bytes of row i / 4, and get column i's four
+    const int lane = threadIdx.x & 63, g = lane >> 5, j = (lane & 15) >> 2, b = (lane >> 4) & 1, c = (lane & 3) >> 1;
+    const uint32_t at = rows + (uint32_t)((4 * g + j) * T::ROW + (lane & 1) * 8);
+    const int x = (2 * b + c) ^ T::turn(4 * g + j);  // of unit 2 b + c; those of 8 rows on differ by 2
 #pragma unroll
     for (int s = 0; s < 2; s++)
 #pragma unroll
-      for (int t = 0; t < DP / 32; t++) {
-        const uint16_t *src = at + 16 * s * PITCH + t * 32;
+      for (int t = 0; t < OT; t++) {
+        constexpr int GROUP = T::UNITS % 16 == 0 ? 16 : T::UNITS % 8 == 0 ? 8 : 4;
+        const uint32_t src = at + (uint32_t)(x ^ ((4 * t) % GROUP)) * 16 + (uint32_t)((4 * t) / GROUP * GROUP * 16 + 16 * s * T::ROW);
+        const uint32_t src8 = at + (uint32_t)(x ^ 2 ^ ((4 * t) % GROUP)) * 16 + (uint32_t)((4 * t) / GROUP * GROUP * 16 + (16 * s + 8) * T::ROW);
         typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
-        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)src));
-        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(src + 8 * PITCH)));
-        gemm_tile::mfma_step<EL>(acc[t], V16{lo[0], lo[1], hi[0], hi[1]}, V16{p.w[4 * s], p.w[4 * s + 1], p.w[4 * s + 2], p.w[4 * s + 3]});
+        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(at_lds<lds_s16x4>(src)));
+        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(at_lds<lds_s16x4>(src8)));
+        f[s * OT + t] = V16{lo[0], lo[1], hi[0], hi[1]};
       }
+  }
+  __device__ __forceinline__ void add(f32x16 (&acc)[OT], const Weights<EL> &p) const {
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+#pragma unroll
+      for (int t = 0; t < OT; t++)
+        gemm_tile::mfma_step<EL>(acc[t], f[s * OT + t], V16{p.w[4 * s], p.w[4 * s + 1], p.w[4 * s + 2], p.w[4 * s + 3]});
+  }
+};
+template <class T, int OT>
+struct RowElements<T, gemm_tile::ElF32, OT> {
+  uint32_t rows;
+  __device__ __forceinline__ void load(uint32_t at) { rows = at; }
+  __device__ __forceinline__ void add(f32x16 (&acc)[OT], const Weights<gemm_tile::ElF32> &p) const {
+    // row 8 (e / 4) + 4 g + e % 4, unit 8 t + c / 4: turn(row) = turn(4 g) ^ turn(8 (e / 4) + e % 4)
+    const int lane = threadIdx.x & 63, g = lane >> 5;
+    const uint32_t at = rows + (uint32_t)(4 * g * T::ROW + (lane & 3) * 4);
+    const int x = ((lane & 31) >> 2) ^ T::turn(4 * g);
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      const int r = (e >> 2) * 8 + (e & 3), turned = T::turn(r);
+#pragma unroll
+      for (int t = 0; t < OT; t++) {
+        const int unit = (8 * t) ^ (turned & ~7);
+        const float v = *at_lds<const lds_float>(at + (uint32_t)(x ^ (turned & 7)) * 16 + (uint32_t)(unit * 16 + r * T::ROW));
+        acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p.w[e], acc[t], 0, 0, 0);
+      }
+    }
+  }
+};
+
+// Two products of 32 rows each, of tiles that lie side by side: a += rows . ca, b += rows T::SIZE further on . cb. Heads of more
+// than 64 in two halves, which is as many registers as a product of one.
+template <class T, class EL, int DP>
+__device__ __forceinline__ void two_scores(f32x16 &a, const Column<EL, DP> &ca, f32x16 &b, const Column<EL, DP> &cb, uint32_t rows) {
+  if constexpr (EL::F32) {
+    rows_by_columns<T>(a, rows, ca);
+    rows_by_columns<T>(b, rows + T::SIZE, cb);
+  } else if constexpr (DP <= 64) {
+    RowVectors<T, EL, DP> x, y;
+    x.load(rows);
+    y.load(rows + T::SIZE);
+    in_order();
+    x.scores(a, ca);
+    y.scores(b, cb);
+  } else {
+    constexpr int STEPS = DP / (2 * EL::VE), HALF = STEPS / 2;
+    RowVectors<T, EL, DP, 0, HALF> x, y;
+    RowVectors<T, EL, DP, HALF, STEPS> z, u;
+    x.load(rows);
+    y.load(rows + T::SIZE);
+    in_order();
+    x.scores(a, ca);
+    z.load(rows);
+    y.scores(b, cb);
+    u.load(rows + T::SIZE);
+    in_order();
+    z.scores(a, ca);
+    u.scores(b, cb);
   }
 }
 
@@ -299,10 +422,12 @@ int attention_operand(const char *op, const nxh_tensor *t, int dt, int64_t b, in
     if (t->shape[k] > 1 && t->strides[k] == 0) return nxh_fail(NXH_INVALID_ARGUMENT, op, NXH_ERR_OUT_ALIASED);
   if (d > 1 && t->strides[3] != 1) return nxh_fail(NXH_FAILURE, op, "rows must be contiguous");
   if (n > 1 && (t->strides[2] < 0 || t->strides[2] > (1 << 23))) return nxh_fail(NXH_FAILURE, op, "rows must follow each other within 2^23 elements");
-  o.base = (const char *)t->data + t->offset * (int64_t)nxh_elem_size(dt);
+  const int64_t es = nxh_elem_size(dt);
+  o.base = (const char *)t->data + t->offset * es;
   o.batch = t->strides[0];
   o.head = t->strides[1];
   o.row = n > 1 ? t->strides[2] : 0;
+  o.direct = (uintptr_t)o.base % 16 == 0 && d * es % 16 == 0 && o.row * es % 16 == 0 && (b <= 1 || o.batch * es % 16 == 0) && (h <= 1 || o.head * es % 16 == 0);
   return NXH_OK;
 }
 
@@ -332,7 +457,7 @@ int attention_arguments(const char *op, AttentionArgs &a, const nxh_tensor *q, c
   if (lse->ndim != 3 || lse->shape[0] != b || lse->shape[1] != h || lse->shape[2] != sq) return nxh_fail(NXH_INVALID_ARGUMENT, op, NXH_ERR_SHAPE);
   for (int n = 0; n < 3 && !grad; n++)
     if (lse->shape[n] > 1 && lse->strides[n] == 0) return nxh_fail(NXH_INVALID_ARGUMENT, op, NXH_ERR_OUT_ALIASED);
-  a.lse = {(const char *)lse->data + lse->offset * 4, lse->strides[0], lse->strides[1], lse->strides[2]};
+  a.lse = {(const char *)lse->data + lse->offset * 4, lse->strides[0], lse->strides[1], lse->strides[2], 0};
   a.lengths = nullptr;
   a.lengths_step = 0;
   if (lengths) {
@@ -341,13 +466,13 @@ int attention_arguments(const char *op, AttentionArgs &a, const nxh_tensor *q, c
     a.lengths = (const int32_t *)lengths->data + lengths->offset;
     a.lengths_step = lengths->strides[0];
   }
-  a.mask = {nullptr, 0, 0, 0};
+  a.mask = {nullptr, 0, 0, 0, 0};
   a.mask_col = 0;
   if (mask) {
     if (mask->dtype != NXH_BOOL) return nxh_fail(NXH_FAILURE, op, NXH_ERR_UNSUPPORTED);
     if (mask->ndim != 4 || mask->shape[0] != b || mask->shape[1] != h || mask->shape[2] != sq || mask->shape[3] != sk)
       return nxh_fail(NXH_INVALID_ARGUMENT, op, NXH_ERR_SHAPE);
-    a.mask = {(const char *)mask->data + mask->offset, mask->strides[0], mask->strides[1], mask->strides[2]};
+    a.mask = {(const char *)mask->data + mask->offset, mask->strides[0], mask->strides[1], mask->strides[2], 0};
     a.mask_col = mask->strides[3];
   }
   a.batch = (int)b;
@@ -360,8 +485,8 @@ int attention_arguments(const char *op, AttentionArgs &a, const nxh_tensor *q, c
   a.shift = (int)(sk - sq);
   a.scale = (float)scale;
   a.c2 = (float)(scale * 1.4426950408889634);
-  a.g = a.dq = a.dk = a.dv = {nullptr, 0, 0, 0};
-  a.delta = a.partial = nullptr;
+  a.g = a.dq = a.dk = a.dv = {nullptr, 0, 0, 0, 0};
+  a.rows = a.partial = nullptr;
   a.parts = 1;
   a.tiles = 0;
   return NXH_OK;

@@ -17,10 +17,10 @@ namespace {
 template <class EL, int DP, int KW>
 __global__ __launch_bounds__(256) void attention_train_kernel(AttentionArgs a) {
   using S = typename EL::S;
-  constexpr int KEYS = EL::F32 ? 32 * KW : 64, QUERIES = 128 / KW, OT = DP / 32;
-  using T = Tile<EL, DP, KEYS>;
-  constexpr int STAGE = 2 * T::SIZE;
-  __shared__ __attribute__((aligned(16))) S stages[2 * STAGE];
+  constexpr int KEYS = !EL::F32 && DP <= 64 ? 64 : 32 * KW, SUBS = KEYS / 32 / KW, QUERIES = 128 / KW, OT = DP / 32;
+  using T = Tile<EL, DP, KEYS, 4>;
+  constexpr int STAGE = 2 * T::SIZE, RING = 3 * STAGE <= 80 * 1024 ? 3 : 2, AHEAD = RING - 1;  // tiles on their way
+  __shared__ __attribute__((aligned(1024))) unsigned char stages[RING * STAGE];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31;
   const int pair = wave / KW, part = wave % KW;
@@ -31,29 +31,31 @@ __global__ __launch_bounds__(256) void attention_train_kernel(AttentionArgs a) {
   const int q0 = tile * QUERIES + pair * 32, qi = q0 + c32;
   const S *K = rows_of<EL>(a.k, b, hk), *V = rows_of<EL>(a.v, b, hk);
   const uint8_t *mask = a.mask.base ? reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)b * a.mask.batch + (int64_t)h * a.mask.head : nullptr;
-  Column<EL, DP> q;
-  q.load(rows_of<EL>(a.q, b, h) + (int64_t)qi * a.q.row, qi < a.sq, a.dim);
 
   int seen = keys;  // by the block's last query
   if (a.causal) seen = min(seen, max(0, min((tile + 1) * QUERIES, a.sq) + a.shift));
   const int steps = (seen + KEYS - 1) / KEYS;
 
+  const uint32_t lds = lds_address(stages);
   T kt, vt;
-  kt.begin(a.k.row);
-  vt.begin(a.v.row);
-  auto fetch = [&](int t) {
-    kt.fetch(K + (int64_t)t * KEYS * a.k.row, keys - t * KEYS, a.dim);
-    vt.fetch(V + (int64_t)t * KEYS * a.v.row, keys - t * KEYS, a.dim);
-  };
-  auto lay = [&](int t) {
-    kt.lay(stages + (t & 1) * STAGE);
-    vt.lay(stages + (t & 1) * STAGE + T::SIZE);
-  };
-  if (steps > 0) {
-    fetch(0);
-    lay(0);
-    if (steps > 1) fetch(1);
+  kt.begin(wave, a.k.row);
+  vt.begin(wave, a.v.row);
+  if (a.dim != DP) {
+    for (int s = 0; s < RING; s++) {
+      kt.clear(lds + s * STAGE, a.dim);
+      vt.clear(lds + s * STAGE + T::SIZE, a.dim);
+    }
+    __syncthreads();
   }
+  auto whole = [&](int t) { return (t + 1) * KEYS <= keys && a.k.direct && a.v.direct; };
+  auto fetch = [&](int t, uint32_t to) {
+    kt.fetch(K + (int64_t)t * KEYS * a.k.row, keys - t * KEYS, a.k, a.dim, to);
+    vt.fetch(V + (int64_t)t * KEYS * a.v.row, keys - t * KEYS, a.v, a.dim, to + T::SIZE);
+  };
+  for (int t = 0; t < AHEAD && t < steps; t++) fetch(t, lds + t * STAGE);
+  Column<EL, DP> q;
+  q.load(rows_of<EL>(a.q, b, h) + (int64_t)qi * a.q.row, qi < a.sq, a.dim);
+
   f32x16 out[OT];
 #pragma unroll
   for (int t = 0; t < OT; t++)
@@ -61,52 +63,72 @@ __global__ __launch_bounds__(256) void attention_train_kernel(AttentionArgs a) {
     for (int e = 0; e < 16; e++) out[t][e] = 0.0f;
   float m = -INF, sum = 0.0f;
   float mc = 0.0f, lim = INF;  // -c m, and +inf before the first score, where exponentials take 0
+  uint32_t stage = lds, ahead = lds + AHEAD * STAGE;
   for (int t = 0; t < steps; t++) {
-    __syncthreads();  // this tile is there, and the one before has been used
-    if (t + 1 < steps) {
-      lay(t + 1);
-      if (t + 2 < steps) fetch(t + 2);
+    // this tile has come, and the stage that is filled next has been used
+    if (AHEAD == 2 && t > 0 && t + 1 < steps && whole(t + 1)) meet<2 * T::LPW>();
+    else meet<0>();
+    if (t + AHEAD < steps) fetch(t + AHEAD, ahead);
+    const uint32_t rows = stage + (uint32_t)(part * 32 * T::ROW);
+    stage = stage == lds + (RING - 1) * STAGE ? lds : stage + STAGE;
+    ahead = ahead == lds + (RING - 1) * STAGE ? lds : ahead + STAGE;
+    const int j0 = t * KEYS + part * 32;
+    if (j0 >= keys || (a.causal && j0 > q0 + 31 + a.shift)) continue;  // nothing of it is seen
+    f32x16 s[SUBS];
+#pragma unroll
+    for (int u = 0; u < SUBS; u++) {
+      RowVectors<T, EL, DP> k;
+      k.load(rows + u * 32 * T::ROW);
+      if constexpr (!EL::F32) in_order();
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[u][e] = 0.0f;
+      k.scores(s[u], q);
     }
-    const S *stage = stages + (t & 1) * STAGE;
+    RowElements<T, EL, OT> v;  // (on their way during the exponentials)
+    v.load(rows + T::SIZE);
+    if constexpr (!EL::F32) in_order();
+    if (mask || j0 + SUBS * 32 > keys || (a.causal && j0 + SUBS * 32 - 1 > q0 + a.shift)) {
 #pragma unroll
-    for (int sub = 0; sub < KEYS / 32; sub += KW) {
-      const int r0 = (sub + part) * 32, j0 = t * KEYS + r0;
-      if (j0 >= keys || (a.causal && j0 > q0 + 31 + a.shift)) continue;  // nothing of it is seen
-      f32x16 s;
+      for (int u = 0; u < SUBS; u++) {
+        const uint32_t see = keys_seen(a, mask, qi, j0 + u * 32, keys);
 #pragma unroll
-      for (int e = 0; e < 16; e++) s[e] = 0.0f;
-      rows_by_columns<EL, DP, T::PITCH>(s, stage + r0 * T::PITCH, q);
-      if (mask || j0 + 32 > keys || (a.causal && j0 + 31 > q0 + a.shift)) {
-        const uint32_t see = keys_seen(a, mask, qi, j0, keys);
-#pragma unroll
-        for (int e = 0; e < 16; e++) s[e] = (see >> e) & 1 ? s[e] : -INF;
+        for (int e = 0; e < 16; e++) s[u][e] = (see >> e) & 1 ? s[u][e] : -INF;
       }
-      float most = s[0];
+    }
+    float most = s[0][0];
 #pragma unroll
-      for (int e = 1; e < 16; e++) most = __builtin_fmaxf(most, s[e]);
-      most = __builtin_fmaxf(most, other_half(most));
-      const bool grow = most > m && __builtin_fmaf(most, a.c2, lim) > 8.0f;
-      if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-        const float mc_new = -most * a.c2;
-        const float alpha = grow ? __builtin_amdgcn_exp2f(__builtin_fmaf(m, a.c2, mc_new)) : 1.0f;
-        m = grow ? most : m;
-        mc = grow ? mc_new : mc;
-        lim = grow ? mc_new : lim;
-        sum = sum * alpha;
+    for (int u = 0; u < SUBS; u++)
 #pragma unroll
-        for (int o = 0; o < OT; o++)
+      for (int e = 0; e < 16; e++) most = __builtin_fmaxf(most, s[u][e]);
+    most = __builtin_fmaxf(most, other_half(most));
+    const bool grow = most > m && __builtin_fmaf(most, a.c2, lim) > 8.0f;
+    if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+      const float mc_new = -most * a.c2;
+      const float alpha = grow ? __builtin_amdgcn_exp2f(__builtin_fmaf(m, a.c2, mc_new)) : 1.0f;
+      m = grow ? most : m;
+      mc = grow ? mc_new : mc;
+      lim = grow ? mc_new : lim;
+      sum = sum * alpha;
 #pragma unroll
-          for (int e = 0; e < 16; e++) out[o][e] = out[o][e] * alpha;
+      for (int o = 0; o < OT; o++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) out[o][e] = out[o][e] * alpha;
+    }
+#pragma unroll
+    for (int u = 0; u < SUBS; u++) {
+      float add = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        s[u][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e], a.c2, mc));
+        add = add + s[u][e];
       }
-#pragma unroll
-      for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.c2, mc));
-      float add = s[0];
-#pragma unroll
-      for (int e = 1; e < 16; e++) add = add + s[e];
       sum = sum + add;
       Weights<EL> p;
-      p.set(s);
-      add_weighted_rows<EL, DP, T::PITCH>(out, stage + T::SIZE + r0 * T::PITCH, p);
+      p.set(s[u]);
+      RowElements<T, EL, OT> next;
+      if (u + 1 < SUBS) next.load(rows + T::SIZE + (u + 1) * 32 * T::ROW);
+      v.add(out, p);
+      if (u + 1 < SUBS) v = next;
     }
   }
   if constexpr (KW == 2) {  // the odd wave of a pair hands over
