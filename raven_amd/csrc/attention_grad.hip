@@ -30,7 +30,7 @@ __device__ __forceinline__ float exponent_of(float lse) {
 
 // Blocks of four waves with 32 queries each.
 template <class EL, int DP>
-__global__ __launch_bounds__(256) void attention_grad_queries_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(EL::F32 && DP > 96 ? 1 : 2))) void attention_grad_queries_kernel(AttentionArgs a) {
   using S = typename EL::S;
   constexpr int KEYS = EL::F32 || DP > 64 ? 32 : 64, QUERIES = 128, OT = DP / 32;
   using T = Tile<EL, DP, KEYS, 4>;
@@ -61,10 +61,12 @@ __global__ __launch_bounds__(256) void attention_grad_queries_kernel(AttentionAr
     }
     __syncthreads();
   }
-  auto whole = [&](int t) { return (t + 1) * KEYS <= keys && a.k.direct && a.v.direct; };
-  auto fetch = [&](int t, uint32_t to) {
-    kt.fetch(K + (int64_t)t * KEYS * a.k.row, keys - t * KEYS, a.k, a.dim, to);
-    vt.fetch(V + (int64_t)t * KEYS * a.v.row, keys - t * KEYS, a.v, a.dim, to + T::SIZE);
+  const bool direct = a.k.direct && a.v.direct;
+  auto fetch = [&](int t, uint32_t to) {  // tile by tile
+    kt.fetch(K, keys - t * KEYS, a.k, a.dim, to);
+    vt.fetch(V, keys - t * KEYS, a.v, a.dim, to + T::SIZE);
+    K += KEYS * a.k.row;
+    V += KEYS * a.v.row;
   };
   if (steps > 0) fetch(0, lds);
   if (steps > 1) fetch(1, lds + STAGE);
@@ -85,19 +87,22 @@ __global__ __launch_bounds__(256) void attention_grad_queries_kernel(AttentionAr
   for (int t = 0; t < OT; t++)
 #pragma unroll
     for (int e = 0; e < 16; e++) dq[t][e] = 0.0f;
+  Places<T, EL> places;
+  places.begin();
   uint32_t stage = lds, ahead = lds + 2 * STAGE;
   for (int t = 0; t < steps; t++) {
     // this tile has come, and the stage that is filled next has been used
-    if (t > 0 && t + 1 < steps && whole(t + 1)) meet<2 * T::LPW>();
+    if (t > 0 && (t + 2) * KEYS <= keys && t + 1 < steps && direct) meet<2 * T::LPW>();
     else meet<0>();
     if (t + 2 < steps) fetch(t + 2, ahead);
-    const uint32_t rows = stage;
+    const uint32_t now = stage;
     stage = stage == lds + 2 * STAGE ? lds : stage + STAGE;
     ahead = ahead == lds + 2 * STAGE ? lds : ahead + STAGE;
-    auto products = [&](int r0, f32x16 &p, f32x16 &ds) {
+    if (a.causal && t * KEYS > q0 + 31 + a.shift) continue;  // nothing of it is seen
+    const Places<T, EL> here = places.in(now);
+    auto begin = [&](f32x16 &p, f32x16 &ds) {
 #pragma unroll
       for (int e = 0; e < 16; e++) p[e] = 0.0f, ds[e] = -delta;
-      two_scores<T>(p, q, ds, g, rows + r0 * T::ROW);
     };
     auto differences = [&](int r0, const f32x16 &p, f32x16 &ds) {
 #pragma unroll
@@ -108,20 +113,21 @@ __global__ __launch_bounds__(256) void attention_grad_queries_kernel(AttentionAr
 #pragma unroll
       for (int e = 0; e < 16; e++) ds[e] = (see >> e) & 1 ? ds[e] : 0.0f;
     };
-    if (a.causal && t * KEYS > q0 + 31 + a.shift) continue;  // nothing of it is seen
     f32x16 p, ds;
     Weights<EL> w;
     RowElements<T, EL, OT> k;  // (on their way during the exponentials; those of heads of 128 would be more registers than there are)
-    products(0, p, ds);
-    if constexpr (DP <= 96) k.load(rows);
+    begin(p, ds);
+    two_scores<T, 0>(p, q, ds, g, here);
+    if constexpr (DP <= 96) k.template load<0>(here);
     if constexpr (!EL::F32) in_order();
     differences(0, p, ds);
-    if constexpr (DP > 96) k.load(rows);
+    if constexpr (DP > 96) k.template load<0>(here);
     w.set(ds);
     if constexpr (KEYS == 64) {
       k.add(dq, w);
-      products(32, p, ds);
-      k.load(rows + 32 * T::ROW);
+      begin(p, ds);
+      two_scores<T, 32 * T::ROW>(p, q, ds, g, here);
+      k.template load<32 * T::ROW>(here);
       in_order();
       differences(32, p, ds);
       w.set(ds);
@@ -133,14 +139,12 @@ __global__ __launch_bounds__(256) void attention_grad_queries_kernel(AttentionAr
 
 // Which of queries i0 + (e / 4) * 8 + g * 4 + e % 4 see key kj, bit e of the result.
 __device__ __forceinline__ uint32_t queries_seeing(const AttentionArgs &a, const uint8_t *mask, int kj, int i0) {
-  const int g = (threadIdx.x >> 5) & 1, first = i0 + g * 4, from = a.causal ? kj - a.shift - first : 0;
-  uint32_t seeing = 0;
-#pragma unroll
-  for (int e = 0; e < 16; e++) seeing |= (uint32_t)(!a.causal || (e >> 2) * 8 + (e & 3) >= from) << e;
+  const int g = (threadIdx.x >> 5) & 1, first = i0 + g * 4;
+  const uint32_t seeing = a.causal ? rows_from(kj - a.shift - first) : 0xffffu;
   if (!mask) return seeing;
   const uint8_t *m = mask + (int64_t)(kj < a.sk ? kj : a.sk - 1) * a.mask_col;
   uint32_t kept = 0;
-#pragma unroll
+#pragma unroll 4
   for (int e = 0; e < 16; e++) {
     const int i = first + (e >> 2) * 8 + (e & 3);
     kept |= (uint32_t)(m[(int64_t)(i < a.sq ? i : a.sq - 1) * a.mask.row] != 0) << e;
@@ -184,12 +188,12 @@ struct KeysWalk {
   }
 };
 
-// A value of each of 32 rows, as the scores lie.
-__device__ __forceinline__ void row_values(uint32_t values, f32x16 &x) {
-  const uint32_t at = values + ((threadIdx.x >> 5) & 1) * 16;
+// A value of each of 32 rows, as the scores lie; `half`: the values' place, and 16 more in the wave's second half.
+template <int OFFSET>
+__device__ __forceinline__ void row_values(uint32_t half, f32x16 &x) {
 #pragma unroll
   for (int e = 0; e < 16; e += 4) {
-    const gemm_tile::f32x4 v = *at_lds<const lds_f32x4>(at + e * 8);
+    const gemm_tile::f32x4 v = *at_lds<const lds_f32x4>(half + (uint32_t)(e * 8 + OFFSET));
 #pragma unroll
     for (int j = 0; j < 4; j++) x[e + j] = v[j];
   }
@@ -239,17 +243,27 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
   }
   const bool direct = a.q.direct && a.g.direct;
   int at = w.at, head = w.head;  // of the step that is worked on (the walk's are of the one that is fetched)
+  const typename EL::S *q_next, *g_next;
+  const float *values_next;
+  auto find = [&]() {  // the walk's place, where it is not behind the last one
+    const int64_t i0 = (int64_t)w.at * QUERIES;
+    q_next = rows_of<EL>(a.q, w.b, w.head) + i0 * a.q.row;
+    g_next = rows_of<EL>(a.g, w.b, w.head) + i0 * a.g.row;
+    values_next = a.rows + (((int64_t)w.b * a.heads + w.head) * a.rows_pitch + i0 + wave * 32) * 2;
+  };
   // The walk's step, and on; whether all of it is on its way past the registers.
   auto fetch = [&](uint32_t to) {
-    const int64_t i0 = (int64_t)w.at * QUERIES;
     const int left = a.sq - w.at * QUERIES;
-    qt.fetch(rows_of<EL>(a.q, w.b, w.head) + i0 * a.q.row, left, a.q, a.dim, to);
-    gt.fetch(rows_of<EL>(a.g, w.b, w.head) + i0 * a.g.row, left, a.g, a.dim, to + T::SIZE);
-    if (wave < QUERIES / 32)
-      load_to_lds4(a.rows + (((int64_t)w.b * a.heads + w.head) * a.rows_pitch + i0 + wave * 32) * 2, (threadIdx.x & 63) * 4, to + VALUES + wave * 256);
-    w.next();
+    qt.fetch(q_next, left, a.q, a.dim, to);
+    gt.fetch(g_next, left, a.g, a.dim, to + T::SIZE);
+    if (wave < QUERIES / 32) load_to_lds4(values_next, (threadIdx.x & 63) * 4, to + VALUES + wave * 256);
+    q_next += QUERIES * a.q.row;
+    g_next += QUERIES * a.g.row;
+    values_next += QUERIES * 2;
+    if (w.next()) find();
     return direct && left >= QUERIES;
   };
+  if (w.steps > 0) find();
   bool whole = false;  // of the step after the one that is worked on
   if (w.steps > 0) fetch(lds);
   if (w.steps > 1) whole = fetch(lds + STAGE);
@@ -261,6 +275,9 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
   for (int t = 0; t < OT; t++)
 #pragma unroll
     for (int e = 0; e < 16; e++) dk[t][e] = dv[t][e] = 0.0f;
+  Places<T, EL> places;
+  places.begin();
+  const uint32_t half16 = ((threadIdx.x >> 5) & 1) * 16;
   uint32_t stage = lds, ahead = lds + 2 * STAGE;
   for (int t = 0; t < w.steps; t++) {
     // this tile has come, and the stage that is filled next has been used
@@ -269,20 +286,16 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
     else meet<2 * T::LPW>();
     whole = false;
     if (t + 2 < w.steps) whole = fetch(ahead);
-    const uint32_t rows = stage;
+    const uint32_t now = stage;
     stage = stage == lds + 2 * STAGE ? lds : stage + STAGE;
     ahead = ahead == lds + 2 * STAGE ? lds : ahead + STAGE;
     const int i0 = at * QUERIES, head_now = head;
     if (++at == w.tiles) at = w.before, head++;
-    auto products = [&](int r0, f32x16 &p, f32x16 &ds) {
-#pragma unroll
-      for (int e = 0; e < 16; e++) p[e] = 0.0f;
-      row_values(rows + VALUES + r0 * 8 + 128, ds);
-      two_scores<T>(p, k, ds, v, rows + r0 * T::ROW);
-    };
-    auto differences = [&](int r0, f32x16 &p, f32x16 &ds) {
-      f32x16 l;
-      row_values(rows + VALUES + r0 * 8, l);
+    if (k0 >= w.keys || (a.causal && k0 > i0 + QUERIES - 1 + a.shift)) continue;  // nothing of the tile sees these keys
+    const Places<T, EL> here = places.in(now);
+    uint32_t values = now + half16;
+    asm("" : "+v"(values));
+    auto differences = [&](int r0, const f32x16 &l, f32x16 &p, f32x16 &ds) {
 #pragma unroll
       for (int e = 0; e < 16; e++) {
         p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[e], a.c2, l[e]));
@@ -298,25 +311,32 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
         ds[e] = keep ? ds[e] : 0.0f;
       }
     };
-    if (k0 >= w.keys || (a.causal && k0 > i0 + QUERIES - 1 + a.shift)) continue;  // nothing of the tile sees these keys
-    f32x16 p, ds;
+    f32x16 p, ds, l;
     Weights<EL> pw, dsw;
     RowElements<T, EL, OT> g, q;  // (on their way during the exponentials)
-    products(0, p, ds);
-    g.load(rows + T::SIZE);
-    q.load(rows);
+#pragma unroll
+    for (int e = 0; e < 16; e++) p[e] = 0.0f;
+    row_values<VALUES + 128>(values, ds);
+    two_scores<T, 0>(p, k, ds, v, here);
+    row_values<VALUES>(values, l);
+    g.template load<T::SIZE>(here);
+    q.template load<0>(here);
     if constexpr (!EL::F32) in_order();
-    differences(0, p, ds);
+    differences(0, l, p, ds);
     pw.set(p);
     dsw.set(ds);
     if constexpr (QUERIES == 64) {
       g.add(dv, pw);
       q.add(dk, dsw);
-      products(32, p, ds);
-      g.load(rows + T::SIZE + 32 * T::ROW);
-      q.load(rows + 32 * T::ROW);
+#pragma unroll
+      for (int e = 0; e < 16; e++) p[e] = 0.0f;
+      row_values<VALUES + 256 + 128>(values, ds);
+      two_scores<T, 32 * T::ROW>(p, k, ds, v, here);
+      row_values<VALUES + 256>(values, l);
+      g.template load<T::SIZE + 32 * T::ROW>(here);
+      q.template load<32 * T::ROW>(here);
       in_order();
-      differences(32, p, ds);
+      differences(32, l, p, ds);
       pw.set(p);
       dsw.set(ds);
     }
@@ -353,14 +373,23 @@ __global__ __launch_bounds__(512) void attention_grad_wide_keys_kernel(Attention
     __syncthreads();
   }
   int at = w.at, head = w.head;  // of the step that this wave works on (the walk's are of the one that is fetched)
-  auto fetch = [&](uint32_t to) {
+  const typename EL::S *next;
+  const float *values_next;
+  auto find = [&]() {  // the walk's place, where it is not behind the last one
     const int64_t i0 = (int64_t)w.at * QUERIES;
+    next = rows_of<EL>(brought, w.b, w.head) + i0 * brought.row;
+    values_next = a.rows + (((int64_t)w.b * a.heads + w.head) * a.rows_pitch + i0) * 2;
+  };
+  auto fetch = [&](uint32_t to) {
     const int left = a.sq - w.at * QUERIES;
-    tile.fetch(rows_of<EL>(brought, w.b, w.head) + i0 * brought.row, left, brought, a.dim, to + (second ? T::SIZE : 0));
-    if (wave == 0) load_to_lds4(a.rows + (((int64_t)w.b * a.heads + w.head) * a.rows_pitch + i0) * 2, lane * 4, to + VALUES);
-    w.next();
+    tile.fetch(next, left, brought, a.dim, to + (second ? T::SIZE : 0));
+    if (wave == 0) load_to_lds4(values_next, lane * 4, to + VALUES);
+    next += QUERIES * brought.row;
+    values_next += QUERIES * 2;
+    if (w.next()) find();
     return brought.direct && left >= QUERIES;
   };
+  if (w.steps > 0) find();
   bool whole = false;  // what is on its way for the step after this one
   if (w.steps > 0) fetch(lds);
   if (AHEAD == 2 && w.steps > 1) whole = fetch(lds + STAGE);
@@ -371,6 +400,9 @@ __global__ __launch_bounds__(512) void attention_grad_wide_keys_kernel(Attention
   for (int t = 0; t < OT; t++)
 #pragma unroll
     for (int e = 0; e < 16; e++) acc[t][e] = 0.0f;
+  Places<T, EL> places;
+  places.begin();
+  const uint32_t half16 = ((threadIdx.x >> 5) & 1) * 16;
   uint32_t stage = lds, ahead = lds + AHEAD * STAGE;
   for (int t = 0; w.steps > 0 && t <= w.steps; t++) {
     // tile t has come, p of the tile before it too, and what is filled next has been used
@@ -384,30 +416,33 @@ __global__ __launch_bounds__(512) void attention_grad_wide_keys_kernel(Attention
     }
     ahead = ahead == lds + (RING - 1) * STAGE ? lds : ahead + STAGE;
     if (second ? t == 0 : t == w.steps) continue;
-    const uint32_t rows = stage;
+    const uint32_t now = stage;
     stage = stage == lds + (RING - 1) * STAGE ? lds : stage + STAGE;
     const int i0 = at * QUERIES, head_now = head;
     if (++at == w.tiles) at = w.before, head++;
     if (k0 >= w.keys || (a.causal && k0 > i0 + 31 + a.shift)) continue;  // nothing of the tile sees these keys
     float(*between)[64][4] = over[(second ? t - 1 : t) & 1][pair];
     const bool inner = !a.mask.base && !(a.causal && k0 + 31 > i0 + a.shift);
+    const Places<T, EL> here = places.in(now + (second ? T::SIZE : 0)), other = places.in(now + (second ? 0 : T::SIZE));
+    uint32_t values = now + half16;
+    asm("" : "+v"(values));
     f32x16 x;
     if (second) {
-      row_values(rows + VALUES + 128, x);
+      row_values<VALUES + 128>(values, x);
     } else {
 #pragma unroll
       for (int e = 0; e < 16; e++) x[e] = 0.0f;
     }
     RowVectors<T, EL, DP> vectors;
-    vectors.load(rows + (second ? T::SIZE : 0));
+    vectors.template load<0>(here);
     if constexpr (!EL::F32) in_order();
     vectors.scores(x, own);
     RowElements<T, EL, OT> elements;  // (on their way during the exponentials)
-    elements.load(rows + (second ? 0 : T::SIZE));
+    elements.template load<0>(other);
     if constexpr (!EL::F32) in_order();
     if (!second) {
       f32x16 l;
-      row_values(rows + VALUES, l);
+      row_values<VALUES>(values, l);
 #pragma unroll
       for (int e = 0; e < 16; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.c2, l[e]));
       if (!inner) {

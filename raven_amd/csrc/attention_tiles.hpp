@@ -228,20 +228,56 @@ struct Column {
 // each use, and each matrix instruction then waits out a read's latency: all of a product's reads are issued first.
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
-// Elements of 32 rows as scores() takes them, steps FROM to TO of the dim: row lane % 32. `rows`: where the first row lies, a
-// multiple of 32 of a tile.
+// Where a lane reads in a tile: its row's vectors, which a scores() takes, and the elements that an add() takes. The places of a
+// tile's units differ by turns, which stay inside groups of four, eight or sixteen: a few addresses, made once for a stage,
+// and constants beside them.
+template <class T, class EL>
+struct Places {
+  static constexpr int GROUP = T::UNITS % 16 == 0 ? 16 : T::UNITS % 8 == 0 ? 8 : 4;
+  static constexpr int VECTORS = GROUP / 2, ELEMENTS = EL::F32 ? (GROUP < 8 ? GROUP : 8) : GROUP / 2;
+  uint32_t vector[VECTORS], element[ELEMENTS];
+  __device__ __forceinline__ void begin() {
+    const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < VECTORS; i++) vector[i] = (uint32_t)(r * T::ROW + (g ^ T::turn(r) ^ (2 * i)) * 16);
+    if constexpr (EL::F32) {
+      // row 8 (e / 4) + 4 g + e % 4, unit 8 t + c / 4: turn(row) = turn(4 g) ^ turn(8 (e / 4) + e % 4)
+#pragma unroll
+      for (int i = 0; i < ELEMENTS; i++) element[i] = (uint32_t)(4 * g * T::ROW + ((r >> 2) ^ T::turn(4 * g) ^ i) * 16 + (lane & 3) * 4);
+    } else {
+      // the transposing load: sixteen lanes read 4 rows of 16 elements, lane i eight bytes of row i / 4, and get column i's four
+      const int j = (lane & 15) >> 2, b = (lane >> 4) & 1, c = (lane & 3) >> 1;
+#pragma unroll
+      for (int i = 0; i < ELEMENTS; i++)  // unit 2 b + c, and those that 4 t and 8 rows on (2) turn it to
+        element[i] = (uint32_t)((4 * g + j) * T::ROW + ((2 * b + c) ^ T::turn(4 * g + j) ^ (2 * i)) * 16 + (lane & 1) * 8);
+    }
+  }
+  __device__ __forceinline__ Places in(uint32_t stage) const {
+    Places p;
+#pragma unroll
+    for (int i = 0; i < VECTORS; i++) {
+      p.vector[i] = vector[i] + stage;
+      asm("" : "+v"(p.vector[i]));  // (what is added to it is the instruction's offset)
+    }
+#pragma unroll
+    for (int i = 0; i < ELEMENTS; i++) {
+      p.element[i] = element[i] + stage;
+      asm("" : "+v"(p.element[i]));
+    }
+    return p;
+  }
+};
+
+// Elements of 32 rows as scores() takes them, steps FROM to TO of the dim: row lane % 32. OFFSET: of the first row in a stage, a
+// multiple of 32 of a tile's.
 template <class T, class EL, int DP, int FROM = 0, int TO = DP / (2 * EL::VE)>
 struct RowVectors {
   V16 f[TO - FROM];
-  __device__ __forceinline__ void load(uint32_t rows) {
-    const int r = threadIdx.x & 31, g = (threadIdx.x >> 5) & 1, x = g ^ T::turn(r);
-    const uint32_t at = rows + (uint32_t)(r * T::ROW);
+  template <int OFFSET>
+  __device__ __forceinline__ void load(const Places<T, EL> &p) {
+    constexpr int GROUP = Places<T, EL>::GROUP;
 #pragma unroll
-    for (int s = FROM; s < TO; s++) {
-      // (turns stay inside groups of four, eight or sixteen units: what lies above is a constant)
-      constexpr int GROUP = T::UNITS % 16 == 0 ? 16 : T::UNITS % 8 == 0 ? 8 : 4;
-      f[s - FROM] = *at_lds<const lds_V16>(at + (uint32_t)(x ^ ((2 * s) % GROUP)) * 16 + (uint32_t)((2 * s) / GROUP * GROUP * 16));
-    }
+    for (int s = FROM; s < TO; s++) f[s - FROM] = *at_lds<const lds_V16>(p.vector[(2 * s) % GROUP / 2] + (uint32_t)((2 * s) / GROUP * GROUP * 16 + OFFSET));
   }
   // acc[e] += row (e / 4) * 8 + g * 4 + e % 4 . this lane's column
   __device__ __forceinline__ void scores(f32x16 &acc, const Column<EL, DP> &column) const {
@@ -249,13 +285,6 @@ struct RowVectors {
     for (int s = FROM; s < TO; s++) gemm_tile::mfma_step<EL>(acc, f[s - FROM], column.f[s]);
   }
 };
-// The same in one, for float32, whose instructions take longer than a read.
-template <class T, class EL, int DP>
-__device__ __forceinline__ void rows_by_columns(f32x16 &acc, uint32_t rows, const Column<EL, DP> &column) {
-  RowVectors<T, EL, DP> v;
-  v.load(rows);
-  v.scores(acc, column);
-}
 
 // Weights of 32 rows and this lane's column, as the second product takes them: rounded to the operands' type, which its
 // matrix instruction wants (float32 as they are).
@@ -274,25 +303,21 @@ struct Weights<gemm_tile::ElF32> {
 };
 
 // Elements of 32 rows as the second product takes them: acc[t][e] += sum over the rows of element 32 t + (e / 4) * 8 + g * 4 +
-// e % 4 of a row times its weight for this lane's column. 16-bit elements are read ahead.
+// e % 4 of a row times its weight for this lane's column. 16-bit elements are read ahead; float32's instructions take longer than a read.
 template <class T, class EL, int OT>
 struct RowElements {
   V16 f[2 * OT];
-  __device__ __forceinline__ void load(uint32_t rows) {
-    // the transposing load: sixteen lanes read 4 rows of 16 elements, lane i eight bytes of row i / 4, and get column i's four
-    const int lane = threadIdx.x & 63, g = lane >> 5, j = (lane & 15) >> 2, b = (lane >> 4) & 1, c = (lane & 3) >> 1;
-    const uint32_t at = rows + (uint32_t)((4 * g + j) * T::ROW + (lane & 1) * 8);
-    const int x = (2 * b + c) ^ T::turn(4 * g + j);  // of unit 2 b + c; those of 8 rows on differ by 2
+  template <int OFFSET>
+  __device__ __forceinline__ void load(const Places<T, EL> &p) {
+    constexpr int GROUP = Places<T, EL>::GROUP;
 #pragma unroll
     for (int s = 0; s < 2; s++)
 #pragma unroll
       for (int t = 0; t < OT; t++) {
-        constexpr int GROUP = T::UNITS % 16 == 0 ? 16 : T::UNITS % 8 == 0 ? 8 : 4;
-        const uint32_t src = at + (uint32_t)(x ^ ((4 * t) % GROUP)) * 16 + (uint32_t)((4 * t) / GROUP * GROUP * 16 + 16 * s * T::ROW);
-        const uint32_t src8 = at + (uint32_t)(x ^ 2 ^ ((4 * t) % GROUP)) * 16 + (uint32_t)((4 * t) / GROUP * GROUP * 16 + (16 * s + 8) * T::ROW);
+        const int i = (4 * t) % GROUP / 2, at = (4 * t) / GROUP * GROUP * 16 + 16 * s * T::ROW + OFFSET;
         typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
-        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(at_lds<lds_s16x4>(src)));
-        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(at_lds<lds_s16x4>(src8)));
+        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(at_lds<lds_s16x4>(p.element[i] + (uint32_t)at)));
+        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(at_lds<lds_s16x4>(p.element[i ^ 1] + (uint32_t)(at + 8 * T::ROW))));
         f[s * OT + t] = V16{lo[0], lo[1], hi[0], hi[1]};
       }
   }
@@ -306,20 +331,17 @@ struct RowElements {
 };
 template <class T, int OT>
 struct RowElements<T, gemm_tile::ElF32, OT> {
-  uint32_t rows;
-  __device__ __forceinline__ void load(uint32_t at) { rows = at; }
+  const Places<T, gemm_tile::ElF32> *places;
+  uint32_t offset;
+  template <int OFFSET>
+  __device__ __forceinline__ void load(const Places<T, gemm_tile::ElF32> &p) { places = &p, offset = OFFSET; }
   __device__ __forceinline__ void add(f32x16 (&acc)[OT], const Weights<gemm_tile::ElF32> &p) const {
-    // row 8 (e / 4) + 4 g + e % 4, unit 8 t + c / 4: turn(row) = turn(4 g) ^ turn(8 (e / 4) + e % 4)
-    const int lane = threadIdx.x & 63, g = lane >> 5;
-    const uint32_t at = rows + (uint32_t)(4 * g * T::ROW + (lane & 3) * 4);
-    const int x = ((lane & 31) >> 2) ^ T::turn(4 * g);
 #pragma unroll
     for (int e = 0; e < 16; e++) {
       const int r = (e >> 2) * 8 + (e & 3), turned = T::turn(r);
 #pragma unroll
       for (int t = 0; t < OT; t++) {
-        const int unit = (8 * t) ^ (turned & ~7);
-        const float v = *at_lds<const lds_float>(at + (uint32_t)(x ^ (turned & 7)) * 16 + (uint32_t)(unit * 16 + r * T::ROW));
+        const float v = *at_lds<const lds_float>(places->element[turned & 7] + (uint32_t)(((8 * t) ^ (turned & ~7)) * 16 + r * T::ROW) + offset);
         acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p.w[e], acc[t], 0, 0, 0);
       }
     }
@@ -328,29 +350,29 @@ struct RowElements<T, gemm_tile::ElF32, OT> {
 
 // Two products of 32 rows each, of tiles that lie side by side: a += rows . ca, b += rows T::SIZE further on . cb. Heads of more
 // than 64 in two halves, which is as many registers as a product of one.
-template <class T, class EL, int DP>
-__device__ __forceinline__ void two_scores(f32x16 &a, const Column<EL, DP> &ca, f32x16 &b, const Column<EL, DP> &cb, uint32_t rows) {
-  if constexpr (EL::F32) {
-    rows_by_columns<T>(a, rows, ca);
-    rows_by_columns<T>(b, rows + T::SIZE, cb);
-  } else if constexpr (DP <= 64) {
+template <class T, int OFFSET, class EL, int DP>
+__device__ __forceinline__ void two_scores(f32x16 &a, const Column<EL, DP> &ca, f32x16 &b, const Column<EL, DP> &cb, const Places<T, EL> &p) {
+  if constexpr (EL::F32 || DP <= 64) {
     RowVectors<T, EL, DP> x, y;
-    x.load(rows);
-    y.load(rows + T::SIZE);
-    in_order();
-    x.scores(a, ca);
+    x.template load<OFFSET>(p);
+    if constexpr (EL::F32) x.scores(a, ca);
+    y.template load<OFFSET + T::SIZE>(p);
+    if constexpr (!EL::F32) {
+      in_order();
+      x.scores(a, ca);
+    }
     y.scores(b, cb);
   } else {
     constexpr int STEPS = DP / (2 * EL::VE), HALF = STEPS / 2;
     RowVectors<T, EL, DP, 0, HALF> x, y;
     RowVectors<T, EL, DP, HALF, STEPS> z, u;
-    x.load(rows);
-    y.load(rows + T::SIZE);
+    x.template load<OFFSET>(p);
+    y.template load<OFFSET + T::SIZE>(p);
     in_order();
     x.scores(a, ca);
-    z.load(rows);
+    z.template load<OFFSET>(p);
     y.scores(b, cb);
-    u.load(rows + T::SIZE);
+    u.template load<OFFSET + T::SIZE>(p);
     in_order();
     z.scores(a, ca);
     u.scores(b, cb);
@@ -385,13 +407,17 @@ __device__ __forceinline__ void store_column(typename EL::S *row, const f32x16 (
     }
 }
 
+// Bits e of the 16 elements a lane has of 32 rows for which row (e / 4) * 8 + e % 4 is at least `from` (of the lane's own, less 4 g).
+__device__ __forceinline__ uint32_t rows_from(int from) {
+  const int q = from >> 3, r = from & 7;  // the first `from` rows: 4 bits for every eight, those of the last
+  const uint32_t below = from <= 0 ? 0u : from >= 32 ? 0xffffu : ((1u << (4 * q)) - 1u) | ((1u << (r < 4 ? r : 4)) - 1u) << (4 * q);
+  return 0xffffu & ~below;
+}
 // Which of keys j0 + (e / 4) * 8 + g * 4 + e % 4 query qi sees, bit e of the result.
 __device__ __forceinline__ uint32_t keys_seen(const AttentionArgs &a, const uint8_t *mask, int qi, int j0, int keys) {
   const int g = (threadIdx.x >> 5) & 1, first = j0 + g * 4;
-  const int end = a.causal && qi + a.shift < keys - 1 ? qi + a.shift : keys - 1, last = end - first;
-  uint32_t seen = 0;
-#pragma unroll
-  for (int e = 0; e < 16; e++) seen |= (uint32_t)((e >> 2) * 8 + (e & 3) <= last) << e;
+  const int end = a.causal && qi + a.shift < keys - 1 ? qi + a.shift : keys - 1;
+  const uint32_t seen = ~rows_from(end + 1 - first) & 0xffffu;
   if (!mask) return seen;
   const uint8_t *m = mask + (int64_t)(qi < a.sq ? qi : a.sq - 1) * a.mask.row;
   uint32_t kept = 0;
@@ -404,7 +430,7 @@ __device__ __forceinline__ uint32_t keys_seen(const AttentionArgs &a, const uint
       for (int j = 0; j < 4; j++) kept |= (uint32_t)(((four >> (8 * j)) & 0xffu) != 0) << (e + j);
     }
   } else {
-#pragma unroll
+#pragma unroll 4
     for (int e = 0; e < 16; e++) {
       const int j = first + (e >> 2) * 8 + (e & 3);
       kept |= (uint32_t)(m[(int64_t)(j < a.sk ? j : a.sk - 1) * a.mask_col] != 0) << e;

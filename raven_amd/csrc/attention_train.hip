@@ -47,10 +47,12 @@ __global__ __launch_bounds__(256) void attention_train_kernel(AttentionArgs a) {
     }
     __syncthreads();
   }
-  auto whole = [&](int t) { return (t + 1) * KEYS <= keys && a.k.direct && a.v.direct; };
-  auto fetch = [&](int t, uint32_t to) {
-    kt.fetch(K + (int64_t)t * KEYS * a.k.row, keys - t * KEYS, a.k, a.dim, to);
-    vt.fetch(V + (int64_t)t * KEYS * a.v.row, keys - t * KEYS, a.v, a.dim, to + T::SIZE);
+  const bool direct = a.k.direct && a.v.direct;
+  auto fetch = [&](int t, uint32_t to) {  // tile by tile
+    kt.fetch(K, keys - t * KEYS, a.k, a.dim, to);
+    vt.fetch(V, keys - t * KEYS, a.v, a.dim, to + T::SIZE);
+    K += KEYS * a.k.row;
+    V += KEYS * a.v.row;
   };
   for (int t = 0; t < AHEAD && t < steps; t++) fetch(t, lds + t * STAGE);
   Column<EL, DP> q;
@@ -63,29 +65,33 @@ __global__ __launch_bounds__(256) void attention_train_kernel(AttentionArgs a) {
     for (int e = 0; e < 16; e++) out[t][e] = 0.0f;
   float m = -INF, sum = 0.0f;
   float mc = 0.0f, lim = INF;  // -c m, and +inf before the first score, where exponentials take 0
+  Places<T, EL> places;
+  places.begin();
   uint32_t stage = lds, ahead = lds + AHEAD * STAGE;
   for (int t = 0; t < steps; t++) {
     // this tile has come, and the stage that is filled next has been used
-    if (AHEAD == 2 && t > 0 && t + 1 < steps && whole(t + 1)) meet<2 * T::LPW>();
+    if (AHEAD == 2 && t > 0 && t + 1 < steps && (t + 2) * KEYS <= keys && direct) meet<2 * T::LPW>();
     else meet<0>();
     if (t + AHEAD < steps) fetch(t + AHEAD, ahead);
-    const uint32_t rows = stage + (uint32_t)(part * 32 * T::ROW);
+    const Places<T, EL> here = places.in(stage + (uint32_t)(part * 32 * T::ROW));
     stage = stage == lds + (RING - 1) * STAGE ? lds : stage + STAGE;
     ahead = ahead == lds + (RING - 1) * STAGE ? lds : ahead + STAGE;
     const int j0 = t * KEYS + part * 32;
     if (j0 >= keys || (a.causal && j0 > q0 + 31 + a.shift)) continue;  // nothing of it is seen
     f32x16 s[SUBS];
+    RowVectors<T, EL, DP> k[SUBS];
+    k[0].template load<0>(here);
+    if constexpr (SUBS == 2) k[1].template load<32 * T::ROW>(here);
+    if constexpr (!EL::F32) in_order();
 #pragma unroll
     for (int u = 0; u < SUBS; u++) {
-      RowVectors<T, EL, DP> k;
-      k.load(rows + u * 32 * T::ROW);
-      if constexpr (!EL::F32) in_order();
 #pragma unroll
       for (int e = 0; e < 16; e++) s[u][e] = 0.0f;
-      k.scores(s[u], q);
+      k[u].scores(s[u], q);
     }
-    RowElements<T, EL, OT> v;  // (on their way during the exponentials)
-    v.load(rows + T::SIZE);
+    RowElements<T, EL, OT> v[SUBS];  // (on their way during the exponentials)
+    v[0].template load<T::SIZE>(here);
+    if constexpr (SUBS == 2) v[1].template load<T::SIZE + 32 * T::ROW>(here);
     if constexpr (!EL::F32) in_order();
     if (mask || j0 + SUBS * 32 > keys || (a.causal && j0 + SUBS * 32 - 1 > q0 + a.shift)) {
 #pragma unroll
@@ -125,10 +131,7 @@ __global__ __launch_bounds__(256) void attention_train_kernel(AttentionArgs a) {
       sum = sum + add;
       Weights<EL> p;
       p.set(s[u]);
-      RowElements<T, EL, OT> next;
-      if (u + 1 < SUBS) next.load(rows + T::SIZE + (u + 1) * 32 * T::ROW);
-      v.add(out, p);
-      if (u + 1 < SUBS) v = next;
+      v[u].add(out, p);
     }
   }
   if constexpr (KW == 2) {  // the odd wave of a pair hands over
