@@ -28,21 +28,23 @@ __device__ __forceinline__ float exponent_of(float lse) {
   return lse == -INF ? -INF : __builtin_fmaf(-lse, LOG2E, LIFT<EL>);
 }
 
-// Blocks of four waves with 32 queries each.
-template <class EL, int DP>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(EL::F32 && DP > 96 ? 1 : 2))) void attention_grad_queries_kernel(AttentionArgs a) {
+// Blocks of four waves. KW = 1: each has 32 queries of 128. KW = 2: two share 32 queries, each takes every other 32 keys of a
+// tile, and their sums are added at the end: twice the blocks, where there are few.
+template <class EL, int DP, int KW>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((EL::F32 || KW == 2) && DP > (KW == 2 && EL::F32 ? 64 : 96) ? 1 : 2))) void attention_grad_queries_kernel(AttentionArgs a) {
   using S = typename EL::S;
-  constexpr int KEYS = EL::F32 || DP > 64 ? 32 : 64, QUERIES = 128, OT = DP / 32;
+  constexpr int KEYS = EL::F32 || DP > 64 ? 32 * KW : 64, SUBS = KEYS / 32 / KW, QUERIES = 128 / KW, OT = DP / 32;
   using T = Tile<EL, DP, KEYS, 4>;
-  constexpr int STAGE = 2 * T::SIZE, RING = 3;
+  constexpr int STAGE = 2 * T::SIZE, RING = 3 * STAGE <= 80 * 1024 ? 3 : 2, AHEAD = RING - 1;  // tiles on their way
   __shared__ __attribute__((aligned(1024))) unsigned char stages[RING * STAGE];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31;
+  const int pair = wave / KW, part = wave % KW;
   const uint32_t heads = (uint32_t)a.batch * (uint32_t)a.heads;
   const int tile = a.tiles - 1 - (int)(blockIdx.x / heads);
   const int bh = (int)(blockIdx.x % heads), b = bh / a.heads, h = bh % a.heads, hk = h / (a.heads / a.kv_heads);
   const int keys = keys_of(a, b);
-  const int q0 = tile * QUERIES + wave * 32, qi = q0 + c32;
+  const int q0 = tile * QUERIES + pair * 32, qi = q0 + c32;
   const bool there = qi < a.sq;
   const S *K = rows_of<EL>(a.k, b, hk), *V = rows_of<EL>(a.v, b, hk);
   const uint8_t *mask = a.mask.base ? reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)b * a.mask.batch + (int64_t)h * a.mask.head : nullptr;
@@ -68,8 +70,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(EL::F32 && 
     K += KEYS * a.k.row;
     V += KEYS * a.v.row;
   };
-  if (steps > 0) fetch(0, lds);
-  if (steps > 1) fetch(1, lds + STAGE);
+  for (int t = 0; t < AHEAD && t < steps; t++) fetch(t, lds + t * STAGE);
   Column<EL, DP> q, g;
   g.load(rows_of<EL>(a.g, b, h) + (int64_t)qi * a.g.row, there, a.dim);
   q.load(rows_of<EL>(a.out, b, h) + (int64_t)qi * a.out.row, there, a.dim);
@@ -78,7 +79,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(EL::F32 && 
   q.load(rows_of<EL>(a.q, b, h) + (int64_t)qi * a.q.row, there, a.dim);
   float power = -INF;
   if (there) power = exponent_of<EL>(reinterpret_cast<const float *>(a.lse.base)[(int64_t)b * a.lse.batch + (int64_t)h * a.lse.head + (int64_t)qi * a.lse.row]);
-  if (qi < a.rows_pitch) {  // for the second launch, 32 rows' powers and then their differences' starts; past the end -inf and 0
+  if (part == 0 && qi < a.rows_pitch) {  // for the second launch, 32 rows' powers and then their differences' starts; past the end -inf and 0
     float *to = a.rows + ((int64_t)bh * a.rows_pitch + q0) * 2;
     to[lane] = lane < 32 ? power : there ? -delta : 0.0f;
   }
@@ -89,17 +90,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(EL::F32 && 
     for (int e = 0; e < 16; e++) dq[t][e] = 0.0f;
   Places<T, EL> places;
   places.begin();
-  uint32_t stage = lds, ahead = lds + 2 * STAGE;
+  uint32_t stage = lds, ahead = lds + AHEAD * STAGE;
   for (int t = 0; t < steps; t++) {
     // this tile has come, and the stage that is filled next has been used
-    if (t > 0 && (t + 2) * KEYS <= keys && t + 1 < steps && direct) meet<2 * T::LPW>();
+    if (AHEAD == 2 && t > 0 && (t + 2) * KEYS <= keys && t + 1 < steps && direct) meet<2 * T::LPW>();
     else meet<0>();
-    if (t + 2 < steps) fetch(t + 2, ahead);
+    if (t + AHEAD < steps) fetch(t + AHEAD, ahead);
     const uint32_t now = stage;
-    stage = stage == lds + 2 * STAGE ? lds : stage + STAGE;
-    ahead = ahead == lds + 2 * STAGE ? lds : ahead + STAGE;
-    if (a.causal && t * KEYS > q0 + 31 + a.shift) continue;  // nothing of it is seen
-    const Places<T, EL> here = places.in(now);
+    stage = stage == lds + (RING - 1) * STAGE ? lds : stage + STAGE;
+    ahead = ahead == lds + (RING - 1) * STAGE ? lds : ahead + STAGE;
+    const int first = t * KEYS + part * 32;
+    if (first >= keys || (a.causal && first > q0 + 31 + a.shift)) continue;  // nothing of it is seen
+    const Places<T, EL> here = places.in(now + (uint32_t)(part * 32 * T::ROW));
     auto begin = [&](f32x16 &p, f32x16 &ds) {
 #pragma unroll
       for (int e = 0; e < 16; e++) p[e] = 0.0f, ds[e] = -delta;
@@ -107,7 +109,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(EL::F32 && 
     auto differences = [&](int r0, const f32x16 &p, f32x16 &ds) {
 #pragma unroll
       for (int e = 0; e < 16; e++) ds[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[e], a.c2, power)) * ds[e];
-      const int j0 = t * KEYS + r0;
+      const int j0 = first + r0;
       if (!mask && j0 + 32 <= keys && !(a.causal && j0 + 31 > q0 + a.shift)) return;
       const uint32_t see = keys_seen(a, mask, qi, j0, keys);
 #pragma unroll
@@ -117,22 +119,39 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(EL::F32 && 
     Weights<EL> w;
     RowElements<T, EL, OT> k;  // (on their way during the exponentials; those of heads of 128 would be more registers than there are)
     begin(p, ds);
-    two_scores<T, 0>(p, q, ds, g, here);
+    two_scores<T, 0>(p, q, ds, g, here, a.dim);
     if constexpr (DP <= 96) k.template load<0>(here);
     if constexpr (!EL::F32) in_order();
     differences(0, p, ds);
     if constexpr (DP > 96) k.template load<0>(here);
     w.set(ds);
-    if constexpr (KEYS == 64) {
+    if constexpr (SUBS == 2) {
       k.add(dq, w);
       begin(p, ds);
-      two_scores<T, 32 * T::ROW>(p, q, ds, g, here);
+      two_scores<T, 32 * T::ROW>(p, q, ds, g, here, a.dim);
       k.template load<32 * T::ROW>(here);
       in_order();
       differences(32, p, ds);
       w.set(ds);
     }
     k.add(dq, w);
+  }
+  if constexpr (KW == 2) {  // the odd wave of a pair hands over
+    static_assert(sizeof(float) * 2 * OT * 16 * 64 <= sizeof(stages), "sums of two waves fit the stages");
+    float(*over)[OT * 16][64] = reinterpret_cast<float(*)[OT * 16][64]>(stages);
+    __syncthreads();
+    if (part == 1) {
+#pragma unroll
+      for (int t = 0; t < OT; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) over[pair][t * 16 + e][lane] = dq[t][e];
+    }
+    __syncthreads();
+    if (part == 1) return;
+#pragma unroll
+    for (int t = 0; t < OT; t++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) dq[t][e] = dq[t][e] + over[pair][t * 16 + e][lane];
   }
   if (there) store_column<EL, DP>(const_cast<S *>(rows_of<EL>(a.dq, b, h)) + (int64_t)qi * a.dq.row, dq, a.scale * UNLIFT<EL>, a.dim);
 }
@@ -317,7 +336,7 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
 #pragma unroll
     for (int e = 0; e < 16; e++) p[e] = 0.0f;
     row_values<VALUES + 128>(values, ds);
-    two_scores<T, 0>(p, k, ds, v, here);
+    two_scores<T, 0>(p, k, ds, v, here, a.dim);
     row_values<VALUES>(values, l);
     g.template load<T::SIZE>(here);
     q.template load<0>(here);
@@ -331,7 +350,7 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
 #pragma unroll
       for (int e = 0; e < 16; e++) p[e] = 0.0f;
       row_values<VALUES + 256 + 128>(values, ds);
-      two_scores<T, 32 * T::ROW>(p, k, ds, v, here);
+      two_scores<T, 32 * T::ROW>(p, k, ds, v, here, a.dim);
       row_values<VALUES + 256>(values, l);
       g.template load<T::SIZE + 32 * T::ROW>(here);
       q.template load<32 * T::ROW>(here);
@@ -491,9 +510,16 @@ __global__ __launch_bounds__(256) void attention_grad_join_kernel(AttentionArgs 
 
 template <class EL, int DP>
 void launch(nxh_context *ctx, AttentionArgs a) {
+  const int units = ctx->compute_units > 0 ? ctx->compute_units : 256;
   if (a.sq > 0 && a.heads > 0) {
     a.tiles = (a.sq + 127) / 128;
-    hipLaunchKernelGGL((attention_grad_queries_kernel<EL, DP>), dim3((unsigned)(a.batch * a.heads * a.tiles)), dim3(256), 0, ctx->stream, a);
+    const int64_t blocks = (int64_t)a.batch * a.heads * a.tiles;
+    if (blocks < 2 * units) {
+      a.tiles = (a.sq + 63) / 64;
+      hipLaunchKernelGGL((attention_grad_queries_kernel<EL, DP, 2>), dim3((unsigned)(a.batch * a.heads * a.tiles)), dim3(256), 0, ctx->stream, a);
+    } else {
+      hipLaunchKernelGGL((attention_grad_queries_kernel<EL, DP, 1>), dim3((unsigned)blocks), dim3(256), 0, ctx->stream, a);
+    }
   }
   if (a.sk == 0) return;
   a.tiles = (a.sk + 127) / 128;

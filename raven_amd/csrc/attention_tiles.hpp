@@ -268,21 +268,21 @@ struct Places {
   }
 };
 
-// Elements of 32 rows as scores() takes them, steps FROM to TO of the dim: row lane % 32. OFFSET: of the first row in a stage, a
-// multiple of 32 of a tile's.
-template <class T, class EL, int DP, int FROM = 0, int TO = DP / (2 * EL::VE)>
+// Elements of 32 rows as scores() takes them: row lane % 32. OFFSET: of the first row in a stage, a multiple of 32 of a tile's.
+template <class T, class EL, int DP>
 struct RowVectors {
-  V16 f[TO - FROM];
+  static constexpr int STEPS = DP / (2 * EL::VE);
+  V16 f[STEPS];
   template <int OFFSET>
   __device__ __forceinline__ void load(const Places<T, EL> &p) {
     constexpr int GROUP = Places<T, EL>::GROUP;
 #pragma unroll
-    for (int s = FROM; s < TO; s++) f[s - FROM] = *at_lds<const lds_V16>(p.vector[(2 * s) % GROUP / 2] + (uint32_t)((2 * s) / GROUP * GROUP * 16 + OFFSET));
+    for (int s = 0; s < STEPS; s++) f[s] = *at_lds<const lds_V16>(p.vector[(2 * s) % GROUP / 2] + (uint32_t)((2 * s) / GROUP * GROUP * 16 + OFFSET));
   }
   // acc[e] += row (e / 4) * 8 + g * 4 + e % 4 . this lane's column
   __device__ __forceinline__ void scores(f32x16 &acc, const Column<EL, DP> &column) const {
 #pragma unroll
-    for (int s = FROM; s < TO; s++) gemm_tile::mfma_step<EL>(acc, f[s - FROM], column.f[s]);
+    for (int s = 0; s < STEPS; s++) gemm_tile::mfma_step<EL>(acc, f[s], column.f[s]);
   }
 };
 
@@ -336,46 +336,50 @@ struct RowElements<T, gemm_tile::ElF32, OT> {
   template <int OFFSET>
   __device__ __forceinline__ void load(const Places<T, gemm_tile::ElF32> &p) { places = &p, offset = OFFSET; }
   __device__ __forceinline__ void add(f32x16 (&acc)[OT], const Weights<gemm_tile::ElF32> &p) const {
-#pragma unroll
-    for (int e = 0; e < 16; e++) {
+    float f[2][OT];  // a row's elements are read while the row before is multiplied
+    auto load = [&](int e) {
       const int r = (e >> 2) * 8 + (e & 3), turned = T::turn(r);
 #pragma unroll
-      for (int t = 0; t < OT; t++) {
-        const float v = *at_lds<const lds_float>(places->element[turned & 7] + (uint32_t)(((8 * t) ^ (turned & ~7)) * 16 + r * T::ROW) + offset);
-        acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p.w[e], acc[t], 0, 0, 0);
-      }
+      for (int t = 0; t < OT; t++)
+        f[e & 1][t] = *at_lds<const lds_float>(places->element[turned & 7] + (uint32_t)(((8 * t) ^ (turned & ~7)) * 16 + r * T::ROW) + offset);
+    };
+    load(0);
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      in_order();
+      if (e < 15) load(e + 1);
+#pragma unroll
+      for (int t = 0; t < OT; t++) acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(f[e & 1][t], p.w[e], acc[t], 0, 0, 0);
     }
   }
 };
 
-// Two products of 32 rows each, of tiles that lie side by side: a += rows . ca, b += rows T::SIZE further on . cb. Heads of more
-// than 64 in two halves, which is as many registers as a product of one.
+// Two products of 32 rows each, of tiles that lie side by side: a += rows . ca, b += rows T::SIZE further on . cb. A few steps' rows
+// are read while the steps before are multiplied. float32 leaves out steps past the head's end, whose instructions are slow.
 template <class T, int OFFSET, class EL, int DP>
-__device__ __forceinline__ void two_scores(f32x16 &a, const Column<EL, DP> &ca, f32x16 &b, const Column<EL, DP> &cb, const Places<T, EL> &p) {
-  if constexpr (EL::F32 || DP <= 64) {
-    RowVectors<T, EL, DP> x, y;
-    x.template load<OFFSET>(p);
-    if constexpr (EL::F32) x.scores(a, ca);
-    y.template load<OFFSET + T::SIZE>(p);
-    if constexpr (!EL::F32) {
-      in_order();
-      x.scores(a, ca);
+__device__ __forceinline__ void two_scores(f32x16 &a, const Column<EL, DP> &ca, f32x16 &b, const Column<EL, DP> &cb, const Places<T, EL> &p, int dim) {
+  constexpr int STEPS = DP / (2 * EL::VE), CHUNK = EL::F32 ? 2 : STEPS % 4 == 0 ? 4 : STEPS < 4 ? STEPS : 3, CHUNKS = STEPS / CHUNK, GROUP = Places<T, EL>::GROUP;
+  static_assert(CHUNKS * CHUNK == STEPS, "whole chunks");
+  V16 f[2][CHUNK];
+  auto load = [&](int i) {
+#pragma unroll
+    for (int k = 0; k < CHUNK; k++) {
+      const int s = i % CHUNKS * CHUNK + k;
+      f[i & 1][k] = *at_lds<const lds_V16>(p.vector[(2 * s) % GROUP / 2] + (uint32_t)((2 * s) / GROUP * GROUP * 16 + OFFSET + i / CHUNKS * T::SIZE));
     }
-    y.scores(b, cb);
-  } else {
-    constexpr int STEPS = DP / (2 * EL::VE), HALF = STEPS / 2;
-    RowVectors<T, EL, DP, 0, HALF> x, y;
-    RowVectors<T, EL, DP, HALF, STEPS> z, u;
-    x.template load<OFFSET>(p);
-    y.template load<OFFSET + T::SIZE>(p);
+  };
+  load(0);
+#pragma unroll
+  for (int i = 0; i < 2 * CHUNKS; i++) {
     in_order();
-    x.scores(a, ca);
-    z.template load<OFFSET>(p);
-    y.scores(b, cb);
-    u.template load<OFFSET + T::SIZE>(p);
-    in_order();
-    z.scores(a, ca);
-    u.scores(b, cb);
+    if (i + 1 < 2 * CHUNKS) load(i + 1);
+    if (EL::F32 && i % CHUNKS * CHUNK * 2 * EL::VE >= dim) continue;
+#pragma unroll
+    for (int k = 0; k < CHUNK; k++) {
+      const int s = i % CHUNKS * CHUNK + k;
+      if (i < CHUNKS) gemm_tile::mfma_step<EL>(a, f[i & 1][k], ca.f[s]);
+      else gemm_tile::mfma_step<EL>(b, f[i & 1][k], cb.f[s]);
+    }
   }
 }
 
