@@ -173,7 +173,7 @@ __device__ __forceinline__ uint32_t queries_seeing(const AttentionArgs &a, const
 
 // Where a block of the second launch is: its keys, and its part of what they are seen by, the query tiles of all heads that share
 // them, one head after the other.
-template <class EL, int QUERIES>
+template <class EL, int QUERIES, int KEYS = 128>
 struct KeysWalk {
   int b, hk, keys, first;  // batch, head, the sequence's keys, the block's first
   int part, steps;
@@ -185,7 +185,7 @@ struct KeysWalk {
     b = bh / a.kv_heads;
     hk = bh % a.kv_heads;
     keys = keys_of(a, b);
-    first = (int)(rest / (uint32_t)a.parts) * 128;  // the first keys first: under a causal mask most queries see them
+    first = (int)(rest / (uint32_t)a.parts) * KEYS;  // the first keys first: under a causal mask most queries see them
     part = (int)(rest % (uint32_t)a.parts);
     tiles = (a.sq + QUERIES - 1) / QUERIES;
     before = a.causal ? min(tiles, max(0, first - a.shift) / QUERIES) : 0;
@@ -370,124 +370,136 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
 // The same for heads of more than 64. Blocks of eight waves, of which two have the same 32 keys: one makes the scores, p and dv,
 // the other g . v, ds and dk, one tile of queries behind the first, whose p it takes from LDS. So a wave holds the vectors and the
 // sums of one operand, not of two, which for heads of 128 are more registers than two waves of a unit's may have.
-template <class EL, int DP>
-__global__ __launch_bounds__(512) void attention_grad_wide_keys_kernel(AttentionArgs a) {
+template <class EL, int DP, int PAIRS>
+__global__ __launch_bounds__(128 * PAIRS) __attribute__((amdgpu_waves_per_eu(2))) void attention_grad_wide_keys_kernel(AttentionArgs a) {
   constexpr int QUERIES = 32, OT = DP / 32;
-  using T = Tile<EL, DP, QUERIES, 4>;  // (four waves bring each operand's)
-  constexpr int STAGE = 2 * T::SIZE + 1024, RING = EL::F32 ? 3 : 4, VALUES = 2 * T::SIZE;
+  using T = Tile<EL, DP, QUERIES, PAIRS>;  // (half of the waves bring each operand's)
+  constexpr int STAGE = 2 * T::SIZE + 1024, RING = EL::F32 || PAIRS == 2 ? 3 : 4, VALUES = 2 * T::SIZE;
   constexpr int AHEAD = RING - 2;  // tiles on their way
   __shared__ __attribute__((aligned(1024))) unsigned char stages[RING * STAGE];
-  __shared__ __attribute__((aligned(16))) float over[2][4][4][64][4];  // p, for the other wave: [tile][pair][e / 4][lane][e % 4]
+  __shared__ __attribute__((aligned(16))) float over[2][PAIRS][4][64][4];  // p, for the other wave: [tile][pair][e / 4][lane][e % 4]
 
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = wave & 3;
-  const bool second = wave >= 4;  // dk
-  KeysWalk<EL, QUERIES> w(a);
-  const int k0 = w.first + pair * 32, kj = k0 + (lane & 31);
-  const HeadOperand &mine = second ? a.v : a.k, &brought = second ? a.g : a.q;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = wave % PAIRS;
   const uint32_t lds = lds_address(stages);
-  T tile;
-  tile.begin(pair, brought.row);
-  if (a.dim != DP) {
-    for (int s = 0; s < RING; s++) tile.clear(lds + s * STAGE + (second ? T::SIZE : 0), a.dim);
-    __syncthreads();
-  }
-  int at = w.at, head = w.head;  // of the step that this wave works on (the walk's are of the one that is fetched)
-  const typename EL::S *next;
-  const float *values_next;
-  auto find = [&]() {  // the walk's place, where it is not behind the last one
-    const int64_t i0 = (int64_t)w.at * QUERIES;
-    next = rows_of<EL>(brought, w.b, w.head) + i0 * brought.row;
-    values_next = a.rows + (((int64_t)w.b * a.heads + w.head) * a.rows_pitch + i0) * 2;
-  };
-  auto fetch = [&](uint32_t to) {
-    const int left = a.sq - w.at * QUERIES;
-    tile.fetch(next, left, brought, a.dim, to + (second ? T::SIZE : 0));
-    if (wave == 0) load_to_lds4(values_next, lane * 4, to + VALUES);
-    next += QUERIES * brought.row;
-    values_next += QUERIES * 2;
-    if (w.next()) find();
-    return brought.direct && left >= QUERIES;
-  };
-  if (w.steps > 0) find();
-  bool whole = false;  // what is on its way for the step after this one
-  if (w.steps > 0) fetch(lds);
-  if (AHEAD == 2 && w.steps > 1) whole = fetch(lds + STAGE);
-  Column<EL, DP> own;
-  own.load(rows_of<EL>(mine, w.b, w.hk) + (int64_t)kj * mine.row, kj < w.keys, a.dim);
-  f32x16 acc[OT];  // of dv, in the second wave of dk
-#pragma unroll
-  for (int t = 0; t < OT; t++)
-#pragma unroll
-    for (int e = 0; e < 16; e++) acc[t][e] = 0.0f;
-  Places<T, EL> places;
-  places.begin();
   const uint32_t half16 = ((threadIdx.x >> 5) & 1) * 16;
-  uint32_t stage = lds, ahead = lds + AHEAD * STAGE;
-  for (int t = 0; w.steps > 0 && t <= w.steps; t++) {
-    // tile t has come, p of the tile before it too, and what is filled next has been used
-    if (t == 0 || !whole) meet<0>();
-    else if (wave == 0) meet<T::LPW + 1>();
-    else meet<T::LPW>();
-    whole = false;
-    if (t + AHEAD < w.steps) {
-      const bool is = fetch(ahead);
-      if (AHEAD == 2) whole = is;
+  // The two kinds of waves have code of their own, which meets at the same barriers.
+  auto run = [&](auto kind) {
+    constexpr bool second = decltype(kind)::value;  // dk
+    KeysWalk<EL, QUERIES, 32 * PAIRS> w(a);
+    const int k0 = w.first + pair * 32, kj = k0 + (lane & 31);
+    const HeadOperand &mine = second ? a.v : a.k, &brought = second ? a.g : a.q;
+    T tile;
+    tile.begin(pair, brought.row);
+    if (a.dim != DP) {
+      for (int s = 0; s < RING; s++) tile.clear(lds + s * STAGE + (second ? T::SIZE : 0), a.dim);
+      meet<0>();
     }
-    ahead = ahead == lds + (RING - 1) * STAGE ? lds : ahead + STAGE;
-    if (second ? t == 0 : t == w.steps) continue;
-    const uint32_t now = stage;
-    stage = stage == lds + (RING - 1) * STAGE ? lds : stage + STAGE;
-    const int i0 = at * QUERIES, head_now = head;
-    if (++at == w.tiles) at = w.before, head++;
-    if (k0 >= w.keys || (a.causal && k0 > i0 + 31 + a.shift)) continue;  // nothing of the tile sees these keys
-    float(*between)[64][4] = over[(second ? t - 1 : t) & 1][pair];
-    const bool inner = !a.mask.base && !(a.causal && k0 + 31 > i0 + a.shift);
-    const Places<T, EL> here = places.in(now + (second ? T::SIZE : 0)), other = places.in(now + (second ? 0 : T::SIZE));
-    uint32_t values = now + half16;
-    asm("" : "+v"(values));
-    f32x16 x;
-    if (second) {
-      row_values<VALUES + 128>(values, x);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; e++) x[e] = 0.0f;
+    int at = w.at, head = w.head;  // of the step that this wave works on (the walk's are of the one that is fetched)
+    const typename EL::S *next;
+    const float *values_next;
+    auto find = [&]() {  // the walk's place, where it is not behind the last one
+      const int64_t i0 = (int64_t)w.at * QUERIES;
+      next = rows_of<EL>(brought, w.b, w.head) + i0 * brought.row;
+      values_next = a.rows + (((int64_t)w.b * a.heads + w.head) * a.rows_pitch + i0) * 2;
+    };
+    auto fetch = [&](uint32_t to) {
+      const int left = a.sq - w.at * QUERIES;
+      tile.fetch(next, left, brought, a.dim, to + (second ? T::SIZE : 0));
+      if (!second && pair == 0) load_to_lds4(values_next, lane * 4, to + VALUES);
+      next += QUERIES * brought.row;
+      values_next += QUERIES * 2;
+      if (w.next()) find();
+      return brought.direct && left >= QUERIES;
+    };
+    bool whole = false;  // what is on its way for the step after this one
+    if (w.steps > 0) {
+      find();
+      fetch(lds);
     }
-    RowVectors<T, EL, DP> vectors;
-    vectors.template load<0>(here);
-    if constexpr (!EL::F32) in_order();
-    vectors.scores(x, own);
-    RowElements<T, EL, OT> elements;  // (on their way during the exponentials)
-    elements.template load<0>(other);
-    if constexpr (!EL::F32) in_order();
-    if (!second) {
-      f32x16 l;
-      row_values<VALUES>(values, l);
+    if (AHEAD == 2 && w.steps > 1) whole = fetch(lds + STAGE);
+    Column<EL, DP> own;
+    own.load(rows_of<EL>(mine, w.b, w.hk) + (int64_t)kj * mine.row, kj < w.keys, a.dim);
+    f32x16 acc[OT];
 #pragma unroll
-      for (int e = 0; e < 16; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.c2, l[e]));
-      if (!inner) {
-        const uint8_t *mask = a.mask.base ? reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)w.b * a.mask.batch + (int64_t)head_now * a.mask.head : nullptr;
-        const uint32_t seeing = queries_seeing(a, mask, kj, i0);
+    for (int t = 0; t < OT; t++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) x[e] = (seeing >> e) & 1 ? x[e] : 0.0f;
+      for (int e = 0; e < 16; e++) acc[t][e] = 0.0f;
+    Places<T, EL> places;
+    places.begin();
+    uint32_t stage = lds, ahead = lds + AHEAD * STAGE;
+    for (int t = 0; w.steps > 0 && t <= w.steps; t++) {
+      // tile t has come, p of the tile before it too, and what is filled next has been used
+      if (t == 0 || !whole) meet<0>();
+      else if (!second && pair == 0) meet<T::LPW + 1>();
+      else meet<T::LPW>();
+      whole = false;
+      if (t + AHEAD < w.steps) {
+        const bool is = fetch(ahead);
+        if (AHEAD == 2) whole = is;
       }
+      ahead = ahead == lds + (RING - 1) * STAGE ? lds : ahead + STAGE;
+      if (second ? t == 0 : t == w.steps) continue;
+      const uint32_t now = stage;
+      stage = stage == lds + (RING - 1) * STAGE ? lds : stage + STAGE;
+      const int i0 = at * QUERIES, head_now = head;
+      if (++at == w.tiles) at = w.before, head++;
+      if (k0 >= w.keys || (a.causal && k0 > i0 + 31 + a.shift)) continue;  // nothing of the tile sees these keys
+      float(*between)[64][4] = over[(second ? t - 1 : t) & 1][pair];
+      const bool inner = !a.mask.base && !(a.causal && k0 + 31 > i0 + a.shift);
+      const Places<T, EL> here = places.in(now);
+      uint32_t values = now + half16;
+      asm("" : "+v"(values));
+      f32x16 x, l;  // l: the rows' powers; in the second wave p, which the first wave left
+      if (second) {
+        row_values<VALUES + 128>(values, x);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) *reinterpret_cast<gemm_tile::f32x4 *>(between[e >> 2][lane]) = gemm_tile::f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
-    } else {
+        for (int e = 0; e < 16; e++) x[e] = 0.0f;
+      }
+      RowVectors<T, EL, DP> vectors;
+      vectors.template load<(second ? T::SIZE : 0)>(here);
+      if constexpr (!EL::F32) in_order();
+      vectors.scores(x, own);
+      if (second) {
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const gemm_tile::f32x4 p = *reinterpret_cast<const gemm_tile::f32x4 *>(between[e >> 2][lane]);
+        for (int e = 0; e < 16; e += 4) {
+          const gemm_tile::f32x4 p = *reinterpret_cast<const gemm_tile::f32x4 *>(between[e >> 2][lane]);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float ds = p[j] * x[e + j];
-          x[e + j] = inner || p[j] != 0.0f ? ds : 0.0f;  // (what a query does not see may be no number)
+          for (int j = 0; j < 4; j++) l[e + j] = p[j];
         }
+      } else {
+        row_values<VALUES>(values, l);
       }
+      RowElements<T, EL, OT> elements;  // (on their way during the exponentials)
+      elements.template load<(second ? 0 : T::SIZE)>(here);
+      if constexpr (!EL::F32) in_order();
+      if (second) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[e] = l[e] * x[e];
+        if (!inner) {
+#pragma unroll
+          for (int e = 0; e < 16; e++) x[e] = l[e] != 0.0f ? x[e] : 0.0f;  // (what a query does not see may be no number)
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.c2, l[e]));
+        if (!inner) {
+          const uint8_t *mask = a.mask.base ? reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)w.b * a.mask.batch + (int64_t)head_now * a.mask.head : nullptr;
+          const uint32_t seeing = queries_seeing(a, mask, kj, i0);
+#pragma unroll
+          for (int e = 0; e < 16; e++) x[e] = (seeing >> e) & 1 ? x[e] : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) *reinterpret_cast<gemm_tile::f32x4 *>(between[e >> 2][lane]) = gemm_tile::f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+      }
+      Weights<EL> y;
+      y.set(x);
+      elements.add(acc, y);
     }
-    Weights<EL> y;
-    y.set(x);
-    elements.add(acc, y);
-  }
-  if (kj < a.sk) store_key<EL, DP>(a, w, kj, second, acc);
+    if (kj < a.sk) store_key<EL, DP>(a, w, kj, second, acc);
+  };
+  if (wave >= PAIRS) run(std::integral_constant<bool, true>{});
+  else run(std::integral_constant<bool, false>{});
 }
 
 // The parts' sums, in order.
@@ -525,7 +537,8 @@ void launch(nxh_context *ctx, AttentionArgs a) {
   a.tiles = (a.sk + 127) / 128;
   const dim3 grid((unsigned)(a.batch * a.kv_heads * a.tiles * a.parts));
   if constexpr (DP <= 64) hipLaunchKernelGGL((attention_grad_keys_kernel<EL, DP>), grid, dim3(256), 0, ctx->stream, a);
-  else hipLaunchKernelGGL((attention_grad_wide_keys_kernel<EL, DP>), grid, dim3(512), 0, ctx->stream, a);
+  else if constexpr (EL::F32) hipLaunchKernelGGL((attention_grad_wide_keys_kernel<EL, DP, 4>), grid, dim3(512), 0, ctx->stream, a);
+  else hipLaunchKernelGGL((attention_grad_wide_keys_kernel<EL, DP, 2>), dim3((unsigned)(a.batch * a.kv_heads * ((a.sk + 63) / 64) * a.parts)), dim3(256), 0, ctx->stream, a);
   if (!a.partial) return;
   const int64_t size = (int64_t)a.batch * a.kv_heads * a.sk * 2 * a.dim;
   hipLaunchKernelGGL((attention_grad_join_kernel<EL>), dim3((unsigned)std::min<int64_t>((size + 255) / 256, 1 << 16)), dim3(256), 0, ctx->stream, a);
