@@ -30,8 +30,8 @@ __device__ __forceinline__ float exponent_of(float lse) {
 
 // Blocks of four waves. KW = 1: each has 32 queries of 128. KW = 2: two share 32 queries, each takes every other 32 keys of a
 // tile, and their sums are added at the end: twice the blocks, where there are few.
-template <class EL, int DP, int KW>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((EL::F32 || KW == 2) && DP > (KW == 2 && EL::F32 ? 64 : 96) ? 1 : 2))) void attention_grad_queries_kernel(AttentionArgs a) {
+template <class EL, int DP, int KW, bool MASK>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((EL::F32 || KW == 2 || MASK) && DP > (EL::F32 && (KW == 2 || MASK) ? 64 : 96) ? 1 : 2))) void attention_grad_queries_kernel(AttentionArgs a) {
   using S = typename EL::S;
   constexpr int KEYS = EL::F32 || DP > 64 ? 32 * KW : 64, SUBS = KEYS / 32 / KW, QUERIES = 128 / KW, OT = DP / 32;
   using T = Tile<EL, DP, KEYS, 4>;
@@ -47,7 +47,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((EL::F32 ||
   const int q0 = tile * QUERIES + pair * 32, qi = q0 + c32;
   const bool there = qi < a.sq;
   const S *K = rows_of<EL>(a.k, b, hk), *V = rows_of<EL>(a.v, b, hk);
-  const uint8_t *mask = a.mask.base ? reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)b * a.mask.batch + (int64_t)h * a.mask.head : nullptr;
+  const uint8_t *mask = reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)b * a.mask.batch + (int64_t)h * a.mask.head;
   int seen = keys;
   if (a.causal) seen = min(seen, max(0, min((tile + 1) * QUERIES, a.sq) + a.shift));
   const int steps = (seen + KEYS - 1) / KEYS;
@@ -102,7 +102,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((EL::F32 ||
     const int first = t * KEYS + part * 32;
     if (first >= keys || (a.causal && first > q0 + 31 + a.shift)) continue;  // nothing of it is seen
     const Places<T, EL> here = places.in(now + (uint32_t)(part * 32 * T::ROW));
-    auto begin = [&](f32x16 &p, f32x16 &ds) {
+    MaskBytes bytes;
+    auto begin = [&](int r0, f32x16 &p, f32x16 &ds) {
+      if constexpr (MASK) bytes.load_keys(a, mask, qi, first + r0);
 #pragma unroll
       for (int e = 0; e < 16; e++) p[e] = 0.0f, ds[e] = -delta;
     };
@@ -110,15 +112,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((EL::F32 ||
 #pragma unroll
       for (int e = 0; e < 16; e++) ds[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[e], a.c2, power)) * ds[e];
       const int j0 = first + r0;
-      if (!mask && j0 + 32 <= keys && !(a.causal && j0 + 31 > q0 + a.shift)) return;
-      const uint32_t see = keys_seen(a, mask, qi, j0, keys);
+      if (!MASK && j0 + 32 <= keys && !(a.causal && j0 + 31 > q0 + a.shift)) return;
+      uint32_t see = keys_seen(a, qi, j0, keys);
+      if constexpr (MASK) see &= bytes.kept();
 #pragma unroll
       for (int e = 0; e < 16; e++) ds[e] = (see >> e) & 1 ? ds[e] : 0.0f;
     };
     f32x16 p, ds;
     Weights<EL> w;
     RowElements<T, EL, OT> k;  // (on their way during the exponentials; those of heads of 128 would be more registers than there are)
-    begin(p, ds);
+    begin(0, p, ds);
     two_scores<T, 0>(p, q, ds, g, here, a.dim);
     if constexpr (DP <= 96) k.template load<0>(here);
     if constexpr (!EL::F32) in_order();
@@ -127,7 +130,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((EL::F32 ||
     w.set(ds);
     if constexpr (SUBS == 2) {
       k.add(dq, w);
-      begin(p, ds);
+      begin(32, p, ds);
       two_scores<T, 32 * T::ROW>(p, q, ds, g, here, a.dim);
       k.template load<32 * T::ROW>(here);
       in_order();
@@ -156,19 +159,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((EL::F32 ||
   if (there) store_column<EL, DP>(const_cast<S *>(rows_of<EL>(a.dq, b, h)) + (int64_t)qi * a.dq.row, dq, a.scale * UNLIFT<EL>, a.dim);
 }
 
-// Which of queries i0 + (e / 4) * 8 + g * 4 + e % 4 see key kj, bit e of the result.
-__device__ __forceinline__ uint32_t queries_seeing(const AttentionArgs &a, const uint8_t *mask, int kj, int i0) {
-  const int g = (threadIdx.x >> 5) & 1, first = i0 + g * 4;
-  const uint32_t seeing = a.causal ? rows_from(kj - a.shift - first) : 0xffffu;
-  if (!mask) return seeing;
-  const uint8_t *m = mask + (int64_t)(kj < a.sk ? kj : a.sk - 1) * a.mask_col;
-  uint32_t kept = 0;
-#pragma unroll 4
-  for (int e = 0; e < 16; e++) {
-    const int i = first + (e >> 2) * 8 + (e & 3);
-    kept |= (uint32_t)(m[(int64_t)(i < a.sq ? i : a.sq - 1) * a.mask.row] != 0) << e;
-  }
-  return seeing & kept;
+// Which of queries i0 + (e / 4) * 8 + g * 4 + e % 4 see key kj, the mask aside, bit e of the result.
+__device__ __forceinline__ uint32_t queries_seeing(const AttentionArgs &a, int kj, int i0) {
+  return a.causal ? rows_from(kj - a.shift - i0 - (int)((threadIdx.x >> 5) & 1) * 4) : 0xffffu;
 }
 
 // Where a block of the second launch is: its keys, and its part of what they are seen by, the query tiles of all heads that share
@@ -239,7 +232,7 @@ __device__ __forceinline__ void store_key(const AttentionArgs &a, const W &w, in
 
 // Blocks of four waves with 32 keys each, for heads of up to 64. What a block walks over is cut into a.parts, a block each, where
 // there would be few blocks; their sums are joined by another launch.
-template <class EL, int DP>
+template <class EL, int DP, bool MASK>
 __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs a) {
   constexpr int QUERIES = EL::F32 ? 32 : 64, OT = DP / 32;
   using T = Tile<EL, DP, QUERIES, 4>;
@@ -314,15 +307,22 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
     const Places<T, EL> here = places.in(now);
     uint32_t values = now + half16;
     asm("" : "+v"(values));
+    MaskBytes bytes;
+    auto begin = [&](int r0, f32x16 &p) {
+      if constexpr (MASK)
+        bytes.load_queries(a, reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)w.b * a.mask.batch + (int64_t)head_now * a.mask.head, kj, i0 + r0);
+#pragma unroll
+      for (int e = 0; e < 16; e++) p[e] = 0.0f;
+    };
     auto differences = [&](int r0, const f32x16 &l, f32x16 &p, f32x16 &ds) {
 #pragma unroll
       for (int e = 0; e < 16; e++) {
         p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[e], a.c2, l[e]));
         ds[e] = p[e] * ds[e];
       }
-      if (!a.mask.base && !(a.causal && k0 + 31 > i0 + r0 + a.shift)) return;
-      const uint8_t *mask = a.mask.base ? reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)w.b * a.mask.batch + (int64_t)head_now * a.mask.head : nullptr;
-      const uint32_t seeing = queries_seeing(a, mask, kj, i0 + r0);
+      if (!MASK && !(a.causal && k0 + 31 > i0 + r0 + a.shift)) return;
+      uint32_t seeing = queries_seeing(a, kj, i0 + r0);
+      if constexpr (MASK) seeing &= bytes.kept();
 #pragma unroll
       for (int e = 0; e < 16; e++) {
         const bool keep = (seeing >> e) & 1;
@@ -333,8 +333,7 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
     f32x16 p, ds, l;
     Weights<EL> pw, dsw;
     RowElements<T, EL, OT> g, q;  // (on their way during the exponentials)
-#pragma unroll
-    for (int e = 0; e < 16; e++) p[e] = 0.0f;
+    begin(0, p);
     row_values<VALUES + 128>(values, ds);
     two_scores<T, 0>(p, k, ds, v, here, a.dim);
     row_values<VALUES>(values, l);
@@ -347,8 +346,7 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
     if constexpr (QUERIES == 64) {
       g.add(dv, pw);
       q.add(dk, dsw);
-#pragma unroll
-      for (int e = 0; e < 16; e++) p[e] = 0.0f;
+      begin(32, p);
       row_values<VALUES + 256 + 128>(values, ds);
       two_scores<T, 32 * T::ROW>(p, k, ds, v, here, a.dim);
       row_values<VALUES + 256>(values, l);
@@ -370,7 +368,7 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
 // The same for heads of more than 64. Blocks of eight waves, of which two have the same 32 keys: one makes the scores, p and dv,
 // the other g . v, ds and dk, one tile of queries behind the first, whose p it takes from LDS. So a wave holds the vectors and the
 // sums of one operand, not of two, which for heads of 128 are more registers than two waves of a unit's may have.
-template <class EL, int DP, int PAIRS>
+template <class EL, int DP, int PAIRS, bool MASK>
 __global__ __launch_bounds__(128 * PAIRS) __attribute__((amdgpu_waves_per_eu(2))) void attention_grad_wide_keys_kernel(AttentionArgs a) {
   constexpr int QUERIES = 32, OT = DP / 32;
   using T = Tile<EL, DP, QUERIES, PAIRS>;  // (half of the waves bring each operand's)
@@ -445,7 +443,10 @@ __global__ __launch_bounds__(128 * PAIRS) __attribute__((amdgpu_waves_per_eu(2))
       if (++at == w.tiles) at = w.before, head++;
       if (k0 >= w.keys || (a.causal && k0 > i0 + 31 + a.shift)) continue;  // nothing of the tile sees these keys
       float(*between)[64][4] = over[(second ? t - 1 : t) & 1][pair];
-      const bool inner = !a.mask.base && !(a.causal && k0 + 31 > i0 + a.shift);
+      const bool inner = !MASK && !(a.causal && k0 + 31 > i0 + a.shift);
+      MaskBytes bytes;
+      if constexpr (!second && MASK)
+        bytes.load_queries(a, reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)w.b * a.mask.batch + (int64_t)head_now * a.mask.head, kj, i0);
       const Places<T, EL> here = places.in(now);
       uint32_t values = now + half16;
       asm("" : "+v"(values));
@@ -484,8 +485,8 @@ __global__ __launch_bounds__(128 * PAIRS) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll
         for (int e = 0; e < 16; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.c2, l[e]));
         if (!inner) {
-          const uint8_t *mask = a.mask.base ? reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)w.b * a.mask.batch + (int64_t)head_now * a.mask.head : nullptr;
-          const uint32_t seeing = queries_seeing(a, mask, kj, i0);
+          uint32_t seeing = queries_seeing(a, kj, i0);
+          if constexpr (MASK) seeing &= bytes.kept();
 #pragma unroll
           for (int e = 0; e < 16; e++) x[e] = (seeing >> e) & 1 ? x[e] : 0.0f;
         }
@@ -520,35 +521,42 @@ __global__ __launch_bounds__(256) void attention_grad_join_kernel(AttentionArgs 
   }
 }
 
-template <class EL, int DP>
+template <class EL, int DP, bool MASK>
 void launch(nxh_context *ctx, AttentionArgs a) {
   const int units = ctx->compute_units > 0 ? ctx->compute_units : 256;
+  const auto blocks_of = [&](int heads, int n) { return dim3((unsigned)(a.batch * heads * n)); };
   if (a.sq > 0 && a.heads > 0) {
     a.tiles = (a.sq + 127) / 128;
-    const int64_t blocks = (int64_t)a.batch * a.heads * a.tiles;
-    if (blocks < 2 * units) {
+    if ((int64_t)a.batch * a.heads * a.tiles < 2 * units) {
       a.tiles = (a.sq + 63) / 64;
-      hipLaunchKernelGGL((attention_grad_queries_kernel<EL, DP, 2>), dim3((unsigned)(a.batch * a.heads * a.tiles)), dim3(256), 0, ctx->stream, a);
+      hipLaunchKernelGGL((attention_grad_queries_kernel<EL, DP, 2, MASK>), blocks_of(a.heads, a.tiles), dim3(256), 0, ctx->stream, a);
     } else {
-      hipLaunchKernelGGL((attention_grad_queries_kernel<EL, DP, 1>), dim3((unsigned)blocks), dim3(256), 0, ctx->stream, a);
+      hipLaunchKernelGGL((attention_grad_queries_kernel<EL, DP, 1, MASK>), blocks_of(a.heads, a.tiles), dim3(256), 0, ctx->stream, a);
     }
   }
   if (a.sk == 0) return;
-  a.tiles = (a.sk + 127) / 128;
-  const dim3 grid((unsigned)(a.batch * a.kv_heads * a.tiles * a.parts));
-  if constexpr (DP <= 64) hipLaunchKernelGGL((attention_grad_keys_kernel<EL, DP>), grid, dim3(256), 0, ctx->stream, a);
-  else if constexpr (EL::F32) hipLaunchKernelGGL((attention_grad_wide_keys_kernel<EL, DP, 4>), grid, dim3(512), 0, ctx->stream, a);
-  else hipLaunchKernelGGL((attention_grad_wide_keys_kernel<EL, DP, 2>), dim3((unsigned)(a.batch * a.kv_heads * ((a.sk + 63) / 64) * a.parts)), dim3(256), 0, ctx->stream, a);
+  if constexpr (DP <= 64) {
+    hipLaunchKernelGGL((attention_grad_keys_kernel<EL, DP, MASK>), blocks_of(a.kv_heads, (a.sk + 127) / 128 * a.parts), dim3(256), 0, ctx->stream, a);
+  } else {
+    constexpr int PAIRS = EL::F32 ? 4 : 2;
+    hipLaunchKernelGGL((attention_grad_wide_keys_kernel<EL, DP, PAIRS, MASK>), blocks_of(a.kv_heads, (a.sk + 32 * PAIRS - 1) / (32 * PAIRS) * a.parts),
+                       dim3(128 * PAIRS), 0, ctx->stream, a);
+  }
   if (!a.partial) return;
   const int64_t size = (int64_t)a.batch * a.kv_heads * a.sk * 2 * a.dim;
   hipLaunchKernelGGL((attention_grad_join_kernel<EL>), dim3((unsigned)std::min<int64_t>((size + 255) / 256, 1 << 16)), dim3(256), 0, ctx->stream, a);
 }
+template <class EL, int DP>
+void launch_mask(nxh_context *ctx, const AttentionArgs &a) {
+  if (a.mask.base) launch<EL, DP, true>(ctx, a);
+  else launch<EL, DP, false>(ctx, a);
+}
 template <class EL>
 void launch_dim(nxh_context *ctx, const AttentionArgs &a) {
-  if (a.dim <= 32) launch<EL, 32>(ctx, a);
-  else if (a.dim <= 64) launch<EL, 64>(ctx, a);
-  else if (a.dim <= 96) launch<EL, 96>(ctx, a);
-  else launch<EL, 128>(ctx, a);
+  if (a.dim <= 32) launch_mask<EL, 32>(ctx, a);
+  else if (a.dim <= 64) launch_mask<EL, 64>(ctx, a);
+  else if (a.dim <= 96) launch_mask<EL, 96>(ctx, a);
+  else launch_mask<EL, 128>(ctx, a);
 }
 
 }  // namespace

@@ -417,30 +417,48 @@ __device__ __forceinline__ uint32_t rows_from(int from) {
   const uint32_t below = from <= 0 ? 0u : from >= 32 ? 0xffffu : ((1u << (4 * q)) - 1u) | ((1u << (r < 4 ? r : 4)) - 1u) << (4 * q);
   return 0xffffu & ~below;
 }
-// Which of keys j0 + (e / 4) * 8 + g * 4 + e % 4 query qi sees, bit e of the result.
-__device__ __forceinline__ uint32_t keys_seen(const AttentionArgs &a, const uint8_t *mask, int qi, int j0, int keys) {
-  const int g = (threadIdx.x >> 5) & 1, first = j0 + g * 4;
-  const int end = a.causal && qi + a.shift < keys - 1 ? qi + a.shift : keys - 1;
-  const uint32_t seen = ~rows_from(end + 1 - first) & 0xffffu;
-  if (!mask) return seen;
-  const uint8_t *m = mask + (int64_t)(qi < a.sq ? qi : a.sq - 1) * a.mask.row;
-  uint32_t kept = 0;
-  if (a.mask_col == 1 && j0 + 32 <= a.sk) {  // four neighbours are one load, of any alignment
+// What the mask holds for the 16 pairs of a lane: requested before the products, looked at behind them.
+struct MaskBytes {
+  uint32_t b[16];
+  // keys j0 + (e / 4) * 8 + g * 4 + e % 4 of query qi: four neighbours are one load, of any alignment, where they lie side by side
+  __device__ __forceinline__ void load_keys(const AttentionArgs &a, const uint8_t *mask, int qi, int j0) {
+    const int first = j0 + ((threadIdx.x >> 5) & 1) * 4;
+    const uint8_t *m = mask + (int64_t)(qi < a.sq ? qi : a.sq - 1) * a.mask.row;
+    if (a.mask_col == 1 && j0 + 32 <= a.sk) {
+      uint32_t four[4];
 #pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      uint32_t four;
-      __builtin_memcpy(&four, m + first + e * 2, 4);
+      for (int e = 0; e < 4; e++) __builtin_memcpy(&four[e], m + first + e * 8, 4);
 #pragma unroll
-      for (int j = 0; j < 4; j++) kept |= (uint32_t)(((four >> (8 * j)) & 0xffu) != 0) << (e + j);
-    }
-  } else {
-#pragma unroll 4
-    for (int e = 0; e < 16; e++) {
-      const int j = first + (e >> 2) * 8 + (e & 3);
-      kept |= (uint32_t)(m[(int64_t)(j < a.sk ? j : a.sk - 1) * a.mask_col] != 0) << e;
+      for (int e = 0; e < 16; e++) b[e] = (four[e >> 2] >> (8 * (e & 3))) & 0xffu;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        const int j = first + (e >> 2) * 8 + (e & 3);
+        b[e] = m[(int64_t)(j < a.sk ? j : a.sk - 1) * a.mask_col];
+      }
     }
   }
-  return seen & kept;
+  // queries i0 + (e / 4) * 8 + g * 4 + e % 4 of key kj
+  __device__ __forceinline__ void load_queries(const AttentionArgs &a, const uint8_t *mask, int kj, int i0) {
+    const int first = i0 + ((threadIdx.x >> 5) & 1) * 4;
+    const uint8_t *m = mask + (int64_t)(kj < a.sk ? kj : a.sk - 1) * a.mask_col;
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      const int i = first + (e >> 2) * 8 + (e & 3);
+      b[e] = m[(int64_t)(i < a.sq ? i : a.sq - 1) * a.mask.row];
+    }
+  }
+  __device__ __forceinline__ uint32_t kept() const {
+    uint32_t k = 0;
+#pragma unroll
+    for (int e = 0; e < 16; e++) k |= (uint32_t)(b[e] != 0) << e;
+    return k;
+  }
+};
+// Which of those keys query qi sees, the mask aside, bit e of the result.
+__device__ __forceinline__ uint32_t keys_seen(const AttentionArgs &a, int qi, int j0, int keys) {
+  const int end = a.causal && qi + a.shift < keys - 1 ? qi + a.shift : keys - 1;
+  return ~rows_from(end + 1 - j0 - (int)((threadIdx.x >> 5) & 1) * 4) & 0xffffu;
 }
 
 // ── host side ───────────────────────────────────────────────────────────────

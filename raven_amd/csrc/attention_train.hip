@@ -14,7 +14,7 @@ namespace {
 
 // Blocks of four waves. KW = 1: each has 32 queries of 128. KW = 2: two share 32 queries, each takes every other 32 keys
 // of a tile, and their results are joined at the end: twice the blocks.
-template <class EL, int DP, int KW>
+template <class EL, int DP, int KW, bool MASK>
 __global__ __launch_bounds__(256) void attention_train_kernel(AttentionArgs a) {
   using S = typename EL::S;
   constexpr int KEYS = !EL::F32 && DP <= 64 ? 64 : 32 * KW, SUBS = KEYS / 32 / KW, QUERIES = 128 / KW, OT = DP / 32;
@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) void attention_train_kernel(AttentionArgs a) {
   const int keys = keys_of(a, b);
   const int q0 = tile * QUERIES + pair * 32, qi = q0 + c32;
   const S *K = rows_of<EL>(a.k, b, hk), *V = rows_of<EL>(a.v, b, hk);
-  const uint8_t *mask = a.mask.base ? reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)b * a.mask.batch + (int64_t)h * a.mask.head : nullptr;
+  const uint8_t *mask = reinterpret_cast<const uint8_t *>(a.mask.base) + (int64_t)b * a.mask.batch + (int64_t)h * a.mask.head;
 
   int seen = keys;  // by the block's last query
   if (a.causal) seen = min(seen, max(0, min((tile + 1) * QUERIES, a.sq) + a.shift));
@@ -78,6 +78,11 @@ __global__ __launch_bounds__(256) void attention_train_kernel(AttentionArgs a) {
     ahead = ahead == lds + (RING - 1) * STAGE ? lds : ahead + STAGE;
     const int j0 = t * KEYS + part * 32;
     if (j0 >= keys || (a.causal && j0 > q0 + 31 + a.shift)) continue;  // nothing of it is seen
+    MaskBytes bytes[SUBS];
+    if constexpr (MASK) {
+#pragma unroll
+      for (int u = 0; u < SUBS; u++) bytes[u].load_keys(a, mask, qi, j0 + u * 32);
+    }
     f32x16 s[SUBS];
     RowVectors<T, EL, DP> k[SUBS];
     k[0].template load<0>(here);
@@ -93,10 +98,11 @@ __global__ __launch_bounds__(256) void attention_train_kernel(AttentionArgs a) {
     v[0].template load<T::SIZE>(here);
     if constexpr (SUBS == 2) v[1].template load<T::SIZE + 32 * T::ROW>(here);
     if constexpr (!EL::F32) in_order();
-    if (mask || j0 + SUBS * 32 > keys || (a.causal && j0 + SUBS * 32 - 1 > q0 + a.shift)) {
+    if (MASK || j0 + SUBS * 32 > keys || (a.causal && j0 + SUBS * 32 - 1 > q0 + a.shift)) {
 #pragma unroll
       for (int u = 0; u < SUBS; u++) {
-        const uint32_t see = keys_seen(a, mask, qi, j0 + u * 32, keys);
+        uint32_t see = keys_seen(a, qi, j0 + u * 32, keys);
+        if constexpr (MASK) see &= bytes[u].kept();
 #pragma unroll
         for (int e = 0; e < 16; e++) s[u][e] = (see >> e) & 1 ? s[u][e] : -INF;
       }
@@ -170,7 +176,9 @@ __global__ __launch_bounds__(256) void attention_train_kernel(AttentionArgs a) {
 template <class EL, int DP, int KW>
 void launch(nxh_context *ctx, AttentionArgs a) {
   a.tiles = (a.sq + 128 / KW - 1) / (128 / KW);
-  hipLaunchKernelGGL((attention_train_kernel<EL, DP, KW>), dim3((unsigned)(a.batch * a.heads * a.tiles)), dim3(256), 0, ctx->stream, a);
+  const dim3 grid((unsigned)(a.batch * a.heads * a.tiles));
+  if (a.mask.base) hipLaunchKernelGGL((attention_train_kernel<EL, DP, KW, true>), grid, dim3(256), 0, ctx->stream, a);
+  else hipLaunchKernelGGL((attention_train_kernel<EL, DP, KW, false>), grid, dim3(256), 0, ctx->stream, a);
 }
 template <class EL, int KW>
 void launch_dim(nxh_context *ctx, const AttentionArgs &a) {
