@@ -417,7 +417,7 @@ int nxh_log_probs_with_grad(nxh_context *ctx, const nxh_tensor *log_p, const nxh
    strides any (heads split from a projection's rows; zero for inputs). Query i sees key j if
    j < lengths[its batch] (int32 [batch]; NULL: all), if mask (bool [batch, heads, queries, keys], any
    strides; NULL: all) is true there, and with causal != 0 if j <= i + keys - queries. Over what it sees,
-   s_j = scale q_i . k_j (0 < scale <= 1e30):
+   s_j = scale q_i . k_j (1e-30 <= scale <= 1e30):
      lse_i = log sum e^(s_j)  (float32 [batch, heads, queries], any strides),  out_i = sum e^(s_j - lse_i) v_j
    A query that sees no key has out 0 and lse -inf. Keys from a sequence's length on are not read. A key
    hidden by the mask or by causal has probability 0, which multiplies its v like any other: an infinity

@@ -503,21 +503,35 @@ __global__ __launch_bounds__(128 * PAIRS) __attribute__((amdgpu_waves_per_eu(2))
   else run(std::integral_constant<bool, false>{});
 }
 
-// The parts' sums, in order.
-template <class EL>
+// The parts' sums, in order, V elements of a row at a time. (There are parts for few rows only: all sizes fit 32 bits.)
+template <class EL, int V>
 __global__ __launch_bounds__(256) void attention_grad_join_kernel(AttentionArgs a) {
   using S = typename EL::S;
-  const int64_t row = 2 * (int64_t)a.dim, size = (int64_t)a.batch * a.kv_heads * a.sk * row;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
-    float sum = a.partial[i];
-    for (int p = 1; p < a.parts; p++) sum = sum + a.partial[(int64_t)p * size + i];
-    const int64_t r = i / row;
-    const int at = (int)(i - r * row), j = (int)(r % a.sk), bh = (int)(r / a.sk), b = bh / a.kv_heads, h = bh % a.kv_heads;
-    const bool is_k = at < a.dim;
-    const HeadOperand &o = is_k ? a.dk : a.dv;
-    S *to = const_cast<S *>(rows_of<EL>(o, b, h)) + (int64_t)j * o.row + (is_k ? at : at - a.dim);
-    if constexpr (EL::F32) *to = sum;
-    else *to = (uint16_t)pack2<EL>(sum, 0.0f);
+  const uint32_t of_row = 2u * (uint32_t)a.dim / V, rows = (uint32_t)a.batch * (uint32_t)a.kv_heads * (uint32_t)a.sk;
+  const int64_t part = (int64_t)rows * 2 * a.dim;
+  const uint32_t each = 256 / of_row, row = blockIdx.x * each + threadIdx.x / of_row;  // (a row has at most 256 elements)
+  if (threadIdx.x >= each * of_row || row >= rows) return;
+  const int at = (int)(threadIdx.x % of_row) * V;
+  const float *from = a.partial + (int64_t)row * 2 * a.dim + at;
+  float sum[V];
+  __builtin_memcpy(sum, from, sizeof sum);
+  for (int p = 1; p < a.parts; p++) {
+    float more[V];
+    __builtin_memcpy(more, from + p * part, sizeof more);
+#pragma unroll
+    for (int j = 0; j < V; j++) sum[j] = sum[j] + more[j];
+  }
+  const uint32_t bh = row / (uint32_t)a.sk, j = row - bh * (uint32_t)a.sk, b = bh / (uint32_t)a.kv_heads, h = bh - b * (uint32_t)a.kv_heads;
+  const bool is_k = at < a.dim;
+  const HeadOperand &o = is_k ? a.dk : a.dv;
+  S *to = const_cast<S *>(rows_of<EL>(o, (int)b, (int)h)) + (int64_t)j * o.row + (is_k ? at : at - a.dim);
+  if constexpr (EL::F32) {
+    __builtin_memcpy(to, sum, sizeof sum);
+  } else if constexpr (V == 4) {
+    const uint32_t w[2] = {pack2<EL>(sum[0], sum[1]), pack2<EL>(sum[2], sum[3])};
+    __builtin_memcpy(to, w, sizeof w);
+  } else {
+    *to = (uint16_t)pack2<EL>(sum[0], 0.0f);
   }
 }
 
@@ -543,8 +557,10 @@ void launch(nxh_context *ctx, AttentionArgs a) {
                        dim3(128 * PAIRS), 0, ctx->stream, a);
   }
   if (!a.partial) return;
-  const int64_t size = (int64_t)a.batch * a.kv_heads * a.sk * 2 * a.dim;
-  hipLaunchKernelGGL((attention_grad_join_kernel<EL>), dim3((unsigned)std::min<int64_t>((size + 255) / 256, 1 << 16)), dim3(256), 0, ctx->stream, a);
+  const int v = a.dim % 4 == 0 ? 4 : 1, each = 256 / (2 * a.dim / v), rows = a.batch * a.kv_heads * a.sk;
+  const dim3 grid((unsigned)((rows + (int64_t)each - 1) / each));
+  if (v == 4) hipLaunchKernelGGL((attention_grad_join_kernel<EL, 4>), grid, dim3(256), 0, ctx->stream, a);
+  else hipLaunchKernelGGL((attention_grad_join_kernel<EL, 1>), grid, dim3(256), 0, ctx->stream, a);
 }
 template <class EL, int DP>
 void launch_mask(nxh_context *ctx, const AttentionArgs &a) {
@@ -581,11 +597,16 @@ NXH_EXPORT int nxh_attention_grad(nxh_context *ctx, const nxh_tensor *dq, const 
   for (const nxh_tensor *r : results)
     for (const nxh_tensor *i : inputs)
       if (same_start(r, i)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "a gradient must not replace an input");
-  // A block has 128 keys of a head and walks over all queries that see them: cut into parts where that leaves units
-  // without work, down to parts of four tiles.
+  // A block has the keys that four waves or pairs of waves share and walks over all queries that see them: cut into parts where
+  // that leaves units without work, down to parts of four tiles. A unit has room for one block of float32 heads of more than 64,
+  // else for two. Under a causal mask the first blocks walk over twice the mean: wide heads take twice as many parts, and the last
+  // ones fill the gaps ([1,16,8192,128] 757 us, and 697 + 15 for the sums; of [4,12,1024,64] 33, and 32 + 11).
   const int units = ctx->compute_units > 0 ? ctx->compute_units : 256;
-  const int64_t blocks = (int64_t)a.batch * a.kv_heads * ((a.sk + 127) / 128), walk = (int64_t)(a.heads / a.kv_heads) * ((a.sq + 31) / 32);
-  a.parts = blocks > 0 && walk > 0 ? (int)std::max<int64_t>(1, std::min<int64_t>({16, 2 * units / blocks, walk / 4})) : 1;
+  const bool wide = a.dim > 64, f32 = dt == NXH_F32;
+  const int tile = wide && !f32 ? 64 : 128;
+  const int64_t blocks = (int64_t)a.batch * a.kv_heads * ((a.sk + tile - 1) / tile), walk = (int64_t)(a.heads / a.kv_heads) * ((a.sq + 31) / 32);
+  const int64_t room = (wide ? (f32 ? 1 : 2) * (a.causal ? 2 : 1) : 2) * (int64_t)units;
+  a.parts = blocks > 0 && walk > 0 ? (int)std::max<int64_t>(1, std::min<int64_t>({16, room / blocks, walk / 4})) : 1;
   if ((double)blocks * a.parts > 2147483647.0) return nxh_fail(NXH_FAILURE, op, "too many rows for one launch");
   std::lock_guard<std::mutex> guard(ctx->mu);
   NXH_HIP(op, hipSetDevice(ctx->device));

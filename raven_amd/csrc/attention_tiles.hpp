@@ -493,7 +493,7 @@ int attention_arguments(const char *op, AttentionArgs &a, const nxh_tensor *q, c
   if (q->ndim != 4 || k->ndim != 4) return nxh_fail(NXH_INVALID_ARGUMENT, op, "operands must be [batch, heads, length, dim]");
   const int64_t b = q->shape[0], h = q->shape[1], sq = q->shape[2], d = q->shape[3], hk = k->shape[1], sk = k->shape[2];
   if (hk == 0 ? h != 0 : h % hk != 0) return nxh_fail(NXH_INVALID_ARGUMENT, op, "heads must be a multiple of the heads of keys and values");
-  if (!(scale > 0.0 && scale <= 1e30)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "scale must be positive and at most 1e30");
+  if (!(scale >= 1e-30 && scale <= 1e30)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "scale must lie in 1e-30 to 1e30");  // (a normal float32)
   if (d < 1) return nxh_fail(NXH_INVALID_ARGUMENT, op, "head dimension must not be 0");
   if (d > 128) return nxh_fail(NXH_FAILURE, op, "head dimension must be at most 128");
   if (sq > 0x3fffff00 || sk > 0x3fffff00) return nxh_fail(NXH_FAILURE, op, "more than 2^30 - 256 queries or keys");

@@ -121,6 +121,24 @@ def test_many_blocks(hip, oracle, d):
     run(hip, oracle, d, 3, 50, 50, 130, 140, 32, True, seed=9)
 
 
+@pytest.mark.parametrize("d", [F32, BF16, F16])
+@pytest.mark.parametrize("dim", [6, 12, 65, 127])
+def test_sums_of_parts(hip, oracle, d, dim):
+    run(hip, oracle, d, 1, 4, 1, 300, 130, dim, seed=14)
+
+
+@pytest.mark.parametrize("d, dim", [(BF16, 64), (BF16, 128), (BF16, 63), (F16, 32), (F16, 96), (F32, 32), (F32, 64), (F32, 90), (F32, 128)])
+@pytest.mark.parametrize("mask", [None, 0.4])
+def test_more_blocks_than_units(hip, oracle, d, dim, mask):
+    """Heads enough for the widest blocks of queries, and for gradients of keys without parts."""
+    run(hip, oracle, d, 4, 64, 32, 260, 140, dim, mask is None, [140, 0, 77, 1], mask, seed=15)
+
+
+@pytest.mark.parametrize("d", [F32, BF16])
+def test_more_blocks_than_units_in_a_projection(hip, oracle, d):
+    run(hip, oracle, d, 2, 128, 128, 270, 100, 40, True, seed=16, view=packed)
+
+
 # ── layouts ─────────────────────────────────────────────────────────────────────────────────────
 
 def packed(hip, storage, d):
@@ -315,7 +333,7 @@ def test_refusals(hip):
         hip.attention_train(q, t(2, 3, 5, 8), t(2, 3, 5, 8), 1.0)
     with pytest.raises(ValueError, match="batch, heads"):
         hip.attention_train(t(4, 6, 8), t(4, 5, 8), t(4, 5, 8), 1.0)
-    for scale in (0.0, -1.0, float("nan"), float("inf")):
+    for scale in (0.0, -1.0, 1e-31, 1e31, float("nan"), float("inf")):
         with pytest.raises(ValueError, match="scale"):
             hip.attention_train(q, k, k, scale)
     with pytest.raises(ValueError, match="shape"):
