@@ -421,15 +421,18 @@ int nxh_log_probs_with_grad(nxh_context *ctx, const nxh_tensor *log_p, const nxh
      lse_i = log sum e^(s_j)  (float32 [batch, heads, queries], any strides),  out_i = sum e^(s_j - lse_i) v_j
    A query that sees no key has out 0 and lse -inf. Keys from a sequence's length on are not read. A key
    hidden by the mask or by causal has probability 0, which multiplies its v like any other: an infinity
-   or a NaN there may reach queries that do not see it. Sums are float32, with one rounding on the way out; f16 and bf16
-   round the exponentials for their product with v. */
+   or a NaN there may reach queries that do not see it. Sums are float32, with one rounding on the way
+   out; f16 and bf16 round the exponentials for their product with v. No result replaces an input or
+   the other (Invalid_argument where they begin at one element; other overlaps are undefined). */
 int nxh_attention_train(nxh_context *ctx, const nxh_tensor *out, const nxh_tensor *lse, const nxh_tensor *q, const nxh_tensor *k,
                         const nxh_tensor *v, const nxh_tensor *lengths, const nxh_tensor *mask, double scale, int causal);
 /* The gradients of q, k and v for g, what flows back into out; out and lse as nxh_attention_train gave
-   them, the other arguments as it took them. dk and dv are summed over the query heads that share them, zeros from a
-   sequence's length on; a query that sees no key has dq 0. f16 and bf16 round the probabilities and the scores'
-   gradients for their products. A gradient never replaces an input (Invalid_argument where both begin
-   at one element; other overlaps are undefined). No atomics: equal calls give equal bits. */
+   them, the other arguments as it took them. dk and dv are summed over the query heads that share them,
+   zeros from a sequence's length on; a query that sees no key has dq 0. f16 and bf16 round the
+   probabilities and the scores' gradients for their products (f16: p (g . v - g . out) beyond 2047 is
+   infinite there). A hidden pair's zeros multiply k, q and g like any others. A gradient replaces no
+   input and no other gradient (Invalid_argument where they begin at one element; other overlaps are
+   undefined). No atomics: equal calls give equal bits. */
 int nxh_attention_grad(nxh_context *ctx, const nxh_tensor *dq, const nxh_tensor *dk, const nxh_tensor *dv, const nxh_tensor *g,
                        const nxh_tensor *q, const nxh_tensor *k, const nxh_tensor *v, const nxh_tensor *out, const nxh_tensor *lse,
                        const nxh_tensor *lengths, const nxh_tensor *mask, double scale, int causal);
@@ -440,23 +443,25 @@ int nxh_attention_grad(nxh_context *ctx, const nxh_tensor *dq, const nxh_tensor 
      (a, b) -> amplitude (a cos(s f_i) - b sin(s f_i), a sin(s f_i) + b cos(s f_i))
    and the other dimensions are copied. flags: bit 0, pairs are neighbours (2 i, 2 i + 1), else halves
    (i, i + n); bit 1, angles negated, which is the gradient. f16/bf16/f32/f64, rows contiguous, other strides any.
-   Angles are float64, sine and cosine float32 (float64 for float64), one rounding on the way out. A result may be its own
-   operand (the same view); other overlaps are undefined. */
+   Angles are float64, sine and cosine float32 (float64 for float64), one rounding on the way out. A
+   result may be its own operand (the same view); both results in one place: Invalid_argument; other
+   overlaps are undefined. */
 int nxh_rotary(nxh_context *ctx, const nxh_tensor *q_out, const nxh_tensor *k_out, const nxh_tensor *q, const nxh_tensor *k,
                const nxh_tensor *positions, const nxh_tensor *frequencies, double amplitude, int flags);
 
 /* A step of AdamW over `count` tensors at once, in place; tensor i of each list has one shape, all are
    contiguous. params (f16/bf16/f32, all of one dtype), grads (of that dtype), masters (NULL, or float32:
    what 16-bit params are the rounding of; then params are only written). With f = factor (float32, one
-   element; NULL: 1), t = step (int32, one element, from 1 on), lr = rate (float32, one element), all three device memory that a recorded
-   graph reads at each replay:
+   element; NULL: 1), t = step (int32, one element, from 1 on), lr = rate (float32, one element), all three
+   device memory that a recorded graph reads at each replay:
      m = beta1 m + (1 - beta1) f g,  v = beta2 v + (1 - beta2) (f g)^2
      p = p (1 - lr decay) - lr / (1 - beta1^t) m / (sqrt v / sqrt (1 - beta2^t) + eps)
    m and v are float32, or, with m_scales and v_scales (float32 [ceil (elements / 256)] each) and key
-   (int32 [2], device memory), float8_e4m3: elements 256 b .. 256 b + 255 of m are their codes times m_scales[b], those of
-   sqrt v likewise, and each is rounded to one of its two neighbours by random bits (nxh_threefry of key; another
-   key each step), sqrt v that is not 0 not to 0. A gradient that is not finite leaves its element (8 bits: its block of 256) not
-   finite. The same tensor twice among those that are written: Invalid_argument. */
+   (int32 [2], device memory), float8_e4m3: elements 256 b .. 256 b + 255 of m are their codes times
+   m_scales[b], those of sqrt v likewise, and each is rounded to one of its two neighbours by random bits
+   (nxh_threefry of key; another key each step), sqrt v that is not 0 not to 0. A gradient that is not
+   finite leaves its element (8 bits: its block of 256) not
+   finite. What is written must not overlap anything else in the lists: Invalid_argument. */
 int nxh_adamw(nxh_context *ctx, int count, const nxh_tensor *const *params, const nxh_tensor *const *grads,
               const nxh_tensor *const *m, const nxh_tensor *const *v, const nxh_tensor *const *masters,
               const nxh_tensor *const *m_scales, const nxh_tensor *const *v_scales, const nxh_tensor *rate,

@@ -319,7 +319,12 @@ NXH_EXPORT int nxh_adamw(nxh_context *ctx, int count, const nxh_tensor *const *p
   if (key && (key->dtype != NXH_I32 || key->ndim != 1 || key->shape[0] != 2)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "key must be two int32");
   if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "beta1 and beta2 must be at least 0 and below 1");
   if (!(eps >= 0.0) || !(decay >= 0.0)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "eps and decay must be >= 0");
-  std::vector<const char *> written;
+  struct Range {
+    const char *begin, *end;
+    bool written;
+  };
+  std::vector<Range> ranges;
+  ranges.reserve((size_t)count * (3 + (masters ? 1 : 0) + (m_scales ? 2 : 0) + 1));
   for (int i = 0; i < count; i++) {
     const nxh_tensor *all[] = {params[i], grads[i], m[i], v[i], masters ? masters[i] : nullptr, m_scales ? m_scales[i] : nullptr, v_scales ? v_scales[i] : nullptr};
     const int kinds[] = {dt, dt, bits == 8 ? NXH_F8E4M3 : NXH_F32, bits == 8 ? NXH_F8E4M3 : NXH_F32, NXH_F32, NXH_F32, NXH_F32};
@@ -333,12 +338,16 @@ NXH_EXPORT int nxh_adamw(nxh_context *ctx, int count, const nxh_tensor *const *p
       if (k < 5 ? !nxh_same_shape(t, params[i]) : t->ndim != 1 || t->shape[0] != (elements(params[i]) + SCALE - 1) / SCALE)
         return nxh_fail(NXH_INVALID_ARGUMENT, op, NXH_ERR_SHAPE);
       if (!dense(t)) return nxh_fail(NXH_FAILURE, op, "tensors must be contiguous");
-      if (k != 1 && elements(t) > 0) written.push_back(start_of(t));
+      if (elements(t) > 0) ranges.push_back({start_of(t), start_of(t) + elements(t) * (int64_t)nxh_elem_size(t->dtype), k != 1});
     }
   }
-  std::sort(written.begin(), written.end());
-  if (std::adjacent_find(written.begin(), written.end()) != written.end())
-    return nxh_fail(NXH_INVALID_ARGUMENT, op, "a tensor that is written appears twice");
+  std::sort(ranges.begin(), ranges.end(), [](const Range &x, const Range &y) { return x.begin < y.begin; });
+  const char *end = nullptr, *written_end = nullptr;  // of the ranges so far, and of those that are written
+  for (const Range &r : ranges) {
+    if (r.begin < (r.written ? end : written_end)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "a tensor that is written appears twice");
+    end = std::max(end, r.end);
+    if (r.written) written_end = std::max(written_end, r.end);
+  }
   const AdamwCall c = {count, dt, params, grads, m, v, masters, m_scales, v_scales};
   auto fill = [&](auto &a) {
     a.rate = (const float *)start_of(rate);

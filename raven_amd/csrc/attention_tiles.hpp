@@ -479,8 +479,11 @@ int attention_operand(const char *op, const nxh_tensor *t, int dt, int64_t b, in
   return NXH_OK;
 }
 
-// Whether two operands begin at one element.
+// Whether two operands that have elements begin at one address.
 bool same_start(const nxh_tensor *a, const nxh_tensor *b) {
+  for (const nxh_tensor *t : {a, b})
+    for (int d = 0; d < t->ndim; d++)
+      if (t->shape[d] == 0) return false;
   return (const char *)a->data + a->offset * (int64_t)nxh_elem_size(a->dtype) == (const char *)b->data + b->offset * (int64_t)nxh_elem_size(b->dtype);
 }
 

@@ -199,6 +199,8 @@ NXH_EXPORT int nxh_rotary(nxh_context *ctx, const nxh_tensor *q_out, const nxh_t
               y->strides[0], y->strides[1], y->strides[2], (int)x->shape[1], (int)((x->shape[1] + HEADS - 1) / HEADS)};
     in_place = in_place && one_view(x, y);
   }
+  if (k && a.x[0].out == a.x[1].out && a.x[0].heads > 0 && a.x[1].heads > 0 && q->shape[0] > 0 && q->shape[2] > 0 && q->shape[3] > 0)
+    return nxh_fail(NXH_INVALID_ARGUMENT, op, "two results in one place");
   const int64_t batch = q->shape[0], length = q->shape[2], dim = q->shape[3];
   if (positions->ndim != 2 || positions->shape[0] != batch || positions->shape[1] != length || frequencies->ndim != 1)
     return nxh_fail(NXH_INVALID_ARGUMENT, op, NXH_ERR_SHAPE);

@@ -364,3 +364,19 @@ def test_refusals(hip):
         hip.adamw(*lists(), r, s, m_scales=[t(1)], v_scales=[t(1)], key=key)
     with pytest.raises(TypeError):
         hip.adamw(5, [], [], [], r, s)
+
+
+def test_overlaps(hip):
+    """Parameters in one buffer, side by side and over each other; gradients may be shared, but not written."""
+    t = lambda *s: hip.buffer(F32, s)  # noqa: E731
+    r, s, flat = one(hip, 0.1, F32), one(hip, 1, I32), t(100)
+    part = lambda a, b: hip.shrink(flat, [(a, b)])  # noqa: E731
+    g = t(50)
+    states = lambda n: ([t(n), t(n)], [t(n), t(n)])  # noqa: E731
+    hip.adamw([part(50, 100), part(0, 50)], [g, g], *states(50), r, s)
+    with pytest.raises(ValueError, match="twice"):
+        hip.adamw([part(0, 50), part(49, 99)], [g, g], *states(50), r, s)
+    with pytest.raises(ValueError, match="twice"):
+        hip.adamw([part(0, 30)], [part(20, 50)], [t(30)], [t(30)], r, s)
+    with pytest.raises(ValueError, match="twice"):
+        hip.adamw([t(30)], [part(20, 50)], [part(49, 79)], [t(30)], r, s)

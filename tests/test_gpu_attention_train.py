@@ -370,3 +370,21 @@ def test_refusals(hip):
         hip.attention_grad(k, q, k, k, *y, 1.0)
     with pytest.raises(RuntimeError, match="dtype"):
         hip.attention_grad(q, q, k, k, y[0], t(2, 4, 6, d=BF16), 1.0)
+
+
+def test_results_in_one_place(hip):
+    t = lambda *s: hip.buffer(F32, s)  # noqa: E731
+    q, k = t(2, 2, 6, 8), t(2, 2, 6, 8)
+    y = hip.attention_train(q, k, k, 1.0)
+    one = t(2, 2, 6, 8)
+    for out in ((one, one, t(2, 2, 6, 8)), (one, t(2, 2, 6, 8), one), (t(2, 2, 6, 8), one, one)):
+        with pytest.raises(ValueError, match="one place"):
+            hip.attention_grad(q, q, k, k, *y, 1.0, out=out)
+    flat = t(2 * 2 * 6 * 8)
+    lse = hip.reshape(hip.shrink(flat, [(0, 24)]), (2, 2, 6))
+    with pytest.raises(ValueError, match="one place"):
+        hip.attention_train(q, k, k, 1.0, out=(hip.reshape(flat, (2, 2, 6, 8)), lse))
+    with pytest.raises(ValueError, match="replace"):
+        hip.attention_train(q, hip.reshape(flat, (2, 2, 6, 8)), k, 1.0, out=(one, lse))
+    with pytest.raises(ValueError, match="replace"):
+        hip.attention_grad(q, q, k, k, y[0], lse, 1.0, out=(hip.reshape(flat, (2, 2, 6, 8)), one, t(2, 2, 6, 8)))

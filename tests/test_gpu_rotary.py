@@ -218,3 +218,5 @@ def test_refusals(hip):
     for amplitude in (float("nan"), float("inf")):
         with pytest.raises(ValueError, match="amplitude"):
             hip.rotary(q, None, p, f, amplitude=amplitude)
+    with pytest.raises(ValueError, match="one place"):
+        hip.rotary(q, t(2, 3, 4, 8), p, f, out=(q, q))
