@@ -9,6 +9,8 @@ AdamW's first step divides a gradient by its own size (m / sqrt v = sign): its e
 up to the rate, those above by 1e-3 / 1e-2 of it, a tenth. So weights are compared after three steps where all three gradients are above
 that: within 3 x 0.1 rates; and no weight is off by more than 6 rates."""
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -139,3 +141,51 @@ def test_recorded_step(hip):
             same_bits(logical(grads[n]), logical(grads_e[n]), n)
             same_bits(logical(recorded.w[n]).copy(), logical(eager.w[n]).copy(), n)
     graph.destroy()
+
+
+def steps_of(hip, seed):
+    """The weights after a problem's steps."""
+    weights, batches, f, lengths = problem(seed)
+    block = Block(hip, weights, f, lengths)
+    for step, (x, positions, target) in enumerate(batches, 1):
+        hip.assign(block.step, tensor(hip, np.array([step], np.int32), dt.int32))
+        block.train(tensor(hip, x), tensor(hip, positions, dt.int32), tensor(hip, target))
+    return {n: logical(block.w[n]).copy() for n in NAMES}
+
+
+def test_deferred_steps(hip):
+    want = steps_of(hip, 3)
+    hip.set_deferred(True)
+    try:
+        got = steps_of(hip, 3)
+    finally:
+        hip.set_deferred(False)
+    for n in NAMES:
+        np.testing.assert_allclose(got[n], want[n], rtol=0, atol=2 * 3 * RATE)  # (fused sums may turn a sign: two rates a step)
+
+
+def test_steps_of_two_threads(hip):
+    """On one context, and on two of the one GPU: the bits that the steps alone get."""
+    want = [steps_of(hip, s) for s in (4, 5)]
+    other = Backend()
+    try:
+        for contexts in ((hip, hip), (hip, other)):
+            errors = []
+
+            def body(i, contexts=contexts, errors=errors):
+                try:
+                    for _ in range(4):
+                        got = steps_of(contexts[i], i + 4)
+                        for n in NAMES:
+                            same_bits(got[n], want[i][n], f"{n} of thread {i}")
+                except BaseException as exc:  # noqa: BLE001 - reported below
+                    errors.append((i, repr(exc)))
+
+            threads = [threading.Thread(target=body, args=(i,)) for i in range(2)]
+            for t in threads:
+                t.start()
+            for t in threads:
+                t.join()
+            assert not errors, errors
+    finally:
+        other.close()
