@@ -326,8 +326,12 @@ NXH_EXPORT int nxh_adamw(nxh_context *ctx, int count, const nxh_tensor *const *p
     const char *begin, *end;
     bool written;
   };
-  std::vector<Range> ranges;
-  ranges.reserve((size_t)count * (3 + (masters ? 1 : 0) + (m_scales ? 2 : 0) + 1));
+  std::vector<Range> ranges;  // (all its room is taken here)
+  try {
+    ranges.reserve((size_t)count * (4 + (masters ? 1 : 0) + (m_scales ? 2 : 0)));
+  } catch (const std::bad_alloc &) {
+    return nxh_fail(NXH_FAILURE, op, "out of host memory");
+  }
   for (int i = 0; i < count; i++) {
     const nxh_tensor *all[] = {params[i], grads[i], m[i], v[i], masters ? masters[i] : nullptr, m_scales ? m_scales[i] : nullptr, v_scales ? v_scales[i] : nullptr};
     const int kinds[] = {dt, dt, bits == 8 ? NXH_F8E4M3 : NXH_F32, bits == 8 ? NXH_F8E4M3 : NXH_F32, NXH_F32, NXH_F32, NXH_F32};

@@ -235,9 +235,11 @@ __device__ __forceinline__ void store_key(const AttentionArgs &a, const W &w, in
   }
 }
 
-// Blocks of four waves with 32 keys each, for heads of up to 64. What a block walks over is cut into a.parts, a block each, where
-// there would be few blocks; their sums are joined by another launch.
-template <class EL, int DP, bool MASK>
+// For heads of up to 64. Blocks of four waves. KW = 1: each has 32 keys. KW = 2: two share 32 keys, each takes every other 32 queries of a
+// tile, and their sums are added at the end: where there would be fewer than two blocks a unit ([4,12,1024,64] bfloat16 causal 32.7 and
+// 30.8 us, [8,12,1024,64] 47 and 52; [2,12,1024,64] not causal 27.9 + 7.2 for sums of parts, and 27.4). What a block walks over is cut into
+// a.parts, a block each, where there would still be few; their sums are joined by another launch.
+template <class EL, int DP, int KW, bool MASK>
 __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs a) {
   constexpr int QUERIES = EL::F32 ? 32 : 64, OT = DP / 32;
   using T = Tile<EL, DP, QUERIES, 4>;
@@ -245,8 +247,9 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
   __shared__ __attribute__((aligned(1024))) unsigned char stages[RING * STAGE];
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  KeysWalk<EL, QUERIES> w(a);
-  const int k0 = w.first + wave * 32, kj = k0 + (threadIdx.x & 31);
+  const int pair = wave / KW, share = wave % KW;
+  KeysWalk<EL, QUERIES, 128 / KW> w(a);
+  const int k0 = w.first + pair * 32, kj = k0 + (threadIdx.x & 31);
   const uint32_t lds = lds_address(stages);
   T qt, gt;
   qt.begin(wave, a.q.row);
@@ -306,11 +309,11 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
     const uint32_t now = stage;
     stage = stage == lds + 2 * STAGE ? lds : stage + STAGE;
     ahead = ahead == lds + 2 * STAGE ? lds : ahead + STAGE;
-    const int i0 = at * QUERIES, head_now = head;
+    const int i0 = at * QUERIES + share * 32, head_now = head;
     if (++at == w.tiles) at = w.before, head++;
-    if (k0 >= w.keys || (a.causal && k0 > i0 + QUERIES - 1 + a.shift)) continue;  // nothing of the tile sees these keys
-    const Places<T, EL> here = places.in(now);
-    uint32_t values = now + half16;
+    if (k0 >= w.keys || (a.causal && k0 > i0 + QUERIES / KW - 1 + a.shift)) continue;  // nothing of the tile sees these keys
+    const Places<T, EL> here = places.in(now + (uint32_t)(share * 32 * T::ROW));
+    uint32_t values = now + (uint32_t)share * 256 + half16;
     asm("" : "+v"(values));
     MaskBytes bytes;
     auto begin = [&](int r0, f32x16 &p) {
@@ -348,7 +351,7 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
     differences(0, l, p, ds);
     pw.set(p);
     dsw.set(ds);
-    if constexpr (QUERIES == 64) {
+    if constexpr (QUERIES / KW == 64) {
       g.add(dv, pw);
       q.add(dk, dsw);
       begin(32, p);
@@ -364,6 +367,24 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
     }
     g.add(dv, pw);
     q.add(dk, dsw);
+  }
+  if constexpr (KW == 2) {  // the odd wave of a pair hands over
+    static_assert(sizeof(float) * 4 * OT * 16 * 64 <= sizeof(stages), "sums of two waves fit the stages");
+    float(*over)[2 * OT * 16][64] = reinterpret_cast<float(*)[2 * OT * 16][64]>(stages);
+    const int lane = threadIdx.x & 63;
+    __syncthreads();
+    if (share == 1) {
+#pragma unroll
+      for (int t = 0; t < OT; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) over[pair][t * 16 + e][lane] = dk[t][e], over[pair][(OT + t) * 16 + e][lane] = dv[t][e];
+    }
+    __syncthreads();
+    if (share == 1) return;
+#pragma unroll
+    for (int t = 0; t < OT; t++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) dk[t][e] = dk[t][e] + over[pair][t * 16 + e][lane], dv[t][e] = dv[t][e] + over[pair][(OT + t) * 16 + e][lane];
   }
   if (kj >= a.sk) return;
   store_key<EL, DP>(a, w, kj, true, dk);
@@ -541,7 +562,7 @@ __global__ __launch_bounds__(256) void attention_grad_join_kernel(AttentionArgs 
 }
 
 template <class EL, int DP, bool MASK>
-void launch(nxh_context *ctx, AttentionArgs a) {
+void launch(nxh_context *ctx, AttentionArgs a, int keys_of_block) {
   const int units = ctx->compute_units > 0 ? ctx->compute_units : 256;
   const auto blocks_of = [&](int heads, int n) { return dim3((unsigned)(a.batch * heads * n)); };
   if (a.sq > 0 && a.heads > 0) {
@@ -555,7 +576,11 @@ void launch(nxh_context *ctx, AttentionArgs a) {
   }
   if (a.sk == 0) return;
   if constexpr (DP <= 64) {
-    hipLaunchKernelGGL((attention_grad_keys_kernel<EL, DP, MASK>), blocks_of(a.kv_heads, (a.sk + 127) / 128 * a.parts), dim3(256), 0, ctx->stream, a);
+    const dim3 grid = blocks_of(a.kv_heads, (a.sk + keys_of_block - 1) / keys_of_block * a.parts);
+    if constexpr (!EL::F32) {
+      if (keys_of_block == 64) hipLaunchKernelGGL((attention_grad_keys_kernel<EL, DP, 2, MASK>), grid, dim3(256), 0, ctx->stream, a);
+    }
+    if (keys_of_block == 128) hipLaunchKernelGGL((attention_grad_keys_kernel<EL, DP, 1, MASK>), grid, dim3(256), 0, ctx->stream, a);
   } else {
     constexpr int PAIRS = EL::F32 ? 4 : 2;
     hipLaunchKernelGGL((attention_grad_wide_keys_kernel<EL, DP, PAIRS, MASK>), blocks_of(a.kv_heads, (a.sk + 32 * PAIRS - 1) / (32 * PAIRS) * a.parts),
@@ -568,16 +593,16 @@ void launch(nxh_context *ctx, AttentionArgs a) {
   else hipLaunchKernelGGL((attention_grad_join_kernel<EL, 1>), grid, dim3(256), 0, ctx->stream, a);
 }
 template <class EL, int DP>
-void launch_mask(nxh_context *ctx, const AttentionArgs &a) {
-  if (a.mask.base) launch<EL, DP, true>(ctx, a);
-  else launch<EL, DP, false>(ctx, a);
+void launch_mask(nxh_context *ctx, const AttentionArgs &a, int keys_of_block) {
+  if (a.mask.base) launch<EL, DP, true>(ctx, a, keys_of_block);
+  else launch<EL, DP, false>(ctx, a, keys_of_block);
 }
 template <class EL>
-void launch_dim(nxh_context *ctx, const AttentionArgs &a) {
-  if (a.dim <= 32) launch_mask<EL, 32>(ctx, a);
-  else if (a.dim <= 64) launch_mask<EL, 64>(ctx, a);
-  else if (a.dim <= 96) launch_mask<EL, 96>(ctx, a);
-  else launch_mask<EL, 128>(ctx, a);
+void launch_dim(nxh_context *ctx, const AttentionArgs &a, int keys_of_block) {
+  if (a.dim <= 32) launch_mask<EL, 32>(ctx, a, keys_of_block);
+  else if (a.dim <= 64) launch_mask<EL, 64>(ctx, a, keys_of_block);
+  else if (a.dim <= 96) launch_mask<EL, 96>(ctx, a, keys_of_block);
+  else launch_mask<EL, 128>(ctx, a, keys_of_block);
 }
 
 }  // namespace
@@ -603,14 +628,15 @@ NXH_EXPORT int nxh_attention_grad(nxh_context *ctx, const nxh_tensor *dq, const 
     for (const nxh_tensor *i : inputs)
       if (same_start(r, i)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "a gradient must not replace an input");
   if (same_start(dq, dk) || same_start(dq, dv) || same_start(dk, dv)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "two gradients in one place");
-  // A block has the keys that four waves or pairs of waves share and walks over all queries that see them: cut into parts where
+  // A block has the keys that four waves or pairs of waves have and walks over all queries that see them: cut into parts where
   // that leaves units without work, down to parts of four tiles. A unit has room for one block of float32 heads of more than 64,
   // else for two. Under a causal mask the first blocks walk over twice the mean: wide heads take twice as many parts, and the last
-  // ones fill the gaps ([1,16,8192,128] 757 us, and 697 + 15 for the sums; of [4,12,1024,64] 33, and 32 + 11).
+  // ones fill the gaps ([1,16,8192,128] 757 us, and 697 + 15 for the sums).
   const int units = ctx->compute_units > 0 ? ctx->compute_units : 256;
   const bool wide = a.dim > 64, f32 = dt == NXH_F32;
-  const int tile = wide && !f32 ? 64 : 128;
-  const int64_t blocks = (int64_t)a.batch * a.kv_heads * ((a.sk + tile - 1) / tile), walk = (int64_t)(a.heads / a.kv_heads) * ((a.sq + 31) / 32);
+  const int64_t heads = (int64_t)a.batch * a.kv_heads;
+  const int keys_of_block = !f32 && (wide || heads * ((a.sk + 127) / 128) < 2 * units) ? 64 : 128;
+  const int64_t blocks = heads * ((a.sk + keys_of_block - 1) / keys_of_block), walk = (int64_t)(a.heads / a.kv_heads) * ((a.sq + 31) / 32);
   const int64_t room = (wide ? (f32 ? 1 : 2) * (a.causal ? 2 : 1) : 2) * (int64_t)units;
   a.parts = blocks > 0 && walk > 0 ? (int)std::max<int64_t>(1, std::min<int64_t>({16, room / blocks, walk / 4})) : 1;
   if ((double)blocks * a.parts > 2147483647.0) return nxh_fail(NXH_FAILURE, op, "too many rows for one launch");
@@ -624,9 +650,9 @@ NXH_EXPORT int nxh_attention_grad(nxh_context *ctx, const nxh_tensor *dq, const 
   a.rows = (float *)space;
   a.partial = sums ? (float *)((char *)space + rows) : nullptr;
   nxh_set_path("attention_grad");
-  if (dt == NXH_F32) launch_dim<gemm_tile::ElF32>(ctx, a);
-  else if (dt == NXH_BF16) launch_dim<gemm_tile::ElBF16>(ctx, a);
-  else launch_dim<gemm_tile::ElF16>(ctx, a);
+  if (dt == NXH_F32) launch_dim<gemm_tile::ElF32>(ctx, a, keys_of_block);
+  else if (dt == NXH_BF16) launch_dim<gemm_tile::ElBF16>(ctx, a, keys_of_block);
+  else launch_dim<gemm_tile::ElF16>(ctx, a, keys_of_block);
   nxh_free_locked(ctx, space);  // (the stream orders its next use behind these launches)
   NXH_HIP(op, hipGetLastError());
   return NXH_OK;

@@ -139,6 +139,12 @@ def test_more_blocks_than_units_in_a_projection(hip, oracle, d):
     run(hip, oracle, d, 2, 128, 128, 270, 100, 40, True, seed=16, view=packed)
 
 
+@pytest.mark.parametrize("d, dim", [(BF16, 64), (F16, 32), (BF16, 41)])
+@pytest.mark.parametrize("mask", [None, 0.4])
+def test_more_blocks_of_keys_than_units(hip, oracle, d, dim, mask):
+    run(hip, oracle, d, 4, 128, 128, 100, 140, dim, mask is None, [140, 0, 77, 1], mask, seed=17)
+
+
 # ── layouts ─────────────────────────────────────────────────────────────────────────────────────
 
 def packed(hip, storage, d):
