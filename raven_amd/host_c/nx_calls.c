@@ -766,7 +766,8 @@ static PyObject *calls_matmul(Calls *self, Args args, Py_ssize_t n, PyObject *kw
 }
 
 /* A step of AdamW. Descriptors lie in memory that is kept from call to call (fresh pages would cost more than filling them);
-   a call that finds it taken by another thread's makes its own. */
+   a call that finds it taken by another thread's makes its own. The lists are read once, into tuples of this call's own: another
+   thread may change a list while the library has the call, and storage that went back to the allocator then would be written to. */
 static nxh_tensor *adamw_space;
 static size_t adamw_room;
 static PyObject *calls_adamw(Calls *self, PyObject *args, PyObject *kw) {
@@ -784,9 +785,9 @@ static PyObject *calls_adamw(Calls *self, PyObject *args, PyObject *kw) {
   size_t room = 0;
   for (int l = 0; l < LISTS && !bad; l++) {
     if (!lists[l] || lists[l] == Py_None) continue;
-    if (!(seq[l] = PySequence_Fast(lists[l], "adamw: tensors come in lists"))) bad = 1;
-    else if (l == 0) count = PySequence_Fast_GET_SIZE(seq[0]);
-    else if (PySequence_Fast_GET_SIZE(seq[l]) != count) {
+    if (!(seq[l] = PySequence_Tuple(lists[l]))) bad = 1;
+    else if (l == 0) count = PyTuple_GET_SIZE(seq[0]);
+    else if (PyTuple_GET_SIZE(seq[l]) != count) {
       PyErr_SetString(PyExc_ValueError, "adamw: the lists have different lengths");
       bad = 1;
     }
@@ -810,13 +811,7 @@ static PyObject *calls_adamw(Calls *self, PyObject *args, PyObject *kw) {
     for (Py_ssize_t i = 0; i < count && seq[l] && !bad; i++) {
       const size_t at = (size_t)l * (size_t)count + (size_t)i;
       p[at] = &d[at];
-      PyObject *o = i < PySequence_Fast_GET_SIZE(seq[l]) ? PySequence_Fast_GET_ITEM(seq[l], i) : NULL; /* (describing one may run code that cuts a list) */
-      if (!o) PyErr_SetString(PyExc_ValueError, "adamw: the lists have different lengths"), bad = 1;
-      else {
-        Py_INCREF(o);
-        bad = describe(&d[at], o);
-        Py_DECREF(o);
-      }
+      bad = describe(&d[at], PyTuple_GET_ITEM(seq[l], i));
     }
   const nxh_tensor *one[ONES] = {NULL};
   for (int k = 0; k < ONES && !bad; k++)
