@@ -151,10 +151,11 @@ void nxh_free_locked(nxh_context *ctx, void *p);
 // cache (non-temporal stores) and NXH_STREAM_IN if what is read should (non-temporal loads of
 // every large input). Caller holds ctx->mu.
 enum { NXH_STREAM_OUT = 1u, NXH_STREAM_IN = 2u };
+constexpr int NXH_CACHE_OPERANDS = 16;  // of one access: the written tensor and those that are read
 uint32_t nxh_cache_hints(nxh_context *ctx, int nop, const void *const *base, const uint64_t *bytes,
                          uint32_t allow = NXH_STREAM_OUT | NXH_STREAM_IN);
 // The same bookkeeping for an entry point whose kernels take no hints: the first n_out
-// tensors are written, the others read (NULL entries are skipped). Takes ctx->mu.
+// tensors are written, the others read, fewer than NXH_CACHE_OPERANDS (NULL entries are skipped). Takes ctx->mu.
 void nxh_cache_touch(nxh_context *ctx, const nxh_tensor *const *tensors, int n, int n_out);
 // An entry point that may touch blocks it does not name. Takes ctx->mu.
 void nxh_cache_opaque(nxh_context *ctx);
@@ -210,6 +211,7 @@ enum { NXH_D_UNARY, NXH_D_BINARY, NXH_D_COMPARE, NXH_D_WHERE, NXH_D_CAST, NXH_D_
   do {                                                                                                        \
     if (ctx) {                                                                                                \
       const nxh_tensor *dts__[] = {__VA_ARGS__};                                                              \
+      static_assert((int)(sizeof dts__ / sizeof *dts__) - (n_out) < NXH_CACHE_OPERANDS, "every read is counted"); \
       if (nxh_defer_active(ctx))                                                                              \
         if (int drc__ = nxh_defer_touch(ctx, dts__, (int)(sizeof dts__ / sizeof *dts__), n_out)) return drc__; \
       nxh_cache_touch(ctx, dts__, (int)(sizeof dts__ / sizeof *dts__), n_out);                                \

@@ -327,8 +327,8 @@ uint32_t nxh_cache_hints(nxh_context *ctx, int nop, const void *const *base, con
     return allow;
   }
   const uint64_t pos = ctx->cache_pos;
-  nxh_context::BlockUse *use[8] = {};
-  if (nop > 8) nop = 8;
+  nxh_context::BlockUse *use[NXH_CACHE_OPERANDS] = {};
+  if (nop > NXH_CACHE_OPERANDS) nop = NXH_CACHE_OPERANDS;
   // reads first: an operand that is also the output is read before it is written
   bool in_tracked = false, in_stream = true, out_stream = false;
   for (int pass = 0; pass < 2; pass++) {
@@ -381,12 +381,12 @@ void nxh_cache_touch(nxh_context *ctx, const nxh_tensor *const *tensors, int n, 
   if (!ctx->cache_hints) return;
   // every written tensor is an access of its own; the tensors read share one
   std::lock_guard<std::mutex> g(ctx->mu);
-  const void *base[8];
-  uint64_t bytes[8];
+  const void *base[NXH_CACHE_OPERANDS];
+  uint64_t bytes[NXH_CACHE_OPERANDS];
   int nop = 1;
   base[0] = nullptr;
   bytes[0] = 0;
-  for (int i = n_out; i < n && nop < 8; i++)
+  for (int i = n_out; i < n && nop < NXH_CACHE_OPERANDS; i++)
     if (tensors[i] && (unsigned)tensors[i]->ndim <= NXH_MAX_NDIM) {
       base[nop] = tensors[i]->data;
       bytes[nop++] = tensor_bytes(tensors[i]);
