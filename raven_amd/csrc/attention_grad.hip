@@ -391,15 +391,16 @@ __global__ __launch_bounds__(256) void attention_grad_keys_kernel(AttentionArgs 
   store_key<EL, DP>(a, w, kj, false, dv);
 }
 
-// The same for heads of more than 64. Blocks of eight waves, of which two have the same 32 keys: one makes the scores, p and dv,
-// the other g . v, ds and dk, one tile of queries behind the first, whose p it takes from LDS. So a wave holds the vectors and the
-// sums of one operand, not of two, which for heads of 128 are more registers than two waves of a unit's may have.
+// The same for heads of more than 64. Blocks of two pairs of waves (float32: four), of which the two of a pair have the same 32 keys: one
+// makes the scores, p and dv, the other g . v, ds and dk, one tile of queries behind the first, whose p it takes from LDS. So a wave holds
+// the vectors and the sums of one operand, not of two, which for heads of 128 are more registers than two waves of a unit's may have.
+// Three stages: the tile that is on its way, and those of the two kinds of waves. (A fourth, for two tiles on their way, is 84 KB
+// of 16-bit heads of 128: over half of a unit's LDS.)
 template <class EL, int DP, int PAIRS, bool MASK>
 __global__ __launch_bounds__(128 * PAIRS) __attribute__((amdgpu_waves_per_eu(2))) void attention_grad_wide_keys_kernel(AttentionArgs a) {
   constexpr int QUERIES = 32, OT = DP / 32;
   using T = Tile<EL, DP, QUERIES, PAIRS>;  // (half of the waves bring each operand's)
-  constexpr int STAGE = 2 * T::SIZE + 1024, RING = EL::F32 || PAIRS == 2 ? 3 : 4, VALUES = 2 * T::SIZE;
-  constexpr int AHEAD = RING - 2;  // tiles on their way
+  constexpr int STAGE = 2 * T::SIZE + 1024, RING = 3, VALUES = 2 * T::SIZE;
   __shared__ __attribute__((aligned(1024))) unsigned char stages[RING * STAGE];
   __shared__ __attribute__((aligned(16))) float over[2][PAIRS][4][64][4];  // p, for the other wave: [tile][pair][e / 4][lane][e % 4]
 
@@ -433,14 +434,11 @@ __global__ __launch_bounds__(128 * PAIRS) __attribute__((amdgpu_waves_per_eu(2))
       next += QUERIES * brought.row;
       values_next += QUERIES * 2;
       if (w.next()) find();
-      return brought.direct && left >= QUERIES;
     };
-    bool whole = false;  // what is on its way for the step after this one
     if (w.steps > 0) {
       find();
       fetch(lds);
     }
-    if (AHEAD == 2 && w.steps > 1) whole = fetch(lds + STAGE);
     Column<EL, DP> own;
     own.load(rows_of<EL>(mine, w.b, w.hk) + (int64_t)kj * mine.row, kj < w.keys, a.dim);
     f32x16 acc[OT];
@@ -450,17 +448,10 @@ __global__ __launch_bounds__(128 * PAIRS) __attribute__((amdgpu_waves_per_eu(2))
       for (int e = 0; e < 16; e++) acc[t][e] = 0.0f;
     Places<T, EL> places;
     places.begin();
-    uint32_t stage = lds, ahead = lds + AHEAD * STAGE;
+    uint32_t stage = lds, ahead = lds + STAGE;
     for (int t = 0; w.steps > 0 && t <= w.steps; t++) {
-      // tile t has come, p of the tile before it too, and what is filled next has been used
-      if (t == 0 || !whole) meet<0>();
-      else if (!second && pair == 0) meet<T::LPW + 1>();
-      else meet<T::LPW>();
-      whole = false;
-      if (t + AHEAD < w.steps) {
-        const bool is = fetch(ahead);
-        if (AHEAD == 2) whole = is;
-      }
+      meet<0>();  // tile t has come, p of the tile before it too, and what is filled next has been used
+      if (t + 1 < w.steps) fetch(ahead);
       ahead = ahead == lds + (RING - 1) * STAGE ? lds : ahead + STAGE;
       if (second ? t == 0 : t == w.steps) continue;
       const uint32_t now = stage;
