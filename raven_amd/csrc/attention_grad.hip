@@ -614,10 +614,10 @@ NXH_EXPORT int nxh_attention_grad(nxh_context *ctx, const nxh_tensor *dq, const 
       (rc = attention_operand(op, dk, dt, a.batch, a.kv_heads, a.sk, a.dim, a.dk, true)) || (rc = attention_operand(op, dv, dt, a.batch, a.kv_heads, a.sk, a.dim, a.dv, true)))
     return rc;
   if (a.batch == 0 || a.kv_heads == 0) return NXH_OK;
-  const nxh_tensor *results[] = {dq, dk, dv}, *inputs[] = {g, q, k, v, out, lse};
+  const nxh_tensor *results[] = {dq, dk, dv}, *inputs[] = {g, q, k, v, out, lse, lengths, mask};
   for (const nxh_tensor *r : results)
     for (const nxh_tensor *i : inputs)
-      if (same_start(r, i)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "a gradient must not replace an input");
+      if (i && same_start(r, i)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "a gradient must not replace an input");
   if (same_start(dq, dk) || same_start(dq, dv) || same_start(dk, dv)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "two gradients in one place");
   // A block has the keys that four waves or pairs of waves have and walks over all queries that see them: cut into parts where
   // that leaves units without work, down to parts of four tiles. A unit has room for one block of float32 heads of more than 64,

@@ -218,8 +218,8 @@ NXH_EXPORT int nxh_attention_train(nxh_context *ctx, const nxh_tensor *out, cons
   AttentionArgs a;
   if ((rc = attention_arguments(op, a, q, k, v, out, lse, lengths, mask, scale, causal, false))) return rc;
   if (a.batch == 0 || a.heads == 0 || a.sq == 0) return NXH_OK;
-  for (const nxh_tensor *i : {q, k, v})
-    if (same_start(out, i) || same_start(lse, i)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "a result must not replace an input");
+  for (const nxh_tensor *i : {q, k, v, lengths, mask})
+    if (i && (same_start(out, i) || same_start(lse, i))) return nxh_fail(NXH_INVALID_ARGUMENT, op, "a result must not replace an input");
   if (same_start(out, lse)) return nxh_fail(NXH_INVALID_ARGUMENT, op, "two results in one place");
   std::lock_guard<std::mutex> guard(ctx->mu);
   NXH_HIP(op, hipSetDevice(ctx->device));
