@@ -460,8 +460,8 @@ int nxh_rotary(nxh_context *ctx, const nxh_tensor *q_out, const nxh_tensor *k_ou
    (int32 [2], device memory), float8_e4m3: elements 256 b .. 256 b + 255 of m are their codes times
    m_scales[b], those of sqrt v likewise, and each is rounded to one of its two neighbours by random bits
    (nxh_threefry of key; another key each step), sqrt v that is not 0 not to 0. A gradient that is not
-   finite leaves its element (8 bits: its block of 256) not
-   finite. What is written must not overlap anything else in the lists: Invalid_argument. */
+   finite leaves its element not finite, an infinity its block of 256 of 8-bit states. What is written must
+   not overlap anything else in the lists, nor rate, step, factor or key: Invalid_argument. */
 int nxh_adamw(nxh_context *ctx, int count, const nxh_tensor *const *params, const nxh_tensor *const *grads,
               const nxh_tensor *const *m, const nxh_tensor *const *v, const nxh_tensor *const *masters,
               const nxh_tensor *const *m_scales, const nxh_tensor *const *v_scales, const nxh_tensor *rate,

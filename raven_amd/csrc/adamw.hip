@@ -328,7 +328,7 @@ NXH_EXPORT int nxh_adamw(nxh_context *ctx, int count, const nxh_tensor *const *p
   };
   std::vector<Range> ranges;  // (all its room is taken here)
   try {
-    ranges.reserve((size_t)count * (4 + (masters ? 1 : 0) + (m_scales ? 2 : 0)));
+    ranges.reserve((size_t)count * (4 + (masters ? 1 : 0) + (m_scales ? 2 : 0)) + 4);
   } catch (const std::bad_alloc &) {
     return nxh_fail(NXH_FAILURE, op, "out of host memory");
   }
@@ -347,6 +347,12 @@ NXH_EXPORT int nxh_adamw(nxh_context *ctx, int count, const nxh_tensor *const *p
       if (!dense(t)) return nxh_fail(NXH_FAILURE, op, "tensors must be contiguous");
       if (elements(t) > 0) ranges.push_back({start_of(t), start_of(t) + elements(t) * (int64_t)nxh_elem_size(t->dtype), k != 1});
     }
+  }
+  for (const nxh_tensor *t : {rate, step, factor, key}) {  // of one or two elements of 4 bytes
+    if (!t) continue;
+    const char *at = start_of(t);
+    const int64_t to = t == key ? t->strides[0] * 4 : 0;
+    ranges.push_back({at + std::min<int64_t>(0, to), at + std::max<int64_t>(0, to) + 4, false});
   }
   std::sort(ranges.begin(), ranges.end(), [](const Range &x, const Range &y) { return x.begin < y.begin; });
   const char *end = nullptr, *written_end = nullptr;  // of the ranges so far, and of those that are written
