@@ -142,6 +142,20 @@ int nxh_hip_fail(const char *op, hipError_t e);
     if (e__ != hipSuccess) return nxh_hip_fail(op, e__); \
   } while (0)
 
+// Of a grid with 2^32 lanes or more along a dimension the runtime launches the rest after division by 2^32 and reports nothing (2^24 + 1
+// blocks of 256: one block ran). Every launch is looked at, and one that is too large leaves an error where hipGetLastError finds it.
+bool nxh_grid_refused();
+static inline bool nxh_grid_fits(const dim3 &grid, const dim3 &block) {
+  const uint64_t x = (uint64_t)grid.x * block.x, y = (uint64_t)grid.y * block.y, z = (uint64_t)grid.z * block.z;
+  return ((x | y | z) >> 32) == 0 || nxh_grid_refused();
+}
+#undef hipLaunchKernelGGL
+#define hipLaunchKernelGGL(kernel, grid, block, lds, stream, ...)                                  \
+  do {                                                                                             \
+    const dim3 grid__ = (grid), block__ = (block);                                                 \
+    if (nxh_grid_fits(grid__, block__)) (kernel)<<<grid__, block__, (lds), (stream)>>>(__VA_ARGS__); \
+  } while (0)
+
 // allocator (runtime.hip)
 int nxh_alloc_locked(nxh_context *ctx, size_t bytes, void **out);
 void nxh_free_locked(nxh_context *ctx, void *p);

@@ -24,7 +24,20 @@ int nxh_fail(int kind, const char *op, const char *msg) {
   nxh_set_error(op, msg);
   return kind;
 }
+// (the number of a device that does not exist: an error without any other effect)
+static thread_local bool grid_refused = false;
+bool nxh_grid_refused() {
+  grid_refused = true;
+  (void)hipSetDevice(-1);
+  return false;
+}
 int nxh_hip_fail(const char *op, hipError_t e) {
+  const bool refused = grid_refused && e == hipErrorInvalidDevice;
+  grid_refused = false;
+  if (refused) {
+    (void)hipGetLastError();
+    return nxh_fail(NXH_FAILURE, op, "too many elements for one launch");
+  }
   // Device-runtime errors are Failure, like the reference's non-argument
   // statuses (nx_c_engine.c:1345-1351).
   char buf[256];
