@@ -11,7 +11,7 @@
 // be what follows. A step's own update uses m and v as they are before they are rounded.
 //
 // What bounds it: memory, 28 bytes an element in float32. GPT-2's tensors, 196 with projections apart (124 million elements, bfloat16 with masters) take 675 us
-// in four launches, 5.2 TB/s, with states of 8 bits 444 us in five, 4.5 TB/s; a few small ones 12 us, of which the device has 7.
+// in four launches, 5.2 TB/s, with states of 8 bits 444 to 448 us in five, 4.5 TB/s; a few small ones 13 us, of which the device has 7.
 // A launch takes as many tensors as its arguments hold; a block finds its tensor among them by halving. A lane requests all that it
 // will change before it makes the step's factors.
 
@@ -361,6 +361,9 @@ NXH_EXPORT int nxh_adamw(nxh_context *ctx, int count, const nxh_tensor *const *p
     end = std::max(end, r.end);
     if (r.written) written_end = std::max(written_end, r.end);
   }
+  if (nxh_defer_active(ctx))  // a deferred window may take a tensor's old contents for a constant
+    for (const nxh_tensor *const *written : {params, m, v, masters, m_scales, v_scales})
+      if (written) nxh_defer_written(ctx, written, count);
   const AdamwCall c = {count, dt, params, grads, m, v, masters, m_scales, v_scales};
   auto fill = [&](auto &a) {
     a.rate = (const float *)start_of(rate);

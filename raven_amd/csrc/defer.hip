@@ -1108,6 +1108,16 @@ int nxh_defer_barrier(nxh_context *ctx, const nxh_tensor *out0, const nxh_tensor
   return rc;
 }
 
+// What the window knew about blocks that such a call writes, where it has more than a barrier names.
+void nxh_defer_written(nxh_context *ctx, const nxh_tensor *const *tensors, int n) {
+  if (!ctx || tls_in_flush) return;
+  Window *w = window_of(ctx, false);
+  if (!w) return;
+  std::lock_guard<std::mutex> g(w->mu);
+  for (int i = 0; i < n; i++)
+    if (tensors[i]) w->known.erase(tensors[i]->data);
+}
+
 // The same for an entry point that names its operands: the first n_out are written, the
 // others read. Only the postponed runs those blocks belong to are written.
 int nxh_defer_touch(nxh_context *ctx, const nxh_tensor *const *tensors, int n, int n_out) {

@@ -203,6 +203,7 @@ bool nxh_defer_active(nxh_context *ctx);
 int nxh_defer_flush(nxh_context *ctx);
 int nxh_defer_barrier(nxh_context *ctx, const nxh_tensor *out0 = nullptr, const nxh_tensor *out1 = nullptr,
                       const nxh_tensor *out2 = nullptr);
+void nxh_defer_written(nxh_context *ctx, const nxh_tensor *const *tensors, int n);
 int nxh_defer_touch(nxh_context *ctx, const nxh_tensor *const *tensors, int n, int n_out);
 int nxh_defer_quiet(nxh_context *ctx);
 int nxh_defer_host_read(nxh_context *ctx, const void *src);
