@@ -13,9 +13,9 @@
 // lie below; a result is scaled back in its last multiplication.
 //
 // What bounds it: the matrix instructions of heads of 128, of which seven products take 7/5 of what the formulas have ([1,16,8192,128]
-// bfloat16 causal 1049 us, 655 TFLOP/s of five products, 917 of seven); of heads of 64 the vector unit beside them ([8,12,1024,64] 34 us
+// bfloat16 causal 1049 to 1075 us, 640 to 655 TFLOP/s of five products, 895 to 917 of seven); of heads of 64 the vector unit beside them ([8,12,1024,64] 34 us
 // dq and 47 dk, dv: matrix instructions are 40 % of the second's cycles); in float32 the matrix instructions ([3,6,777,80] with a mask
-// 165 us).
+// 165 to 174 us).
 
 #include "attention_tiles.hpp"
 

@@ -10,11 +10,11 @@
 //
 // A lane has a query: scores come transposed (K Q^T), so its maximum and sum need one exchange between the wave's halves, and as they
 // lie they are the second product's operand, of whose 32 keys an instruction takes those that one half of the wave holds.
-// Tiles of keys go to LDS past the registers, two on their way (Tile, Places).
+// Tiles of keys go to LDS past the registers, two on their way where three stages fit half of a unit's LDS, else one (Tile, Places).
 //
-// What bounds it: of heads of 128 the matrix instructions and the vector unit by turns ([1,16,8192,128] bfloat16 causal 305 us, 901
+// What bounds it: of heads of 128 the matrix instructions and the vector unit by turns ([1,16,8192,128] bfloat16 causal 305 to 314 us, 875 to 901
 // TFLOP/s; a product of 8192^3 reaches 1259 here); of heads of 64, whose 32 x 32 scores take 256 cycles of products and about 560 of
-// exponentials, sums and rounding, the vector unit and each block's walk from tile to tile ([8,12,1024,64] 27 us).
+// exponentials, sums and rounding, the vector unit and each block's walk from tile to tile ([8,12,1024,64] 27 to 28 us).
 
 #include "attention_tiles.hpp"
 
@@ -188,9 +188,10 @@ void launch_waves(nxh_context *ctx, AttentionArgs a) {
   if (a.mask.base) hipLaunchKernelGGL((attention_train_kernel<EL, DP, KW, true>), grid, dim3(256), 0, ctx->stream, a);
   else hipLaunchKernelGGL((attention_train_kernel<EL, DP, KW, false>), grid, dim3(256), 0, ctx->stream, a);
 }
-// Blocks of 128 queries where there are three for each unit, else of 64: [b,12,1024,64] bfloat16 causal, b = 1 / 2 / 4 / 8, 19.0 / 19.4 /
-// 22.5 / 28.2 us and 15.6 / 17.3 / 19.8 / 32.7;
-// [1,32,2048,128] with 4 heads of keys 75 and 60, [1,16,8192,128] 337 and 383; float32 [4,8,512,64] 45 and 27.
+// Blocks of 128 queries where there are three for each unit, else of 64. Causal, us with blocks of 128 and of 64: bfloat16 [b,12,1024,64],
+// b = 1, 2, 4, 5 (0.4 to 1.9 blocks of 128 a unit) 19 / 16, 20 / 17, 21 / 19, 24 / 21; 6, 7 (2.3 and 2.6) 24.4 / 25.2, 26.1 / 29.1; 8, 9, 16 (3
+// to 6) 27 / 31, 29 / 36, 45 / 56; [1,32,2048,128] with 4 heads of keys (2) 70 / 56, [1,16,8192,128] (4) 303 / 341; float32 [4,8,512,64]
+// (0.5) 44 / 26, [8,8,1024,64] (2) 109 / 85. The border lies between 2 and 2.3; from there to 3 the rule costs up to a tenth.
 template <class EL, int DP>
 void launch(nxh_context *ctx, const AttentionArgs &a) {
   const int64_t blocks = (int64_t)a.batch * a.heads * ((a.sq + 127) / 128);
